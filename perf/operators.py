@@ -382,11 +382,11 @@ def _tables_plain(s):
     pos = ctx[req] + at
     slots = table[req, (pos // page).clamp(max=width - 1)].long() * page + pos % page
     slots = torch.where(admitted[req], slots, torch.full_like(slots, -1))
-    status = (fits & ~admitted).any().int() + 2 * (~fits).any().int()
+    status = (fits & ~admitted).int() + 2 * (~fits).int()          # of each request: 0, or why it was refused
     out_take = torch.where(admitted, take, torch.zeros_like(take)).sum()
     out = [table, free, torch.cat((torch.zeros_like(cu[:1]), cu)).int(),
            torch.where(admitted, ctx + new, torch.zeros_like(ctx)).int(), slots, pos.int(), req.int(),
-           torch.where(admitted, want, held).int(), (top - out_take).int(), status.view(1)]
+           torch.where(admitted, want, held).int(), (top - out_take).int(), status]
     if s["parents"] is not None:
         # ancestors: step every token's pointer to its parent until all have left their tree
         first = (cu - new)[req]
