@@ -25,6 +25,8 @@ SYMBOLS = (
     "dsv41_router_topk", "dsv41_moe_forward_logits",
     "dsv41_ep_peer_buffer_size", "dsv41_ep_peer_alloc", "dsv41_ep_peer_open", "dsv41_ep_peer_close", "dsv41_ep_peer_free",
     "dsv41_ep_peer_forward", "dsv41_ep_peer_read_status",
+    "dsv41_step_tables", "dsv41_store_kv", "dsv41_tree_attention_workspace_size", "dsv41_tree_attention",
+    "dsv41_w4_layout_size", "dsv41_w4_pack", "dsv41_w4_linear", "dsv41_w4_gated",
     "dsv41_set_stage_timing", "dsv41_read_stage_times",
 )
 ABI_VERSION = 2
@@ -55,6 +57,41 @@ class RouterOptions(C.Structure):
 class EpPeerGroup(C.Structure):
     _fields_ = [("rank", C.c_int32), ("world", C.c_int32), ("num_global_experts", C.c_int32),
                 ("tokens_cap", C.c_int32), ("bases", C.c_void_p * MAX_PEERS), ("wait_limit_us", C.c_int32)]
+
+
+class StepTablesArgs(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("width", C.c_int32), ("page_size", C.c_int32), ("num_tokens", C.c_int32),
+                ("context_lens", C.c_void_p), ("new_lens", C.c_void_p), ("held_pages", C.c_void_p),
+                ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("free_pages", C.c_void_p),
+                ("free_count", C.c_void_p), ("free_capacity", C.c_int32), ("mask_words", C.c_int32),
+                ("parents", C.c_void_p), ("cu_lens", C.c_void_p), ("seq_lens", C.c_void_p), ("slots", C.c_void_p),
+                ("positions", C.c_void_p), ("requests", C.c_void_p), ("held_out", C.c_void_p),
+                ("free_count_out", C.c_void_p), ("status", C.c_void_p), ("tree_mask", C.c_void_p)]
+
+
+class StoreKvArgs(C.Structure):
+    _fields_ = [("num_tokens", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("num_pages", C.c_int32),
+                ("page_size", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p), ("k_stride_token", C.c_int64),
+                ("k_stride_head", C.c_int64), ("v_stride_token", C.c_int64), ("v_stride_head", C.c_int64),
+                ("slots", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("stride_page", C.c_int64),
+                ("stride_slot", C.c_int64), ("stride_head", C.c_int64)]
+
+
+class TreeAttentionArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("batch", C.c_int32), ("num_tokens", C.c_int32), ("max_new", C.c_int32),
+                ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32),
+                ("num_pages", C.c_int32), ("max_keys", C.c_int32), ("q", C.c_void_p), ("q_stride_token", C.c_int64),
+                ("q_stride_head", C.c_int64), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+                ("stride_page", C.c_int64), ("stride_slot", C.c_int64), ("stride_head", C.c_int64),
+                ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("seq_lens", C.c_void_p),
+                ("cu_lens", C.c_void_p), ("tree_mask", C.c_void_p), ("mask_words", C.c_int32), ("scale", C.c_float),
+                ("out", C.c_void_p), ("out_stride_token", C.c_int64), ("out_stride_head", C.c_int64),
+                ("lse", C.c_void_p)]
+
+
+class W4WeightC(C.Structure):
+    _fields_ = [("n", C.c_int32), ("k", C.c_int32), ("group", C.c_int32), ("has_zeros", C.c_int32),
+                ("scale_dtype", C.c_int32), ("data", C.c_void_p)]
 
 
 class Dsv41Error(RuntimeError):
@@ -131,6 +168,23 @@ def load(path: str | None = None):
                                             C.c_float, i32, vp, vp]
         L.dsv41_ep_peer_read_status.restype = C.c_int
         L.dsv41_ep_peer_read_status.argtypes = [gp, C.POINTER(MoeLayer), i32, i32, vp, C.POINTER(C.c_int32)]
+        L.dsv41_step_tables.restype = C.c_int
+        L.dsv41_step_tables.argtypes = [C.POINTER(StepTablesArgs), vp]
+        L.dsv41_store_kv.restype = C.c_int
+        L.dsv41_store_kv.argtypes = [C.POINTER(StoreKvArgs), vp]
+        L.dsv41_tree_attention_workspace_size.restype = C.c_int
+        L.dsv41_tree_attention_workspace_size.argtypes = [i32, C.POINTER(C.c_size_t)]
+        L.dsv41_tree_attention.restype = C.c_int
+        L.dsv41_tree_attention.argtypes = [C.POINTER(TreeAttentionArgs), vp, C.c_size_t, vp]
+        wp = C.POINTER(W4WeightC)
+        L.dsv41_w4_layout_size.restype = C.c_int
+        L.dsv41_w4_layout_size.argtypes = [i32, i32, i32, i32, C.POINTER(C.c_size_t)]
+        L.dsv41_w4_pack.restype = C.c_int
+        L.dsv41_w4_pack.argtypes = [vp, vp, vp, i32, i32, i32, vp, C.c_size_t, vp]
+        L.dsv41_w4_linear.restype = C.c_int
+        L.dsv41_w4_linear.argtypes = [wp, vp, i32, C.c_int64, i32, vp, i32, C.c_int64, i32, vp]
+        L.dsv41_w4_gated.restype = C.c_int
+        L.dsv41_w4_gated.argtypes = [wp, wp, vp, i32, C.c_int64, i32, C.c_float, vp, i32, C.c_int64, vp]
         L.dsv41_set_stage_timing.restype = C.c_int
         L.dsv41_set_stage_timing.argtypes = [i32]
         L.dsv41_read_stage_times.restype = C.c_int

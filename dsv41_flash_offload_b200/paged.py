@@ -1,0 +1,215 @@
+"""A paged key/value cache for decode steps with drafted tokens: the step's page tables and slot maps, the
+store of new keys and values, and the attention of drafted trees over the cache.
+
+A cache is a pair of tensors [num_pages, page_size, kv_heads, head_dim]; slot s is token s % page_size of page
+s // page_size, and row b of a block table lists the pages of request b. One step of a layer stack is
+
+    t = step_tables(context_lens, new_lens, held_pages, block_table, free_pages, free_count, page_size, N, parents=...)
+    per layer:  store_kv(k, v, t.slots, k_cache, v_cache)
+                out = tree_attention(q, k_cache, v_cache, block_table, t.seq_lens, t.cu_lens, max_new, tree_mask=t.tree_mask)
+
+All lengths stay on the GPU, nothing synchronises the host, and after the first tree_attention on a stream
+(whose workspace is kept per device, stream and head size) only outputs are allocated, so a step can be
+captured in a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+import threading
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+MAX_REQUESTS = 2048
+MAX_MASK_WORDS = 4
+NO_PAGES, TOO_WIDE, BAD_PARENT, BIG_TREE = 1, 2, 4, 8   # status bits of a request
+
+
+class StepTables(NamedTuple):
+    """What one step of the layer stack reads (all on the GPU)."""
+    cu_lens: torch.Tensor            # int32 [B + 1] running sums of the new tokens
+    seq_lens: torch.Tensor           # int32 [B] context + new tokens (0: the request was refused)
+    slots: torch.Tensor              # int64 [N] cache slot of each new token (-1: none)
+    positions: torch.Tensor          # int32 [N] position of each new token (context + depth in its tree)
+    requests: torch.Tensor           # int32 [N] request of each new token (-1: padding)
+    held_pages: torch.Tensor         # int32 [B] pages held after the step's exchange
+    free_count: torch.Tensor         # int32 [1] height of the stack of free pages after it
+    status: torch.Tensor             # int32 [B] 0, or why a request was refused / its tree is broken
+    tree_mask: torch.Tensor | None   # int64 [N, mask_words] ancestors of each drafted token
+
+
+def _stream(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _vector(t: torch.Tensor, name: str, n: int, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != dev:
+        raise ValueError(f"{name} must be {str(dtype)[6:]} [{n}] on {dev}")
+    return t.contiguous()
+
+
+def step_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, held_pages: torch.Tensor, block_table: torch.Tensor,
+                free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int, num_tokens: int, *,
+                parents: torch.Tensor | None = None, mask_words: int = 1) -> StepTables:
+    """Bring every request's pages in line with its length and build the step's maps, in one launch.
+
+    Request b holds held_pages[b] pages (row b of block_table) for context_lens[b] tokens and brings new_lens[b]
+    (all int32 [B]); surplus pages go back on the stack free_pages[:free_count], missing ones come off it, in
+    request order. block_table [B, W] and free_pages are updated in place; held_pages and free_count come back
+    as new tensors for the next step. A finished request has lengths 0: its pages go back. Rejected drafts:
+    pass the accepted context length and the surplus goes back. num_tokens is the length of the step's token
+    batch, >= sum(new_lens). parents (int32 [num_tokens]): index within its request of each drafted token's
+    parent, which must lie before it, -1 for the context; then positions are context + depth and tree_mask is
+    built, for trees of up to 64 * mask_words tokens. A request that finds no pages is refused: status bit,
+    seq_lens 0, slots -1."""
+    dev = context_lens.device
+    if not context_lens.is_cuda or context_lens.dim() != 1 or not 1 <= context_lens.shape[0] <= MAX_REQUESTS:
+        raise ValueError(f"context_lens must be a CUDA int32 [B] with B in 1..{MAX_REQUESTS}")
+    B, N = context_lens.shape[0], int(num_tokens)
+    context_lens = _vector(context_lens, "context_lens", B, torch.int32, dev)
+    new_lens = _vector(new_lens, "new_lens", B, torch.int32, dev)
+    held_pages = _vector(held_pages, "held_pages", B, torch.int32, dev)
+    free_count = _vector(free_count, "free_count", 1, torch.int32, dev)
+    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.device != dev
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+        raise ValueError(f"block_table must be int32 [{B}, width] with contiguous rows on {dev}")
+    if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous() or free_pages.device != dev:
+        raise ValueError(f"free_pages must be a contiguous int32 vector on {dev}")
+    if N < 0:
+        raise ValueError("num_tokens is negative")
+    mask = None
+    if parents is not None:
+        if not 1 <= mask_words <= MAX_MASK_WORDS:
+            raise ValueError(f"mask_words must be 1..{MAX_MASK_WORDS}")
+        parents = _vector(parents, "parents", N, torch.int32, dev)
+        mask = torch.empty((N, mask_words), dtype=torch.int64, device=dev)
+    pad = (N + 3) // 4 * 4
+    ints = torch.empty(2 * pad + 4 * B + 2, dtype=torch.int32, device=dev)
+    positions, _, requests, _, cu, seq, held, count, status = ints.split((N, pad - N, N, pad - N, B + 1, B, B, 1, B))
+    slots = torch.empty(N, dtype=torch.int64, device=dev)
+    base = ints.data_ptr()
+    args = _lib.StepTablesArgs(
+        B, block_table.shape[1], int(page_size), N, context_lens.data_ptr(), new_lens.data_ptr(), held_pages.data_ptr(),
+        block_table.data_ptr(), block_table.stride(0) if B > 1 else block_table.shape[1], free_pages.data_ptr(),
+        free_count.data_ptr(), free_pages.shape[0], int(mask_words), parents.data_ptr() if parents is not None else None,
+        cu.data_ptr(), seq.data_ptr(), slots.data_ptr(), base, base + 4 * pad, held.data_ptr(), count.data_ptr(),
+        status.data_ptr(), mask.data_ptr() if mask is not None else None)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().dsv41_step_tables(C.byref(args), _stream(dev)), "dsv41_step_tables")
+    return StepTables(cu, seq, slots, positions, requests, held, count, status, mask)
+
+
+def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype or k_cache.stride() != v_cache.stride():
+        raise ValueError("the caches must be [num_pages, page_size, kv_heads, head_dim], alike in shape, dtype and strides")
+    if not k_cache.is_cuda or v_cache.device != k_cache.device:
+        raise ValueError("the caches must live on one CUDA device")
+    if k_cache.dtype not in _DTYPES:
+        raise TypeError(f"unsupported cache dtype {k_cache.dtype} (fp16 or bf16)")
+    if k_cache.shape[3] % 8 or k_cache.shape[3] == 0:
+        raise ValueError("head_dim must be a multiple of 8")
+    if k_cache.stride(3) != 1 or any(s % 8 for s in k_cache.stride()[:3]) or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+        raise ValueError("the caches must have contiguous, 16-byte aligned heads")
+
+
+def _heads(t: torch.Tensor, name: str, unit: int, tokens: int, heads: int, dim: int, like: torch.Tensor) -> torch.Tensor:
+    """t [tokens, heads, dim] in a form the kernels read in pieces of `unit` elements (copied if it is not)."""
+    if t.dim() != 3 or tuple(t.shape) != (tokens, heads, dim) or t.device != like.device:
+        raise ValueError(f"{name} must be [{tokens}, {heads}, {dim}] on {like.device}")
+    if t.dtype != like.dtype:
+        raise TypeError(f"{name} is {t.dtype}, the cache {like.dtype}")
+    if t.stride(2) != 1 or t.stride(0) % unit or t.stride(1) % unit or t.data_ptr() % (2 * unit):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def store_kv(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
+    """k_cache[slots[t]] = k[t] and v_cache[slots[t]] = v[t] for new keys and values [N, kv_heads, head_dim] (any
+    strides with contiguous heads, e.g. slices of a fused projection); slots int64 [N], -1 stores nothing."""
+    _check_cache(k_cache, v_cache)
+    pages, page_size, heads, dim = k_cache.shape
+    N = slots.shape[0]
+    slots = _vector(slots, "slots", N, torch.int64, k_cache.device)
+    k = _heads(k, "k", 8, N, heads, dim, k_cache)
+    v = _heads(v, "v", 8, N, heads, dim, k_cache)
+    args = _lib.StoreKvArgs(N, heads, dim, pages, page_size, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
+                            v.stride(1), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0),
+                            k_cache.stride(1), k_cache.stride(2))
+    with torch.cuda.device(k_cache.device):
+        _lib.check(_lib.load().dsv41_store_kv(C.byref(args), _stream(k_cache.device)), "dsv41_store_kv")
+
+
+# one zeroed workspace per (device, stream, padded head size): its counters are zero between calls, and calls
+# that overlap on several streams get one each
+_ws_lock = threading.Lock()
+_ws: dict = {}
+
+
+def _workspace(dev: torch.device, stream: int, head_dim: int) -> torch.Tensor:
+    key = (dev.index, stream, 64 if head_dim <= 64 else 128 if head_dim <= 128 else 256)
+    buf = _ws.get(key)
+    if buf is None:
+        with _ws_lock:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("dsv41: workspace must be allocated before CUDA-graph capture (run once eagerly)")
+            size = C.c_size_t()
+            _lib.check(_lib.load().dsv41_tree_attention_workspace_size(head_dim, C.byref(size)), "workspace_size")
+            buf = _ws.setdefault(key, torch.zeros(size.value, dtype=torch.uint8, device=dev))
+    return buf
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                   seq_lens: torch.Tensor, cu_lens: torch.Tensor, max_new: int, *, tree_mask: torch.Tensor | None = None,
+                   scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
+    """Attention of the step's new tokens over the paged cache that already holds their keys and values.
+
+    q [N, q_heads, head_dim] (the caches' dtype, head_dim up to 256); request b owns rows cu_lens[b]:cu_lens[b + 1]
+    and the first seq_lens[b] slots of its pages, the last of them its new tokens. With tree_mask (int64 [N, words],
+    step_tables) a token sees the context and the new tokens of its bits, without it the context and the new tokens
+    up to itself. max_new is an upper bound on a request's new tokens, scale defaults to head_dim ** -0.5. Query head
+    h reads KV head h // (q_heads / kv_heads). A row that sees nothing is 0 with lse -inf. Returns out [N, q_heads,
+    head_dim] in q's dtype, or (out, lse fp32 [N, q_heads]); rows past cu_lens[B] are not written."""
+    _check_cache(k_cache, v_cache)
+    pages, page_size, kv_heads, dim = k_cache.shape
+    dev = k_cache.device
+    if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % kv_heads:
+        raise ValueError(f"q must be [N, q_heads, {dim}] with q_heads a multiple of {kv_heads}")
+    N, q_heads = q.shape[0], q.shape[1]
+    q = _heads(q, "q", 2, N, q_heads, dim, k_cache)
+    if seq_lens.dim() != 1:
+        raise ValueError("seq_lens must be int32 [B]")
+    B = seq_lens.shape[0]
+    seq_lens = _vector(seq_lens, "seq_lens", B, torch.int32, dev)
+    cu_lens = _vector(cu_lens, "cu_lens", B + 1, torch.int32, dev)
+    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.device != dev
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+        raise ValueError(f"block_table must be int32 [{B}, width] with contiguous rows on {dev}")
+    words = 1
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != N or tree_mask.device != dev:
+            raise ValueError(f"tree_mask must be int64 [{N}, words] on {dev}")
+        words = tree_mask.shape[1]
+        tree_mask = tree_mask.contiguous()
+    if out is None:
+        out = torch.empty((N, q_heads, dim), dtype=q.dtype, device=dev)
+    elif (tuple(out.shape) != (N, q_heads, dim) or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1
+          or out.stride(0) % 2 or out.stride(1) % 2 or out.data_ptr() % 4):
+        raise ValueError("out must be like q, with contiguous heads")
+    lse = torch.empty((N, q_heads), dtype=torch.float32, device=dev) if return_lse else None
+    stream = _stream(dev)
+    width = block_table.shape[1]
+    args = _lib.TreeAttentionArgs(
+        _DTYPES[q.dtype], B, N, int(max_new), q_heads, kv_heads, dim, page_size, pages, min(width * page_size, 0x7fffff00),
+        q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
+        k_cache.stride(2), block_table.data_ptr(), block_table.stride(0) if B > 1 else width, seq_lens.data_ptr(),
+        cu_lens.data_ptr(), tree_mask.data_ptr() if tree_mask is not None else None, words,
+        1.0 / math.sqrt(dim) if scale is None else float(scale), out.data_ptr(), out.stride(0), out.stride(1),
+        lse.data_ptr() if lse is not None else None)
+    with torch.cuda.device(dev):
+        ws = _workspace(dev, stream, dim)
+        _lib.check(_lib.load().dsv41_tree_attention(C.byref(args), ws.data_ptr(), ws.numel(), stream), "dsv41_tree_attention")
+    return (out, lse) if return_lse else out

@@ -232,6 +232,133 @@ int dsv41_ep_peer_forward(const dsv41_moe_layer* local_layer, const dsv41_ep_pee
 int dsv41_ep_peer_read_status(const dsv41_ep_peer_group* group, const dsv41_moe_layer* local_layer, int32_t topk,
                               int32_t fat_threshold, void* stream, int32_t* status);
 
+/* ------------------------------------------------------------------------------------------
+ * A decode step with drafted tokens around the routed experts (no counterpart in the reference,
+ * whose serving engine brings its own cache and attention): the page tables and slot maps of the
+ * step, the store of the new keys and values, attention of the drafted tokens over the paged cache,
+ * and products with 4-bit weights (projections, shared expert, head).
+ *
+ * A paged cache is [num_pages][page_size][kv_heads][head_dim] for keys and the same for values; slot
+ * s is token s % page_size of page s / page_size. block_table[b][c] is the page of tokens
+ * c * page_size .. of request b.
+ * ------------------------------------------------------------------------------------------ */
+#define DSV41_MAX_REQUESTS 2048
+#define DSV41_MAX_MASK_WORDS 4
+
+/* Status bits of one request after dsv41_step_tables. A refused request (NO_PAGES, TOO_WIDE) keeps the
+ * pages it holds, gets seq_lens 0 and slots -1. */
+enum {
+    DSV41_TABLES_NO_PAGES = 1,   /* the free pages do not reach to it (requests are served in order) */
+    DSV41_TABLES_TOO_WIDE = 2,   /* its pages exceed the table's width */
+    DSV41_TABLES_BAD_PARENT = 4, /* a parent is not an earlier token of the request (taken as -1) */
+    DSV41_TABLES_BIG_TREE = 8    /* tokens past 64 * mask_words: they are in no mask */
+};
+
+/* Bring the pages of every request in line with its length. Request b has context_lens[b] tokens in the
+ * cache, new_lens[b] new ones in this step and holds held_pages[b] pages, listed in its row of block_table.
+ * It needs ceil((context + new) / page_size): surplus pages go back on the stack of free pages (in request
+ * order), missing ones then come off its top (in request order) into the row. Entries of a row past its
+ * pages are stale. All pointers are device memory; num_tokens >= sum of new_lens (the caller knows it as
+ * the length of the step's token batch; later entries get slot -1, position 0, request -1).
+ * Outputs: cu_lens [batch + 1] running sums of new_lens; seq_lens [batch] = context + new; held_out [batch];
+ * free_count_out [1]; status [batch]; per token: slots (int64), positions, requests (its b). Without
+ * parents a token's position is context + its index; with parents ([num_tokens], index of the parent
+ * within the request, -1 = the context) it is context + its depth, and tree_mask [num_tokens][mask_words]
+ * holds a bit for each ancestor and itself. The int32 outputs may not overlap the inputs. slots,
+ * positions and requests must be 16-byte aligned. */
+typedef struct dsv41_step_tables_args {
+    int32_t batch, width, page_size, num_tokens;
+    const int32_t* context_lens;
+    const int32_t* new_lens;
+    const int32_t* held_pages;
+    int32_t* block_table;         /* [batch][table_stride], updated */
+    int64_t table_stride;
+    int32_t* free_pages;          /* [free_capacity], updated */
+    const int32_t* free_count;    /* [1] */
+    int32_t free_capacity;
+    int32_t mask_words;           /* 1..DSV41_MAX_MASK_WORDS (with parents) */
+    const int32_t* parents;       /* or NULL */
+    int32_t* cu_lens;
+    int32_t* seq_lens;
+    int64_t* slots;
+    int32_t* positions;
+    int32_t* requests;
+    int32_t* held_out;
+    int32_t* free_count_out;
+    int32_t* status;
+    int64_t* tree_mask;           /* or NULL (without parents) */
+} dsv41_step_tables_args;
+int dsv41_step_tables(const dsv41_step_tables_args* args, void* stream);
+
+/* cache[slots[t]] = k[t], v[t]; a slot outside the cache (-1) stores nothing. 16-bit elements; head_dim a
+ * multiple of 8, addresses 16-byte aligned, strides (in elements) multiples of 8. Slots that repeat within a call
+ * leave one of their tokens, whichever. */
+typedef struct dsv41_store_kv_args {
+    int32_t num_tokens, kv_heads, head_dim, num_pages, page_size;
+    const void* k;
+    const void* v;
+    int64_t k_stride_token, k_stride_head, v_stride_token, v_stride_head;
+    const int64_t* slots;
+    void* k_cache;
+    void* v_cache;
+    int64_t stride_page, stride_slot, stride_head;   /* of both caches */
+} dsv41_store_kv_args;
+int dsv41_store_kv(const dsv41_store_kv_args* args, void* stream);
+
+/* out[t][hq] = softmax(scale * q . k) v over the keys that token t of its request sees. Request b owns rows
+ * cu_lens[b] .. cu_lens[b + 1] - 1 of q, its keys are the first seq_lens[b] of its pages, the last of them its
+ * new tokens. Token i sees the whole context and, with tree_mask, the new tokens of its bits; without, the
+ * new tokens up to itself. Keys and values that a row does not see never reach it, whatever they hold. A row
+ * that sees nothing is 0 (lse -inf); so are the rows of a request with seq_lens[b] < its new tokens or >
+ * max_keys. Query head hq reads KV head hq / (q_heads / kv_heads). head_dim a multiple of 8 up to 256. dtype of q,
+ * caches and out: fp16 or bf16. max_new: upper bound on a request's new tokens (a hint that picks the row
+ * tile). lse [num_tokens][q_heads] (natural logarithm of the sums) or NULL. The workspace is zeroed once
+ * after allocation; every call leaves its counters zero. One workspace serves one stream. */
+typedef struct dsv41_tree_attention_args {
+    int32_t dtype, batch, num_tokens, max_new;
+    int32_t q_heads, kv_heads, head_dim, page_size, num_pages, max_keys;
+    const void* q;
+    int64_t q_stride_token, q_stride_head;
+    const void* k_cache;
+    const void* v_cache;
+    int64_t stride_page, stride_slot, stride_head;
+    const int32_t* block_table;
+    int64_t table_stride;
+    const int32_t* seq_lens;
+    const int32_t* cu_lens;
+    const int64_t* tree_mask;     /* [num_tokens][mask_words] or NULL */
+    int32_t mask_words;
+    float scale;
+    void* out;
+    int64_t out_stride_token, out_stride_head;
+    float* lse;
+} dsv41_tree_attention_args;
+int dsv41_tree_attention_workspace_size(int32_t head_dim, size_t* bytes);
+int dsv41_tree_attention(const dsv41_tree_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* 4-bit weights: w[n][k] = scale[n][k / group] * (code - zero[n][k / group]), codes 0..15, zero points
+ * 0..15 (8 where there are none), groups of 32, 64 or 128 inputs, k a multiple of the group, any n.
+ * dsv41_w4_pack lays a matrix out once: codes [n][k / 2] uint8 (even k in the low nibble), scales
+ * [n][k / group] fp16 or bf16, zeros [n][k / group] uint8 or NULL -> data, dsv41_w4_layout_size bytes. */
+typedef struct dsv41_w4_weight {
+    int32_t n, k, group;
+    int32_t has_zeros;
+    int32_t scale_dtype;          /* DSV41_DTYPE_F16 or DSV41_DTYPE_BF16 */
+    const void* data;
+} dsv41_w4_weight;
+int dsv41_w4_layout_size(int32_t n, int32_t k, int32_t group, int32_t has_zeros, size_t* bytes);
+int dsv41_w4_pack(const void* codes, const void* scales, const void* zeros, int32_t n, int32_t k, int32_t group,
+                  void* data, size_t data_bytes, void* stream);
+/* out[t][n] = sum_k w[n][k] x[t][k], fp32 sums, x fp16 or bf16 [tokens][x_stride] (16-byte aligned, x_stride a
+ * multiple of 8), out fp32, fp16 or bf16 [tokens][out_stride]; accumulate (fp32 out only) adds into out. */
+int dsv41_w4_linear(const dsv41_w4_weight* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t tokens,
+                    void* out, int32_t out_dtype, int64_t out_stride, int32_t accumulate, void* stream);
+/* out[t][n] = min(silu(g), limit) * clamp(u, -limit, limit) with g, u the products with gate and up (same n,
+ * k and group); limit 0 = no clamp (the routed experts' SwiGLU). */
+int dsv41_w4_gated(const dsv41_w4_weight* gate, const dsv41_w4_weight* up, const void* x, int32_t x_dtype,
+                   int64_t x_stride, int32_t tokens, float limit, void* out, int32_t out_dtype, int64_t out_stride,
+                   void* stream);
+
 /* Profiling (no counterpart in the reference; used by bench.py to time each kernel on the stream
  * it runs on). While enabled, dsv41_moe_forward records CUDA events at its stage boundaries for up
  * to DSV41_TIMING_MAX_CALLS calls (not under stream capture). dsv41_read_stage_times synchronises
