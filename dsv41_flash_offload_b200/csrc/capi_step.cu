@@ -211,16 +211,14 @@ int dsv41_tree_attention(const dsv41_tree_attention_args* a, void* workspace, si
         return set_error(DSV41_E_INVALID, "NULL pointer");
     if (a->tree_mask && (a->mask_words < 1 || a->mask_words > kMaxMaskWords))
         return set_error(DSV41_E_INVALID, "mask_words=%d (1..%d)", a->mask_words, kMaxMaskWords);
-    if (!aligned(a->q, 4) || !aligned(a->out, 4) || !aligned(a->k_cache, 16) || !aligned(a->v_cache, 16))
-        return set_error(DSV41_E_INVALID, "q and out must be 4-byte, the caches 16-byte aligned");
+    if (!aligned(a->q, 16) || !aligned(a->out, 16) || !aligned(a->k_cache, 16) || !aligned(a->v_cache, 16))
+        return set_error(DSV41_E_INVALID, "q, out and the caches must be 16-byte aligned");
     if (!aligned(workspace, 256)) return set_error(DSV41_E_INVALID, "the workspace must be 256-byte aligned");
     if (workspace_bytes < need) return set_error(DSV41_E_WORKSPACE, "workspace %zu bytes < required %zu", workspace_bytes, need);
-    const int64_t even[] = {a->q_stride_token, a->q_stride_head, a->out_stride_token, a->out_stride_head};
-    for (int64_t s : even)
-        if (s < 0 || s % 2) return set_error(DSV41_E_INVALID, "q or out stride %lld is odd", (long long)s);
-    const int64_t eights[] = {a->stride_page, a->stride_slot, a->stride_head};
-    for (int64_t s : eights)
-        if (s < 0 || s % 8) return set_error(DSV41_E_INVALID, "cache stride %lld is not a multiple of 8 elements", (long long)s);
+    const int64_t strides[] = {a->q_stride_token, a->q_stride_head, a->out_stride_token, a->out_stride_head,
+                               a->stride_page, a->stride_slot, a->stride_head};
+    for (int64_t s : strides)
+        if (s < 0 || s % 8) return set_error(DSV41_E_INVALID, "stride %lld is not a multiple of 8 elements", (long long)s);
     if (!std::isfinite(a->scale)) return set_error(DSV41_E_INVALID, "scale %g", a->scale);
     TreeAttnParams p{};
     p.q = a->q;
@@ -242,6 +240,7 @@ int dsv41_tree_attention(const dsv41_tree_attention_args* a, void* workspace, si
     p.lse = a->lse;
     const AttnWorkspace w = tree_attn_workspace(a->head_dim);
     unsigned char* ws = static_cast<unsigned char*>(workspace);
+    p.status = reinterpret_cast<int*>(ws);
     p.counters = reinterpret_cast<int*>(ws + w.counters);
     p.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
     p.part_o = reinterpret_cast<float*>(ws + w.part_o);
@@ -256,6 +255,7 @@ int dsv41_tree_attention(const dsv41_tree_attention_args* a, void* workspace, si
     p.max_keys = a->max_keys;
     p.mask_words = a->mask_words;
     p.page_div = FastDiv::make(a->page_size);
+    p.group_div = FastDiv::make(p.group);
     p.scale_log2 = a->scale * 1.4426950408889634f;
     const int64_t rows = (int64_t)(a->max_new ? a->max_new : 1) * p.group;
     return launched(launch_tree_attn(p, a->dtype, (int)(rows > 1024 ? 1024 : rows), static_cast<cudaStream_t>(stream)),

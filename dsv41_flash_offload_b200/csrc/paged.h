@@ -67,18 +67,20 @@ struct TreeAttnParams {
     float2* part_ml;
     float* part_o;
     int* counters;                                     // zero between calls
+    int* status;
     int batch, num_tokens, q_heads, kv_heads, group, head_dim, page_size, num_pages, max_keys, mask_words;
-    FastDiv page_div;
+    FastDiv page_div, group_div;
     float scale_log2;                                  // scale * log2(e)
 };
 
-struct AttnWorkspace {
+struct AttnWorkspace {   // the status word lies at 0
     size_t counters, part_ml, part_o, total;
 };
 AttnWorkspace tree_attn_workspace(int head_dim);
 
 // dtype 0 fp16, 1 bf16; max_rows: upper bound on a request's new tokens times the group (picks the row tile)
 cudaError_t launch_tree_attn(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st);
+cudaError_t launch_tree_attn_tc(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st);   // head_dim <= 128
 cudaError_t launch_step_tables(const StepTablesParams& p, cudaStream_t st);
 cudaError_t launch_store_kv(const StoreKvParams& p, cudaStream_t st);
 

@@ -14,11 +14,8 @@
 // resident CTA, whatever the lengths are; the cut is computed in the kernel from the lengths (the host does
 // not know them). A segment (the units of one row tile) that crosses CTAs leaves (m, l, O) per part in the
 // workspace and the CTA that arrives last joins the parts in order: one launch, results independent of timing.
-#include <cuda_bf16.h>
-
-#include "common.cuh"
 #include "internal.h"
-#include "paged.h"
+#include "tree_attn.cuh"
 
 namespace dsv41 {
 
@@ -37,140 +34,10 @@ struct AttnCfg {
     static constexpr int buf_b = wn > 1 ? rt * DT * 4 : kAttnWarps * 16 * tn * 4;   // joins of warps / P of a dirty tile
     static constexpr int ml_off = stages * 2 * tile_b + buf_b;
     static constexpr int smem = ml_off + wn * rt * 8;
-    static constexpr int per_sm = smem <= 56 * 1024 ? 4 : smem <= 74 * 1024 ? 3 : smem <= 113 * 1024 ? 2 : 1;
+    static constexpr int per_sm = smem <= 113 * 1024 ? 2 : 1;
     static_assert(tn >= 16 && tn % 16 == 0, "a warp's keys are whole k16 steps");
     static_assert(kMaxRequests * 8 <= stages * 2 * tile_b, "the prefix sums live in the stages");
 };
-
-template <typename T>
-__device__ __forceinline__ void mma_t(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-{
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
-        mma_16816(d, a, b0, b1);
-    } else {
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b)
-{
-    if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t v)
-{
-    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
-    else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
-}
-template <typename T>
-__device__ constexpr uint32_t exp_bits()
-{
-    return std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-}
-// the pair with infinities and NaN replaced by zero
-template <typename T>
-__device__ __forceinline__ uint32_t finite2(uint32_t v)
-{
-    constexpr uint32_t e = exp_bits<T>();
-    if ((v & e) == e) v &= 0xffff0000u;
-    if ((v & (e << 16)) == (e << 16)) v &= 0x0000ffffu;
-    return v;
-}
-template <typename T>
-__device__ __forceinline__ bool any_nonfinite(uint4 v)
-{
-    constexpr uint32_t e = exp_bits<T>();
-    auto bad = [](uint32_t w) { return (w & e) == e || (w & (e << 16)) == (e << 16); };
-    return bad(v.x) || bad(v.y) || bad(v.z) || bad(v.w);
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&a)[4], uint32_t addr)
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-                 : "r"(addr));
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live)
-{
-    const int n = live ? 16 : 0;   // 0: sixteen zero bytes
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait()
-{
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ float exp2_fast(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// One request as the kernel sees it: n new tokens from row q0 of the batch, seq keys (0 when the lengths do
-// not hold the new tokens: a refused request, whose rows see nothing), clamped to what the arrays hold.
-struct AttnReq {
-    int q0, n, seq;
-};
-__device__ __forceinline__ AttnReq attn_req(const TreeAttnParams& p, int b)
-{
-    AttnReq r;
-    r.q0 = min(max(p.cu_lens[b], 0), p.num_tokens);
-    r.n = max(min(p.cu_lens[b + 1], p.num_tokens) - r.q0, 0);
-    r.seq = p.seq_lens[b];
-    if (r.seq < r.n || r.seq > p.max_keys) r.seq = 0;
-    return r;
-}
-
-// Position in the list of units: request, KV head, row tile, key tile.
-template <int RT, int KT>
-struct UnitCursor {
-    int b, h, rt, kt, nrt, nkt;
-    AttnReq r;
-    __device__ __forceinline__ void enter(const TreeAttnParams& p)
-    {
-        r = attn_req(p, b);
-        nrt = (r.n * p.group + RT - 1) / RT;
-        nkt = max((r.seq + KT - 1) / KT, 1);
-    }
-    __device__ __forceinline__ void next(const TreeAttnParams& p)
-    {
-        if (++kt < nkt) return;
-        kt = 0;
-        if (++rt < nrt) return;
-        rt = 0;
-        if (++h < p.kv_heads) return;
-        h = 0;
-        while (++b < p.batch) {
-            enter(p);
-            if (r.n > 0) return;
-        }
-    }
-};
-
-// bits j0 .. j0 + 63 of what new token i sees, bit x for new token j0 + x; a negative j is context: seen
-__device__ __forceinline__ uint64_t seen_window(const TreeAttnParams& p, const AttnReq& r, int i, int j0)
-{
-    auto word = [&](int w) -> uint64_t {
-        if (w < 0) return ~0ull;
-        if (p.tree_mask) return w < p.mask_words ? (uint64_t)p.tree_mask[(int64_t)(r.q0 + i) * p.mask_words + w] : 0ull;
-        return w < (i >> 6) ? ~0ull : w > (i >> 6) ? 0ull : (~0ull >> (63 - (i & 63)));
-    };
-    const int w = j0 >> 6, sh = j0 & 63;
-    uint64_t v = word(w) >> sh;
-    if (sh) v |= word(w + 1) << (64 - sh);
-    const int left = r.n - j0;   // new tokens from j0 on
-    return left >= 64 ? v : left <= 0 ? 0ull : v & (~0ull >> (64 - left));
-}
 
 template <typename T, int DT, int WM>
 __global__ void __launch_bounds__(kAttnThreads, AttnCfg<DT, WM>::per_sm) tree_attn_kernel(const TreeAttnParams p)
@@ -613,26 +480,23 @@ static cudaError_t launch_attn_rows(const TreeAttnParams& p, int rows, cudaStrea
 
 cudaError_t launch_tree_attn(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st)
 {
-    auto by_dim = [&](auto t) {
-        using T = decltype(t);
-        if (p.head_dim <= 64) return launch_attn_rows<T, 64>(p, max_rows, st);
-        if (p.head_dim <= 128) return launch_attn_rows<T, 128>(p, max_rows, st);
-        return launch_attn_rows<T, 256>(p, max_rows, st);
-    };
-    return dtype == 0 ? by_dim(__half{}) : by_dim(__nv_bfloat16{});
+    if (p.head_dim <= 128) return launch_tree_attn_tc(p, dtype, max_rows, st);
+    return dtype == 0 ? launch_attn_rows<__half, 256>(p, max_rows, st) : launch_attn_rows<__nv_bfloat16, 256>(p, max_rows, st);
 }
 
-// most parts a call can leave: two per CTA, 4 CTAs per SM at most, 64 rows of the padded head size
+// Most parts a call can leave: two per CTA (one CTA per SM and up to 256 rows on the tensor-memory path, two CTAs
+// per SM and up to 64 rows on the other), of the padded head size.
 AttnWorkspace tree_attn_workspace(int head_dim)
 {
-    const int dt = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-    const int64_t ctas = (int64_t)num_sms() * 4, slots = 2 * ctas;
+    const bool tc = head_dim <= 128;
+    const int64_t dt = head_dim <= 64 ? 64 : tc ? 128 : 256;
+    const int64_t ctas = (int64_t)num_sms() * (tc ? 1 : 2), rows = 2 * ctas * (tc ? 256 : 64);
     AttnWorkspace w;
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-    w.counters = 0;
-    w.part_ml = up(ctas * sizeof(int));
-    w.part_o = w.part_ml + up(slots * 64 * sizeof(float2));
-    w.total = w.part_o + up(slots * 64 * dt * sizeof(float));
+    w.counters = 256;
+    w.part_ml = w.counters + up(2 * ctas * sizeof(int));
+    w.part_o = w.part_ml + up(rows * sizeof(float2));
+    w.total = w.part_o + up(rows * dt * sizeof(float));
     return w;
 }
 

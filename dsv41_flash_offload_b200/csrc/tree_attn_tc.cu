@@ -1,0 +1,799 @@
+// Attention of drafted tokens over a paged cache on the fifth-generation tensor cores (head sizes up to 128;
+// the mathematics, the rows and the cut of the work into runs are those of tree_attn.cu).
+//
+// One CTA per SM walks its run of (request, KV head, row tile, key tile) units:
+//   producers (4 warps)  copy key and value tiles of 128 keys (page by page, 16-byte cp.async) into a ring of
+//                        units in the 128-byte swizzle the tensor cores read; a ring of byte offsets, one per
+//                        key, is looked up one tile ahead
+//   Q loader (1 warp)    the rows of the segment
+//   issuer (1 thread)    S = Q K^T (A and B from shared memory) and O += P V (A from tensor memory, V read as it
+//                        lies, N-major), fp32 accumulators in tensor memory
+//   softmax (4 warps per 128 rows; thread = row)  S out of tensor memory, running maximum and sum, P back into
+//                        tensor memory as 16-bit pairs; at the end of a segment O out
+// The product of tile i + 1 runs while tile i is in the softmax (two S and P buffers for up to 128 rows; two row
+// tiles take turns for up to 256).
+//
+// Few rows (REP 4 or 2): the tensor cores compute 128 rows whatever they hold, so 32 (64) rows are repeated 4
+// (2) times and each repeat takes a quarter (half) of a tile's keys: its P is zero elsewhere, so the four warps
+// share the exponentials of the few rows, and the repeats are joined like any split over keys.
+//
+// The accumulator is rescaled only when a row's maximum grows by more than 2^8: P stays below 2^8, its rounding
+// is relative, and the sums are fp32, so the deferral costs no accuracy; a rescale has to wait for the product
+// in flight, the deferral makes that rare.
+#include "internal.h"
+#include "tree_attn.cuh"
+
+namespace dsv41 {
+
+template <int DT, int MT, int REP>
+struct TcCfg {
+    static_assert(MT == 1 || REP == 1, "repeats are for a single tile of 128 rows");
+    static constexpr int kt = 128;                           // keys per tile
+    static constexpr int rt = MT * 128 / REP;                // rows per tile
+    static constexpr int kw = kt / REP;                      // keys of a tile per softmax thread
+    static constexpr int soft_warps = 4 * MT;
+    static constexpr int w_prod = soft_warps, w_q = w_prod + 4, w_mma = w_q + 1;
+    static constexpr int threads = (w_mma + 1) * 32;
+    static constexpr int block_b = 128 * 128;                // 128 rows x 64 columns of 16 bits, swizzled
+    static constexpr int blocks = DT / 64;
+    static constexpr int unit_b = blocks * block_b;          // a key or value tile
+    static constexpr int q_b = MT * unit_b;
+    static constexpr int stage_b = soft_warps * 32 * 17 * 4; // O on its way out, 16 columns at a time
+    static constexpr int off_b = 4 * kt * 8;                 // byte offsets of the keys of four tiles
+    static constexpr int ml_b = MT * 128 * 8;
+    static constexpr int bars_b = 1024;
+    static constexpr int fixed_b = 1024 + q_b + stage_b + off_b + ml_b + bars_b;
+    static constexpr int units_fit = (232448 - fixed_b) / unit_b;
+    static constexpr int units = units_fit < 10 ? units_fit : 10;
+    static constexpr int lag = units - 2;                    // units a producer has in flight when it issues the next
+    static constexpr int smem = fixed_b + units * unit_b;
+    static_assert(units >= 4, "ring too short");
+    // tensor memory columns
+    __host__ __device__ static constexpr int s_col(int b) { return b * 128; }
+    __host__ __device__ static constexpr int p_col(int b) { return MT == 1 ? 256 + b * 64 : b * 128; }
+    __host__ __device__ static constexpr int o_col(int t) { return MT == 1 ? 384 : 256 + t * 128; }
+};
+
+// ---- tcgen05 ----------------------------------------------------------------------------------
+__device__ __forceinline__ void tcf_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tcf_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_proxy_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// swizzled-128B operand, rows of 128 bytes, 8-row atoms of 1024 bytes. K-major: lbo unused. N-major: lbo is the
+// distance of the 64-column blocks.
+__device__ __forceinline__ uint64_t tc_desc(uint32_t saddr, uint32_t lbo)
+{
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// tensor memory loads with their wait, in one statement: the registers are valid once it has run
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, float* v)
+{
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, float* v)
+{
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        " tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ uint32_t tc_ld1(uint32_t taddr)
+{
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n tcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(taddr) : "memory");
+    return r;
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+template <typename T, int DT, int MT, int REP>
+__global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_kernel(const TreeAttnParams p)
+{
+    using Cfg = TcCfg<DT, MT, REP>;
+    constexpr int KT = Cfg::kt, RT = Cfg::rt, KW = Cfg::kw, NU = Cfg::units, LAG = Cfg::lag, CPR = DT / 8;
+    using Cursor = UnitCursor<RT, KT>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* sq = smem;
+    unsigned char* su = sq + Cfg::q_b;
+    float* stage = reinterpret_cast<float*>(su + NU * Cfg::unit_b);
+    int64_t* key_off = reinterpret_cast<int64_t*>(reinterpret_cast<unsigned char*>(stage) + Cfg::stage_b);
+    float2* ml = reinterpret_cast<float2*>(key_off + 4 * KT);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(ml + MT * 128);
+    uint64_t* full = bars;                 // [NU] a unit's copies have landed (4 producer warps)
+    uint64_t* empty = full + NU;           // [NU] its products are done
+    uint64_t* q_full = empty + NU;         // the segment's rows have landed
+    uint64_t* q_free = q_full + 1;         // its last S product is done
+    uint64_t* s_full = q_free + 1;         // [2] S buffer computed
+    uint64_t* p_full = s_full + 2;         // [2] P buffer written (4 softmax warps)
+    uint64_t* pv_done = p_full + 2;        // [2] O updated (per row tile)
+    uint64_t* all_done = pv_done + 2;
+    int* dirty = reinterpret_cast<int*>(all_done + 1);   // [NU] 1 + ring position of a unit that held infinities or NaN
+    int* s_last = dirty + NU;              // [2]
+    volatile int* abort_flag = s_last + 2;
+    uint32_t* tmem_slot = const_cast<uint32_t*>(reinterpret_cast<volatile uint32_t*>(abort_flag)) + 1;
+    __shared__ int64_t warp_tot[Cfg::threads / 32];
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+    // ---- this CTA's run of units ----
+    int64_t* pre = reinterpret_cast<int64_t*>(su);
+    int64_t total = 0;
+    {
+        const int per = (p.batch + Cfg::threads - 1) / Cfg::threads;
+        const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+        auto units_of = [&](int b) -> int64_t {
+            const AttnReq r = attn_req(p, b);
+            return r.n > 0 ? (int64_t)((r.n * p.group + RT - 1) / RT) * max((r.seq + KT - 1) / KT, 1) * p.kv_heads : 0;
+        };
+        int64_t sum = 0;
+        for (int b = b0; b < b1; ++b) sum += units_of(b);
+        int64_t inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        if (lane == 31) warp_tot[warp] = inc;
+        __syncthreads();
+        int64_t base = inc - sum;
+        for (int w = 0; w < Cfg::threads / 32; ++w) {
+            if (w < warp) base += warp_tot[w];
+            total += warp_tot[w];
+        }
+        for (int b = b0; b < b1; ++b) {
+            pre[b] = base;
+            base += units_of(b);
+        }
+        __syncthreads();
+    }
+    const int64_t run = (total + gridDim.x - 1) / gridDim.x;
+    const int64_t u0 = run * blockIdx.x;
+    const int count = (int)max(min(run, total - u0), (int64_t)0);
+    if (count <= 0) return;
+    Cursor cur;
+    {
+        int lo = 0, hi = p.batch;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (pre[mid] <= u0) lo = mid;
+            else hi = mid;
+        }
+        cur.b = lo;
+        cur.enter(p);
+        int64_t at = u0 - pre[lo];
+        const int64_t per_head = (int64_t)cur.nrt * cur.nkt;
+        cur.h = (int)(at / per_head);
+        at -= cur.h * per_head;
+        cur.rt = (int)(at / cur.nkt);
+        cur.kt = (int)(at - (int64_t)cur.rt * cur.nkt);
+    }
+    __syncthreads();   // the prefix sums lie in the ring
+
+    if (tid == 0) {
+        for (int i = 0; i < NU; ++i) {
+            mbar_init(&full[i], 4);
+            mbar_init(&empty[i], 1);
+            dirty[i] = 0;
+        }
+        mbar_init(q_full, 1);
+        mbar_init(q_free, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&pv_done[i], 1);
+        }
+        mbar_init(all_done, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == Cfg::w_mma) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (p.head_dim % 16) {   // the last 16-column step of Q K^T reads past the head size: zeros there
+        uint4* z = reinterpret_cast<uint4*>(sq);
+        for (int i = tid; i < (Cfg::q_b + NU * Cfg::unit_b) / 16; i += Cfg::threads) z[i] = make_uint4(0, 0, 0, 0);
+        fence_proxy_smem();
+    }
+    tcf_before();
+    __syncthreads();
+    tcf_after();
+    const uint32_t tmem = *tmem_slot;
+    const int ksteps = (p.head_dim + 15) / 16;
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, abort_flag, p.status); };
+    // ring position of tile i's keys and values: K0 K1 V0 K2 V1 ... (the order in which they are needed)
+    auto k_pos = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
+    auto v_pos = [&](int i) { return i == count - 1 ? 2 * i + 1 : 2 * i + 2; };
+
+    if (warp >= Cfg::w_prod && warp < Cfg::w_prod + 4) {
+        // ---------------------------------- producers ----------------------------------
+        const int pt = tid - Cfg::w_prod * 32, chunk = pt % CPR, row0 = pt / CPR;
+        constexpr int kRowStep = 128 / CPR;
+        const bool col_live = chunk * 8 < p.head_dim;
+        const uint32_t col_at = (chunk >> 3) * Cfg::block_b;
+        const uint32_t ring = smem_addr(su);
+        uint32_t hist = 0;   // bit k: the unit issued k units ago holds new tokens' values
+        auto arrive = [&](int n, bool check) {   // this thread's copies of unit n have landed
+            const int slot = n % NU;
+            if (check && col_live) {
+                // infinities and NaN among new tokens' values would reach rows that do not see them (0 * NaN):
+                // zero them here and leave a mark; the softmax warps add them to the rows that do see them
+                bool bad = false;
+                for (int row = row0; row < KT; row += kRowStep) {
+                    uint4* at = reinterpret_cast<uint4*>(su + slot * Cfg::unit_b + col_at + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+                    uint4 v = *at;
+                    if (any_nonfinite<T>(v)) {
+                        v.x = finite2<T>(v.x), v.y = finite2<T>(v.y), v.z = finite2<T>(v.z), v.w = finite2<T>(v.w);
+                        *at = v;
+                        bad = true;
+                    }
+                }
+                if (bad) *reinterpret_cast<volatile int*>(dirty + slot) = n + 1;
+            }
+            fence_proxy_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[slot]);
+        };
+        auto issue = [&](int n, const void* cache, const int64_t* offs, bool check) {
+            const int slot = n % NU;
+            wait(&empty[slot], ((n / NU) & 1) ^ 1);
+            if (col_live) {
+                const uint32_t dst = ring + slot * Cfg::unit_b + col_at;
+#pragma unroll 8
+                for (int row = row0; row < KT; row += kRowStep) {
+                    const int64_t off = offs[row];
+                    cp_async16(dst + row * 128 + (((chunk & 7) ^ (row & 7)) << 4),
+                               static_cast<const T*>(cache) + (off < 0 ? 0 : off + chunk * 8), off >= 0);
+                }
+            }
+            cp_async_commit();
+            hist = (hist << 1) | (check ? 1u : 0u);
+            cp_async_wait<LAG>();
+            if (n >= LAG) arrive(n - LAG, (hist >> LAG) & 1);
+        };
+        // element offset of key `pt` of the cursor's tile (-1: past the end, or not a page of this cache)
+        auto offset_of = [&](const Cursor& c) -> int64_t {
+            const int pos = c.kt * KT + pt;
+            if (pos >= c.r.seq) return -1;
+            const int pg = p.page_div.div(pos);
+            const int id = __ldg(p.block_table + (int64_t)c.b * p.table_stride + pg);
+            if ((unsigned)id >= (unsigned)p.num_pages) return -1;
+            return id * p.stride_page + (pos - pg * p.page_size) * p.stride_slot + c.h * p.stride_head;
+        };
+        int64_t next_off = offset_of(cur);
+        bool tail = false, tail_before = false;
+        int n = 0;
+        for (int step = 0; step <= count; ++step) {
+            if (step < count) {
+                key_off[(step & 3) * KT + pt] = next_off;
+                tail_before = tail;
+                tail = cur.kt * KT + KT > cur.r.seq - cur.r.n;
+                if (step + 1 < count) {
+                    cur.next(p);
+                    next_off = offset_of(cur);
+                }
+                named_bar_sync(3, 128);
+                issue(n++, p.k_cache, key_off + (step & 3) * KT, false);
+            } else {
+                tail_before = tail;
+            }
+            if (step > 0) issue(n++, p.v_cache, key_off + ((step - 1) & 3) * KT, tail_before);
+        }
+        cp_async_wait<0>();
+        for (int u = max(n - LAG, 0); u < n; ++u) arrive(u, (hist >> (n - 1 - u)) & 1);
+    } else if (warp == Cfg::w_q) {
+        // ---------------------------------- Q loader ----------------------------------
+        const int chunk = lane % CPR;
+        constexpr int kRowStep = 32 / CPR;
+        int seg = 0;
+        for (int it = 0; it < count; ++it) {
+            if (it == 0 || cur.kt == 0) {
+                wait(q_free, (seg & 1) ^ 1);
+                const int rows = min(RT, cur.r.n * p.group - cur.rt * RT);
+                if (chunk * 8 < p.head_dim) {
+#pragma unroll 4
+                    for (int r = lane / CPR; r < MT * 128; r += kRowStep) {
+                        const int row = r % RT;
+                        if (row >= rows) continue;   // rows of no token: whatever lies there, nothing of it is read
+                        const int at = cur.rt * RT + row, i = p.group_div.div(at), g = at - i * p.group;
+                        const T* src = static_cast<const T*>(p.q) + (int64_t)(cur.r.q0 + i) * p.q_stride_token +
+                                       (int64_t)(cur.h * p.group + g) * p.q_stride_head + chunk * 8;
+                        cp_async16(smem_addr(sq) + (r >> 7) * Cfg::unit_b + (chunk >> 3) * Cfg::block_b + (r & 127) * 128 +
+                                       (((chunk & 7) ^ (r & 7)) << 4),
+                                   src, true);
+                    }
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                fence_proxy_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+                ++seg;
+            }
+            cur.next(p);
+        }
+    } else if (warp == Cfg::w_mma) {
+        // ---------------------------------- issuer ----------------------------------
+        if (lane == 0) {
+            constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
+            constexpr uint32_t kBase = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(128 >> 4) << 24);
+            constexpr uint32_t idesc_s = kBase | ((uint32_t)(KT >> 3) << 17);
+            const uint32_t idesc_o = kBase | (1u << 16) | ((uint32_t)(ksteps * 16 >> 3) << 17);   // V is N-major
+            const uint32_t q_at = smem_addr(sq), ring = smem_addr(su);
+            bool ok = true;
+            Cursor cq = cur;          // cursor of the S products
+            int seg_q = 0;            // segments whose rows have been awaited
+            int used[2] = {0, 0};     // MT == 2: tiles of each row tile so far (S products issued)
+            auto first_of = [&](const Cursor& c, int i) { return i == 0 || c.kt == 0; };
+            auto k_ready = [&](int i) {
+                const int n = k_pos(i);
+                if (ok && first_of(cq, i)) ok = wait(q_full, seg_q++ & 1);
+                ok = ok && wait(&full[n % NU], (n / NU) & 1);
+            };
+            auto s_product = [&](int i, int t, int buf) {
+                const int n = k_pos(i);
+                const uint32_t kb = ring + (n % NU) * Cfg::unit_b, qb = q_at + t * Cfg::unit_b;
+                tcf_after();
+                for (int kk = 0; kk < ksteps; ++kk) {
+                    const uint32_t at = (kk >> 2) * Cfg::block_b + (kk & 3) * 32;
+                    tc_mma_ss(tmem + Cfg::s_col(buf), tc_desc(qb + at, 16), tc_desc(kb + at, 16), idesc_s, kk > 0);
+                }
+                tc_commit(&s_full[buf]);
+            };
+            auto k_done = [&](int i) {   // after the tile's last S product
+                tc_commit(&empty[k_pos(i) % NU]);
+                if (cq.kt == cq.nkt - 1 || i == count - 1) tc_commit(q_free);
+                cq.next(p);
+            };
+            auto o_product = [&](int i, int t, int buf, bool first) {
+                const uint32_t vb = ring + (v_pos(i) % NU) * Cfg::unit_b;
+                tcf_after();
+#pragma unroll
+                for (int kk = 0; kk < KT / 16; ++kk)
+                    tc_mma_ts(tmem + Cfg::o_col(t), tmem + Cfg::p_col(buf) + kk * 8, tc_desc(vb + kk * 2048, Cfg::block_b),
+                              idesc_o, !(first && kk == 0));
+                tc_commit(&pv_done[t]);
+            };
+            auto v_ready = [&](int i) {
+                const int n = v_pos(i);
+                ok = ok && wait(&full[n % NU], (n / NU) & 1);
+            };
+            if (MT == 1) {
+                k_ready(0);
+                if (ok) s_product(0, 0, 0);
+                if (ok) k_done(0);
+                bool first = true;
+                for (int i = 0; i < count && ok; ++i) {
+                    const bool more = i + 1 < count, crossing = more && first_of(cq, i + 1);
+                    auto next_s = [&]() {
+                        k_ready(i + 1);
+                        if (ok) s_product(i + 1, 0, (i + 1) & 1);
+                        if (ok) k_done(i + 1);
+                    };
+                    // the P and S buffers of tile i - 1 are free (awaited before product i is issued: see the softmax)
+                    if (more && i > 0) ok = ok && wait(&pv_done[0], (i - 1) & 1);
+                    if (more && !crossing) next_s();
+                    v_ready(i);
+                    ok = ok && wait(&p_full[i & 1], (i >> 1) & 1);
+                    if (!ok) break;
+                    o_product(i, 0, i & 1, first);
+                    tc_commit(&empty[v_pos(i) % NU]);
+                    if (crossing) next_s();   // the next segment's rows may still be on their way: not before this product
+                    first = crossing;
+                }
+            } else {
+                auto both = [&](const Cursor& c) { return min(RT, c.r.n * p.group - c.rt * RT) > 128; };
+                bool two = both(cq);
+                k_ready(0);
+                if (ok) {
+                    s_product(0, 0, 0), ++used[0];
+                    if (two) s_product(0, 1, 1), ++used[1];
+                    k_done(0);
+                }
+                bool first = true;
+                for (int i = 0; i < count && ok; ++i) {
+                    const bool more = i + 1 < count, crossing = more && first_of(cq, i + 1);
+                    v_ready(i);
+                    for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
+                        const uint32_t ph = (used[t] - 1) & 1;
+                        ok = wait(&p_full[t], ph);
+                        if (!ok) break;
+                        o_product(i, t, t, first);
+                        if (t == (two ? 1 : 0)) tc_commit(&empty[v_pos(i) % NU]);
+                        if (more && !crossing) {
+                            if (t == 0) k_ready(i + 1);
+                            ok = ok && wait(&pv_done[t], ph);
+                            if (ok) s_product(i + 1, t, t), ++used[t];
+                        }
+                    }
+                    if (more && !crossing && ok) k_done(i + 1);
+                    first = crossing;
+                    if (crossing && ok) {
+                        const bool next_two = both(cq);
+                        k_ready(i + 1);
+                        for (int t = 0; t < (next_two ? 2 : 1) && ok; ++t) {
+                            // the buffer's last product (an earlier segment may have used only the first)
+                            if (used[t] > 0) ok = wait(&pv_done[t], (used[t] - 1) & 1);
+                            if (ok) s_product(i + 1, t, t), ++used[t];
+                        }
+                        if (ok) k_done(i + 1);
+                        two = next_two;
+                    }
+                }
+            }
+            // every product has ended before the tensor memory goes back (also after a wait that ran out)
+            tc_commit(all_done);
+            const uint64_t t0 = globaltimer_ns();
+            while (!mbar_try_wait(all_done, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {}
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------- softmax ----------------------------------
+        const int t = warp >> 2, wq = warp & 3;                       // row tile, lane quarter of tensor memory
+        const int tw = wq % (4 / REP), kq = wq / (4 / REP) * KW;      // 32-row group, first key of this repeat
+        const uint32_t lanes = tmem + ((uint32_t)(wq * 32) << 16);
+        const int row = t * 128 + tw * 32 + lane;                     // row within the row tile
+        const int gtid = tid - t * 128;                               // thread within the row tile's 128
+        if (REP > 1) {   // P is zero outside the repeat's keys, for good
+            uint32_t z[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) z[i] = 0;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) tc_st16(lanes + Cfg::p_col(0) + c * 16, z);
+            tc_wait_st();
+        }
+        float m = -INFINITY, l = 0.0f;
+        int done = 0;   // tiles of this row tile
+        for (int it = 0; it < count; ++it, cur.next(p)) {
+            const int rows = min(RT, cur.r.n * p.group - cur.rt * RT);
+            if (MT == 2 && t == 1 && rows <= 128) continue;
+            const int buf = MT == 1 ? it & 1 : t;
+            const uint32_t s_par = MT == 1 ? (it >> 1) & 1 : done & 1, o_par = MT == 1 ? it & 1 : done & 1;
+            const bool live = t * 128 + tw * 32 < rows;
+            const bool first = it == 0 || cur.kt == 0;
+            if (first) m = -INFINITY, l = 0.0f;
+            const int pos0 = cur.kt * KT, ctx = cur.r.seq - cur.r.n;
+            const bool tail = pos0 + KT > ctx;
+            uint64_t win[KW / 64 + (KW < 64)];
+            if (tail) {
+                const int i = p.group_div.div(min(cur.rt * RT + row, cur.r.n * p.group - 1));
+#pragma unroll
+                for (int w = 0; w < KW / 64 + (KW < 64); ++w)
+                    win[w] = cur.r.seq > 0 ? seen_window(p, cur.r, i, pos0 + kq + 64 * w - ctx) : 0ull;
+            }
+            wait(&s_full[buf], s_par);
+            tcf_after();
+            if (live) {
+                const uint32_t s_at = lanes + Cfg::s_col(buf) + kq, p_at = lanes + Cfg::p_col(buf) + kq / 2;
+                const float f = tail ? 1.0f : p.scale_log2;   // in tail tiles the scores come scaled and masked
+                auto load = [&](int c, float* v) {
+                    tc_ld32(s_at + c * 32, v);
+                    if (tail) {
+                        const uint32_t bits = (uint32_t)(win[c >> 1] >> ((c & 1) * 32));
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = (bits >> j) & 1 ? v[j] * p.scale_log2 : -INFINITY;
+                    }
+                };
+                constexpr bool kHold = KW <= 64;   // scores stay in registers between the two passes
+                float v[kHold ? KW : 32];
+                float mt = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < KW / 32; ++c) {
+                    float* w = v + (kHold ? c * 32 : 0);
+                    load(c, w);
+                    float a[4];
+                    if (f >= 0.0f) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) a[j] = w[j];
+#pragma unroll
+                        for (int j = 4; j < 32; ++j) a[j & 3] = fmaxf(a[j & 3], w[j]);
+                        mt = fmaxf(mt, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * f);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) a[j] = w[j];
+#pragma unroll
+                        for (int j = 4; j < 32; ++j) a[j & 3] = fminf(a[j & 3], w[j]);
+                        mt = fmaxf(mt, fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) * f);
+                    }
+                }
+                if (first) {
+                    m = mt;
+                } else {
+                    const bool grow = mt > m + 8.0f || (m == -INFINITY && mt > m);
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float alpha = grow ? exp2_fast(m - mt) : 1.0f;
+                        if (grow) m = mt;
+                        l *= alpha;
+                        wait(&pv_done[t], o_par ^ 1);   // the previous tile's product
+                        tcf_after();
+#pragma unroll 1
+                        for (int c = 0; c < ksteps; ++c) {
+                            float o[16];
+                            tc_ld16(lanes + Cfg::o_col(t) + c * 16, o);
+                            uint32_t u[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(o[j] * alpha);
+                            tc_st16(lanes + Cfg::o_col(t) + c * 16, u);
+                        }
+                        tc_wait_st();
+                    }
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < KW / 32; ++c) {
+                    float* w = v + (kHold ? c * 32 : 0);
+                    if (!kHold) load(c, w);
+                    uint32_t u[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float a = exp2_fast(fmaf(w[2 * j], f, -base)), b = exp2_fast(fmaf(w[2 * j + 1], f, -base));
+                        sum[j & 3] += a + b;
+                        u[j] = pack2<T>(a, b);
+                    }
+                    tc_st16(p_at + c * 16, u);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tc_wait_st();
+            }
+            bool fix = false;
+            if (tail) {
+                const int n = v_pos(it);
+                wait(&full[n % NU], (n / NU) & 1);
+                fix = *reinterpret_cast<volatile int*>(dirty + n % NU) == n + 1;
+            }
+            // Where this tile's product will be waited for, wait for the one before it now, while the barrier can be in
+            // no later phase: a wait for a parity cannot tell a phase from the one two later.
+            const bool last = cur.kt == cur.nkt - 1 || it == count - 1;
+            if (last || fix) wait(&pv_done[t], o_par ^ 1);
+            tcf_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[buf]);
+            if (fix && live) {
+                // infinities and NaN of new tokens: add p * v to the rows that see them (their products were zeros)
+                wait(&pv_done[t], o_par);
+                tcf_after();
+                for (int c = 0; c < ksteps; ++c) {
+                    float o[16];
+                    tc_ld16(lanes + Cfg::o_col(t) + c * 16, o);
+                    for (int x = max(ctx - pos0, kq); x < min(cur.r.seq - pos0, kq + KW); ++x) {
+                        __syncwarp();
+                        const uint32_t pair = tc_ld1(lanes + Cfg::p_col(buf) + x / 2);
+                        const float2 pp = unpack2<T>(pair);
+                        const float px = x & 1 ? pp.y : pp.x;
+                        const bool see = (win[(x - kq) >> 6] >> ((x - kq) & 63)) & 1;
+                        const int pos = pos0 + x, pg = p.page_div.div(pos);
+                        const int id = p.block_table[(int64_t)cur.b * p.table_stride + pg];
+                        if ((unsigned)id >= (unsigned)p.num_pages) continue;
+                        const T* src = static_cast<const T*>(p.v_cache) + id * p.stride_page +
+                                       (pos - pg * p.page_size) * p.stride_slot + cur.h * p.stride_head + c * 16;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            if (c * 16 + 2 * j >= p.head_dim) break;
+                            const uint32_t raw = reinterpret_cast<const uint32_t*>(src)[j], fin = finite2<T>(raw);
+                            if (raw == fin || !see) continue;
+                            const float2 a = unpack2<T>(raw);
+                            if ((raw ^ fin) & 0xffffu) o[2 * j] += px * a.x;
+                            if ((raw ^ fin) >> 16) o[2 * j + 1] += px * a.y;
+                        }
+                    }
+                    __syncwarp();
+                    uint32_t u[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(o[j]);
+                    tc_st16(lanes + Cfg::o_col(t) + c * 16, u);
+                }
+                tc_wait_st();
+                tcf_before();
+            }
+            ++done;
+            if (!last) continue;
+
+            // ---- end of the segment, or of this CTA's run ----
+            const int bar = 1 + t;
+            wait(&pv_done[t], o_par);
+            tcf_after();
+            float scale_o = 1.0f;   // of this thread's O row
+            float mm = m, ll = l;
+            if (REP > 1) {
+                ml[gtid] = make_float2(m, l);
+                named_bar_sync(bar, 128);
+                mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+                for (int r = 0; r < REP; ++r) mm = fmaxf(mm, ml[r * RT + tw * 32 + lane].x);
+                const float safe = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+                for (int r = 0; r < REP; ++r) {
+                    const float2 v = ml[r * RT + tw * 32 + lane];
+                    ll += v.y * exp2_fast(v.x - safe);
+                }
+                scale_o = exp2_fast(m - safe);
+            }
+            const int64_t seg0 = u0 + it - cur.kt, seg1 = seg0 + cur.nkt;
+            const bool whole = seg0 >= u0 && seg1 <= u0 + count;
+            if (whole) scale_o *= ll == 0.0f ? 0.0f : 1.0f / ll;
+            if (whole && ll == 0.0f) scale_o = 0.0f;
+            const int slot = 2 * blockIdx.x + (seg0 < u0 ? 0 : 1);
+            float* part = p.part_o + (int64_t)slot * RT * DT;
+            auto out_ptr = [&](int r, int d) {
+                const int at = cur.rt * RT + r, i = p.group_div.div(at), g = at - i * p.group;
+                return static_cast<T*>(p.out) + (int64_t)(cur.r.q0 + i) * p.out_stride_token +
+                       (int64_t)(cur.h * p.group + g) * p.out_stride_head + d;
+            };
+            auto put_lse = [&](int r, float top, float sum) {
+                const int at = cur.rt * RT + r, i = p.group_div.div(at), g = at - i * p.group;
+                p.lse[(int64_t)(cur.r.q0 + i) * p.q_heads + cur.h * p.group + g] =
+                    sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+            };
+            auto put2 = [&](int r, int d, float a, float b) {   // two neighbouring columns of row r (of the row tile)
+                if (whole) {
+                    if (d < p.head_dim) *reinterpret_cast<uint32_t*>(out_ptr(r, d)) = pack2<T>(a, b);
+                } else {
+                    *reinterpret_cast<float2*>(part + (int64_t)r * DT + d) = make_float2(a, b);
+                }
+            };
+            float* mine = stage + (t * 4 + wq) * 32 * 17;
+#pragma unroll 1
+            for (int c = 0; c < ksteps; ++c) {
+                if (live) {
+                    float o[16];
+                    tc_ld16(lanes + Cfg::o_col(t) + c * 16, o);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) mine[lane * 17 + j] = scale_o == 0.0f ? 0.0f : o[j] * scale_o;
+                }
+                if (REP == 1) {
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int r = e * 4 + (lane >> 3), j = (lane & 7) * 2;
+                        if (t * 128 + wq * 32 + r < rows) put2(t * 128 + wq * 32 + r, c * 16 + j, mine[r * 17 + j], mine[r * 17 + j + 1]);
+                    }
+                    __syncwarp();
+                } else {
+                    named_bar_sync(bar, 128);
+                    for (int e = gtid; e < rows * 8; e += 128) {
+                        const int r = e >> 3, j = (e & 7) * 2;
+                        float a = 0.0f, b = 0.0f;
+#pragma unroll
+                        for (int rep = 0; rep < REP; ++rep) {
+                            const float* s = stage + (rep * RT + r) * 17 + j;
+                            a += s[0], b += s[1];
+                        }
+                        put2(r, c * 16 + j, a, b);
+                    }
+                    named_bar_sync(bar, 128);
+                }
+            }
+            const bool owner = live && kq == 0 && row < rows;   // one thread per row
+            if (whole) {
+                if (owner && p.lse) put_lse(row, mm, ll);
+                tcf_before();
+                continue;
+            }
+            if (owner) p.part_ml[(int64_t)slot * RT + row] = make_float2(mm, ll);
+            const int fc = (int)(seg0 / run), lc = (int)((seg1 - 1) / run);
+            int* counter = p.counters + 2 * fc + t;
+            __threadfence();
+            named_bar_sync(bar, 128);
+            if (gtid == 0) s_last[t] = atomicAdd(counter, 1) == lc - fc;
+            named_bar_sync(bar, 128);
+            if (*reinterpret_cast<volatile int*>(s_last + t)) {
+                __threadfence();
+                const int r0 = t * 128, r1 = min(rows, r0 + 128);
+                for (int e = gtid; e < (r1 - r0) * (DT / 4); e += 128) {
+                    const int r = r0 + e / (DT / 4), d = (e % (DT / 4)) * 4;
+                    if (d >= p.head_dim) continue;
+                    float top = -INFINITY, sum = 0.0f;
+                    float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+                    for (int c = fc; c <= lc; ++c) {
+                        const int64_t at = (int64_t)(2 * c + (c == fc ? 1 : 0)) * RT + r;
+                        const float2 v = __ldcg(p.part_ml + at);
+                        const float4 po = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * DT + d));
+                        const float big = fmaxf(top, v.x), safe = big == -INFINITY ? 0.0f : big;
+                        const float fa = exp2_fast(top - safe), fb = exp2_fast(v.x - safe);
+                        acc.x = acc.x * fa + po.x * fb;
+                        acc.y = acc.y * fa + po.y * fb;
+                        acc.z = acc.z * fa + po.z * fb;
+                        acc.w = acc.w * fa + po.w * fb;
+                        sum = sum * fa + v.y * fb;
+                        top = big;
+                    }
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    uint32_t* dst = reinterpret_cast<uint32_t*>(out_ptr(r, d));
+                    dst[0] = pack2<T>(acc.x * inv, acc.y * inv);
+                    dst[1] = pack2<T>(acc.z * inv, acc.w * inv);
+                    if (p.lse && d == 0) put_lse(r, top, sum);
+                }
+                if (gtid == 0) *counter = 0;   // ready for the next call
+            }
+            named_bar_sync(bar, 128);
+            tcf_before();
+        }
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+    if (warp == Cfg::w_mma) {
+        tcf_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+template <typename T, int DT, int MT, int REP>
+static cudaError_t launch_tc(const TreeAttnParams& p, cudaStream_t st)
+{
+    using Cfg = TcCfg<DT, MT, REP>;
+    auto kernel = tree_attn_tc_kernel<T, DT, MT, REP>;
+    static bool ready[64] = {};   // the attribute is per device and kernel, and stays
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    if (dev >= 64 || !ready[dev]) {
+        if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem)) != cudaSuccess) return err;
+        if (dev < 64) ready[dev] = true;
+    }
+    kernel<<<num_sms(), Cfg::threads, Cfg::smem, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T, int DT>
+static cudaError_t launch_tc_rows(const TreeAttnParams& p, int rows, cudaStream_t st)
+{
+    if (rows <= 32) return launch_tc<T, DT, 1, 4>(p, st);
+    if (rows <= 64) return launch_tc<T, DT, 1, 2>(p, st);
+    if (rows <= 128) return launch_tc<T, DT, 1, 1>(p, st);
+    return launch_tc<T, DT, 2, 1>(p, st);
+}
+
+cudaError_t launch_tree_attn_tc(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st)
+{
+    if (dtype == 0)
+        return p.head_dim <= 64 ? launch_tc_rows<__half, 64>(p, max_rows, st) : launch_tc_rows<__half, 128>(p, max_rows, st);
+    return p.head_dim <= 64 ? launch_tc_rows<__nv_bfloat16, 64>(p, max_rows, st)
+                            : launch_tc_rows<__nv_bfloat16, 128>(p, max_rows, st);
+}
+
+}  // namespace dsv41

@@ -162,6 +162,20 @@ def _workspace(dev: torch.device, stream: int, head_dim: int) -> torch.Tensor:
     return buf
 
 
+def read_status(device=None) -> int:
+    """Synchronise the current stream; return (then clear) the status of its tree_attention calls: 0 = ok, 1 = a
+    bounded device-side wait ran out (results since the last read are invalid)."""
+    dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    stream, worst = _stream(dev), 0
+    for (index, s, _), buf in list(_ws.items()):
+        if index == dev.index and s == stream:
+            st = C.c_int32()
+            with torch.cuda.device(dev):
+                _lib.check(_lib.load().dsv41_read_status(buf.data_ptr(), stream, C.byref(st)), "read_status")
+            worst = max(worst, st.value)
+    return worst
+
+
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                    seq_lens: torch.Tensor, cu_lens: torch.Tensor, max_new: int, *, tree_mask: torch.Tensor | None = None,
                    scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
@@ -179,7 +193,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % kv_heads:
         raise ValueError(f"q must be [N, q_heads, {dim}] with q_heads a multiple of {kv_heads}")
     N, q_heads = q.shape[0], q.shape[1]
-    q = _heads(q, "q", 2, N, q_heads, dim, k_cache)
+    q = _heads(q, "q", 8, N, q_heads, dim, k_cache)
     if seq_lens.dim() != 1:
         raise ValueError("seq_lens must be int32 [B]")
     B = seq_lens.shape[0]
@@ -197,8 +211,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if out is None:
         out = torch.empty((N, q_heads, dim), dtype=q.dtype, device=dev)
     elif (tuple(out.shape) != (N, q_heads, dim) or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1
-          or out.stride(0) % 2 or out.stride(1) % 2 or out.data_ptr() % 4):
-        raise ValueError("out must be like q, with contiguous heads")
+          or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16):
+        raise ValueError("out must be like q, with contiguous, 16-byte aligned heads")
     lse = torch.empty((N, q_heads), dtype=torch.float32, device=dev) if return_lse else None
     stream = _stream(dev)
     width = block_table.shape[1]

@@ -316,6 +316,7 @@ def attend(s, **kw):
 
 def check(s, what="", scale=None):
     out, lse = attend(s, return_lse=True, scale=scale)
+    assert paged.read_status() == 0, what    # no device wait ran out
     ref, bound, ref_lse = reference(s, scale)
     over = (out.cpu().double() - ref).abs() - bound
     assert not torch.isnan(out).any(), what

@@ -103,8 +103,8 @@ def _attn(ws=FAKE, nbytes=1 << 40, **kw):
 def test_attention_refusals():
     for kw, text in ((dict(dtype=2), b"dtype"), (dict(batch=0), b"batch"), (dict(batch=2049), b"batch"), (dict(q_heads=5), b"q_heads"),
                      (dict(head_dim=264), b"head_dim"), (dict(head_dim=60), b"head_dim"), (dict(page_size=0), b"page_size"),
-                     (dict(max_new=-1), b"max_new"), (dict(q=None), b"NULL"), (dict(ws=None), b"NULL"), (dict(q=FAKE + 2), b"4-byte"),
-                     (dict(k_cache=FAKE + 8), b"16-byte"), (dict(ws=FAKE + 64), b"256-byte"), (dict(q_stride_head=63), b"stride"),
+                     (dict(max_new=-1), b"max_new"), (dict(q=None), b"NULL"), (dict(ws=None), b"NULL"), (dict(q=FAKE + 8), b"16-byte"),
+                     (dict(k_cache=FAKE + 8), b"16-byte"), (dict(ws=FAKE + 64), b"256-byte"), (dict(q_stride_head=68), b"stride"),
                      (dict(stride_slot=132), b"stride"), (dict(scale=float("inf")), b"scale"), (dict(max_keys=-1), b"max_keys"),
                      (dict(tree_mask=FAKE, mask_words=5), b"mask_words"), (dict(num_tokens=1 << 30), b"2^31")):
         _err(_attn(**kw), text)
