@@ -6,8 +6,9 @@
 //                        units in the 128-byte swizzle the tensor cores read; a ring of byte offsets, one per
 //                        key, is looked up one tile ahead
 //   Q loader (1 warp)    the rows of the segment
-//   issuer (1 thread)    S = Q K^T (A and B from shared memory) and O += P V (A from tensor memory, V read as it
-//                        lies, N-major), fp32 accumulators in tensor memory
+//   two issuers (1 thread each)  S = Q K^T (A and B from shared memory) and O += P V (A from tensor memory, V read
+//                        as it lies, N-major), fp32 accumulators in tensor memory. One thread for both left the tensor
+//                        pipe idle between its waits and commits: a unit then took 3400 cycles, of which 2900 in issuing
 //   softmax (4 warps per 128 rows; thread = row)  S out of tensor memory, running maximum and sum, P back into
 //                        tensor memory as 16-bit pairs; at the end of a segment O out
 // The product of tile i + 1 runs while tile i is in the softmax (two S and P buffers for up to 128 rows; two row
@@ -32,8 +33,8 @@ struct TcCfg {
     static constexpr int rt = MT * 128 / REP;                // rows per tile
     static constexpr int kw = kt / REP;                      // keys of a tile per softmax thread
     static constexpr int soft_warps = 4 * MT;
-    static constexpr int w_prod = soft_warps, w_q = w_prod + 4, w_mma = w_q + 1;
-    static constexpr int threads = (w_mma + 1) * 32;
+    static constexpr int w_prod = soft_warps, w_q = w_prod + 4, w_s = w_q + 1, w_o = w_s + 1;
+    static constexpr int threads = (w_o + 1) * 32;
     static constexpr int block_b = 128 * 128;                // 128 rows x 64 columns of 16 bits, swizzled
     static constexpr int blocks = DT / 64;
     static constexpr int unit_b = blocks * block_b;          // a key or value tile
@@ -84,21 +85,63 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-// tensor memory loads with their wait, in one statement: the registers are valid once it has run
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, float* v)
+// N (a multiple of 32) columns of this thread's lane: all loads, one wait. The empty statements after the wait tie
+// the registers to it, so no use of them is scheduled before.
+template <int N>
+__device__ __forceinline__ void tc_ld(uint32_t taddr, float* v)
 {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
+    uint32_t r[N];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int c = 0; c < N; c += 32)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+            "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+            : "=r"(r[c]), "=r"(r[c + 1]), "=r"(r[c + 2]), "=r"(r[c + 3]), "=r"(r[c + 4]), "=r"(r[c + 5]), "=r"(r[c + 6]),
+              "=r"(r[c + 7]), "=r"(r[c + 8]), "=r"(r[c + 9]), "=r"(r[c + 10]), "=r"(r[c + 11]), "=r"(r[c + 12]), "=r"(r[c + 13]),
+              "=r"(r[c + 14]), "=r"(r[c + 15]), "=r"(r[c + 16]), "=r"(r[c + 17]), "=r"(r[c + 18]), "=r"(r[c + 19]),
+              "=r"(r[c + 20]), "=r"(r[c + 21]), "=r"(r[c + 22]), "=r"(r[c + 23]), "=r"(r[c + 24]), "=r"(r[c + 25]),
+              "=r"(r[c + 26]), "=r"(r[c + 27]), "=r"(r[c + 28]), "=r"(r[c + 29]), "=r"(r[c + 30]), "=r"(r[c + 31])
+            : "r"(taddr + c)
+            : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < N; c += 8)
+        asm volatile("" : "+r"(r[c]), "+r"(r[c + 1]), "+r"(r[c + 2]), "+r"(r[c + 3]), "+r"(r[c + 4]), "+r"(r[c + 5]),
+                          "+r"(r[c + 6]), "+r"(r[c + 7]));
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
+}
+// pairs of fp32 in one instruction
+__device__ __forceinline__ uint64_t pair(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c)
+{
+    float r;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 __device__ __forceinline__ void tc_ld16(uint32_t taddr, float* v)
 {
@@ -143,14 +186,14 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
     float2* ml = reinterpret_cast<float2*>(key_off + 4 * KT);
     uint64_t* bars = reinterpret_cast<uint64_t*>(ml + MT * 128);
     uint64_t* full = bars;                 // [NU] a unit's copies have landed (4 producer warps)
-    uint64_t* empty = full + NU;           // [NU] its products are done
+    uint64_t* empty = full + NU;           // [NU] its products are done (keys: told by a softmax thread, values: by the S issuer)
     uint64_t* q_full = empty + NU;         // the segment's rows have landed
     uint64_t* q_free = q_full + 1;         // its last S product is done
     uint64_t* s_full = q_free + 1;         // [2] S buffer computed
     uint64_t* p_full = s_full + 2;         // [2] P buffer written (4 softmax warps)
-    uint64_t* pv_done = p_full + 2;        // [2] O updated (per row tile)
-    uint64_t* all_done = pv_done + 2;
-    int* dirty = reinterpret_cast<int*>(all_done + 1);   // [NU] 1 + ring position of a unit that held infinities or NaN
+    uint64_t* pv_done = p_full + 2;        // [2] the product of a P buffer is done
+    uint64_t* all_done = pv_done + 2;      // [2] per issuer
+    int* dirty = reinterpret_cast<int*>(all_done + 2);   // [NU] 1 + ring position of a unit that held infinities or NaN
     int* s_last = dirty + NU;              // [2]
     volatile int* abort_flag = s_last + 2;
     uint32_t* tmem_slot = const_cast<uint32_t*>(reinterpret_cast<volatile uint32_t*>(abort_flag)) + 1;
@@ -225,11 +268,12 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             mbar_init(&p_full[i], 4);
             mbar_init(&pv_done[i], 1);
         }
-        mbar_init(all_done, 1);
+        mbar_init(&all_done[0], 1);
+        mbar_init(&all_done[1], 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == Cfg::w_mma) {
+    if (warp == Cfg::w_s) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -243,6 +287,8 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
     tcf_after();
     const uint32_t tmem = *tmem_slot;
     const int ksteps = (p.head_dim + 15) / 16;
+    constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
+    constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(128 >> 4) << 24);   // fp32 sums, M = 128
     auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, abort_flag, p.status); };
     // ring position of tile i's keys and values: K0 K1 V0 K2 V1 ... (the order in which they are needed)
     auto k_pos = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
@@ -282,11 +328,18 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             wait(&empty[slot], ((n / NU) & 1) ^ 1);
             if (col_live) {
                 const uint32_t dst = ring + slot * Cfg::unit_b + col_at;
-#pragma unroll 8
-                for (int row = row0; row < KT; row += kRowStep) {
-                    const int64_t off = offs[row];
-                    cp_async16(dst + row * 128 + (((chunk & 7) ^ (row & 7)) << 4),
-                               static_cast<const T*>(cache) + (off < 0 ? 0 : off + chunk * 8), off >= 0);
+                constexpr int kBatch = 8;   // offsets of a batch of rows first: a copy is a barrier to the compiler's loads
+#pragma unroll
+                for (int r = 0; r < KT / kRowStep; r += kBatch) {
+                    int64_t off[kBatch];
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) off[i] = offs[row0 + (r + i) * kRowStep];
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        const int row = row0 + (r + i) * kRowStep;
+                        cp_async16(dst + row * 128 + (((chunk & 7) ^ (row & 7)) << 4),
+                                   static_cast<const T*>(cache) + (off[i] < 0 ? 0 : off[i] + chunk * 8), off[i] >= 0);
+                    }
                 }
             }
             cp_async_commit();
@@ -355,119 +408,70 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             }
             cur.next(p);
         }
-    } else if (warp == Cfg::w_mma) {
-        // ---------------------------------- issuer ----------------------------------
+    } else if (warp == Cfg::w_s) {
+        // ---------------------------------- S issuer ----------------------------------
+        // Buffers: two per row tile for up to 128 rows (tile i uses buffer i % 2), one each for two row tiles. A buffer's
+        // S, then P, are free once its product is done.
         if (lane == 0) {
-            constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
-            constexpr uint32_t kBase = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(128 >> 4) << 24);
-            constexpr uint32_t idesc_s = kBase | ((uint32_t)(KT >> 3) << 17);
-            const uint32_t idesc_o = kBase | (1u << 16) | ((uint32_t)(ksteps * 16 >> 3) << 17);   // V is N-major
+            const uint32_t idesc = kIdesc | ((uint32_t)(KT >> 3) << 17);
             const uint32_t q_at = smem_addr(sq), ring = smem_addr(su);
             bool ok = true;
-            Cursor cq = cur;          // cursor of the S products
-            int seg_q = 0;            // segments whose rows have been awaited
-            int used[2] = {0, 0};     // MT == 2: tiles of each row tile so far (S products issued)
-            auto first_of = [&](const Cursor& c, int i) { return i == 0 || c.kt == 0; };
-            auto k_ready = [&](int i) {
+            int seg = 0, used[2] = {0, 0};   // segments so far; S products per buffer
+            int freed = 0;                   // tiles whose values' slot has been handed back
+            for (int i = 0; i < count && ok; ++i, cur.next(p)) {
+                const int rows = min(RT, cur.r.n * p.group - cur.rt * RT), tiles = MT == 2 && rows > 128 ? 2 : 1;
+                if (i == 0 || cur.kt == 0) ok = wait(q_full, seg++ & 1);
                 const int n = k_pos(i);
-                if (ok && first_of(cq, i)) ok = wait(q_full, seg_q++ & 1);
-                ok = ok && wait(&full[n % NU], (n / NU) & 1);
-            };
-            auto s_product = [&](int i, int t, int buf) {
-                const int n = k_pos(i);
-                const uint32_t kb = ring + (n % NU) * Cfg::unit_b, qb = q_at + t * Cfg::unit_b;
-                tcf_after();
-                for (int kk = 0; kk < ksteps; ++kk) {
-                    const uint32_t at = (kk >> 2) * Cfg::block_b + (kk & 3) * 32;
-                    tc_mma_ss(tmem + Cfg::s_col(buf), tc_desc(qb + at, 16), tc_desc(kb + at, 16), idesc_s, kk > 0);
-                }
-                tc_commit(&s_full[buf]);
-            };
-            auto k_done = [&](int i) {   // after the tile's last S product
-                tc_commit(&empty[k_pos(i) % NU]);
-                if (cq.kt == cq.nkt - 1 || i == count - 1) tc_commit(q_free);
-                cq.next(p);
-            };
-            auto o_product = [&](int i, int t, int buf, bool first) {
-                const uint32_t vb = ring + (v_pos(i) % NU) * Cfg::unit_b;
-                tcf_after();
-#pragma unroll
-                for (int kk = 0; kk < KT / 16; ++kk)
-                    tc_mma_ts(tmem + Cfg::o_col(t), tmem + Cfg::p_col(buf) + kk * 8, tc_desc(vb + kk * 2048, Cfg::block_b),
-                              idesc_o, !(first && kk == 0));
-                tc_commit(&pv_done[t]);
-            };
-            auto v_ready = [&](int i) {
-                const int n = v_pos(i);
-                ok = ok && wait(&full[n % NU], (n / NU) & 1);
-            };
-            if (MT == 1) {
-                k_ready(0);
-                if (ok) s_product(0, 0, 0);
-                if (ok) k_done(0);
-                bool first = true;
-                for (int i = 0; i < count && ok; ++i) {
-                    const bool more = i + 1 < count, crossing = more && first_of(cq, i + 1);
-                    auto next_s = [&]() {
-                        k_ready(i + 1);
-                        if (ok) s_product(i + 1, 0, (i + 1) & 1);
-                        if (ok) k_done(i + 1);
-                    };
-                    // the P and S buffers of tile i - 1 are free (awaited before product i is issued: see the softmax)
-                    if (more && i > 0) ok = ok && wait(&pv_done[0], (i - 1) & 1);
-                    if (more && !crossing) next_s();
-                    v_ready(i);
-                    ok = ok && wait(&p_full[i & 1], (i >> 1) & 1);
+                for (int t = 0; t < tiles && ok; ++t) {
+                    const int buf = MT == 1 ? i & 1 : t;
+                    if (used[buf] > 0) ok = wait(&pv_done[buf], (used[buf] - 1) & 1);
+                    if (t == tiles - 1 && ok) {
+                        if (MT == 2 && tiles == 1 && used[1] > 0) ok = wait(&pv_done[1], (used[1] - 1) & 1);
+                        // products of tiles before i (two row tiles) or i - 1 have ended: their values' slots are free
+                        for (; freed < (MT == 1 ? i - 1 : i); ++freed) mbar_arrive(&empty[v_pos(freed) % NU]);
+                    }
+                    if (t == 0) ok = ok && wait(&full[n % NU], (n / NU) & 1);
                     if (!ok) break;
-                    o_product(i, 0, i & 1, first);
-                    tc_commit(&empty[v_pos(i) % NU]);
-                    if (crossing) next_s();   // the next segment's rows may still be on their way: not before this product
-                    first = crossing;
-                }
-            } else {
-                auto both = [&](const Cursor& c) { return min(RT, c.r.n * p.group - c.rt * RT) > 128; };
-                bool two = both(cq);
-                k_ready(0);
-                if (ok) {
-                    s_product(0, 0, 0), ++used[0];
-                    if (two) s_product(0, 1, 1), ++used[1];
-                    k_done(0);
-                }
-                bool first = true;
-                for (int i = 0; i < count && ok; ++i) {
-                    const bool more = i + 1 < count, crossing = more && first_of(cq, i + 1);
-                    v_ready(i);
-                    for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
-                        const uint32_t ph = (used[t] - 1) & 1;
-                        ok = wait(&p_full[t], ph);
-                        if (!ok) break;
-                        o_product(i, t, t, first);
-                        if (t == (two ? 1 : 0)) tc_commit(&empty[v_pos(i) % NU]);
-                        if (more && !crossing) {
-                            if (t == 0) k_ready(i + 1);
-                            ok = ok && wait(&pv_done[t], ph);
-                            if (ok) s_product(i + 1, t, t), ++used[t];
-                        }
+                    tcf_after();
+                    const uint32_t kb = ring + (n % NU) * Cfg::unit_b, qb = q_at + t * Cfg::unit_b;
+                    for (int kk = 0; kk < ksteps; ++kk) {
+                        const uint32_t at = (kk >> 2) * Cfg::block_b + (kk & 3) * 32;
+                        tc_mma_ss(tmem + Cfg::s_col(buf), tc_desc(qb + at, 16), tc_desc(kb + at, 16), idesc, kk > 0);
                     }
-                    if (more && !crossing && ok) k_done(i + 1);
-                    first = crossing;
-                    if (crossing && ok) {
-                        const bool next_two = both(cq);
-                        k_ready(i + 1);
-                        for (int t = 0; t < (next_two ? 2 : 1) && ok; ++t) {
-                            // the buffer's last product (an earlier segment may have used only the first)
-                            if (used[t] > 0) ok = wait(&pv_done[t], (used[t] - 1) & 1);
-                            if (ok) s_product(i + 1, t, t), ++used[t];
-                        }
-                        if (ok) k_done(i + 1);
-                        two = next_two;
-                    }
+                    tc_commit(&s_full[buf]);
+                    ++used[buf];
                 }
             }
-            // every product has ended before the tensor memory goes back (also after a wait that ran out)
-            tc_commit(all_done);
-            const uint64_t t0 = globaltimer_ns();
-            while (!mbar_try_wait(all_done, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {}
+            tc_commit(&all_done[0]);
+        }
+        __syncwarp();
+    } else if (warp == Cfg::w_o) {
+        // ---------------------------------- O issuer ----------------------------------
+        if (lane == 0) {
+            const uint32_t idesc = kIdesc | (1u << 16) | ((uint32_t)(ksteps * 16 >> 3) << 17);   // V is N-major
+            const uint32_t ring = smem_addr(su);
+            bool ok = true;
+            int used[2] = {0, 0};
+            for (int i = 0; i < count && ok; ++i, cur.next(p)) {
+                const int rows = min(RT, cur.r.n * p.group - cur.rt * RT), tiles = MT == 2 && rows > 128 ? 2 : 1;
+                const bool first = i == 0 || cur.kt == 0;
+                const int n = v_pos(i);
+                ok = wait(&full[n % NU], (n / NU) & 1);
+                for (int t = 0; t < tiles && ok; ++t) {
+                    const int buf = MT == 1 ? i & 1 : t;
+                    ok = wait(&p_full[buf], used[buf] & 1);
+                    if (!ok) break;
+                    tcf_after();
+                    const uint32_t vb = ring + (n % NU) * Cfg::unit_b;
+#pragma unroll
+                    for (int kk = 0; kk < KT / 16; ++kk)
+                        tc_mma_ts(tmem + Cfg::o_col(t), tmem + Cfg::p_col(buf) + kk * 8, tc_desc(vb + kk * 2048, Cfg::block_b),
+                                  idesc, !(first && kk == 0));
+                    tc_commit(&pv_done[buf]);
+                    ++used[buf];
+                }
+            }
+            tc_commit(&all_done[1]);
         }
         __syncwarp();
     } else {
@@ -491,7 +495,8 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             const int rows = min(RT, cur.r.n * p.group - cur.rt * RT);
             if (MT == 2 && t == 1 && rows <= 128) continue;
             const int buf = MT == 1 ? it & 1 : t;
-            const uint32_t s_par = MT == 1 ? (it >> 1) & 1 : done & 1, o_par = MT == 1 ? it & 1 : done & 1;
+            const uint32_t par = (MT == 1 ? it >> 1 : done) & 1;   // of every barrier of this buffer
+            const bool last = cur.kt == cur.nkt - 1 || it == count - 1;
             const bool live = t * 128 + tw * 32 < rows;
             const bool first = it == 0 || cur.kt == 0;
             if (first) m = -INFINITY, l = 0.0f;
@@ -504,38 +509,49 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                 for (int w = 0; w < KW / 64 + (KW < 64); ++w)
                     win[w] = cur.r.seq > 0 ? seen_window(p, cur.r, i, pos0 + kq + 64 * w - ctx) : 0ull;
             }
-            wait(&s_full[buf], s_par);
+            wait(&s_full[buf], par);
             tcf_after();
+            if (wq == 0 && lane == 0 && (MT == 1 || t == 1 || rows <= 128)) {   // the tile's S products have all ended
+                mbar_arrive(&empty[k_pos(it) % NU]);
+                if (last) mbar_arrive(q_free);
+            }
             if (live) {
                 const uint32_t s_at = lanes + Cfg::s_col(buf) + kq, p_at = lanes + Cfg::p_col(buf) + kq / 2;
                 const float f = tail ? 1.0f : p.scale_log2;   // in tail tiles the scores come scaled and masked
-                auto load = [&](int c, float* v) {
-                    tc_ld32(s_at + c * 32, v);
+                constexpr int HB = KW < 64 ? KW : 64;   // scores held in registers at a time
+                auto load = [&](int c, float* v) {      // HB scores from the c-th such run on
+                    tc_ld<HB>(s_at + c * HB, v);
                     if (tail) {
-                        const uint32_t bits = (uint32_t)(win[c >> 1] >> ((c & 1) * 32));
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = (bits >> j) & 1 ? v[j] * p.scale_log2 : -INFINITY;
+                        for (int j = 0; j < HB; ++j) {
+                            const int x = c * HB + j;
+                            v[j] = (uint32_t)(win[x >> 6] >> ((x & 32) ? 32 : 0)) >> (x & 31) & 1 ? v[j] * p.scale_log2 : -INFINITY;
+                        }
                     }
                 };
-                constexpr bool kHold = KW <= 64;   // scores stay in registers between the two passes
-                float v[kHold ? KW : 32];
+                float v[HB];
                 float mt = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < KW / 32; ++c) {
-                    float* w = v + (kHold ? c * 32 : 0);
-                    load(c, w);
+                for (int c = 0; c < KW / HB; ++c) {
+                    load(c, v);
                     float a[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a[j] = v[j];
                     if (f >= 0.0f) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) a[j] = w[j];
+                        for (int j = 4; j + 8 <= HB; j += 8)
 #pragma unroll
-                        for (int j = 4; j < 32; ++j) a[j & 3] = fmaxf(a[j & 3], w[j]);
+                            for (int q = 0; q < 4; ++q) a[q] = max3(a[q], v[j + 2 * q], v[j + 2 * q + 1]);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) a[q] = fmaxf(a[q], v[HB - 4 + q]);
                         mt = fmaxf(mt, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * f);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) a[j] = w[j];
+                        for (int j = 4; j + 8 <= HB; j += 8)
 #pragma unroll
-                        for (int j = 4; j < 32; ++j) a[j & 3] = fminf(a[j & 3], w[j]);
+                            for (int q = 0; q < 4; ++q) a[q] = min3(a[q], v[j + 2 * q], v[j + 2 * q + 1]);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) a[q] = fminf(a[q], v[HB - 4 + q]);
                         mt = fmaxf(mt, fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) * f);
                     }
                 }
@@ -547,7 +563,8 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                         const float alpha = grow ? exp2_fast(m - mt) : 1.0f;
                         if (grow) m = mt;
                         l *= alpha;
-                        wait(&pv_done[t], o_par ^ 1);   // the previous tile's product
+                        // the previous tile's product: the other buffer's, or this one's last
+                        if (MT == 1) wait(&pv_done[buf ^ 1], ((it - 1) >> 1) & 1);
                         tcf_after();
 #pragma unroll 1
                         for (int c = 0; c < ksteps; ++c) {
@@ -562,21 +579,30 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                     }
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t f2 = pair(f, f), base2 = pair(-base, -base);
+                uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                for (int c = 0; c < KW / 32; ++c) {
-                    float* w = v + (kHold ? c * 32 : 0);
-                    if (!kHold) load(c, w);
-                    uint32_t u[16];
+                for (int c = 0; c < KW / HB; ++c) {
+                    if (HB < KW) load(c, v);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float a = exp2_fast(fmaf(w[2 * j], f, -base)), b = exp2_fast(fmaf(w[2 * j + 1], f, -base));
-                        sum[j & 3] += a + b;
-                        u[j] = pack2<T>(a, b);
+                    for (int c16 = 0; c16 < HB / 32; ++c16) {
+                        uint32_t u[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int x = c16 * 32 + 2 * j;
+                            float a, b;
+                            unpair(fma_pair(pair(v[x], v[x + 1]), f2, base2), a, b);
+                            a = exp2_fast(a), b = exp2_fast(b);
+                            sum[j & 1] = add_pair(sum[j & 1], pair(a, b));
+                            u[j] = pack2<T>(a, b);
+                        }
+                        tc_st16(p_at + c * (HB / 2) + c16 * 16, u);
                     }
-                    tc_st16(p_at + c * 16, u);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                float s0, s1, s2, s3;
+                unpair(sum[0], s0, s1);
+                unpair(sum[1], s2, s3);
+                l += (s0 + s1) + (s2 + s3);
                 tc_wait_st();
             }
             bool fix = false;
@@ -585,16 +611,12 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                 wait(&full[n % NU], (n / NU) & 1);
                 fix = *reinterpret_cast<volatile int*>(dirty + n % NU) == n + 1;
             }
-            // Where this tile's product will be waited for, wait for the one before it now, while the barrier can be in
-            // no later phase: a wait for a parity cannot tell a phase from the one two later.
-            const bool last = cur.kt == cur.nkt - 1 || it == count - 1;
-            if (last || fix) wait(&pv_done[t], o_par ^ 1);
             tcf_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[buf]);
             if (fix && live) {
                 // infinities and NaN of new tokens: add p * v to the rows that see them (their products were zeros)
-                wait(&pv_done[t], o_par);
+                wait(&pv_done[buf], par);
                 tcf_after();
                 for (int c = 0; c < ksteps; ++c) {
                     float o[16];
@@ -634,7 +656,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
 
             // ---- end of the segment, or of this CTA's run ----
             const int bar = 1 + t;
-            wait(&pv_done[t], o_par);
+            wait(&pv_done[buf], par);
             tcf_after();
             float scale_o = 1.0f;   // of this thread's O row
             float mm = m, ll = l;
@@ -756,7 +778,11 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
     }
     cp_async_wait<0>();
     __syncthreads();
-    if (warp == Cfg::w_mma) {
+    if (warp == Cfg::w_s) {
+        // every product has ended before the tensor memory goes back (also after a wait that ran out)
+        const uint64_t t0 = globaltimer_ns();
+        for (int i = 0; i < 2; ++i)
+            while (!mbar_try_wait(&all_done[i], 0) && globaltimer_ns() - t0 < kWaitLimitNs) {}
         tcf_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
