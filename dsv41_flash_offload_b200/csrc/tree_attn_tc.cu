@@ -9,8 +9,10 @@
 //   two issuers (1 thread each)  S = Q K^T (A and B from shared memory) and O += P V (A from tensor memory, V read
 //                        as it lies, N-major), fp32 accumulators in tensor memory. One thread for both left the tensor
 //                        pipe idle between its waits and commits: a unit then took 3400 cycles, of which 2900 in issuing
-//   softmax (4 warps per 128 rows; thread = row)  S out of tensor memory, running maximum and sum, P back into
-//                        tensor memory as 16-bit pairs; at the end of a segment O out
+//   softmax (4 or 8 warps per 128 rows; one or two threads per row, who share its keys)  S out of tensor memory,
+//                        running maximum and sum, P back into tensor memory as 16-bit pairs; at the end of a segment
+//                        O out. A single warp per sub-partition spends most of its time on latencies: with 4 warps a
+//                        tile of 128 rows took 4700 cycles for 128 exponentials a thread.
 // The product of tile i + 1 runs while tile i is in the softmax (two S and P buffers for up to 128 rows; two row
 // tiles take turns for up to 256).
 //
@@ -31,19 +33,24 @@ struct TcCfg {
     static_assert(MT == 1 || REP == 1, "repeats are for a single tile of 128 rows");
     static constexpr int kt = 128;                           // keys per tile
     static constexpr int rt = MT * 128 / REP;                // rows per tile
-    static constexpr int kw = kt / REP;                      // keys of a tile per softmax thread
-    static constexpr int soft_warps = 4 * MT;
+    static constexpr int split = REP == 4 ? 1 : 2;           // softmax threads that share a row's keys
+    static constexpr int kw = kt / REP / split;              // keys of a tile per softmax thread
+    static constexpr int hold = MT == 2 ? 32 : kw;           // scores a thread holds at a time (registers)
+    static constexpr int group = 128 * split;                // softmax threads per 128 rows
+    static constexpr int soft_warps = 4 * split * MT;
     static constexpr int w_prod = soft_warps, w_q = w_prod + 4, w_s = w_q + 1, w_o = w_s + 1;
     static constexpr int threads = (w_o + 1) * 32;
     static constexpr int block_b = 128 * 128;                // 128 rows x 64 columns of 16 bits, swizzled
     static constexpr int blocks = DT / 64;
     static constexpr int unit_b = blocks * block_b;          // a key or value tile
     static constexpr int q_b = MT * unit_b;
-    static constexpr int stage_b = soft_warps * 32 * 17 * 4; // O on its way out, 16 columns at a time
+    static constexpr int sc = MT == 2 ? 8 : 16;              // columns of O on their way out at a time
+    static constexpr int stage_b = soft_warps * 32 * (sc + 1) * 4;
     static constexpr int off_b = 4 * kt * 8;                 // byte offsets of the keys of four tiles
-    static constexpr int ml_b = MT * 128 * 8;
+    static constexpr int ml_b = MT * 2 * 128 * 8;
+    static constexpr int mx_b = MT * 4 * 128 * 4;            // tile maxima of the threads that share a row
     static constexpr int bars_b = 1024;
-    static constexpr int fixed_b = 1024 + q_b + stage_b + off_b + ml_b + bars_b;
+    static constexpr int fixed_b = 1024 + q_b + stage_b + off_b + ml_b + mx_b + bars_b;
     static constexpr int units_fit = (232448 - fixed_b) / unit_b;
     static constexpr int units = units_fit < 10 ? units_fit : 10;
     static constexpr int lag = units - 2;                    // units a producer has in flight when it issues the next
@@ -51,7 +58,12 @@ struct TcCfg {
     static_assert(units >= 4, "ring too short");
     // tensor memory columns
     __host__ __device__ static constexpr int s_col(int b) { return b * 128; }
-    __host__ __device__ static constexpr int p_col(int b) { return MT == 1 ? 256 + b * 64 : b * 128; }
+    // P of key x of buffer b (two keys a column). Two row tiles leave no room of its own: P then lies over S, each
+    // softmax thread's over its own keys', which it alone reads.
+    __host__ __device__ static constexpr int p_col(int b, int x)
+    {
+        return MT == 1 ? 256 + b * 64 + x / 2 : b * 128 + (x / kw) * kw + (x % kw) / 2;
+    }
     __host__ __device__ static constexpr int o_col(int t) { return MT == 1 ? 384 : 256 + t * 128; }
 };
 
@@ -64,25 +76,22 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-// swizzled-128B operand, rows of 128 bytes, 8-row atoms of 1024 bytes. K-major: lbo unused. N-major: lbo is the
-// distance of the 64-column blocks.
-__device__ __forceinline__ uint64_t tc_desc(uint32_t saddr, uint32_t lbo)
-{
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+// Operand descriptors: swizzled-128B, rows of 128 bytes, 8-row atoms of 1024 bytes. The low word holds the address
+// and, for N-major operands, the distance of the 64-column blocks (K-major: unused); both in units of 16 bytes.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t tc_desc_low(uint32_t saddr, uint32_t block) { return ((saddr & 0x3FFFFu) >> 4) | ((block >> 4) << 16); }
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc)
 {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh)
         : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc)
 {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh)
         : "memory");
 }
 // N (a multiple of 32) columns of this thread's lane: all loads, one wait. The empty statements after the wait tie
@@ -184,13 +193,14 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
     float* stage = reinterpret_cast<float*>(su + NU * Cfg::unit_b);
     int64_t* key_off = reinterpret_cast<int64_t*>(reinterpret_cast<unsigned char*>(stage) + Cfg::stage_b);
     float2* ml = reinterpret_cast<float2*>(key_off + 4 * KT);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(ml + MT * 128);
+    float* mx = reinterpret_cast<float*>(ml + MT * 2 * 128);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(mx + MT * 4 * 128);
     uint64_t* full = bars;                 // [NU] a unit's copies have landed (4 producer warps)
     uint64_t* empty = full + NU;           // [NU] its products are done (keys: told by a softmax thread, values: by the S issuer)
     uint64_t* q_full = empty + NU;         // the segment's rows have landed
     uint64_t* q_free = q_full + 1;         // its last S product is done
     uint64_t* s_full = q_free + 1;         // [2] S buffer computed
-    uint64_t* p_full = s_full + 2;         // [2] P buffer written (4 softmax warps)
+    uint64_t* p_full = s_full + 2;         // [2] P buffer written (every softmax warp of the row tile)
     uint64_t* pv_done = p_full + 2;        // [2] the product of a P buffer is done
     uint64_t* all_done = pv_done + 2;      // [2] per issuer
     int* dirty = reinterpret_cast<int*>(all_done + 2);   // [NU] 1 + ring position of a unit that held infinities or NaN
@@ -265,7 +275,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
         mbar_init(q_free, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[i], 4 * Cfg::split);
             mbar_init(&pv_done[i], 1);
         }
         mbar_init(&all_done[0], 1);
@@ -290,6 +300,11 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
     constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(128 >> 4) << 24);   // fp32 sums, M = 128
     auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, abort_flag, p.status); };
+    // by a whole warp, which goes on converged (the tensor memory instructions need that)
+    auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
+        wait(bar, parity);
+        __syncwarp();
+    };
     // ring position of tile i's keys and values: K0 K1 V0 K2 V1 ... (the order in which they are needed)
     auto k_pos = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
     auto v_pos = [&](int i) { return i == count - 1 ? 2 * i + 1 : 2 * i + 2; };
@@ -322,10 +337,11 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             fence_proxy_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[slot]);
+            __syncwarp();
         };
         auto issue = [&](int n, const void* cache, const int64_t* offs, bool check) {
             const int slot = n % NU;
-            wait(&empty[slot], ((n / NU) & 1) ^ 1);
+            wait_warp(&empty[slot], ((n / NU) & 1) ^ 1);
             if (col_live) {
                 const uint32_t dst = ring + slot * Cfg::unit_b + col_at;
                 constexpr int kBatch = 8;   // offsets of a batch of rows first: a copy is a barrier to the compiler's loads
@@ -384,7 +400,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
         int seg = 0;
         for (int it = 0; it < count; ++it) {
             if (it == 0 || cur.kt == 0) {
-                wait(q_free, (seg & 1) ^ 1);
+                wait_warp(q_free, (seg & 1) ^ 1);
                 const int rows = min(RT, cur.r.n * p.group - cur.rt * RT);
                 if (chunk * 8 < p.head_dim) {
 #pragma unroll 4
@@ -433,10 +449,13 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                     if (t == 0) ok = ok && wait(&full[n % NU], (n / NU) & 1);
                     if (!ok) break;
                     tcf_after();
-                    const uint32_t kb = ring + (n % NU) * Cfg::unit_b, qb = q_at + t * Cfg::unit_b;
-                    for (int kk = 0; kk < ksteps; ++kk) {
-                        const uint32_t at = (kk >> 2) * Cfg::block_b + (kk & 3) * 32;
-                        tc_mma_ss(tmem + Cfg::s_col(buf), tc_desc(qb + at, 16), tc_desc(kb + at, 16), idesc, kk > 0);
+                    const uint32_t kd = tc_desc_low(ring + (n % NU) * Cfg::unit_b, 16), qd = tc_desc_low(q_at + t * Cfg::unit_b, 16);
+                    const uint32_t dst = tmem + Cfg::s_col(buf);
+#pragma unroll
+                    for (int kk = 0; kk < DT / 16; ++kk) {
+                        constexpr int kStep = 32 >> 4, kBlock = Cfg::block_b >> 4;
+                        const int at = (kk >> 2) * kBlock + (kk & 3) * kStep;
+                        if (kk < ksteps) tc_mma_ss(dst, qd + at, kd + at, idesc, kk > 0);
                     }
                     tc_commit(&s_full[buf]);
                     ++used[buf];
@@ -462,11 +481,11 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                     ok = wait(&p_full[buf], used[buf] & 1);
                     if (!ok) break;
                     tcf_after();
-                    const uint32_t vb = ring + (n % NU) * Cfg::unit_b;
+                    const uint32_t vd = tc_desc_low(ring + (n % NU) * Cfg::unit_b, Cfg::block_b);
+                    const uint32_t dst = tmem + Cfg::o_col(t);
 #pragma unroll
                     for (int kk = 0; kk < KT / 16; ++kk)
-                        tc_mma_ts(tmem + Cfg::o_col(t), tmem + Cfg::p_col(buf) + kk * 8, tc_desc(vb + kk * 2048, Cfg::block_b),
-                                  idesc, !(first && kk == 0));
+                        tc_mma_ts(dst, tmem + Cfg::p_col(buf, kk * 16), vd + kk * (2048 >> 4), idesc, !(first && kk == 0));
                     tc_commit(&pv_done[buf]);
                     ++used[buf];
                 }
@@ -476,17 +495,21 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
         __syncwarp();
     } else {
         // ---------------------------------- softmax ----------------------------------
-        const int t = warp >> 2, wq = warp & 3;                       // row tile, lane quarter of tensor memory
-        const int tw = wq % (4 / REP), kq = wq / (4 / REP) * KW;      // 32-row group, first key of this repeat
+        constexpr int SPLIT = Cfg::split, HB = Cfg::hold, GT = Cfg::group, SC = Cfg::sc;
+        const int t = warp / (4 * SPLIT), half = (warp >> 2) % SPLIT, wq = warp & 3;   // row tile, share, lane quarter
+        const int rep = wq / (4 / REP), tw = wq % (4 / REP);          // repeat, 32-row group
+        const int kq = rep * (KT / REP) + half * KW;                  // first key of this thread's share of a tile
         const uint32_t lanes = tmem + ((uint32_t)(wq * 32) << 16);
         const int row = t * 128 + tw * 32 + lane;                     // row within the row tile
-        const int gtid = tid - t * 128;                               // thread within the row tile's 128
-        if (REP > 1) {   // P is zero outside the repeat's keys, for good
+        const int gtid = tid - t * GT;                                // thread within the row tile's group
+        const int bar_group = 1 + t, bar_pair = 4 + t * 4 + wq, bar_half = 12 + half;   // 3: the producers
+        if (REP > 1 && half == 0) {   // P is zero outside the repeat's keys, for good
             uint32_t z[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) z[i] = 0;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) tc_st16(lanes + Cfg::p_col(0) + c * 16, z);
+            for (int c = 0; c < 8; ++c)
+                if ((c & 3) / (4 / REP) != rep) tc_st16(lanes + Cfg::p_col(c >> 2, (c & 3) * 32), z);
             tc_wait_st();
         }
         float m = -INFINITY, l = 0.0f;
@@ -502,30 +525,27 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             if (first) m = -INFINITY, l = 0.0f;
             const int pos0 = cur.kt * KT, ctx = cur.r.seq - cur.r.n;
             const bool tail = pos0 + KT > ctx;
-            uint64_t win[KW / 64 + (KW < 64)];
-            if (tail) {
-                const int i = p.group_div.div(min(cur.rt * RT + row, cur.r.n * p.group - 1));
-#pragma unroll
-                for (int w = 0; w < KW / 64 + (KW < 64); ++w)
-                    win[w] = cur.r.seq > 0 ? seen_window(p, cur.r, i, pos0 + kq + 64 * w - ctx) : 0ull;
-            }
-            wait(&s_full[buf], par);
+            static_assert(KW <= 64, "one mask window per thread");
+            uint64_t win = 0;
+            const int tok = p.group_div.div(min(cur.rt * RT + row, cur.r.n * p.group - 1));   // this row's new token
+            if (tail && cur.r.seq > 0) win = seen_window(p, cur.r, tok, pos0 + kq - ctx);
+            wait_warp(&s_full[buf], par);
             tcf_after();
-            if (wq == 0 && lane == 0 && (MT == 1 || t == 1 || rows <= 128)) {   // the tile's S products have all ended
+            if (wq == 0 && half == 0 && lane == 0 && (MT == 1 || t == 1 || rows <= 128)) {   // the tile's S products have all ended
                 mbar_arrive(&empty[k_pos(it) % NU]);
                 if (last) mbar_arrive(q_free);
             }
+            __syncwarp();
             if (live) {
-                const uint32_t s_at = lanes + Cfg::s_col(buf) + kq, p_at = lanes + Cfg::p_col(buf) + kq / 2;
+                const uint32_t s_at = lanes + Cfg::s_col(buf) + kq, p_at = lanes + Cfg::p_col(buf, kq);
                 const float f = tail ? 1.0f : p.scale_log2;   // in tail tiles the scores come scaled and masked
-                constexpr int HB = KW < 64 ? KW : 64;   // scores held in registers at a time
                 auto load = [&](int c, float* v) {      // HB scores from the c-th such run on
                     tc_ld<HB>(s_at + c * HB, v);
                     if (tail) {
 #pragma unroll
                         for (int j = 0; j < HB; ++j) {
                             const int x = c * HB + j;
-                            v[j] = (uint32_t)(win[x >> 6] >> ((x & 32) ? 32 : 0)) >> (x & 31) & 1 ? v[j] * p.scale_log2 : -INFINITY;
+                            v[j] = ((uint32_t)(win >> (x & 32)) >> (x & 31)) & 1 ? v[j] * p.scale_log2 : -INFINITY;
                         }
                     }
                 };
@@ -555,6 +575,12 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                         mt = fmaxf(mt, fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) * f);
                     }
                 }
+                if (SPLIT == 2) {   // the row's other thread
+                    float* at = mx + ((t * 2 + (done & 1)) * 2 + half) * 128 + wq * 32 + lane;
+                    *at = mt;
+                    named_bar_sync(bar_pair, 64);
+                    mt = fmaxf(mt, mx[((t * 2 + (done & 1)) * 2 + (half ^ 1)) * 128 + wq * 32 + lane]);
+                }
                 if (first) {
                     m = mt;
                 } else {
@@ -564,10 +590,10 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                         if (grow) m = mt;
                         l *= alpha;
                         // the previous tile's product: the other buffer's, or this one's last
-                        if (MT == 1) wait(&pv_done[buf ^ 1], ((it - 1) >> 1) & 1);
+                        if (MT == 1) wait_warp(&pv_done[buf ^ 1], ((it - 1) >> 1) & 1);
                         tcf_after();
 #pragma unroll 1
-                        for (int c = 0; c < ksteps; ++c) {
+                        for (int c = half; c < ksteps; c += SPLIT) {
                             float o[16];
                             tc_ld16(lanes + Cfg::o_col(t) + c * 16, o);
                             uint32_t u[16];
@@ -608,45 +634,70 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             bool fix = false;
             if (tail) {
                 const int n = v_pos(it);
-                wait(&full[n % NU], (n / NU) & 1);
-                fix = *reinterpret_cast<volatile int*>(dirty + n % NU) == n + 1;
+                wait_warp(&full[n % NU], (n / NU) & 1);
+                fix = live && *reinterpret_cast<volatile int*>(dirty + n % NU) == n + 1;
+            }
+            // Infinities and NaN of new tokens entered the product as zeros. A row that sees such a value takes
+            // p * v, which is +inf, -inf or NaN (also where p is 0): two bits per row and column, +inf and -inf, both
+            // for NaN, found now, while P is there, and added to O after the product.
+            constexpr int kFix = DT / 16 / SPLIT;
+            uint32_t flags[kFix];   // of this thread's 16-column chunks: low half +inf, high half -inf
+#pragma unroll
+            for (int k = 0; k < kFix; ++k) flags[k] = 0;
+            if (fix) {
+                if (SPLIT == 2) {   // this thread's columns need P of all the row's keys
+                    tcf_before();
+                    named_bar_sync(bar_pair, 64);
+                    tcf_after();
+                }
+                const int x0 = rep * (KT / REP);
+                for (int x = max(ctx - pos0, x0); x < min(cur.r.seq - pos0, x0 + KT / REP); ++x) {
+                    const int pos = pos0 + x, pg = p.page_div.div(pos);
+                    const int id = p.block_table[(int64_t)cur.b * p.table_stride + pg];
+                    if ((unsigned)id >= (unsigned)p.num_pages) continue;
+                    const T* src = static_cast<const T*>(p.v_cache) + id * p.stride_page + (pos - pg * p.page_size) * p.stride_slot +
+                                   cur.h * p.stride_head;
+                    __syncwarp();
+                    const float2 pp = unpack2<T>(tc_ld1(lanes + Cfg::p_col(buf, x)));
+                    const bool zero = (x & 1 ? pp.y : pp.x) == 0.0f;
+                    if (!(seen_window(p, cur.r, tok, pos - ctx) & 1)) continue;
+#pragma unroll
+                    for (int k = 0; k < kFix; ++k) {
+                        const int c = k * SPLIT + half;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            if (c * 16 + 2 * j >= p.head_dim) break;
+                            const uint32_t raw = reinterpret_cast<const uint32_t*>(src)[c * 8 + j];
+                            if (raw == finite2<T>(raw)) continue;
+                            const float2 v = unpack2<T>(raw);
+                            if (!(fabsf(v.x) < INFINITY)) flags[k] |= (v.x < 0 && !zero ? 0u : 1u << (2 * j)) | (v.x > 0 && !zero ? 0u : 0x10000u << (2 * j));
+                            if (!(fabsf(v.y) < INFINITY)) flags[k] |= (v.y < 0 && !zero ? 0u : 2u << (2 * j)) | (v.y > 0 && !zero ? 0u : 0x20000u << (2 * j));
+                        }
+                    }
+                }
+                __syncwarp();
             }
             tcf_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[buf]);
-            if (fix && live) {
-                // infinities and NaN of new tokens: add p * v to the rows that see them (their products were zeros)
-                wait(&pv_done[buf], par);
+            __syncwarp();
+            if (fix) {
+                wait_warp(&pv_done[buf], par);
                 tcf_after();
-                for (int c = 0; c < ksteps; ++c) {
-                    float o[16];
-                    tc_ld16(lanes + Cfg::o_col(t) + c * 16, o);
-                    for (int x = max(ctx - pos0, kq); x < min(cur.r.seq - pos0, kq + KW); ++x) {
-                        __syncwarp();
-                        const uint32_t pair = tc_ld1(lanes + Cfg::p_col(buf) + x / 2);
-                        const float2 pp = unpack2<T>(pair);
-                        const float px = x & 1 ? pp.y : pp.x;
-                        const bool see = (win[(x - kq) >> 6] >> ((x - kq) & 63)) & 1;
-                        const int pos = pos0 + x, pg = p.page_div.div(pos);
-                        const int id = p.block_table[(int64_t)cur.b * p.table_stride + pg];
-                        if ((unsigned)id >= (unsigned)p.num_pages) continue;
-                        const T* src = static_cast<const T*>(p.v_cache) + id * p.stride_page +
-                                       (pos - pg * p.page_size) * p.stride_slot + cur.h * p.stride_head + c * 16;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (c * 16 + 2 * j >= p.head_dim) break;
-                            const uint32_t raw = reinterpret_cast<const uint32_t*>(src)[j], fin = finite2<T>(raw);
-                            if (raw == fin || !see) continue;
-                            const float2 a = unpack2<T>(raw);
-                            if ((raw ^ fin) & 0xffffu) o[2 * j] += px * a.x;
-                            if ((raw ^ fin) >> 16) o[2 * j + 1] += px * a.y;
-                        }
-                    }
-                    __syncwarp();
+                for (int k = 0; k < kFix; ++k) {
+                    if (!__any_sync(0xffffffffu, flags[k] != 0)) continue;
+                    const uint32_t at = lanes + Cfg::o_col(t) + (k * SPLIT + half) * 16;
+                    float o[16];
+                    tc_ld16(at, o);
                     uint32_t u[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(o[j]);
-                    tc_st16(lanes + Cfg::o_col(t) + c * 16, u);
+                    for (int j = 0; j < 16; ++j) {
+                        if ((flags[k] >> j) & 1) o[j] += INFINITY;
+                        if ((flags[k] >> (16 + j)) & 1) o[j] -= INFINITY;
+                        u[j] = __float_as_uint(o[j]);
+                    }
+                    tc_st16(at, u);
                 }
                 tc_wait_st();
                 tcf_before();
@@ -655,29 +706,29 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             if (!last) continue;
 
             // ---- end of the segment, or of this CTA's run ----
-            const int bar = 1 + t;
-            wait(&pv_done[buf], par);
+            wait_warp(&pv_done[buf], par);
             tcf_after();
-            float scale_o = 1.0f;   // of this thread's O row
-            float mm = m, ll = l;
-            if (REP > 1) {
-                ml[gtid] = make_float2(m, l);
-                named_bar_sync(bar, 128);
+            float mm = m, ll = l, scale_o = 1.0f;   // of the row; scale_o: of this thread's O row
+            if (REP > 1 || SPLIT == 2) {
+                float2* mine = ml + t * 256;        // [share][repeat and row]
+                mine[half * 128 + wq * 32 + lane] = make_float2(m, l);
+                named_bar_sync(bar_group, GT);
                 mm = -INFINITY, ll = 0.0f;
+                const int r0 = REP == 1 ? wq * 32 + lane : tw * 32 + lane;
 #pragma unroll
-                for (int r = 0; r < REP; ++r) mm = fmaxf(mm, ml[r * RT + tw * 32 + lane].x);
+                for (int r = 0; r < REP; ++r) mm = fmaxf(mm, mine[r * RT * (REP > 1) + r0].x);
                 const float safe = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
                 for (int r = 0; r < REP; ++r) {
-                    const float2 v = ml[r * RT + tw * 32 + lane];
+                    float2 v = mine[r * RT * (REP > 1) + r0];
+                    if (SPLIT == 2) v.y += mine[128 + r * RT * (REP > 1) + r0].y;
                     ll += v.y * exp2_fast(v.x - safe);
                 }
                 scale_o = exp2_fast(m - safe);
             }
             const int64_t seg0 = u0 + it - cur.kt, seg1 = seg0 + cur.nkt;
             const bool whole = seg0 >= u0 && seg1 <= u0 + count;
-            if (whole) scale_o *= ll == 0.0f ? 0.0f : 1.0f / ll;
-            if (whole && ll == 0.0f) scale_o = 0.0f;
+            if (whole) scale_o = ll == 0.0f ? 0.0f : scale_o / ll;
             const int slot = 2 * blockIdx.x + (seg0 < u0 ? 0 : 1);
             float* part = p.part_o + (int64_t)slot * RT * DT;
             auto out_ptr = [&](int r, int d) {
@@ -697,41 +748,46 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                     *reinterpret_cast<float2*>(part + (int64_t)r * DT + d) = make_float2(a, b);
                 }
             };
-            float* mine = stage + (t * 4 + wq) * 32 * 17;
+            float* mine = stage + warp * 32 * (SC + 1);
 #pragma unroll 1
-            for (int c = 0; c < ksteps; ++c) {
-                if (live) {
-                    float o[16];
-                    tc_ld16(lanes + Cfg::o_col(t) + c * 16, o);
+            for (int c = half; c < ksteps; c += SPLIT) {   // 16 columns a turn, the row's threads in turn
+                float o[16];
+                __syncwarp();
+                tc_ld16(lanes + Cfg::o_col(t) + c * 16, o);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) mine[lane * 17 + j] = scale_o == 0.0f ? 0.0f : o[j] * scale_o;
-                }
-                if (REP == 1) {
-                    __syncwarp();
+                for (int part16 = 0; part16 < 16; part16 += SC) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int r = e * 4 + (lane >> 3), j = (lane & 7) * 2;
-                        if (t * 128 + wq * 32 + r < rows) put2(t * 128 + wq * 32 + r, c * 16 + j, mine[r * 17 + j], mine[r * 17 + j + 1]);
-                    }
-                    __syncwarp();
-                } else {
-                    named_bar_sync(bar, 128);
-                    for (int e = gtid; e < rows * 8; e += 128) {
-                        const int r = e >> 3, j = (e & 7) * 2;
-                        float a = 0.0f, b = 0.0f;
+                    for (int j = 0; j < SC; ++j) mine[lane * (SC + 1) + j] = scale_o == 0.0f ? 0.0f : o[part16 + j] * scale_o;
+                    constexpr int kPairs = SC / 2;
+                    if (REP == 1) {
+                        __syncwarp();
 #pragma unroll
-                        for (int rep = 0; rep < REP; ++rep) {
-                            const float* s = stage + (rep * RT + r) * 17 + j;
-                            a += s[0], b += s[1];
+                        for (int e = 0; e < kPairs; ++e) {
+                            const int r = e * (32 / kPairs) + lane / kPairs, j = (lane % kPairs) * 2;
+                            if (t * 128 + wq * 32 + r < rows)
+                                put2(t * 128 + wq * 32 + r, c * 16 + part16 + j, mine[r * (SC + 1) + j], mine[r * (SC + 1) + j + 1]);
                         }
-                        put2(r, c * 16 + j, a, b);
+                        __syncwarp();
+                    } else {
+                        named_bar_sync(bar_half, 128);
+                        for (int e = wq * 32 + lane; e < rows * kPairs; e += 128) {
+                            const int r = e / kPairs, j = (e % kPairs) * 2;
+                            float a = 0.0f, b = 0.0f;
+#pragma unroll
+                            for (int q = 0; q < REP; ++q) {
+                                const float* s = stage + (half * 128 + q * RT + r) * (SC + 1) + j;
+                                a += s[0], b += s[1];
+                            }
+                            put2(r, c * 16 + part16 + j, a, b);
+                        }
+                        named_bar_sync(bar_half, 128);
                     }
-                    named_bar_sync(bar, 128);
                 }
             }
-            const bool owner = live && kq == 0 && row < rows;   // one thread per row
+            const bool owner = half == 0 && rep == 0 && row < rows;   // one thread per row
             if (whole) {
                 if (owner && p.lse) put_lse(row, mm, ll);
+                __syncwarp();
                 tcf_before();
                 continue;
             }
@@ -739,40 +795,54 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             const int fc = (int)(seg0 / run), lc = (int)((seg1 - 1) / run);
             int* counter = p.counters + 2 * fc + t;
             __threadfence();
-            named_bar_sync(bar, 128);
+            named_bar_sync(bar_group, GT);
             if (gtid == 0) s_last[t] = atomicAdd(counter, 1) == lc - fc;
-            named_bar_sync(bar, 128);
+            named_bar_sync(bar_group, GT);
             if (*reinterpret_cast<volatile int*>(s_last + t)) {
                 __threadfence();
-                const int r0 = t * 128, r1 = min(rows, r0 + 128);
-                for (int e = gtid; e < (r1 - r0) * (DT / 4); e += 128) {
-                    const int r = r0 + e / (DT / 4), d = (e % (DT / 4)) * 4;
-                    if (d >= p.head_dim) continue;
+                // join: a thread takes 16 columns of a row (four 16-byte pieces, neighbours interleaved), the row's maxima
+                // and sums first, then the parts' values, 16 loads in flight
+                constexpr int kCols = DT / 16;
+                const int r0 = t * 128, items = (min(rows, r0 + 128) - r0) * kCols;
+                for (int e = gtid; e < items; e += GT) {
+                    const int r = r0 + e / kCols, d0 = (e % kCols) * 4;
+                    auto at = [&](int c) { return (int64_t)(2 * c + (c == fc ? 1 : 0)) * RT + r; };
                     float top = -INFINITY, sum = 0.0f;
-                    float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+                    for (int c = fc; c <= lc; ++c) top = fmaxf(top, __ldcg(&p.part_ml[at(c)].x));
+                    const float safe = top == -INFINITY ? 0.0f : top;
+                    float4 acc[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[k] = make_float4(0, 0, 0, 0);
 #pragma unroll 4
                     for (int c = fc; c <= lc; ++c) {
-                        const int64_t at = (int64_t)(2 * c + (c == fc ? 1 : 0)) * RT + r;
-                        const float2 v = __ldcg(p.part_ml + at);
-                        const float4 po = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * DT + d));
-                        const float big = fmaxf(top, v.x), safe = big == -INFINITY ? 0.0f : big;
-                        const float fa = exp2_fast(top - safe), fb = exp2_fast(v.x - safe);
-                        acc.x = acc.x * fa + po.x * fb;
-                        acc.y = acc.y * fa + po.y * fb;
-                        acc.z = acc.z * fa + po.z * fb;
-                        acc.w = acc.w * fa + po.w * fb;
-                        sum = sum * fa + v.y * fb;
-                        top = big;
+                        const float2 v = __ldcg(p.part_ml + at(c));
+                        const float w = exp2_fast(v.x - safe);
+                        sum += v.y * w;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float4 po = __ldcg(reinterpret_cast<const float4*>(p.part_o + at(c) * DT + d0 + k * (DT / 4)));
+                            acc[k].x += po.x * w;
+                            acc[k].y += po.y * w;
+                            acc[k].z += po.z * w;
+                            acc[k].w += po.w * w;
+                        }
                     }
                     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    uint32_t* dst = reinterpret_cast<uint32_t*>(out_ptr(r, d));
-                    dst[0] = pack2<T>(acc.x * inv, acc.y * inv);
-                    dst[1] = pack2<T>(acc.z * inv, acc.w * inv);
-                    if (p.lse && d == 0) put_lse(r, top, sum);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int d = d0 + k * (DT / 4);
+                        if (d >= p.head_dim) continue;
+                        uint32_t* dst = reinterpret_cast<uint32_t*>(out_ptr(r, d));
+                        dst[0] = pack2<T>(acc[k].x * inv, acc[k].y * inv);
+                        dst[1] = pack2<T>(acc[k].z * inv, acc[k].w * inv);
+                    }
+                    if (p.lse && d0 == 0) put_lse(r, top, sum);
                 }
                 if (gtid == 0) *counter = 0;   // ready for the next call
             }
-            named_bar_sync(bar, 128);
+            named_bar_sync(bar_group, GT);
+            __syncwarp();
             tcf_before();
         }
     }
