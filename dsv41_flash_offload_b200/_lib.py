@@ -9,6 +9,8 @@ import ctypes as C
 import os
 import threading
 
+import torch
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libdsv41_b200.so")
 
@@ -199,3 +201,23 @@ def check(rc: int, what: str) -> None:
     if rc != OK:
         msg = load().dsv41_last_error().decode(errors="replace")
         raise Dsv41Error(f"{what} failed ({rc}): {msg}")
+
+
+# The handle of a device's current stream as an integer. The object-building public call costs 2 us a time, more
+# than half of what a small kernel takes to launch.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def current_stream(dev: torch.device) -> int:
+    return _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+def call(dev: torch.device, fn, *args) -> None:
+    """fn(*args) of the library with `dev` current; raises what it reports."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args)
+    if rc != OK:
+        check(rc, fn.__name__)

@@ -111,8 +111,8 @@ int dsv41_step_tables(const dsv41_step_tables_args* a, void* stream)
         return set_error(DSV41_E_INVALID, "NULL pointer");
     if (a->held_out == a->held_pages || a->free_count_out == a->free_count)
         return set_error(DSV41_E_INVALID, "an output overlaps its input");
-    if (!aligned(a->slots, 16) || !aligned(a->positions, 16) || !aligned(a->requests, 16))
-        return set_error(DSV41_E_INVALID, "slots, positions and requests must be 16-byte aligned");
+    if (!aligned(a->slots, 8) || !aligned(a->positions, 4) || !aligned(a->requests, 4))
+        return set_error(DSV41_E_INVALID, "slots, positions or requests are misaligned");
     if (a->parents) {
         if (a->mask_words < 1 || a->mask_words > kMaxMaskWords)
             return set_error(DSV41_E_INVALID, "mask_words=%d (1..%d)", a->mask_words, kMaxMaskWords);

@@ -168,7 +168,9 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
     };
 
     if (!p.parents) {
-        // token-parallel, kTabTokens consecutive tokens per thread
+        // token-parallel, kTabTokens consecutive tokens per thread; 16-byte stores where the arrays allow them
+        const bool vector = ((reinterpret_cast<uintptr_t>(p.positions) | reinterpret_cast<uintptr_t>(p.requests) |
+                              reinterpret_cast<uintptr_t>(p.slots)) & 15) == 0;
         for (int64_t t0 = (int64_t)first * kTabTokens; t0 < p.num_tokens; t0 += (int64_t)stride * kTabTokens) {
             int64_t slot[kTabTokens];
             int pos[kTabTokens], req[kTabTokens];
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
                 pos[i] = (int)at;
                 req[i] = b;
             }
-            if (t0 + kTabTokens <= p.num_tokens) {
+            if (vector && t0 + kTabTokens <= p.num_tokens) {
                 *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
                 *reinterpret_cast<int4*>(p.requests + t0) = make_int4(req[0], req[1], req[2], req[3]);
                 *reinterpret_cast<longlong2*>(p.slots + t0) = make_longlong2(slot[0], slot[1]);

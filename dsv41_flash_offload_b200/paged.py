@@ -15,7 +15,6 @@ captured in a CUDA graph.
 from __future__ import annotations
 
 import ctypes as C
-import math
 import threading
 from typing import NamedTuple
 
@@ -42,14 +41,22 @@ class StepTables(NamedTuple):
     tree_mask: torch.Tensor | None   # int64 [N, mask_words] ancestors of each drafted token
 
 
-def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
 def _vector(t: torch.Tensor, name: str, n: int, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != dev:
+    if t.dtype is not dtype or t.shape != (n,) or t.device != dev:
         raise ValueError(f"{name} must be {str(dtype)[6:]} [{n}] on {dev}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _table(t: torch.Tensor, batch: int, dev: torch.device) -> tuple[int, int, int]:
+    """Address, width and row stride of a block table."""
+    if t.dtype is torch.int32 and t.dim() == 2 and t.device == dev:
+        rows, width = t.shape
+        if rows == batch:
+            if t.is_contiguous():
+                return t.data_ptr(), width, width
+            if t.stride(1) == 1 and t.stride(0) >= width:
+                return t.data_ptr(), width, t.stride(0)
+    raise ValueError(f"block_table must be int32 [{batch}, width] with contiguous rows on {dev}")
 
 
 def step_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, held_pages: torch.Tensor, block_table: torch.Tensor,
@@ -74,9 +81,7 @@ def step_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, held_pages: 
     new_lens = _vector(new_lens, "new_lens", B, torch.int32, dev)
     held_pages = _vector(held_pages, "held_pages", B, torch.int32, dev)
     free_count = _vector(free_count, "free_count", 1, torch.int32, dev)
-    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.device != dev
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
-        raise ValueError(f"block_table must be int32 [{B}, width] with contiguous rows on {dev}")
+    table, width, table_stride = _table(block_table, B, dev)
     if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous() or free_pages.device != dev:
         raise ValueError(f"free_pages must be a contiguous int32 vector on {dev}")
     if N < 0:
@@ -86,43 +91,46 @@ def step_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, held_pages: 
         if not 1 <= mask_words <= MAX_MASK_WORDS:
             raise ValueError(f"mask_words must be 1..{MAX_MASK_WORDS}")
         parents = _vector(parents, "parents", N, torch.int32, dev)
-        mask = torch.empty((N, mask_words), dtype=torch.int64, device=dev)
-    pad = (N + 3) // 4 * 4
-    ints = torch.empty(2 * pad + 4 * B + 2, dtype=torch.int32, device=dev)
-    positions, _, requests, _, cu, seq, held, count, status = ints.split((N, pad - N, N, pad - N, B + 1, B, B, 1, B))
-    slots = torch.empty(N, dtype=torch.int64, device=dev)
+        mask = parents.new_empty((N, mask_words), dtype=torch.int64)
+    ints = context_lens.new_empty(2 * N + 4 * B + 2)
+    positions, requests, cu, seq, held, count, status = ints.split_with_sizes((N, N, B + 1, B, B, 1, B))
+    slots = context_lens.new_empty(N, dtype=torch.int64)
     base = ints.data_ptr()
+    at = base + 8 * N
     args = _lib.StepTablesArgs(
-        B, block_table.shape[1], int(page_size), N, context_lens.data_ptr(), new_lens.data_ptr(), held_pages.data_ptr(),
-        block_table.data_ptr(), block_table.stride(0) if B > 1 else block_table.shape[1], free_pages.data_ptr(),
-        free_count.data_ptr(), free_pages.shape[0], int(mask_words), parents.data_ptr() if parents is not None else None,
-        cu.data_ptr(), seq.data_ptr(), slots.data_ptr(), base, base + 4 * pad, held.data_ptr(), count.data_ptr(),
-        status.data_ptr(), mask.data_ptr() if mask is not None else None)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().dsv41_step_tables(C.byref(args), _stream(dev)), "dsv41_step_tables")
+        B, width, int(page_size), N, context_lens.data_ptr(), new_lens.data_ptr(), held_pages.data_ptr(), table,
+        table_stride, free_pages.data_ptr(), free_count.data_ptr(), free_pages.shape[0], int(mask_words), parents.data_ptr() if parents is not None else None,
+        at, at + 4 * B + 4, slots.data_ptr(), base, base + 4 * N, at + 8 * B + 4, at + 12 * B + 4, at + 12 * B + 8,
+        mask.data_ptr() if mask is not None else None)
+    _lib.call(dev, _lib.load().dsv41_step_tables, C.byref(args), _lib.current_stream(dev))
     return StepTables(cu, seq, slots, positions, requests, held, count, status, mask)
 
 
-def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype or k_cache.stride() != v_cache.stride():
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[torch.Size, tuple, torch.device]:
+    """Shape, strides and device of a pair of caches, checked."""
+    shape, strides, dev = k_cache.shape, k_cache.stride(), k_cache.device
+    if len(shape) != 4 or shape != v_cache.shape or strides != v_cache.stride() or k_cache.dtype is not v_cache.dtype:
         raise ValueError("the caches must be [num_pages, page_size, kv_heads, head_dim], alike in shape, dtype and strides")
-    if not k_cache.is_cuda or v_cache.device != k_cache.device:
+    if not k_cache.is_cuda or v_cache.device != dev:
         raise ValueError("the caches must live on one CUDA device")
     if k_cache.dtype not in _DTYPES:
         raise TypeError(f"unsupported cache dtype {k_cache.dtype} (fp16 or bf16)")
-    if k_cache.shape[3] % 8 or k_cache.shape[3] == 0:
+    if shape[3] % 8 or shape[3] == 0:
         raise ValueError("head_dim must be a multiple of 8")
-    if k_cache.stride(3) != 1 or any(s % 8 for s in k_cache.stride()[:3]) or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+    if (strides[3] != 1 or strides[0] % 8 or strides[1] % 8 or strides[2] % 8 or k_cache.data_ptr() % 16
+            or v_cache.data_ptr() % 16):
         raise ValueError("the caches must have contiguous, 16-byte aligned heads")
+    return shape, strides, dev
 
 
-def _heads(t: torch.Tensor, name: str, unit: int, tokens: int, heads: int, dim: int, like: torch.Tensor) -> torch.Tensor:
-    """t [tokens, heads, dim] in a form the kernels read in pieces of `unit` elements (copied if it is not)."""
-    if t.dim() != 3 or tuple(t.shape) != (tokens, heads, dim) or t.device != like.device:
-        raise ValueError(f"{name} must be [{tokens}, {heads}, {dim}] on {like.device}")
-    if t.dtype != like.dtype:
+def _heads(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor) -> torch.Tensor:
+    """t of this shape with contiguous, 16-byte aligned heads (copied if they are not)."""
+    if t.shape != shape or t.device != like.device:
+        raise ValueError(f"{name} must be {list(shape)} on {like.device}")
+    if t.dtype is not like.dtype:
         raise TypeError(f"{name} is {t.dtype}, the cache {like.dtype}")
-    if t.stride(2) != 1 or t.stride(0) % unit or t.stride(1) % unit or t.data_ptr() % (2 * unit):
+    s = t.stride()
+    if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -130,17 +138,15 @@ def _heads(t: torch.Tensor, name: str, unit: int, tokens: int, heads: int, dim: 
 def store_kv(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
     """k_cache[slots[t]] = k[t] and v_cache[slots[t]] = v[t] for new keys and values [N, kv_heads, head_dim] (any
     strides with contiguous heads, e.g. slices of a fused projection); slots int64 [N], -1 stores nothing."""
-    _check_cache(k_cache, v_cache)
-    pages, page_size, heads, dim = k_cache.shape
-    N = slots.shape[0]
-    slots = _vector(slots, "slots", N, torch.int64, k_cache.device)
-    k = _heads(k, "k", 8, N, heads, dim, k_cache)
-    v = _heads(v, "v", 8, N, heads, dim, k_cache)
-    args = _lib.StoreKvArgs(N, heads, dim, pages, page_size, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
-                            v.stride(1), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0),
-                            k_cache.stride(1), k_cache.stride(2))
-    with torch.cuda.device(k_cache.device):
-        _lib.check(_lib.load().dsv41_store_kv(C.byref(args), _stream(k_cache.device)), "dsv41_store_kv")
+    (pages, page_size, heads, dim), cs, dev = _cache(k_cache, v_cache)
+    N = slots.shape[0] if slots.dim() else 0
+    slots = _vector(slots, "slots", N, torch.int64, dev)
+    k = _heads(k, "k", (N, heads, dim), k_cache)
+    v = _heads(v, "v", (N, heads, dim), k_cache)
+    ks, vs = k.stride(), v.stride()
+    args = _lib.StoreKvArgs(N, heads, dim, pages, page_size, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
+                            slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2])
+    _lib.call(dev, _lib.load().dsv41_store_kv, C.byref(args), _lib.current_stream(dev))
 
 
 # one zeroed workspace per (device, stream, padded head size): its counters are zero between calls, and calls
@@ -149,29 +155,30 @@ _ws_lock = threading.Lock()
 _ws: dict = {}
 
 
-def _workspace(dev: torch.device, stream: int, head_dim: int) -> torch.Tensor:
+def _workspace(dev: torch.device, stream: int, head_dim: int) -> tuple[int, int]:
+    """Address and size of the stream's workspace."""
     key = (dev.index, stream, 64 if head_dim <= 64 else 128 if head_dim <= 128 else 256)
-    buf = _ws.get(key)
-    if buf is None:
-        with _ws_lock:
+    got = _ws.get(key)
+    if got is None:
+        with _ws_lock, torch.cuda.device(dev):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("dsv41: workspace must be allocated before CUDA-graph capture (run once eagerly)")
             size = C.c_size_t()
             _lib.check(_lib.load().dsv41_tree_attention_workspace_size(head_dim, C.byref(size)), "workspace_size")
-            buf = _ws.setdefault(key, torch.zeros(size.value, dtype=torch.uint8, device=dev))
-    return buf
+            buf = torch.zeros(size.value, dtype=torch.uint8, device=dev)
+            got = _ws.setdefault(key, (buf.data_ptr(), size.value, buf))
+    return got[:2]
 
 
 def read_status(device=None) -> int:
     """Synchronise the current stream; return (then clear) the status of its tree_attention calls: 0 = ok, 1 = a
     bounded device-side wait ran out (results since the last read are invalid)."""
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-    stream, worst = _stream(dev), 0
-    for (index, s, _), buf in list(_ws.items()):
+    stream, worst = _lib.current_stream(dev), 0
+    for (index, s, _), (_, _, buf) in list(_ws.items()):
         if index == dev.index and s == stream:
             st = C.c_int32()
-            with torch.cuda.device(dev):
-                _lib.check(_lib.load().dsv41_read_status(buf.data_ptr(), stream, C.byref(st)), "read_status")
+            _lib.call(dev, _lib.load().dsv41_read_status, buf.data_ptr(), stream, C.byref(st))
             worst = max(worst, st.value)
     return worst
 
@@ -187,43 +194,40 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     up to itself. max_new is an upper bound on a request's new tokens, scale defaults to head_dim ** -0.5. Query head
     h reads KV head h // (q_heads / kv_heads). A row that sees nothing is 0 with lse -inf. Returns out [N, q_heads,
     head_dim] in q's dtype, or (out, lse fp32 [N, q_heads]); rows past cu_lens[B] are not written."""
-    _check_cache(k_cache, v_cache)
-    pages, page_size, kv_heads, dim = k_cache.shape
-    dev = k_cache.device
+    (pages, page_size, kv_heads, dim), cs, dev = _cache(k_cache, v_cache)
     if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % kv_heads:
         raise ValueError(f"q must be [N, q_heads, {dim}] with q_heads a multiple of {kv_heads}")
-    N, q_heads = q.shape[0], q.shape[1]
-    q = _heads(q, "q", 8, N, q_heads, dim, k_cache)
+    N, q_heads, _ = q.shape
+    q = _heads(q, "q", (N, q_heads, dim), k_cache)
     if seq_lens.dim() != 1:
         raise ValueError("seq_lens must be int32 [B]")
     B = seq_lens.shape[0]
     seq_lens = _vector(seq_lens, "seq_lens", B, torch.int32, dev)
     cu_lens = _vector(cu_lens, "cu_lens", B + 1, torch.int32, dev)
-    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.device != dev
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
-        raise ValueError(f"block_table must be int32 [{B}, width] with contiguous rows on {dev}")
-    words = 1
+    table, width, table_stride = _table(block_table, B, dev)
+    words, mask = 1, None
     if tree_mask is not None:
-        if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != N or tree_mask.device != dev:
+        if tree_mask.dtype is not torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != N or tree_mask.device != dev:
             raise ValueError(f"tree_mask must be int64 [{N}, words] on {dev}")
         words = tree_mask.shape[1]
         tree_mask = tree_mask.contiguous()
+        mask = tree_mask.data_ptr()
     if out is None:
-        out = torch.empty((N, q_heads, dim), dtype=q.dtype, device=dev)
-    elif (tuple(out.shape) != (N, q_heads, dim) or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1
-          or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16):
-        raise ValueError("out must be like q, with contiguous, 16-byte aligned heads")
-    lse = torch.empty((N, q_heads), dtype=torch.float32, device=dev) if return_lse else None
-    stream = _stream(dev)
-    width = block_table.shape[1]
+        out = q.new_empty((N, q_heads, dim))
+        os = (q_heads * dim, dim)
+    else:
+        os = out.stride()
+        if (out.shape != (N, q_heads, dim) or out.dtype is not q.dtype or out.device != dev or os[2] != 1 or os[0] % 8
+                or os[1] % 8 or out.data_ptr() % 16):
+            raise ValueError("out must be like q, with contiguous, 16-byte aligned heads")
+    lse = q.new_empty((N, q_heads), dtype=torch.float32) if return_lse else None
+    stream = _lib.current_stream(dev)
+    ws, ws_bytes = _workspace(dev, stream, dim)
+    qs = q.stride()
     args = _lib.TreeAttentionArgs(
         _DTYPES[q.dtype], B, N, int(max_new), q_heads, kv_heads, dim, page_size, pages, min(width * page_size, 0x7fffff00),
-        q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
-        k_cache.stride(2), block_table.data_ptr(), block_table.stride(0) if B > 1 else width, seq_lens.data_ptr(),
-        cu_lens.data_ptr(), tree_mask.data_ptr() if tree_mask is not None else None, words,
-        1.0 / math.sqrt(dim) if scale is None else float(scale), out.data_ptr(), out.stride(0), out.stride(1),
-        lse.data_ptr() if lse is not None else None)
-    with torch.cuda.device(dev):
-        ws = _workspace(dev, stream, dim)
-        _lib.check(_lib.load().dsv41_tree_attention(C.byref(args), ws.data_ptr(), ws.numel(), stream), "dsv41_tree_attention")
+        q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], table, table_stride,
+        seq_lens.data_ptr(), cu_lens.data_ptr(), mask, words, dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
+        os[0], os[1], lse.data_ptr() if lse is not None else None)
+    _lib.call(dev, _lib.load().dsv41_tree_attention, C.byref(args), ws, ws_bytes, stream)
     return (out, lse) if return_lse else out

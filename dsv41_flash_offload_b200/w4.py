@@ -21,10 +21,6 @@ _X_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 _OUT_DTYPES = {**_X_DTYPES, torch.float32: _lib.DTYPE_F32}
 
 
-def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
 class W4Weight:
     """A 4-bit matrix [n, k] on the GPU, laid out for the kernels.
 
@@ -54,10 +50,11 @@ class W4Weight:
         _lib.check(L.dsv41_w4_layout_size(n, k, group, int(zeros is not None), C.byref(size)), "dsv41_w4_layout_size")
         self.n, self.k, self.group, self.device = n, k, group, codes.device
         self.data = torch.empty(size.value, dtype=torch.uint8, device=codes.device)
-        with torch.cuda.device(self.device):
-            _lib.check(L.dsv41_w4_pack(codes.data_ptr(), scales.data_ptr(), zeros.data_ptr() if zeros is not None else None,
-                                       n, k, group, self.data.data_ptr(), size.value, _stream(self.device)), "dsv41_w4_pack")
+        _lib.call(self.device, L.dsv41_w4_pack, codes.data_ptr(), scales.data_ptr(),
+                  zeros.data_ptr() if zeros is not None else None, n, k, group, self.data.data_ptr(), size.value,
+                  _lib.current_stream(self.device))
         self._c = _lib.W4WeightC(n, k, group, int(zeros is not None), _X_DTYPES[scales.dtype], self.data.data_ptr())
+        self._ref = C.byref(self._c)
 
     @classmethod
     def quantize(cls, weight: torch.Tensor, group: int = 128, symmetric: bool = True) -> "W4Weight":
@@ -88,20 +85,34 @@ def _rows(x: torch.Tensor, w: W4Weight) -> torch.Tensor:
         raise ValueError("x must live on the weight's device")
     if x.dim() != 2:
         x = x.reshape(-1, w.k)
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < w.k or x.data_ptr() % 16:
+    if not x.is_contiguous() and (x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < w.k):
+        x = x.contiguous()
+    if x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
 
-def _output(x: torch.Tensor, tokens: int, w: W4Weight, out: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor:
+def _product(fn, weights, x: torch.Tensor, w: W4Weight, out: torch.Tensor | None, out_dtype: torch.dtype | None,
+             tail) -> torch.Tensor:
+    rows = _rows(x, w)
+    n, tokens = w.n, rows.shape[0]
+    stride = n
     if out is None:
-        if dtype not in _OUT_DTYPES:
-            raise TypeError(f"unsupported output dtype {dtype}")
-        return torch.empty((*x.shape[:-1], w.n), dtype=dtype, device=w.device)
-    if out.shape != (*x.shape[:-1], w.n) or out.dtype not in _OUT_DTYPES or out.device != w.device:
-        raise ValueError("out must be a fp32, fp16 or bf16 tensor of x's leading shape and n columns on the weight's device")
-    if not out.is_contiguous() and not (out.dim() == 2 and out.stride(1) == 1 and out.stride(0) >= w.n):
-        raise ValueError("out must have contiguous rows")
+        out_dtype = out_dtype or x.dtype
+        if out_dtype not in _OUT_DTYPES:
+            raise TypeError(f"unsupported output dtype {out_dtype}")
+        out = x.new_empty((tokens, n) if x.dim() == 2 else (*x.shape[:-1], n), dtype=out_dtype)
+    else:
+        if out.shape != (*x.shape[:-1], n) or out.dtype not in _OUT_DTYPES or out.device != w.device:
+            raise ValueError("out must be a fp32, fp16 or bf16 tensor of x's leading shape and n columns on the weight's device")
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError("out and out_dtype differ")
+        if not out.is_contiguous():
+            if out.dim() != 2 or out.stride(1) != 1 or out.stride(0) < n:
+                raise ValueError("out must have contiguous rows")
+            stride = out.stride(0)
+    _lib.call(w.device, fn, *weights, rows.data_ptr(), _X_DTYPES[rows.dtype], max(rows.stride(0), w.k) if tokens > 1 else w.k,
+              tokens, *tail[0], out.data_ptr(), _OUT_DTYPES[out.dtype], stride, *tail[1], _lib.current_stream(w.device))
     return out
 
 
@@ -109,38 +120,19 @@ def linear(x: torch.Tensor, weight: W4Weight, *, out: torch.Tensor | None = None
            accumulate: bool = False) -> torch.Tensor:
     """x [..., k] (fp16 or bf16) times the transposed 4-bit matrix -> [..., n] in out_dtype (default x's; fp32,
     fp16 or bf16). accumulate adds into a given fp32 `out`."""
-    rows = _rows(x, weight)
     if accumulate and (out is None or out.dtype != torch.float32):
         raise ValueError("accumulate needs an fp32 out")
-    out = _output(x, rows.shape[0], weight, out, out_dtype or x.dtype)
-    if out_dtype is not None and out.dtype != out_dtype:
-        raise ValueError("out and out_dtype differ")
-    stride = out.stride(0) if out.dim() == 2 and rows.shape[0] > 1 else weight.n
-    with torch.cuda.device(weight.device):
-        _lib.check(_lib.load().dsv41_w4_linear(C.byref(weight._c), rows.data_ptr(), _X_DTYPES[rows.dtype],
-                                               max(rows.stride(0), weight.k), rows.shape[0], out.data_ptr(),
-                                               _OUT_DTYPES[out.dtype], stride, int(accumulate), _stream(weight.device)),
-                   "dsv41_w4_linear")
-    return out
+    return _product(_lib.load().dsv41_w4_linear, (weight._ref,), x, weight, out, out_dtype, ((), (int(accumulate),)))
 
 
 def gated(x: torch.Tensor, gate: W4Weight, up: W4Weight, limit: float | None = None, *,
           out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """min(silu(x gate^T), limit) * clamp(x up^T, -limit, limit) -> [..., n] in out_dtype (default x's): the
     routed experts' SwiGLU (limit None or 0: no clamp)."""
-    rows = _rows(x, gate)
     if up.device != gate.device:
         raise ValueError("gate and up must live on one device")
-    out = _output(x, rows.shape[0], gate, out, out_dtype or x.dtype)
-    if out_dtype is not None and out.dtype != out_dtype:
-        raise ValueError("out and out_dtype differ")
-    stride = out.stride(0) if out.dim() == 2 and rows.shape[0] > 1 else gate.n
     lim = float(limit) if limit is not None and limit > 0 else 0.0
-    with torch.cuda.device(gate.device):
-        _lib.check(_lib.load().dsv41_w4_gated(C.byref(gate._c), C.byref(up._c), rows.data_ptr(), _X_DTYPES[rows.dtype],
-                                              max(rows.stride(0), gate.k), rows.shape[0], lim, out.data_ptr(),
-                                              _OUT_DTYPES[out.dtype], stride, _stream(gate.device)), "dsv41_w4_gated")
-    return out
+    return _product(_lib.load().dsv41_w4_gated, (gate._ref, up._ref), x, gate, out, out_dtype, ((lim,), ()))
 
 
 def shared_expert(x: torch.Tensor, gate: W4Weight, up: W4Weight, down: W4Weight, limit: float | None = None, *,

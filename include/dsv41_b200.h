@@ -264,8 +264,7 @@ enum {
  * free_count_out [1]; status [batch]; per token: slots (int64), positions, requests (its b). Without
  * parents a token's position is context + its index; with parents ([num_tokens], index of the parent
  * within the request, -1 = the context) it is context + its depth, and tree_mask [num_tokens][mask_words]
- * holds a bit for each ancestor and itself. The int32 outputs may not overlap the inputs. slots,
- * positions and requests must be 16-byte aligned. */
+ * holds a bit for each ancestor and itself. The outputs may not overlap the inputs. */
 typedef struct dsv41_step_tables_args {
     int32_t batch, width, page_size, num_tokens;
     const int32_t* context_lens;
