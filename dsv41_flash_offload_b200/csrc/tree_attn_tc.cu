@@ -5,7 +5,7 @@
 //   producers (4 warps)  copy key and value tiles of 128 keys (page by page, 16-byte cp.async) into a ring of
 //                        units in the 128-byte swizzle the tensor cores read; a ring of byte offsets, one per
 //                        key, is looked up one tile ahead
-//   Q loader (1 warp)    the rows of the segment
+//   Q loaders (2 warps)  the rows of the segment
 //   two issuers (1 thread each)  S = Q K^T (A and B from shared memory) and O += P V (A from tensor memory, V read
 //                        as it lies, N-major), fp32 accumulators in tensor memory. One thread for both left the tensor
 //                        pipe idle between its waits and commits: a unit then took 3400 cycles, of which 2900 in issuing
@@ -28,6 +28,12 @@
 
 namespace dsv41 {
 
+#ifndef DSV41_ATTN_EXTRA
+#define DSV41_ATTN_EXTRA 2
+#endif
+#ifndef DSV41_ATTN_EXTRA2
+#define DSV41_ATTN_EXTRA2 1
+#endif
 template <int DT, int MT, int REP>
 struct TcCfg {
     static_assert(MT == 1 || REP == 1, "repeats are for a single tile of 128 rows");
@@ -38,14 +44,15 @@ struct TcCfg {
     static constexpr int hold = MT == 2 ? 32 : kw;           // scores a thread holds at a time (registers)
     static constexpr int group = 128 * split;                // softmax threads per 128 rows
     static constexpr int soft_warps = 4 * split * MT;
-    static constexpr int w_prod = soft_warps, w_q = w_prod + 4, w_s = w_q + 1, w_o = w_s + 1;
+    static constexpr int w_prod = soft_warps, w_q = w_prod + 4, w_s = w_q + 2, w_o = w_s + 1;
     static constexpr int threads = (w_o + 1) * 32;
     static constexpr int block_b = 128 * 128;                // 128 rows x 64 columns of 16 bits, swizzled
     static constexpr int blocks = DT / 64;
     static constexpr int unit_b = blocks * block_b;          // a key or value tile
     static constexpr int q_b = MT * unit_b;
-    static constexpr int sc = MT == 2 ? 8 : 16;              // columns of O on their way out at a time
-    static constexpr int stage_b = soft_warps * 32 * (sc + 1) * 4;
+    static constexpr int own = 32 / REP;                     // of 32 columns of O, those a repeat's warps put out
+    static constexpr int stage_b = soft_warps * (32 - own) * 32 * 4;   // the others', on their way to their repeat
+    static constexpr int extra = MT == 1 ? DSV41_ATTN_EXTRA : DSV41_ATTN_EXTRA2;   // cost of a segment, in tiles
     static constexpr int off_b = 4 * kt * 8;                 // byte offsets of the keys of four tiles
     static constexpr int ml_b = MT * 2 * 128 * 8;
     static constexpr int mx_b = MT * 4 * 128 * 4;            // tile maxima of the threads that share a row
@@ -55,7 +62,7 @@ struct TcCfg {
     static constexpr int units = units_fit < 10 ? units_fit : 10;
     static constexpr int lag = units - 2;                    // units a producer has in flight when it issues the next
     static constexpr int smem = fixed_b + units * unit_b;
-    static_assert(units >= 4, "ring too short");
+    static_assert(units >= 4 && lag <= 8, "ring length");
     // tensor memory columns
     __host__ __device__ static constexpr int s_col(int b) { return b * 128; }
     // P of key x of buffer b (two keys a column). Two row tiles leave no room of its own: P then lies over S, each
@@ -66,6 +73,17 @@ struct TcCfg {
     }
     __host__ __device__ static constexpr int o_col(int t) { return MT == 1 ? 384 : 256 + t * 128; }
 };
+
+// whether a phase is complete, without waiting for it
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok)
+                 : "r"(smem_addr(bar)), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
 
 // ---- tcgen05 ----------------------------------------------------------------------------------
 __device__ __forceinline__ void tcf_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -180,6 +198,13 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r)
         : "memory");
 }
 
+__device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t* r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
 template <typename T, int DT, int MT, int REP>
 __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_kernel(const TreeAttnParams p)
 {
@@ -207,63 +232,8 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
     int* s_last = dirty + NU;              // [2]
     volatile int* abort_flag = s_last + 2;
     uint32_t* tmem_slot = const_cast<uint32_t*>(reinterpret_cast<volatile uint32_t*>(abort_flag)) + 1;
-    __shared__ int64_t warp_tot[Cfg::threads / 32];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-
-    // ---- this CTA's run of units ----
-    int64_t* pre = reinterpret_cast<int64_t*>(su);
-    int64_t total = 0;
-    {
-        const int per = (p.batch + Cfg::threads - 1) / Cfg::threads;
-        const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
-        auto units_of = [&](int b) -> int64_t {
-            const AttnReq r = attn_req(p, b);
-            return r.n > 0 ? (int64_t)((r.n * p.group + RT - 1) / RT) * max((r.seq + KT - 1) / KT, 1) * p.kv_heads : 0;
-        };
-        int64_t sum = 0;
-        for (int b = b0; b < b1; ++b) sum += units_of(b);
-        int64_t inc = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += y;
-        }
-        if (lane == 31) warp_tot[warp] = inc;
-        __syncthreads();
-        int64_t base = inc - sum;
-        for (int w = 0; w < Cfg::threads / 32; ++w) {
-            if (w < warp) base += warp_tot[w];
-            total += warp_tot[w];
-        }
-        for (int b = b0; b < b1; ++b) {
-            pre[b] = base;
-            base += units_of(b);
-        }
-        __syncthreads();
-    }
-    const int64_t run = (total + gridDim.x - 1) / gridDim.x;
-    const int64_t u0 = run * blockIdx.x;
-    const int count = (int)max(min(run, total - u0), (int64_t)0);
-    if (count <= 0) return;
-    Cursor cur;
-    {
-        int lo = 0, hi = p.batch;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (pre[mid] <= u0) lo = mid;
-            else hi = mid;
-        }
-        cur.b = lo;
-        cur.enter(p);
-        int64_t at = u0 - pre[lo];
-        const int64_t per_head = (int64_t)cur.nrt * cur.nkt;
-        cur.h = (int)(at / per_head);
-        at -= cur.h * per_head;
-        cur.rt = (int)(at / cur.nkt);
-        cur.kt = (int)(at - (int64_t)cur.rt * cur.nkt);
-    }
-    __syncthreads();   // the prefix sums lie in the ring
 
     if (tid == 0) {
         for (int i = 0; i < NU; ++i) {
@@ -271,21 +241,86 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             mbar_init(&empty[i], 1);
             dirty[i] = 0;
         }
-        mbar_init(q_full, 1);
+        mbar_init(q_full, 2);
         mbar_init(q_free, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4 * Cfg::split);
             mbar_init(&pv_done[i], 1);
+            mbar_init(&all_done[i], 1);
         }
-        mbar_init(&all_done[0], 1);
-        mbar_init(&all_done[1], 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
     if (warp == Cfg::w_s) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // ---- this CTA's run ----
+    // A segment of nkt tiles costs what nkt + extra tiles do (its rows' loads, its end), so the runs are cut from a line
+    // on which each segment begins with `extra` empty places. Every thread sums its requests' places and tiles; the
+    // one whose request holds the run's first place, and the one that holds its end, tell the others.
+    __shared__ int64_t warp_sum[Cfg::threads / 32][2];
+    __shared__ int64_t s_first[3], s_end;   // first: request, segment of the request, place in the segment; tiles before
+    __shared__ int64_t s_tiles0;
+    struct SegState {
+        Cursor c;
+        int64_t v_seg;   // place on the line where the segment begins
+    };
+    __shared__ SegState s_seg[Cfg::soft_warps];
+    int64_t run, v0;
+    {
+        const int per = (p.batch + Cfg::threads - 1) / Cfg::threads;
+        const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+        auto segments = [&](const AttnReq& r) { return r.n > 0 ? (int64_t)((r.n * p.group + RT - 1) / RT) * p.kv_heads : 0; };
+        auto tiles = [&](const AttnReq& r) { return max((r.seq + KT - 1) / KT, 1); };
+        int64_t sum[2] = {0, 0};   // segments' places, tiles
+        AttnReq mine;
+        for (int b = b0; b < b1; ++b) {
+            mine = attn_req(p, b);
+            const int64_t n = segments(mine);
+            sum[0] += n * (tiles(mine) + Cfg::extra);
+            sum[1] += n * tiles(mine);
+        }
+        int64_t inc[2] = {sum[0], sum[1]};
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, inc[k], o);
+                if (lane >= o) inc[k] += y;
+            }
+        }
+        if (lane == 31) warp_sum[warp][0] = inc[0], warp_sum[warp][1] = inc[1];
+        __syncthreads();
+        int64_t at = inc[0] - sum[0], before = inc[1] - sum[1], total = 0, all = 0;
+        for (int w = 0; w < Cfg::threads / 32; ++w) {
+            if (w < warp) at += warp_sum[w][0], before += warp_sum[w][1];
+            total += warp_sum[w][0];
+            all += warp_sum[w][1];
+        }
+        run = (total + gridDim.x - 1) / gridDim.x;
+        v0 = run * blockIdx.x;
+        const int64_t v1 = min(v0 + run, total);
+        if (tid == 0 && v1 >= total) s_end = all;
+        for (int b = b0; b < b1; ++b) {
+            if (per > 1) mine = attn_req(p, b);
+            const int64_t nt = tiles(mine), len = nt + Cfg::extra, places = segments(mine) * len;
+            auto tiles_before = [&](int64_t v) {   // tiles before place v of this request
+                const int64_t g = v / len, in = v - g * len;
+                return before + g * nt + max(in - Cfg::extra, (int64_t)0);
+            };
+            if (v0 >= at && v0 < at + places) {
+                s_first[0] = b;
+                s_first[1] = (v0 - at) / len;
+                s_first[2] = (v0 - at) % len;
+                s_tiles0 = tiles_before(v0 - at);
+            }
+            if (v1 < total && v1 >= at && v1 < at + places) s_end = tiles_before(v1 - at);
+            at += places;
+            before += segments(mine) * nt;
+        }
+        if (v0 >= total && tid == 0) s_tiles0 = all;
     }
     if (p.head_dim % 16) {   // the last 16-column step of Q K^T reads past the head size: zeros there
         uint4* z = reinterpret_cast<uint4*>(sq);
@@ -296,6 +331,17 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
     __syncthreads();
     tcf_after();
     const uint32_t tmem = *tmem_slot;
+    const int count = (int)(s_end - s_tiles0);   // tiles of the run
+    if (count <= 0) {
+        if (warp == Cfg::w_s) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        return;
+    }
+    Cursor cur;
+    cur.b = (int)s_first[0];
+    cur.enter(p);
+    cur.h = (int)s_first[1] / cur.nrt;
+    cur.rt = (int)s_first[1] - cur.h * cur.nrt;
+    cur.kt = max((int)s_first[2] - Cfg::extra, 0);
     const int ksteps = (p.head_dim + 15) / 16;
     constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(128 >> 4) << 24);   // fp32 sums, M = 128
@@ -316,6 +362,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
         const bool col_live = chunk * 8 < p.head_dim;
         const uint32_t col_at = (chunk >> 3) * Cfg::block_b;
         const uint32_t ring = smem_addr(su);
+        int arrived = 0;     // units handed over
         uint32_t hist = 0;   // bit k: the unit issued k units ago holds new tokens' values
         auto arrive = [&](int n, bool check) {   // this thread's copies of unit n have landed
             const int slot = n % NU;
@@ -339,9 +386,32 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             if (lane == 0) mbar_arrive(&full[slot]);
             __syncwarp();
         };
+        // hand over the units in flight before unit n, each as soon as it has landed, until stop()
+        auto flush = [&](int n, auto stop) {
+            bool stopped = false;
+            auto one = [&](auto left) {
+                constexpr int k = decltype(left)::value;   // units that may still be in flight
+                if (stopped || arrived > n - 1 - k) return;
+                cp_async_wait<k>();
+                arrive(arrived++, (hist >> k) & 1);
+                stopped = stop();
+            };
+            if (LAG > 7) one(std::integral_constant<int, 7>());
+            if (LAG > 6) one(std::integral_constant<int, 6>());
+            if (LAG > 5) one(std::integral_constant<int, 5>());
+            if (LAG > 4) one(std::integral_constant<int, 4>());
+            if (LAG > 3) one(std::integral_constant<int, 3>());
+            if (LAG > 2) one(std::integral_constant<int, 2>());
+            one(std::integral_constant<int, 1>());
+            one(std::integral_constant<int, 0>());
+            return stopped;
+        };
         auto issue = [&](int n, const void* cache, const int64_t* offs, bool check) {
             const int slot = n % NU;
-            wait_warp(&empty[slot], ((n / NU) & 1) ^ 1);
+            const uint32_t par = ((n / NU) & 1) ^ 1;
+            // A full ring: hand over what is on its way while waiting, the consumers may need it to go on.
+            auto vacant = [&]() { return __all_sync(0xffffffffu, mbar_test(&empty[slot], par)); };
+            if (!vacant() && !flush(n, vacant)) wait_warp(&empty[slot], par);
             if (col_live) {
                 const uint32_t dst = ring + slot * Cfg::unit_b + col_at;
                 constexpr int kBatch = 8;   // offsets of a batch of rows first: a copy is a barrier to the compiler's loads
@@ -361,7 +431,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             cp_async_commit();
             hist = (hist << 1) | (check ? 1u : 0u);
             cp_async_wait<LAG>();
-            if (n >= LAG) arrive(n - LAG, (hist >> LAG) & 1);
+            if (arrived <= n - LAG) arrive(arrived++, (hist >> LAG) & 1);
         };
         // element offset of key `pt` of the cursor's tile (-1: past the end, or not a page of this cache)
         auto offset_of = [&](const Cursor& c) -> int64_t {
@@ -372,47 +442,52 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             if ((unsigned)id >= (unsigned)p.num_pages) return -1;
             return id * p.stride_page + (pos - pg * p.page_size) * p.stride_slot + c.h * p.stride_head;
         };
-        int64_t next_off = offset_of(cur);
-        bool tail = false, tail_before = false;
+        // offsets are looked up two tiles ahead (a length, then a table entry: two trips to L2 where a request begins)
+        auto reaches_new = [](const Cursor& c) { return c.kt * KT + KT > c.r.seq - c.r.n; };
+        int64_t off[2] = {offset_of(cur), -1};
+        bool tail[2] = {reaches_new(cur), false}, tail_before = false;
+        auto look_ahead = [&](int tile) {
+            if (tile >= count) return;
+            cur.next(p);
+            off[1] = offset_of(cur);
+            tail[1] = reaches_new(cur);
+        };
+        look_ahead(1);
         int n = 0;
         for (int step = 0; step <= count; ++step) {
             if (step < count) {
-                key_off[(step & 3) * KT + pt] = next_off;
-                tail_before = tail;
-                tail = cur.kt * KT + KT > cur.r.seq - cur.r.n;
-                if (step + 1 < count) {
-                    cur.next(p);
-                    next_off = offset_of(cur);
-                }
+                key_off[(step & 3) * KT + pt] = off[0];
                 named_bar_sync(3, 128);
                 issue(n++, p.k_cache, key_off + (step & 3) * KT, false);
-            } else {
-                tail_before = tail;
             }
             if (step > 0) issue(n++, p.v_cache, key_off + ((step - 1) & 3) * KT, tail_before);
+            tail_before = tail[0];
+            off[0] = off[1];
+            tail[0] = tail[1];
+            look_ahead(step + 2);
         }
-        cp_async_wait<0>();
-        for (int u = max(n - LAG, 0); u < n; ++u) arrive(u, (hist >> (n - 1 - u)) & 1);
-    } else if (warp == Cfg::w_q) {
-        // ---------------------------------- Q loader ----------------------------------
-        const int chunk = lane % CPR;
-        constexpr int kRowStep = 32 / CPR;
+        flush(n, [] { return false; });
+    } else if (warp < Cfg::w_s && warp >= Cfg::w_q) {
+        // ---------------------------------- Q loaders ----------------------------------
+        const int ql = tid - Cfg::w_q * 32, chunk = ql % CPR;
+        constexpr int kRowStep = 64 / CPR;
+        const uint32_t dst = smem_addr(sq) + (chunk >> 3) * Cfg::block_b;
         int seg = 0;
         for (int it = 0; it < count; ++it) {
             if (it == 0 || cur.kt == 0) {
                 wait_warp(q_free, (seg & 1) ^ 1);
+                // rows of no token stay what they are: nothing of them is read
                 const int rows = min(RT, cur.r.n * p.group - cur.rt * RT);
                 if (chunk * 8 < p.head_dim) {
+                    const T* base = static_cast<const T*>(p.q) + (int64_t)cur.r.q0 * p.q_stride_token +
+                                    (int64_t)(cur.h * p.group) * p.q_stride_head + chunk * 8;
 #pragma unroll 4
-                    for (int r = lane / CPR; r < MT * 128; r += kRowStep) {
-                        const int row = r % RT;
-                        if (row >= rows) continue;   // rows of no token: whatever lies there, nothing of it is read
+                    for (int row = ql / CPR; row < rows; row += kRowStep) {
                         const int at = cur.rt * RT + row, i = p.group_div.div(at), g = at - i * p.group;
-                        const T* src = static_cast<const T*>(p.q) + (int64_t)(cur.r.q0 + i) * p.q_stride_token +
-                                       (int64_t)(cur.h * p.group + g) * p.q_stride_head + chunk * 8;
-                        cp_async16(smem_addr(sq) + (r >> 7) * Cfg::unit_b + (chunk >> 3) * Cfg::block_b + (r & 127) * 128 +
-                                       (((chunk & 7) ^ (r & 7)) << 4),
-                                   src, true);
+                        const T* src = base + i * p.q_stride_token + g * p.q_stride_head;
+#pragma unroll
+                        for (int r = row; r < MT * 128; r += RT)
+                            cp_async16(dst + (r >> 7) * Cfg::unit_b + (r & 127) * 128 + (((chunk & 7) ^ (r & 7)) << 4), src, true);
                     }
                 }
                 cp_async_commit();
@@ -436,7 +511,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             int freed = 0;                   // tiles whose values' slot has been handed back
             for (int i = 0; i < count && ok; ++i, cur.next(p)) {
                 const int rows = min(RT, cur.r.n * p.group - cur.rt * RT), tiles = MT == 2 && rows > 128 ? 2 : 1;
-                if (i == 0 || cur.kt == 0) ok = wait(q_full, seg++ & 1);
+                const bool fresh = i == 0 || cur.kt == 0;
                 const int n = k_pos(i);
                 for (int t = 0; t < tiles && ok; ++t) {
                     const int buf = MT == 1 ? i & 1 : t;
@@ -446,6 +521,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                         // products of tiles before i (two row tiles) or i - 1 have ended: their values' slots are free
                         for (; freed < (MT == 1 ? i - 1 : i); ++freed) mbar_arrive(&empty[v_pos(freed) % NU]);
                     }
+                    if (t == 0 && fresh) ok = ok && wait(q_full, seg++ & 1);
                     if (t == 0) ok = ok && wait(&full[n % NU], (n / NU) & 1);
                     if (!ok) break;
                     tcf_after();
@@ -495,7 +571,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
         __syncwarp();
     } else {
         // ---------------------------------- softmax ----------------------------------
-        constexpr int SPLIT = Cfg::split, HB = Cfg::hold, GT = Cfg::group, SC = Cfg::sc;
+        constexpr int SPLIT = Cfg::split, HB = Cfg::hold, GT = Cfg::group;
         const int t = warp / (4 * SPLIT), half = (warp >> 2) % SPLIT, wq = warp & 3;   // row tile, share, lane quarter
         const int rep = wq / (4 / REP), tw = wq % (4 / REP);          // repeat, 32-row group
         const int kq = rep * (KT / REP) + half * KW;                  // first key of this thread's share of a tile
@@ -513,22 +589,44 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             tc_wait_st();
         }
         float m = -INFINITY, l = 0.0f;
-        int done = 0;   // tiles of this row tile
-        for (int it = 0; it < count; ++it, cur.next(p)) {
-            const int rows = min(RT, cur.r.n * p.group - cur.rt * RT);
+        // What changes only with the segment lies in shared memory, one copy per warp: registers are short here, and
+        // spilled ones cost a trip to L2 each (the ring leaves no L1).
+        SegState* const seg = s_seg + warp;
+        seg->c = cur;
+        seg->v_seg = v0 - s_first[2];
+        __syncwarp();
+        int kt = cur.kt, nkt = cur.nkt, kt_first = kt;
+        int rows = min(RT, cur.r.n * p.group - cur.rt * RT);
+        int ctx = cur.r.seq - cur.r.n;   // negative for a refused request (no keys)
+        int done = 0;                    // tiles of this row tile
+        for (int it = 0; it < count; ++it) {
+            if (it > 0 && ++kt == nkt) {
+                __syncwarp();
+                Cursor c = seg->c;
+                c.kt = nkt - 1;
+                c.next(p);
+                seg->c = c;
+                seg->v_seg += nkt + Cfg::extra;
+                __syncwarp();
+                kt = kt_first = 0;
+                nkt = c.nkt;
+                rows = min(RT, c.r.n * p.group - c.rt * RT);
+                ctx = c.r.seq - c.r.n;
+            }
             if (MT == 2 && t == 1 && rows <= 128) continue;
             const int buf = MT == 1 ? it & 1 : t;
             const uint32_t par = (MT == 1 ? it >> 1 : done) & 1;   // of every barrier of this buffer
-            const bool last = cur.kt == cur.nkt - 1 || it == count - 1;
+            const bool last = kt == nkt - 1 || it == count - 1;
             const bool live = t * 128 + tw * 32 < rows;
-            const bool first = it == 0 || cur.kt == 0;
+            const bool first = kt == kt_first;
             if (first) m = -INFINITY, l = 0.0f;
-            const int pos0 = cur.kt * KT, ctx = cur.r.seq - cur.r.n;
+            const int pos0 = kt * KT;
             const bool tail = pos0 + KT > ctx;
             static_assert(KW <= 64, "one mask window per thread");
             uint64_t win = 0;
-            const int tok = p.group_div.div(min(cur.rt * RT + row, cur.r.n * p.group - 1));   // this row's new token
-            if (tail && cur.r.seq > 0) win = seen_window(p, cur.r, tok, pos0 + kq - ctx);
+            // this row's new token
+            auto token = [&]() { return p.group_div.div(min(seg->c.rt * RT + row, seg->c.r.n * p.group - 1)); };
+            if (tail && seg->c.r.seq > 0) win = seen_window(p, seg->c.r, token(), pos0 + kq - ctx);
             wait_warp(&s_full[buf], par);
             tcf_after();
             if (wq == 0 && half == 0 && lane == 0 && (MT == 1 || t == 1 || rows <= 128)) {   // the tile's S products have all ended
@@ -611,18 +709,18 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                 for (int c = 0; c < KW / HB; ++c) {
                     if (HB < KW) load(c, v);
 #pragma unroll
-                    for (int c16 = 0; c16 < HB / 32; ++c16) {
-                        uint32_t u[16];
+                    for (int x0 = 0; x0 < HB; x0 += 16) {
+                        uint32_t u[8];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int x = c16 * 32 + 2 * j;
+                        for (int j = 0; j < 8; ++j) {
+                            const int x = x0 + 2 * j;
                             float a, b;
                             unpair(fma_pair(pair(v[x], v[x + 1]), f2, base2), a, b);
                             a = exp2_fast(a), b = exp2_fast(b);
                             sum[j & 1] = add_pair(sum[j & 1], pair(a, b));
                             u[j] = pack2<T>(a, b);
                         }
-                        tc_st16(p_at + c * (HB / 2) + c16 * 16, u);
+                        tc_st8(p_at + c * (HB / 2) + x0 / 2, u);
                     }
                 }
                 float s0, s1, s2, s3;
@@ -650,24 +748,25 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                     named_bar_sync(bar_pair, 64);
                     tcf_after();
                 }
-                const int x0 = rep * (KT / REP);
-                for (int x = max(ctx - pos0, x0); x < min(cur.r.seq - pos0, x0 + KT / REP); ++x) {
+                const Cursor c = seg->c;
+                const int x0 = rep * (KT / REP), tok = token();
+                for (int x = max(ctx - pos0, x0); x < min(c.r.seq - pos0, x0 + KT / REP); ++x) {
                     const int pos = pos0 + x, pg = p.page_div.div(pos);
-                    const int id = p.block_table[(int64_t)cur.b * p.table_stride + pg];
+                    const int id = p.block_table[(int64_t)c.b * p.table_stride + pg];
                     if ((unsigned)id >= (unsigned)p.num_pages) continue;
                     const T* src = static_cast<const T*>(p.v_cache) + id * p.stride_page + (pos - pg * p.page_size) * p.stride_slot +
-                                   cur.h * p.stride_head;
+                                   c.h * p.stride_head;
                     __syncwarp();
                     const float2 pp = unpack2<T>(tc_ld1(lanes + Cfg::p_col(buf, x)));
                     const bool zero = (x & 1 ? pp.y : pp.x) == 0.0f;
-                    if (!(seen_window(p, cur.r, tok, pos - ctx) & 1)) continue;
+                    if (!(seen_window(p, c.r, tok, pos - ctx) & 1)) continue;
 #pragma unroll
                     for (int k = 0; k < kFix; ++k) {
-                        const int c = k * SPLIT + half;
+                        const int col = (k * SPLIT + half) * 16;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            if (c * 16 + 2 * j >= p.head_dim) break;
-                            const uint32_t raw = reinterpret_cast<const uint32_t*>(src)[c * 8 + j];
+                            if (col + 2 * j >= p.head_dim) break;
+                            const uint32_t raw = reinterpret_cast<const uint32_t*>(src)[col / 2 + j];
                             if (raw == finite2<T>(raw)) continue;
                             const float2 v = unpack2<T>(raw);
                             if (!(fabsf(v.x) < INFINITY)) flags[k] |= (v.x < 0 && !zero ? 0u : 1u << (2 * j)) | (v.x > 0 && !zero ? 0u : 0x10000u << (2 * j));
@@ -726,62 +825,72 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                 }
                 scale_o = exp2_fast(m - safe);
             }
-            const int64_t seg0 = u0 + it - cur.kt, seg1 = seg0 + cur.nkt;
-            const bool whole = seg0 >= u0 && seg1 <= u0 + count;
+            const Cursor c = seg->c;
+            const bool whole = kt_first == 0 && kt == nkt - 1;
             if (whole) scale_o = ll == 0.0f ? 0.0f : scale_o / ll;
-            const int slot = 2 * blockIdx.x + (seg0 < u0 ? 0 : 1);
+            const int slot = 2 * blockIdx.x + (kt_first > 0 ? 0 : 1);   // a part: its segment began in an earlier run, or not
             float* part = p.part_o + (int64_t)slot * RT * DT;
             auto out_ptr = [&](int r, int d) {
-                const int at = cur.rt * RT + r, i = p.group_div.div(at), g = at - i * p.group;
-                return static_cast<T*>(p.out) + (int64_t)(cur.r.q0 + i) * p.out_stride_token +
-                       (int64_t)(cur.h * p.group + g) * p.out_stride_head + d;
+                const int at = c.rt * RT + r, i = p.group_div.div(at), g = at - i * p.group;
+                return static_cast<T*>(p.out) + (int64_t)(c.r.q0 + i) * p.out_stride_token +
+                       (int64_t)(c.h * p.group + g) * p.out_stride_head + d;
             };
             auto put_lse = [&](int r, float top, float sum) {
-                const int at = cur.rt * RT + r, i = p.group_div.div(at), g = at - i * p.group;
-                p.lse[(int64_t)(cur.r.q0 + i) * p.q_heads + cur.h * p.group + g] =
+                const int at = c.rt * RT + r, i = p.group_div.div(at), g = at - i * p.group;
+                p.lse[(int64_t)(c.r.q0 + i) * p.q_heads + c.h * p.group + g] =
                     sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
             };
-            auto put2 = [&](int r, int d, float a, float b) {   // two neighbouring columns of row r (of the row tile)
+            // 32 columns at a time, the row's two threads half the columns each. A thread's columns of a row are whole
+            // 16-byte pieces, so they go out from its registers.
+            T* out_row = row < rows ? out_ptr(row, 0) : nullptr;
+            float* part_row = part + (int64_t)row * DT;
+            auto put8 = [&](int d, const float* v) {
+                if (row >= rows || d >= p.head_dim) return;
                 if (whole) {
-                    if (d < p.head_dim) *reinterpret_cast<uint32_t*>(out_ptr(r, d)) = pack2<T>(a, b);
+                    *reinterpret_cast<uint4*>(out_row + d) =
+                        make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
                 } else {
-                    *reinterpret_cast<float2*>(part + (int64_t)r * DT + d) = make_float2(a, b);
+                    *reinterpret_cast<float4*>(part_row + d) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4*>(part_row + d + 4) = make_float4(v[4], v[5], v[6], v[7]);
                 }
             };
-            float* mine = stage + warp * 32 * (SC + 1);
 #pragma unroll 1
-            for (int c = half; c < ksteps; c += SPLIT) {   // 16 columns a turn, the row's threads in turn
-                float o[16];
+            for (int col = half * (DT / SPLIT); col < (half + 1) * (DT / SPLIT); col += 32) {
+                float o[32];
                 __syncwarp();
-                tc_ld16(lanes + Cfg::o_col(t) + c * 16, o);
+                tc_ld<32>(lanes + Cfg::o_col(t) + col, o);   // columns past the head size hold anything: not put out
 #pragma unroll
-                for (int part16 = 0; part16 < 16; part16 += SC) {
+                for (int j = 0; j < 32; ++j) o[j] = scale_o == 0.0f ? 0.0f : o[j] * scale_o;
+                if (REP == 1) {
 #pragma unroll
-                    for (int j = 0; j < SC; ++j) mine[lane * (SC + 1) + j] = scale_o == 0.0f ? 0.0f : o[part16 + j] * scale_o;
-                    constexpr int kPairs = SC / 2;
-                    if (REP == 1) {
-                        __syncwarp();
+                    for (int j = 0; j < 32; j += 8) put8(col + j, o + j);
+                } else {
+                    // each repeat sums and puts out its own `own` of the 32 columns: [warp][other repeat][column][lane]
+                    constexpr int OWN = Cfg::own, NX = REP - 1;
+                    float sum[OWN];
 #pragma unroll
-                        for (int e = 0; e < kPairs; ++e) {
-                            const int r = e * (32 / kPairs) + lane / kPairs, j = (lane % kPairs) * 2;
-                            if (t * 128 + wq * 32 + r < rows)
-                                put2(t * 128 + wq * 32 + r, c * 16 + part16 + j, mine[r * (SC + 1) + j], mine[r * (SC + 1) + j + 1]);
+                    for (int q = 0; q < REP; ++q) {
+                        if (q == rep) {
+#pragma unroll
+                            for (int j = 0; j < OWN; ++j) sum[j] = o[q * OWN + j];
+                        } else {
+                            float* to = stage + ((warp * NX + (q - rep - 1 + REP) % REP) * OWN) * 32 + lane;
+#pragma unroll
+                            for (int j = 0; j < OWN; ++j) to[j * 32] = o[q * OWN + j];
                         }
-                        __syncwarp();
-                    } else {
-                        named_bar_sync(bar_half, 128);
-                        for (int e = wq * 32 + lane; e < rows * kPairs; e += 128) {
-                            const int r = e / kPairs, j = (e % kPairs) * 2;
-                            float a = 0.0f, b = 0.0f;
-#pragma unroll
-                            for (int q = 0; q < REP; ++q) {
-                                const float* s = stage + (half * 128 + q * RT + r) * (SC + 1) + j;
-                                a += s[0], b += s[1];
-                            }
-                            put2(r, c * 16 + part16 + j, a, b);
-                        }
-                        named_bar_sync(bar_half, 128);
                     }
+                    named_bar_sync(bar_half, 128);
+#pragma unroll
+                    for (int q = 0; q < REP; ++q) {
+                        if (q == rep) continue;
+                        const int from = half * 4 + q * (4 / REP) + tw;
+                        const float* src = stage + ((from * NX + (rep - q - 1 + REP) % REP) * OWN) * 32 + lane;
+#pragma unroll
+                        for (int j = 0; j < OWN; ++j) sum[j] += src[j * 32];
+                    }
+#pragma unroll
+                    for (int j = 0; j < OWN; j += 8) put8(col + rep * OWN + j, sum + j);
+                    named_bar_sync(bar_half, 128);
                 }
             }
             const bool owner = half == 0 && rep == 0 && row < rows;   // one thread per row
@@ -792,36 +901,40 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                 continue;
             }
             if (owner) p.part_ml[(int64_t)slot * RT + row] = make_float2(mm, ll);
-            const int fc = (int)(seg0 / run), lc = (int)((seg1 - 1) / run);
+            const int64_t v_seg = seg->v_seg;
+            const int fc = (int)((v_seg + Cfg::extra) / run), lc = (int)((v_seg + nkt + Cfg::extra - 1) / run);   // runs with tiles of it
             int* counter = p.counters + 2 * fc + t;
-            __threadfence();
             named_bar_sync(bar_group, GT);
-            if (gtid == 0) s_last[t] = atomicAdd(counter, 1) == lc - fc;
+            if (gtid == 0) {
+                __threadfence();   // the group's stores, ordered before this thread by the barrier
+                const bool all_in = atomicAdd(counter, 1) == lc - fc;
+                if (all_in) __threadfence();
+                s_last[t] = all_in;
+            }
             named_bar_sync(bar_group, GT);
             if (*reinterpret_cast<volatile int*>(s_last + t)) {
-                __threadfence();
                 // join: a thread takes 16 columns of a row (four 16-byte pieces, neighbours interleaved), the row's maxima
                 // and sums first, then the parts' values, 16 loads in flight
                 constexpr int kCols = DT / 16;
                 const int r0 = t * 128, items = (min(rows, r0 + 128) - r0) * kCols;
                 for (int e = gtid; e < items; e += GT) {
                     const int r = r0 + e / kCols, d0 = (e % kCols) * 4;
-                    auto at = [&](int c) { return (int64_t)(2 * c + (c == fc ? 1 : 0)) * RT + r; };
+                    auto at = [&](int q) { return (int64_t)(2 * q + (q == fc ? 1 : 0)) * RT + r; };
                     float top = -INFINITY, sum = 0.0f;
 #pragma unroll 8
-                    for (int c = fc; c <= lc; ++c) top = fmaxf(top, __ldcg(&p.part_ml[at(c)].x));
+                    for (int q = fc; q <= lc; ++q) top = fmaxf(top, __ldcg(&p.part_ml[at(q)].x));
                     const float safe = top == -INFINITY ? 0.0f : top;
                     float4 acc[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) acc[k] = make_float4(0, 0, 0, 0);
 #pragma unroll 4
-                    for (int c = fc; c <= lc; ++c) {
-                        const float2 v = __ldcg(p.part_ml + at(c));
+                    for (int q = fc; q <= lc; ++q) {
+                        const float2 v = __ldcg(p.part_ml + at(q));
                         const float w = exp2_fast(v.x - safe);
                         sum += v.y * w;
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const float4 po = __ldcg(reinterpret_cast<const float4*>(p.part_o + at(c) * DT + d0 + k * (DT / 4)));
+                            const float4 po = __ldcg(reinterpret_cast<const float4*>(p.part_o + at(q) * DT + d0 + k * (DT / 4)));
                             acc[k].x += po.x * w;
                             acc[k].y += po.y * w;
                             acc[k].z += po.z * w;
