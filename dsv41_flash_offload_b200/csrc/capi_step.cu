@@ -29,6 +29,7 @@ static int check_weight(const dsv41_w4_weight* w, const char* name)
     if (w->n <= 0 || w->k <= 0) return set_error(DSV41_E_INVALID, "%s weight n=%d k=%d", name, w->n, w->k);
     if (w->group != 32 && w->group != 64 && w->group != 128)
         return set_error(DSV41_E_INVALID, "%s weight group %d (32, 64 or 128)", name, w->group);
+    if ((int64_t)(w->n / 16 + 1) * (w->k / 128 + 1) > 0x7fffffffll) return set_error(DSV41_E_INVALID, "%s weight n=%d k=%d is too large", name, w->n, w->k);
     if (w->k % w->group) return set_error(DSV41_E_INVALID, "%s weight k=%d is not a multiple of its group %d", name, w->k, w->group);
     if (w->scale_dtype != DSV41_DTYPE_F16 && w->scale_dtype != DSV41_DTYPE_BF16)
         return set_error(DSV41_E_INVALID, "%s weight scales must be fp16 or bf16", name);
@@ -54,8 +55,9 @@ static int w4_run(const dsv41_w4_weight* a, const dsv41_w4_weight* b, const void
     if (rc) return rc;
     if (b) {
         if ((rc = check_weight(b, "up"))) return rc;
-        if (b->n != a->n || b->k != a->k || b->group != a->group || b->scale_dtype != a->scale_dtype)
-            return set_error(DSV41_E_INVALID, "gate and up differ in size, group or scale type");
+        if (b->n != a->n || b->k != a->k || b->group != a->group || b->scale_dtype != a->scale_dtype ||
+            !b->has_zeros != !a->has_zeros)
+            return set_error(DSV41_E_INVALID, "gate and up differ in size, group, zero points or scale type");
     }
     if (x_dtype != DSV41_DTYPE_F16 && x_dtype != DSV41_DTYPE_BF16)
         return set_error(DSV41_E_INVALID, "x dtype %d (fp16 or bf16)", x_dtype);
@@ -81,8 +83,7 @@ static int w4_run(const dsv41_w4_weight* a, const dsv41_w4_weight* b, const void
     p.n = a->n;
     p.k = a->k;
     p.n16 = l.n16;
-    p.k64 = l.k64;
-    p.groups = l.groups;
+    p.k128 = l.k128;
     p.scale_bf16 = a->scale_dtype == DSV41_DTYPE_BF16;
     p.out_dtype = out_dtype;
     p.accumulate = accumulate;
