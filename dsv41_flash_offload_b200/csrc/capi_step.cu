@@ -257,7 +257,9 @@ int dsv41_tree_attention(const dsv41_tree_attention_args* a, void* workspace, si
     p.mask_words = a->mask_words;
     p.page_div = FastDiv::make(a->page_size);
     p.group_div = FastDiv::make(p.group);
-    p.scale_log2 = a->scale * 1.4426950408889634f;
+    // a scale of 0 (every key counts alike) becomes one that no score survives
+    p.scale_log2 = std::fmax(std::fabs(a->scale) * 1.4426950408889634f, 1e-37f);
+    p.flip = a->scale < 0.0f;
     const int64_t rows = (int64_t)(a->max_new ? a->max_new : 1) * p.group;
     return launched(launch_tree_attn(p, a->dtype, (int)(rows > 1024 ? 1024 : rows), static_cast<cudaStream_t>(stream)),
                     "tree attention");

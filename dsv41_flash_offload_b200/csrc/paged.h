@@ -70,7 +70,8 @@ struct TreeAttnParams {
     int* status;
     int batch, num_tokens, q_heads, kv_heads, group, head_dim, page_size, num_pages, max_keys, mask_words;
     FastDiv page_div, group_div;
-    float scale_log2;                                  // scale * log2(e)
+    float scale_log2;                                  // |scale| * log2(e), not 0 (inf * 0 is NaN)
+    int flip;                                          // the scale is negative
 };
 
 struct AttnWorkspace {   // the status word lies at 0

@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<DT, WM>::per_sm) tree_at
         cp_async_commit();
     }
 
+    const float scale = p.flip ? -p.scale_log2 : p.scale_log2;
     uint32_t qf[DT / 16][4];
     float o[NT][4];
     float m[2], l[2];
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<DT, WM>::per_sm) tree_at
         for (int j = 0; j < TN / 8; ++j) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float t = s[j][e] * p.scale_log2;
+                float t = s[j][e] * scale;
                 if (tail && !((win[e >> 1] >> (wk * TN + j * 8 + col0 + (e & 1))) & 1)) t = -INFINITY;
                 s[j][e] = t;
                 mx[e >> 1] = fmaxf(mx[e >> 1], t);

@@ -164,12 +164,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ float min3(float a, float b, float c)
-{
-    float r;
-    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
 __device__ __forceinline__ void tc_ld16(uint32_t taddr, float* v)
 {
     uint32_t r[16];
@@ -600,7 +594,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
         int ctx = cur.r.seq - cur.r.n;   // negative for a refused request (no keys)
         int done = 0;                    // tiles of this row tile
         for (int it = 0; it < count; ++it) {
-            if (it > 0 && ++kt == nkt) {
+            if (__builtin_expect(it > 0 && ++kt == nkt, 0)) {
                 __syncwarp();
                 Cursor c = seg->c;
                 c.kt = nkt - 1;
@@ -636,43 +630,41 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             __syncwarp();
             if (live) {
                 const uint32_t s_at = lanes + Cfg::s_col(buf) + kq, p_at = lanes + Cfg::p_col(buf, kq);
-                const float f = tail ? 1.0f : p.scale_log2;   // in tail tiles the scores come scaled and masked
-                auto load = [&](int c, float* v) {      // HB scores from the c-th such run on
-                    tc_ld<HB>(s_at + c * HB, v);
-                    if (tail) {
+                // Tiles that reach the new tokens: keys that the row does not see become -inf in place, before the common
+                // path below (a negative scale is turned around there too, so that a maximum stays a maximum).
+                if (__builtin_expect(tail || p.flip, 0)) {
+#pragma unroll 1
+                    for (int c = 0; c < KW; c += 16) {
+                        float w[16];
+                        uint32_t u[16];
+                        tc_ld16(s_at + c, w);
 #pragma unroll
-                        for (int j = 0; j < HB; ++j) {
-                            const int x = c * HB + j;
-                            v[j] = ((uint32_t)(win >> (x & 32)) >> (x & 31)) & 1 ? v[j] * p.scale_log2 : -INFINITY;
+                        for (int j = 0; j < 16; ++j) {
+                            const bool see = !tail || ((win >> (c + j)) & 1);
+                            u[j] = __float_as_uint(see ? (p.flip ? -w[j] : w[j]) : -INFINITY);
                         }
+                        tc_st16(s_at + c, u);
                     }
-                };
+                    tc_wait_st();
+                }
+                const float f = p.scale_log2;
                 float v[HB];
                 float mt = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < KW / HB; ++c) {
-                    load(c, v);
+                for (int c = 0; c < KW; c += HB) {
+                    tc_ld<HB>(s_at + c, v);
                     float a[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) a[j] = v[j];
-                    if (f >= 0.0f) {
 #pragma unroll
-                        for (int j = 4; j + 8 <= HB; j += 8)
+                    for (int j = 4; j + 8 <= HB; j += 8)
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) a[q] = max3(a[q], v[j + 2 * q], v[j + 2 * q + 1]);
+                        for (int q = 0; q < 4; ++q) a[q] = max3(a[q], v[j + 2 * q], v[j + 2 * q + 1]);
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) a[q] = fmaxf(a[q], v[HB - 4 + q]);
-                        mt = fmaxf(mt, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * f);
-                    } else {
-#pragma unroll
-                        for (int j = 4; j + 8 <= HB; j += 8)
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) a[q] = min3(a[q], v[j + 2 * q], v[j + 2 * q + 1]);
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) a[q] = fminf(a[q], v[HB - 4 + q]);
-                        mt = fmaxf(mt, fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) * f);
-                    }
+                    for (int q = 0; q < 4; ++q) a[q] = fmaxf(a[q], v[HB - 4 + q]);
+                    mt = fmaxf(mt, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
                 }
+                mt *= f;
                 if (SPLIT == 2) {   // the row's other thread
                     float* at = mx + ((t * 2 + (done & 1)) * 2 + half) * 128 + wq * 32 + lane;
                     *at = mt;
@@ -683,7 +675,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                     m = mt;
                 } else {
                     const bool grow = mt > m + 8.0f || (m == -INFINITY && mt > m);
-                    if (__any_sync(0xffffffffu, grow)) {
+                    if (__builtin_expect(__any_sync(0xffffffffu, grow), 0)) {
                         const float alpha = grow ? exp2_fast(m - mt) : 1.0f;
                         if (grow) m = mt;
                         l *= alpha;
@@ -706,8 +698,8 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                 const uint64_t f2 = pair(f, f), base2 = pair(-base, -base);
                 uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                for (int c = 0; c < KW / HB; ++c) {
-                    if (HB < KW) load(c, v);
+                for (int c = 0; c < KW; c += HB) {
+                    if (HB < KW) tc_ld<HB>(s_at + c, v);
 #pragma unroll
                     for (int x0 = 0; x0 < HB; x0 += 16) {
                         uint32_t u[8];
@@ -720,7 +712,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                             sum[j & 1] = add_pair(sum[j & 1], pair(a, b));
                             u[j] = pack2<T>(a, b);
                         }
-                        tc_st8(p_at + c * (HB / 2) + x0 / 2, u);
+                        tc_st8(p_at + (c + x0) / 2, u);
                     }
                 }
                 float s0, s1, s2, s3;
@@ -730,7 +722,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                 tc_wait_st();
             }
             bool fix = false;
-            if (tail) {
+            if (__builtin_expect(tail, 0)) {
                 const int n = v_pos(it);
                 wait_warp(&full[n % NU], (n / NU) & 1);
                 fix = live && *reinterpret_cast<volatile int*>(dirty + n % NU) == n + 1;
@@ -742,7 +734,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             uint32_t flags[kFix];   // of this thread's 16-column chunks: low half +inf, high half -inf
 #pragma unroll
             for (int k = 0; k < kFix; ++k) flags[k] = 0;
-            if (fix) {
+            if (__builtin_expect(fix, 0)) {
                 if (SPLIT == 2) {   // this thread's columns need P of all the row's keys
                     tcf_before();
                     named_bar_sync(bar_pair, 64);
@@ -780,7 +772,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[buf]);
             __syncwarp();
-            if (fix) {
+            if (__builtin_expect(fix, 0)) {
                 wait_warp(&pv_done[buf], par);
                 tcf_after();
 #pragma unroll
@@ -802,7 +794,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                 tcf_before();
             }
             ++done;
-            if (!last) continue;
+            if (__builtin_expect(!last, 1)) continue;
 
             // ---- end of the segment, or of this CTA's run ----
             wait_warp(&pv_done[buf], par);
