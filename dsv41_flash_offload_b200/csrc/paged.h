@@ -70,6 +70,7 @@ struct TreeAttnParams {
     int* status;
     int batch, num_tokens, q_heads, kv_heads, group, head_dim, page_size, num_pages, max_keys, mask_words;
     FastDiv page_div, group_div;
+    int box, slot_first;                               // tensor copies: tokens, and whether slots lie within heads (set by the launch)
     float scale_log2;                                  // |scale| * log2(e), not 0 (inf * 0 is NaN)
     int flip;                                          // the scale is negative
 };

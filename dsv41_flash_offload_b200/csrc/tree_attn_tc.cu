@@ -23,6 +23,9 @@
 // The accumulator is rescaled only when a row's maximum grows by more than 2^8: P stays below 2^8, its rounding
 // is relative, and the sums are fp32, so the deferral costs no accuracy; a rescale has to wait for the product
 // in flight, the deferral makes that rare.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "internal.h"
 #include "tree_attn.cuh"
 
@@ -32,9 +35,9 @@ namespace dsv41 {
 #define DSV41_ATTN_EXTRA 2
 #endif
 #ifndef DSV41_ATTN_EXTRA2
-#define DSV41_ATTN_EXTRA2 1
+#define DSV41_ATTN_EXTRA2 2
 #endif
-template <int DT, int MT, int REP>
+template <int DT, int MT, int REP, bool TMA>
 struct TcCfg {
     static_assert(MT == 1 || REP == 1, "repeats are for a single tile of 128 rows");
     static constexpr int kt = 128;                           // keys per tile
@@ -44,7 +47,8 @@ struct TcCfg {
     static constexpr int hold = MT == 2 ? 32 : kw;           // scores a thread holds at a time (registers)
     static constexpr int group = 128 * split;                // softmax threads per 128 rows
     static constexpr int soft_warps = 4 * split * MT;
-    static constexpr int w_prod = soft_warps, w_q = w_prod + 4, w_s = w_q + 2, w_o = w_s + 1;
+    static constexpr int prod_warps = TMA ? 1 : 4, q_warps = TMA && MT == 2 ? 1 : 2;
+    static constexpr int w_prod = soft_warps, w_q = w_prod + prod_warps, w_s = w_q + q_warps, w_o = w_s + 1;
     static constexpr int threads = (w_o + 1) * 32;
     static constexpr int block_b = 128 * 128;                // 128 rows x 64 columns of 16 bits, swizzled
     static constexpr int blocks = DT / 64;
@@ -199,10 +203,156 @@ __device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t* r)
                  : "memory");
 }
 
-template <typename T, int DT, int MT, int REP>
-__global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_kernel(const TreeAttnParams p)
+// The paths that few tiles take are functions of their own: inlined, they crowd the common path out of the
+// instruction cache.
+
+// Infinities and NaN among new tokens' values would reach rows that do not see them (0 * NaN): zero those of this
+// thread's pieces of a tile and say whether there were any; the softmax warps add them to the rows that do see them.
+// A first look only: a half-word's exponent bits, turned, are zero in a value that is not finite, and the minimum over
+// all words finds one.
+template <typename T, int ROWS>
+__device__ __noinline__ bool clear_nonfinite(unsigned char* base, int row0, int step, int chunk)
 {
-    using Cfg = TcCfg<DT, MT, REP>;
+    constexpr uint32_t kExp = exp_bits<T>() * 0x10001u;
+    auto piece = [&](int i) {
+        const int row = row0 + i * step;
+        return reinterpret_cast<uint4*>(base + row * 128 + ((chunk ^ (row & 7)) << 4));
+    };
+    uint32_t least = 0xffffffffu;
+#pragma unroll 8
+    for (int i = 0; i < ROWS; ++i) {
+        const uint4 v = *piece(i);
+        least = __vminu2(least, __vminu2(__vminu2((v.x & kExp) ^ kExp, (v.y & kExp) ^ kExp), __vminu2((v.z & kExp) ^ kExp, (v.w & kExp) ^ kExp)));
+    }
+    if ((least & 0xffffu) != 0 && (least >> 16) != 0) return false;
+#pragma unroll 1
+    for (int i = 0; i < ROWS; ++i) {
+        uint4 v = *piece(i);
+        v.x = finite2<T>(v.x), v.y = finite2<T>(v.y), v.z = finite2<T>(v.z), v.w = finite2<T>(v.w);
+        *piece(i) = v;
+    }
+    return true;
+}
+
+// The same for a tile of whole pages, by `threads` threads together, before its product: values past the last key
+// (rows from `rows` on, which may hold anything) are cleared too, without a mark. The mark is set before a value is
+// cleared: who finds it cleared (another group of threads looks at the same tile) finds the mark.
+template <typename T, int N>
+__device__ __noinline__ void clear_tile(unsigned char* unit, int thread, int threads, int rows, volatile int* mark, int value)
+{
+    constexpr uint32_t kExp = exp_bits<T>() * 0x10001u;
+    uint32_t least = 0xffffffffu;
+    uint4* at = reinterpret_cast<uint4*>(unit) + thread;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint4 v = at[i * threads];
+        least = __vminu2(least, __vminu2(__vminu2((v.x & kExp) ^ kExp, (v.y & kExp) ^ kExp), __vminu2((v.z & kExp) ^ kExp, (v.w & kExp) ^ kExp)));
+    }
+    if ((least & 0xffffu) == 0 || (least >> 16) == 0) {
+#pragma unroll 1
+        for (int i = 0; i < N; ++i) {
+            uint4 v = at[i * threads];
+            if (!any_nonfinite<T>(v)) continue;
+            if (((thread + i * threads) >> 3) % 128 < rows) *mark = value;   // 128-byte rows, 128 of them a block
+            __threadfence_block();
+            v.x = finite2<T>(v.x), v.y = finite2<T>(v.y), v.z = finite2<T>(v.z), v.w = finite2<T>(v.w);
+            at[i * threads] = v;
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Infinities and NaN of new tokens entered the product as zeros. A row that sees such a value takes p * v, which is
+// +inf, -inf or NaN (also where p is 0): two bits per row and column, +inf and -inf, both for NaN.
+// flags[k]: of columns col0 + k * step .. + 15, low half +inf, high half -inf. Keys x0 .. x1 - 1 of the tile at pos0.
+template <typename T, int NF, typename PCol>
+__device__ __noinline__ void find_nonfinite(const TreeAttnParams& p, const AttnReq& r, int b, int h, int tok, int pos0, int x0,
+                                            int x1, int col0, int step, PCol p_col, uint32_t (&flags)[NF])
+{
+#pragma unroll
+    for (int k = 0; k < NF; ++k) flags[k] = 0;
+    const int ctx = r.seq - r.n;
+#pragma unroll 1
+    for (int x = x0; x < min(r.seq - pos0, x1); ++x) {
+        const int pos = pos0 + x, pg = p.page_div.div(pos);
+        const int id = p.block_table[(int64_t)b * p.table_stride + pg];
+        if ((unsigned)id >= (unsigned)p.num_pages) continue;
+        const T* src = static_cast<const T*>(p.v_cache) + id * p.stride_page + (pos - pg * p.page_size) * p.stride_slot + h * p.stride_head;
+        __syncwarp();
+        const float2 pp = unpack2<T>(tc_ld1(p_col(x)));
+        const bool zero = (x & 1 ? pp.y : pp.x) == 0.0f;
+        if (!(seen_window(p, r, tok, pos - ctx) & 1)) continue;
+#pragma unroll
+        for (int k = 0; k < NF; ++k) {
+            const int col = col0 + k * step;
+#pragma unroll 1
+            for (int j = 0; j < 8; ++j) {
+                if (col + 2 * j >= p.head_dim) break;
+                const uint32_t raw = reinterpret_cast<const uint32_t*>(src)[col / 2 + j];
+                if (raw == finite2<T>(raw)) continue;
+                const float2 v = unpack2<T>(raw);
+                if (!(fabsf(v.x) < INFINITY)) flags[k] |= (v.x < 0 && !zero ? 0u : 1u << (2 * j)) | (v.x > 0 && !zero ? 0u : 0x10000u << (2 * j));
+                if (!(fabsf(v.y) < INFINITY)) flags[k] |= (v.y < 0 && !zero ? 0u : 2u << (2 * j)) | (v.y > 0 && !zero ? 0u : 0x20000u << (2 * j));
+            }
+        }
+    }
+    __syncwarp();
+}
+
+// Join of a segment's parts (runs fc .. lc): a thread takes 16 columns of a row (four 16-byte pieces, neighbours
+// interleaved), the row's maxima and sums first, then the parts' values, 16 loads in flight. Rows r0 .. r0 + rows - 1 of the
+// row tile at c, by `threads` threads.
+template <typename T, int DT, int RT, typename Cursor>
+__device__ __noinline__ void join_parts(const TreeAttnParams& p, const Cursor& c, int fc, int lc, int r0, int rows, int thread,
+                                        int threads)
+{
+    constexpr int kCols = DT / 16;
+    for (int e = thread; e < rows * kCols; e += threads) {
+        const int r = r0 + e / kCols, d0 = (e % kCols) * 4;
+        auto at = [&](int q) { return (int64_t)(2 * q + (q == fc ? 1 : 0)) * RT + r; };
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll 8
+        for (int q = fc; q <= lc; ++q) top = fmaxf(top, __ldcg(&p.part_ml[at(q)].x));
+        const float safe = top == -INFINITY ? 0.0f : top;
+        float4 acc[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+        for (int q = fc; q <= lc; ++q) {
+            const float2 v = __ldcg(p.part_ml + at(q));
+            const float w = exp2_fast(v.x - safe);
+            sum += v.y * w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float4 po = __ldcg(reinterpret_cast<const float4*>(p.part_o + at(q) * DT + d0 + k * (DT / 4)));
+                acc[k].x += po.x * w;
+                acc[k].y += po.y * w;
+                acc[k].z += po.z * w;
+                acc[k].w += po.w * w;
+            }
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int row = c.rt * RT + r, i = p.group_div.div(row), g = row - i * p.group;
+        T* out = static_cast<T*>(p.out) + (int64_t)(c.r.q0 + i) * p.out_stride_token + (int64_t)(c.h * p.group + g) * p.out_stride_head;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int d = d0 + k * (DT / 4);
+            if (d >= p.head_dim) continue;
+            uint32_t* dst = reinterpret_cast<uint32_t*>(out + d);
+            dst[0] = pack2<T>(acc[k].x * inv, acc[k].y * inv);
+            dst[1] = pack2<T>(acc[k].z * inv, acc[k].w * inv);
+        }
+        if (p.lse && d0 == 0)
+            p.lse[(int64_t)(c.r.q0 + i) * p.q_heads + c.h * p.group + g] =
+                sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    }
+}
+
+template <typename T, int DT, int MT, int REP, bool TMA>
+__global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn_tc_kernel(const __grid_constant__ TreeAttnParams p, const __grid_constant__ CUtensorMap tm_k,
+                                                                                      const __grid_constant__ CUtensorMap tm_v)
+{
+    using Cfg = TcCfg<DT, MT, REP, TMA>;
     constexpr int KT = Cfg::kt, RT = Cfg::rt, KW = Cfg::kw, NU = Cfg::units, LAG = Cfg::lag, CPR = DT / 8;
     using Cursor = UnitCursor<RT, KT>;
     extern __shared__ unsigned char smem_raw[];
@@ -231,11 +381,11 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
 
     if (tid == 0) {
         for (int i = 0; i < NU; ++i) {
-            mbar_init(&full[i], 4);
+            mbar_init(&full[i], Cfg::prod_warps);
             mbar_init(&empty[i], 1);
             dirty[i] = 0;
         }
-        mbar_init(q_full, 2);
+        mbar_init(q_full, Cfg::q_warps);
         mbar_init(q_free, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
@@ -349,7 +499,63 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
     auto k_pos = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
     auto v_pos = [&](int i) { return i == count - 1 ? 2 * i + 1 : 2 * i + 2; };
 
-    if (warp >= Cfg::w_prod && warp < Cfg::w_prod + 4) {
+    if (TMA && warp == Cfg::w_prod) {
+        // ---------------------------------- producer, whole pages ----------------------------------
+        // A tile is boxes of `box` tokens (a page, or 128 tokens of a larger one) and 64 columns; lane: one of them.
+        // Boxes past the last key are left out: their keys are masked, their values are cleared by the softmax warps.
+        const int per = KT / p.box, in_tile = lane % per, block = lane / per;
+        const uint32_t dst0 = smem_addr(su) + block * Cfg::block_b + in_tile * p.box * 128;
+        struct Box {
+            int page, slot, head, live;
+        };
+        auto look_up = [&](const Cursor& c) {
+            Box b;
+            const int pos = c.kt * KT + in_tile * p.box, pg = p.page_div.div(pos);
+            b.live = block < Cfg::blocks && pos < c.r.seq;
+            b.page = b.live ? __ldg(p.block_table + (int64_t)c.b * p.table_stride + pg) : 0;
+            b.slot = pos - pg * p.page_size;
+            b.head = c.h;
+            return b;
+        };
+        auto issue = [&](int n, const CUtensorMap* map, const Box& b) {
+            const int slot = n % NU;
+            wait_warp(&empty[slot], ((n / NU) & 1) ^ 1);
+            const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, b.live));
+            if (lane == 0) mbar_arrive_expect_tx(&full[slot], boxes * p.box * 128);
+            __syncwarp();
+            if (b.live && !*abort_flag) {
+                // (a page that is not the cache's lies outside the map: zeros)
+                asm volatile(
+                    "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                        dst0 + slot * Cfg::unit_b),
+                    "l"(reinterpret_cast<uint64_t>(map)), "r"(block * 64), "r"(p.slot_first ? b.slot : b.head), "r"(p.slot_first ? b.head : b.slot), "r"(b.page), "r"(smem_addr(&full[slot]))
+                    : "memory");
+            }
+            __syncwarp();
+        };
+        // pages are looked up two tiles ahead (a length, then a table entry: two trips to L2 where a request begins)
+        Box box[3] = {look_up(cur), Box{}, Box{}};   // this tile, the next, the one before
+        auto look_ahead = [&](int tile) {
+            if (tile >= count) return;
+            cur.next(p);
+            box[1] = look_up(cur);
+        };
+        look_ahead(1);
+        int n = 0;
+        for (int step = 0; step <= count; ++step) {
+            if (step < count) issue(n++, &tm_k, box[0]);
+            if (step > 0) issue(n++, &tm_v, box[2]);
+            box[2] = box[0];
+            box[0] = box[1];
+            look_ahead(step + 2);
+        }
+        // on an abort, let the copies already issued land before the CTA exits
+        for (int u = max(n - NU, 0); u < n && *abort_flag; ++u) {
+            const uint64_t t0 = globaltimer_ns();
+            while (!mbar_try_wait(&full[u % NU], (u / NU) & 1) && globaltimer_ns() - t0 < kWaitLimitNs) {}
+        }
+        __syncwarp();
+    } else if (!TMA && warp >= Cfg::w_prod && warp < Cfg::w_prod + 4) {
         // ---------------------------------- producers ----------------------------------
         const int pt = tid - Cfg::w_prod * 32, chunk = pt % CPR, row0 = pt / CPR;
         constexpr int kRowStep = 128 / CPR;
@@ -360,20 +566,9 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
         uint32_t hist = 0;   // bit k: the unit issued k units ago holds new tokens' values
         auto arrive = [&](int n, bool check) {   // this thread's copies of unit n have landed
             const int slot = n % NU;
-            if (check && col_live) {
-                // infinities and NaN among new tokens' values would reach rows that do not see them (0 * NaN):
-                // zero them here and leave a mark; the softmax warps add them to the rows that do see them
-                bool bad = false;
-                for (int row = row0; row < KT; row += kRowStep) {
-                    uint4* at = reinterpret_cast<uint4*>(su + slot * Cfg::unit_b + col_at + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
-                    uint4 v = *at;
-                    if (any_nonfinite<T>(v)) {
-                        v.x = finite2<T>(v.x), v.y = finite2<T>(v.y), v.z = finite2<T>(v.z), v.w = finite2<T>(v.w);
-                        *at = v;
-                        bad = true;
-                    }
-                }
-                if (bad) *reinterpret_cast<volatile int*>(dirty + slot) = n + 1;
+            if (__builtin_expect(check && col_live, 0)) {
+                if (clear_nonfinite<T, KT / kRowStep>(su + slot * Cfg::unit_b + col_at, row0, kRowStep, chunk & 7))
+                    *reinterpret_cast<volatile int*>(dirty + slot) = n + 1;
             }
             fence_proxy_smem();
             __syncwarp();
@@ -464,7 +659,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
     } else if (warp < Cfg::w_s && warp >= Cfg::w_q) {
         // ---------------------------------- Q loaders ----------------------------------
         const int ql = tid - Cfg::w_q * 32, chunk = ql % CPR;
-        constexpr int kRowStep = 64 / CPR;
+        constexpr int kRowStep = 32 * Cfg::q_warps / CPR;
         const uint32_t dst = smem_addr(sq) + (chunk >> 3) * Cfg::block_b;
         int seg = 0;
         for (int it = 0; it < count; ++it) {
@@ -725,54 +920,29 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             if (__builtin_expect(tail, 0)) {
                 const int n = v_pos(it);
                 wait_warp(&full[n % NU], (n / NU) & 1);
+                if (TMA) {
+                    clear_tile<T, Cfg::unit_b / 16 / GT>(su + (n % NU) * Cfg::unit_b, gtid, GT, ctx + seg->c.r.n - pos0, dirty + n % NU, n + 1);
+                    named_bar_sync(bar_group, GT);
+                    __syncwarp();
+                }
                 fix = live && *reinterpret_cast<volatile int*>(dirty + n % NU) == n + 1;
             }
-            // Infinities and NaN of new tokens entered the product as zeros. A row that sees such a value takes
-            // p * v, which is +inf, -inf or NaN (also where p is 0): two bits per row and column, +inf and -inf, both
-            // for NaN, found now, while P is there, and added to O after the product.
-            constexpr int kFix = DT / 16 / SPLIT;
-            uint32_t flags[kFix];   // of this thread's 16-column chunks: low half +inf, high half -inf
-#pragma unroll
-            for (int k = 0; k < kFix; ++k) flags[k] = 0;
             if (__builtin_expect(fix, 0)) {
+                // found now, while P is there, and added to O after the product
+                constexpr int kFix = DT / 16 / SPLIT;
+                uint32_t flags[kFix];
                 if (SPLIT == 2) {   // this thread's columns need P of all the row's keys
                     tcf_before();
                     named_bar_sync(bar_pair, 64);
                     tcf_after();
                 }
                 const Cursor c = seg->c;
-                const int x0 = rep * (KT / REP), tok = token();
-                for (int x = max(ctx - pos0, x0); x < min(c.r.seq - pos0, x0 + KT / REP); ++x) {
-                    const int pos = pos0 + x, pg = p.page_div.div(pos);
-                    const int id = p.block_table[(int64_t)c.b * p.table_stride + pg];
-                    if ((unsigned)id >= (unsigned)p.num_pages) continue;
-                    const T* src = static_cast<const T*>(p.v_cache) + id * p.stride_page + (pos - pg * p.page_size) * p.stride_slot +
-                                   c.h * p.stride_head;
-                    __syncwarp();
-                    const float2 pp = unpack2<T>(tc_ld1(lanes + Cfg::p_col(buf, x)));
-                    const bool zero = (x & 1 ? pp.y : pp.x) == 0.0f;
-                    if (!(seen_window(p, c.r, tok, pos - ctx) & 1)) continue;
-#pragma unroll
-                    for (int k = 0; k < kFix; ++k) {
-                        const int col = (k * SPLIT + half) * 16;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (col + 2 * j >= p.head_dim) break;
-                            const uint32_t raw = reinterpret_cast<const uint32_t*>(src)[col / 2 + j];
-                            if (raw == finite2<T>(raw)) continue;
-                            const float2 v = unpack2<T>(raw);
-                            if (!(fabsf(v.x) < INFINITY)) flags[k] |= (v.x < 0 && !zero ? 0u : 1u << (2 * j)) | (v.x > 0 && !zero ? 0u : 0x10000u << (2 * j));
-                            if (!(fabsf(v.y) < INFINITY)) flags[k] |= (v.y < 0 && !zero ? 0u : 2u << (2 * j)) | (v.y > 0 && !zero ? 0u : 0x20000u << (2 * j));
-                        }
-                    }
-                }
+                find_nonfinite<T>(p, c.r, c.b, c.h, token(), pos0, rep * (KT / REP), (rep + 1) * (KT / REP), half * 16, SPLIT * 16,
+                                  [=](int x) { return lanes + Cfg::p_col(buf, x); }, flags);
+                tcf_before();
                 __syncwarp();
-            }
-            tcf_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[buf]);
-            __syncwarp();
-            if (__builtin_expect(fix, 0)) {
+                if (lane == 0) mbar_arrive(&p_full[buf]);
+                __syncwarp();
                 wait_warp(&pv_done[buf], par);
                 tcf_after();
 #pragma unroll
@@ -792,6 +962,11 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
                 }
                 tc_wait_st();
                 tcf_before();
+            } else {
+                tcf_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[buf]);
+                __syncwarp();
             }
             ++done;
             if (__builtin_expect(!last, 1)) continue;
@@ -905,45 +1080,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
             }
             named_bar_sync(bar_group, GT);
             if (*reinterpret_cast<volatile int*>(s_last + t)) {
-                // join: a thread takes 16 columns of a row (four 16-byte pieces, neighbours interleaved), the row's maxima
-                // and sums first, then the parts' values, 16 loads in flight
-                constexpr int kCols = DT / 16;
-                const int r0 = t * 128, items = (min(rows, r0 + 128) - r0) * kCols;
-                for (int e = gtid; e < items; e += GT) {
-                    const int r = r0 + e / kCols, d0 = (e % kCols) * 4;
-                    auto at = [&](int q) { return (int64_t)(2 * q + (q == fc ? 1 : 0)) * RT + r; };
-                    float top = -INFINITY, sum = 0.0f;
-#pragma unroll 8
-                    for (int q = fc; q <= lc; ++q) top = fmaxf(top, __ldcg(&p.part_ml[at(q)].x));
-                    const float safe = top == -INFINITY ? 0.0f : top;
-                    float4 acc[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[k] = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-                    for (int q = fc; q <= lc; ++q) {
-                        const float2 v = __ldcg(p.part_ml + at(q));
-                        const float w = exp2_fast(v.x - safe);
-                        sum += v.y * w;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float4 po = __ldcg(reinterpret_cast<const float4*>(p.part_o + at(q) * DT + d0 + k * (DT / 4)));
-                            acc[k].x += po.x * w;
-                            acc[k].y += po.y * w;
-                            acc[k].z += po.z * w;
-                            acc[k].w += po.w * w;
-                        }
-                    }
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int d = d0 + k * (DT / 4);
-                        if (d >= p.head_dim) continue;
-                        uint32_t* dst = reinterpret_cast<uint32_t*>(out_ptr(r, d));
-                        dst[0] = pack2<T>(acc[k].x * inv, acc[k].y * inv);
-                        dst[1] = pack2<T>(acc[k].z * inv, acc[k].w * inv);
-                    }
-                    if (p.lse && d0 == 0) put_lse(r, top, sum);
-                }
+                join_parts<T, DT, RT>(p, c, fc, lc, t * 128, min(rows - t * 128, 128), gtid, GT);
                 if (gtid == 0) *counter = 0;   // ready for the next call
             }
             named_bar_sync(bar_group, GT);
@@ -963,11 +1100,42 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP>::threads, 1) tree_attn_tc_k
     }
 }
 
-template <typename T, int DT, int MT, int REP>
-static cudaError_t launch_tc(const TreeAttnParams& p, cudaStream_t st)
+static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_fn()
 {
-    using Cfg = TcCfg<DT, MT, REP>;
-    auto kernel = tree_attn_tc_kernel<T, DT, MT, REP>;
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        cudaDriverEntryPointQueryResult q;
+        void* f = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    return fn;
+}
+
+// a cache as [page][slot][head][column] (or heads outside the slots, by their strides: each stride of a map is to be a
+// multiple of the one before), boxes of 64 columns, one head, `box` slots; zeros outside
+static bool cache_map(CUtensorMap* m, const void* base, const TreeAttnParams& p, bool bf16)
+{
+    auto fn = tensor_map_fn();
+    if (!fn) return false;
+    auto bytes = [](int64_t s) { return (cuuint64_t)(s > 8 ? s : 8) * 2; };   // (the stride of a dimension of one may be anything)
+    const int h = p.slot_first ? 2 : 1, t = 3 - h;   // dimension of heads, of slots
+    cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, 0, 0, (cuuint64_t)p.num_pages}, strides[3] = {0, 0, bytes(p.stride_page)};
+    cuuint32_t box[4] = {64, 1, 1, 1};
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    dims[h] = (cuuint64_t)p.kv_heads, dims[t] = (cuuint64_t)p.page_size;
+    strides[h - 1] = bytes(p.stride_head), strides[t - 1] = bytes(p.stride_slot);
+    box[t] = (cuuint32_t)p.box;
+    return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides,
+              box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DT, int MT, int REP, bool TMA>
+static cudaError_t launch_tc(const TreeAttnParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st)
+{
+    using Cfg = TcCfg<DT, MT, REP, TMA>;
+    auto kernel = tree_attn_tc_kernel<T, DT, MT, REP, TMA>;
     static bool ready[64] = {};   // the attribute is per device and kernel, and stays
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
@@ -976,25 +1144,38 @@ static cudaError_t launch_tc(const TreeAttnParams& p, cudaStream_t st)
         if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem)) != cudaSuccess) return err;
         if (dev < 64) ready[dev] = true;
     }
-    kernel<<<num_sms(), Cfg::threads, Cfg::smem, st>>>(p);
+    kernel<<<num_sms(), Cfg::threads, Cfg::smem, st>>>(p, tm_k, tm_v);
     return cudaGetLastError();
 }
 
-template <typename T, int DT>
-static cudaError_t launch_tc_rows(const TreeAttnParams& p, int rows, cudaStream_t st)
+template <typename T, int DT, bool TMA>
+static cudaError_t launch_tc_rows(const TreeAttnParams& p, const CUtensorMap& k, const CUtensorMap& v, int rows, cudaStream_t st)
 {
-    if (rows <= 32) return launch_tc<T, DT, 1, 4>(p, st);
-    if (rows <= 64) return launch_tc<T, DT, 1, 2>(p, st);
-    if (rows <= 128) return launch_tc<T, DT, 1, 1>(p, st);
-    return launch_tc<T, DT, 2, 1>(p, st);
+    if (rows <= 32) return launch_tc<T, DT, 1, 4, TMA>(p, k, v, st);
+    if (rows <= 64) return launch_tc<T, DT, 1, 2, TMA>(p, k, v, st);
+    if (rows <= 128) return launch_tc<T, DT, 1, 1, TMA>(p, k, v, st);
+    return launch_tc<T, DT, 2, 1, TMA>(p, k, v, st);
+}
+
+template <typename T>
+static cudaError_t launch_tc_typed(TreeAttnParams p, int max_rows, cudaStream_t st)
+{
+    // Whole pages go by tensor copies where a tile is whole pages (or a page whole tiles) of at least a swizzle atom's
+    // 8 rows; other page sizes are gathered key by key.
+    CUtensorMap k{}, v{};
+    p.box = p.page_size < 128 ? p.page_size : 128;
+    p.slot_first = p.stride_slot < p.stride_head;
+    constexpr bool bf16 = !std::is_same<T, __half>::value;
+    const bool pages = p.num_pages > 0 && p.box >= 8 && 128 % p.box == 0 && p.page_size % p.box == 0 &&
+                       cache_map(&k, p.k_cache, p, bf16) && cache_map(&v, p.v_cache, p, bf16);
+    if (pages)
+        return p.head_dim <= 64 ? launch_tc_rows<T, 64, true>(p, k, v, max_rows, st) : launch_tc_rows<T, 128, true>(p, k, v, max_rows, st);
+    return p.head_dim <= 64 ? launch_tc_rows<T, 64, false>(p, k, v, max_rows, st) : launch_tc_rows<T, 128, false>(p, k, v, max_rows, st);
 }
 
 cudaError_t launch_tree_attn_tc(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st)
 {
-    if (dtype == 0)
-        return p.head_dim <= 64 ? launch_tc_rows<__half, 64>(p, max_rows, st) : launch_tc_rows<__half, 128>(p, max_rows, st);
-    return p.head_dim <= 64 ? launch_tc_rows<__nv_bfloat16, 64>(p, max_rows, st)
-                            : launch_tc_rows<__nv_bfloat16, 128>(p, max_rows, st);
+    return dtype == 0 ? launch_tc_typed<__half>(p, max_rows, st) : launch_tc_typed<__nv_bfloat16>(p, max_rows, st);
 }
 
 }  // namespace dsv41

@@ -417,6 +417,24 @@ def test_unseen_infinities_and_nan_do_not_spread(heads, kv, dim, new, dtype, tre
     assert torch.equal(got[~seen], clean.cpu()[~seen]) and bool(torch.isnan(got[seen]).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim,page,new", [(4, 2, 64, 16, [6, 3]), (8, 1, 128, 7, [9, 4]), (2, 1, 256, 16, [7, 1]),
+                                                   (16, 2, 128, 32, [20, 11]), (4, 4, 128, 64, [3, 2])])
+def test_nan_in_the_context_reaches_every_row(heads, kv, dim, page, new, dtype):
+    """A value that every row sees: in a whole tile of the context, and in the tile that the new tokens share."""
+    s = build([300, 16], new, heads, kv, dim, page, dtype, seed=dim)
+    clean = attend(s)
+    for at in (5, 290):
+        pg, off = int(s["table"][0, at // page]), at % page
+        old = s["vc"][pg, off].clone()
+        s["vc"][pg, off, :, 3] = float("nan")
+        got = attend(s)
+        assert bool(torch.isnan(got[:new[0], :, 3]).all()), at
+        same = [d for d in range(dim) if d != 3]
+        assert torch.equal(got[:, :, same], clean[:, :, same]) and torch.equal(got[new[0]:], clean[new[0]:])
+        s["vc"][pg, off] = old
+
+
 def test_refused_requests_are_zero_and_do_not_disturb():
     s = build([70, 30, 50], [4, 6, 2], 8, 2, 128, 16, torch.bfloat16, seed=6)
     clean = attend(s)
@@ -436,6 +454,20 @@ def test_requests_without_new_tokens():
     check(s)
     s = build([7, 8], [0, 0], 8, 2, 64, 16, torch.float16, seed=7)
     assert attend(s).shape == (0, 8, 64)
+
+
+@pytest.mark.parametrize("page,layout", [(16, "heads"), (128, "heads"), (256, "slots"), (256, "heads"), (24, "heads"), (8, "slots")])
+def test_cache_layouts_and_page_sizes(page, layout):
+    check(build([70, 300, 0], [5, 9, 20], 8, 2, 128, page, torch.float16, seed=page, layout=layout), f"{page} {layout}")
+    check(build([70, 300, 0], [5, 9, 20], 4, 1, 64, page, torch.bfloat16, seed=page, layout=layout), f"{page} {layout}")
+
+
+def test_keys_and_values_side_by_side():
+    """Both caches as slices of one tensor: equal strides, neither contiguous."""
+    s = build([70, 200], [5, 9], 8, 2, 128, 16, torch.float16, seed=21)
+    want = check(s)
+    both = torch.stack((s["kc"], s["vc"]), 1)
+    assert torch.equal(attend(dict(s, kc=both[:, 0], vc=both[:, 1])), want)
 
 
 def test_strided_query_output_and_head_major_cache():
