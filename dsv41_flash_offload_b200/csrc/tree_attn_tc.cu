@@ -47,7 +47,8 @@ struct TcCfg {
     static constexpr int hold = MT == 2 ? 32 : kw;           // scores a thread holds at a time (registers)
     static constexpr int group = 128 * split;                // softmax threads per 128 rows
     static constexpr int soft_warps = 4 * split * MT;
-    static constexpr int prod_warps = TMA ? 1 : 4, q_warps = TMA && MT == 2 ? 1 : 2;
+    // one warp's tensor copies of 16-token pages (16 a unit) take 1200 cycles to issue; two share them where there is room
+    static constexpr int prod_warps = TMA ? (MT == 2 ? 1 : 2) : 4, q_warps = TMA && MT == 2 ? 1 : 2;
     static constexpr int w_prod = soft_warps, w_q = w_prod + prod_warps, w_s = w_q + q_warps, w_o = w_s + 1;
     static constexpr int threads = (w_o + 1) * 32;
     static constexpr int block_b = 128 * 128;                // 128 rows x 64 columns of 16 bits, swizzled
@@ -499,11 +500,11 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
     auto k_pos = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
     auto v_pos = [&](int i) { return i == count - 1 ? 2 * i + 1 : 2 * i + 2; };
 
-    if (TMA && warp == Cfg::w_prod) {
+    if (TMA && warp >= Cfg::w_prod && warp < Cfg::w_q) {
         // ---------------------------------- producer, whole pages ----------------------------------
         // A tile is boxes of `box` tokens (a page, or 128 tokens of a larger one) and 64 columns; lane: one of them.
         // Boxes past the last key are left out: their keys are masked, their values are cleared by the softmax warps.
-        const int per = KT / p.box, in_tile = lane % per, block = lane / per;
+        const int per = KT / p.box, mine = lane * Cfg::prod_warps + warp - Cfg::w_prod, in_tile = mine % per, block = mine / per;
         const uint32_t dst0 = smem_addr(su) + block * Cfg::block_b + in_tile * p.box * 128;
         struct Box {
             int page, slot, head, live;
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             while (!mbar_try_wait(&full[u % NU], (u / NU) & 1) && globaltimer_ns() - t0 < kWaitLimitNs) {}
         }
         __syncwarp();
-    } else if (!TMA && warp >= Cfg::w_prod && warp < Cfg::w_prod + 4) {
+    } else if (!TMA && warp >= Cfg::w_prod && warp < Cfg::w_q) {
         // ---------------------------------- producers ----------------------------------
         const int pt = tid - Cfg::w_prod * 32, chunk = pt % CPR, row0 = pt / CPR;
         constexpr int kRowStep = 128 / CPR;
