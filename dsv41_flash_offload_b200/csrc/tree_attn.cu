@@ -1,4 +1,5 @@
-// Attention of drafted tokens over a paged cache (dsv41_tree_attention).
+// Attention of drafted tokens over a paged cache (dsv41_tree_attention): the mathematics, and the kernel for head
+// sizes over 128 (tree_attn_tc.cu has the others).
 //
 // For request b with s_b keys in the cache, the last n_b of them its new tokens, token i and query head
 // hq = h * G + g:
@@ -14,6 +15,10 @@
 // resident CTA, whatever the lengths are; the cut is computed in the kernel from the lengths (the host does
 // not know them). A segment (the units of one row tile) that crosses CTAs leaves (m, l, O) per part in the
 // workspace and the CTA that arrives last joins the parts in order: one launch, results independent of timing.
+//
+// Here: warp-level matrix instructions with Q and O in registers, keys and values through a three-stage ring of
+// cp.async copies. For few rows the warps share a tile's keys (WN = 4 / WM of them per row tile) and are joined at the
+// end of a segment.
 #include "internal.h"
 #include "tree_attn.cuh"
 
@@ -24,13 +29,13 @@ constexpr int kAttnThreads = kAttnWarps * 32;
 
 template <int DT, int WM>
 struct AttnCfg {
-    static constexpr int kt = (DT == 256 && WM > 1) ? 32 : 64;       // keys per tile
+    static constexpr int kt = WM > 1 ? 32 : 64;                      // keys per tile
     static constexpr int rt = 16 * WM;                               // rows per tile
     static constexpr int wn = kAttnWarps / WM;                       // warps that share a row tile's keys
     static constexpr int tn = kt / wn;                               // keys of a tile per warp
     static constexpr int row_b = DT * 2;
     static constexpr int tile_b = kt * row_b;                        // one K or V tile
-    static constexpr int stages = DT == 64 ? 4 : 3;
+    static constexpr int stages = 3;
     static constexpr int buf_b = wn > 1 ? rt * DT * 4 : kAttnWarps * 16 * tn * 4;   // joins of warps / P of a dirty tile
     static constexpr int ml_off = stages * 2 * tile_b + buf_b;
     static constexpr int smem = ml_off + wn * rt * 8;
@@ -197,7 +202,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<DT, WM>::per_sm) tree_at
         for (int j = 0; j < TN / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < DT / 16; ++kk) {
-            if (DT > 64 && kk * 16 >= p.head_dim) break;
+            if (kk * 16 >= p.head_dim) break;
 #pragma unroll
             for (int j = 0; j < TN / 16; ++j) {
                 const int row = wk * TN + j * 16 + ((lane >> 4) << 3) + (lane & 7);
@@ -275,7 +280,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<DT, WM>::per_sm) tree_at
             const int row = wk * TN + j * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
 #pragma unroll
             for (int n2 = 0; n2 < DT / 16; ++n2) {
-                if (DT > 64 && n2 * 16 >= p.head_dim) break;
+                if (n2 * 16 >= p.head_dim) break;
                 const int chunk = n2 * 2 + (lane >> 4);
                 uint32_t vf[4];
                 ldmatrix_x4_trans(vf, sv + row * Cfg::row_b + ((chunk ^ (row & 7)) << 4));

@@ -2,17 +2,18 @@
 // the mathematics, the rows and the cut of the work into runs are those of tree_attn.cu).
 //
 // One CTA per SM walks its run of (request, KV head, row tile, key tile) units:
-//   producers (4 warps)  copy key and value tiles of 128 keys (page by page, 16-byte cp.async) into a ring of
-//                        units in the 128-byte swizzle the tensor cores read; a ring of byte offsets, one per
-//                        key, is looked up one tile ahead
-//   Q loaders (2 warps)  the rows of the segment
+//   producers            key and value tiles of 128 keys into a ring of units, in the 128-byte swizzle the tensor cores
+//                        read. Whole pages go by tensor copies (one or two warps, a lane per page and 64 columns); page
+//                        sizes that do not make up a tile are gathered key by key by four warps of cp.async, whose
+//                        issue rate then bounds a call (16 tokens x 8 rows over 4 x 64-128k keys: 323 us for 288)
+//   Q loaders            the rows of the segment
 //   two issuers (1 thread each)  S = Q K^T (A and B from shared memory) and O += P V (A from tensor memory, V read
 //                        as it lies, N-major), fp32 accumulators in tensor memory. One thread for both left the tensor
-//                        pipe idle between its waits and commits: a unit then took 3400 cycles, of which 2900 in issuing
+//                        pipe idle between its waits and commits (2900 cycles of issuing per tile)
 //   softmax (4 or 8 warps per 128 rows; one or two threads per row, who share its keys)  S out of tensor memory,
 //                        running maximum and sum, P back into tensor memory as 16-bit pairs; at the end of a segment
 //                        O out. A single warp per sub-partition spends most of its time on latencies: with 4 warps a
-//                        tile of 128 rows took 4700 cycles for 128 exponentials a thread.
+//                        tile of 128 rows took 4700 cycles for 128 exponentials a thread
 // The product of tile i + 1 runs while tile i is in the softmax (two S and P buffers for up to 128 rows; two row
 // tiles take turns for up to 256).
 //
@@ -22,7 +23,13 @@
 //
 // The accumulator is rescaled only when a row's maximum grows by more than 2^8: P stays below 2^8, its rounding
 // is relative, and the sums are fp32, so the deferral costs no accuracy; a rescale has to wait for the product
-// in flight, the deferral makes that rare.
+// in flight, the deferral makes that rare. P is rounded to the cache's type (the second product's operand), which is
+// half a unit of each weight, as much as the output's own rounding; the sum of weights is of the unrounded ones.
+//
+// Measured, 4 requests of 32-64k keys, 8 KV heads of 128, bf16, pages of 64 (floor 120 us of HBM): 32 rows 153 us,
+// 5.1 TB/s; 128 rows 172 us, 4.6 TB/s, 585 TFLOP/s; 256 rows 267 us, 753 TFLOP/s. The first two are bound by the key
+// stream and, at the ends of a run, by latency; the last by the softmax warps' issue (16 warps, a third of the issue
+// slots, exponentials at 40% of their pipe).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -31,12 +38,6 @@
 
 namespace dsv41 {
 
-#ifndef DSV41_ATTN_EXTRA
-#define DSV41_ATTN_EXTRA 2
-#endif
-#ifndef DSV41_ATTN_EXTRA2
-#define DSV41_ATTN_EXTRA2 2
-#endif
 template <int DT, int MT, int REP, bool TMA>
 struct TcCfg {
     static_assert(MT == 1 || REP == 1, "repeats are for a single tile of 128 rows");
@@ -57,7 +58,9 @@ struct TcCfg {
     static constexpr int q_b = MT * unit_b;
     static constexpr int own = 32 / REP;                     // of 32 columns of O, those a repeat's warps put out
     static constexpr int stage_b = soft_warps * (32 - own) * 32 * 4;   // the others', on their way to their repeat
-    static constexpr int extra = MT == 1 ? DSV41_ATTN_EXTRA : DSV41_ATTN_EXTRA2;   // cost of a segment, in tiles
+    // what a segment costs beside its tiles (rows' loads, its end), in tiles. 1, 2, 3, 4, 5: 32 x 64 tokens of 4 rows over
+    // 1-8k keys 271, 246, 231, 228, 228 us; 16 x 5-13 tokens over 0.1-4k keys 54, 50, 50, 57, 56 us; long lengths within 2%
+    static constexpr int extra = 3;
     static constexpr int off_b = 4 * kt * 8;                 // byte offsets of the keys of four tiles
     static constexpr int ml_b = MT * 2 * 128 * 8;
     static constexpr int mx_b = MT * 4 * 128 * 4;            // tile maxima of the threads that share a row
@@ -65,7 +68,7 @@ struct TcCfg {
     static constexpr int fixed_b = 1024 + q_b + stage_b + off_b + ml_b + mx_b + bars_b;
     static constexpr int units_fit = (232448 - fixed_b) / unit_b;
     static constexpr int units = units_fit < 10 ? units_fit : 10;
-    static constexpr int lag = units - 2;                    // units a producer has in flight when it issues the next
+    static constexpr int lag = units - 2;                    // cp.async: units in flight when the next is issued
     static constexpr int smem = fixed_b + units * unit_b;
     static_assert(units >= 4 && lag <= 8, "ring length");
     // tensor memory columns
