@@ -16,10 +16,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdsv41_b200.so")
 SOURCES = ["capi.cu", "permute.cu", "transform.cu", "gemv.cu", "gemm.cu", "noalloc.cu", "ep_peer.cu", "router.cu",
-           "paged.cu", "tree_attn.cu", "tree_attn_tc.cu", "w4.cu", "w4_f16.cu",
+           "paged.cu", "tree_attn.cu", "tree_attn_f16.cu", "tree_attn_bf16.cu", "w4.cu", "w4_f16.cu",
            "w4_bf16.cu", "capi_step.cu"]
-HEADERS = ["common.cuh", "internal.h", "gemm.h", "paged.h", "tree_attn.cuh", "w4.h",
-           "w4_kernel.cuh"]
+HEADERS = ["common.cuh", "internal.h", "gemm.h", "paged.h", "tree_attn.cuh", "tree_attn_kernel.cuh",
+           "w4.h", "w4_kernel.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

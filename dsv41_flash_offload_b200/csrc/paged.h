@@ -82,7 +82,8 @@ AttnWorkspace tree_attn_workspace(int head_dim);
 
 // dtype 0 fp16, 1 bf16; max_rows: upper bound on a request's new tokens times the group (picks the row tile)
 cudaError_t launch_tree_attn(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st);
-cudaError_t launch_tree_attn_tc(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st);   // head_dim <= 128
+cudaError_t launch_tree_attn_f16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
+cudaError_t launch_tree_attn_bf16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
 cudaError_t launch_step_tables(const StepTablesParams& p, cudaStream_t st);
 cudaError_t launch_store_kv(const StoreKvParams& p, cudaStream_t st);
 

@@ -1,4 +1,4 @@
-// Device helpers shared by the attention kernels (tree_attn.cu, tree_attn_tc.cu): 16-bit pairs, asynchronous
+// Device helpers of the attention kernel: 16-bit pairs, asynchronous
 // copies, the kernel's view of a request, positions in the list of units, and the mask windows.
 #pragma once
 #include <cuda_bf16.h>
@@ -10,18 +10,6 @@
 
 namespace dsv41 {
 
-template <typename T>
-__device__ __forceinline__ void mma_t(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-{
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
-        mma_16816(d, a, b0, b1);
-    } else {
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b)
 {
@@ -59,12 +47,6 @@ __device__ __forceinline__ bool any_nonfinite(uint4 v)
     constexpr uint32_t e = exp_bits<T>();
     auto bad = [](uint32_t w) { return (w & e) == e || (w & (e << 16)) == (e << 16); };
     return bad(v.x) || bad(v.y) || bad(v.z) || bad(v.w);
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&a)[4], uint32_t addr)
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-                 : "r"(addr));
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live)
 {

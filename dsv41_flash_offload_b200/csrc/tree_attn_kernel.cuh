@@ -1,11 +1,12 @@
-// Attention of drafted tokens over a paged cache on the fifth-generation tensor cores (head sizes up to 128;
-// the mathematics, the rows and the cut of the work into runs are those of tree_attn.cu).
+// Attention of drafted tokens over a paged cache on the fifth-generation tensor cores (tree_attn.cu has the
+// mathematics, the rows and the cut of the work into runs).
 //
 // One CTA per SM walks its run of (request, KV head, row tile, key tile) units:
-//   producers            key and value tiles of 128 keys into a ring of units, in the 128-byte swizzle the tensor cores
-//                        read. Whole pages go by tensor copies (one or two warps, a lane per page and 64 columns); page
-//                        sizes that do not make up a tile are gathered key by key by four warps of cp.async, whose
-//                        issue rate then bounds a call (16 tokens x 8 rows over 4 x 64-128k keys: 323 us for 288)
+//   producers            key and value tiles (128 keys; 64 for head sizes over 128) into a ring of units, in the
+//                        128-byte swizzle the tensor cores read. Whole pages go by tensor copies (one or two warps, a lane
+//                        per page and 64 columns); page sizes that do not make up a tile are gathered key by key by four
+//                        warps of cp.async, whose issue rate then bounds a call (16 tokens x 8 rows over 4 x 64-128k keys:
+//                        323 us for 288)
 //   Q loaders            the rows of the segment
 //   two issuers (1 thread each)  S = Q K^T (A and B from shared memory) and O += P V (A from tensor memory, V read
 //                        as it lies, N-major), fp32 accumulators in tensor memory. One thread for both left the tensor
@@ -29,7 +30,10 @@
 // Measured, 4 requests of 32-64k keys, 8 KV heads of 128, bf16, pages of 64 (floor 120 us of HBM): 32 rows 153 us,
 // 5.1 TB/s; 128 rows 172 us, 4.6 TB/s, 585 TFLOP/s; 256 rows 267 us, 753 TFLOP/s. The first two are bound by the key
 // stream and, at the ends of a run, by latency; the last by the softmax warps' issue (16 warps, a third of the issue
-// slots, exponentials at 40% of their pipe).
+// slots, exponentials at 40% of their pipe). Heads of 256 (floor 240 us): 285 us, 5.5 TB/s; 368 us; 592 us (two tiles of
+// 128 rows, a second trip of the keys), 680 TFLOP/s. Warp-level matrix instructions took 780 us for the first and reached
+// 120 TFLOP/s in the last.
+#pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -41,7 +45,8 @@ namespace dsv41 {
 template <int DT, int MT, int REP, bool TMA>
 struct TcCfg {
     static_assert(MT == 1 || REP == 1, "repeats are for a single tile of 128 rows");
-    static constexpr int kt = 128;                           // keys per tile
+    static_assert(MT == 1 || DT <= 128, "tensor memory holds one row tile of 256 columns");
+    static constexpr int kt = DT == 256 ? 64 : 128;          // keys per tile (256 columns of O leave room for two S of 64)
     static constexpr int rt = MT * 128 / REP;                // rows per tile
     static constexpr int split = REP == 4 ? 1 : 2;           // softmax threads that share a row's keys
     static constexpr int kw = kt / REP / split;              // keys of a tile per softmax thread
@@ -52,10 +57,11 @@ struct TcCfg {
     static constexpr int prod_warps = TMA ? (MT == 2 ? 1 : 2) : 4, q_warps = TMA && MT == 2 ? 1 : 2;
     static constexpr int w_prod = soft_warps, w_q = w_prod + prod_warps, w_s = w_q + q_warps, w_o = w_s + 1;
     static constexpr int threads = (w_o + 1) * 32;
-    static constexpr int block_b = 128 * 128;                // 128 rows x 64 columns of 16 bits, swizzled
-    static constexpr int blocks = DT / 64;
+    static constexpr int blocks = DT / 64;                   // blocks of 64 columns (128 bytes), swizzled
+    static constexpr int block_b = kt * 128;
     static constexpr int unit_b = blocks * block_b;          // a key or value tile
-    static constexpr int q_b = MT * unit_b;
+    static constexpr int q_block_b = 128 * 128, q_tile_b = blocks * q_block_b;
+    static constexpr int q_b = MT * q_tile_b;
     static constexpr int own = 32 / REP;                     // of 32 columns of O, those a repeat's warps put out
     static constexpr int stage_b = soft_warps * (32 - own) * 32 * 4;   // the others', on their way to their repeat
     // what a segment costs beside its tiles (rows' loads, its end), in tiles. 1, 2, 3, 4, 5: 32 x 64 tokens of 4 rows over
@@ -72,14 +78,14 @@ struct TcCfg {
     static constexpr int smem = fixed_b + units * unit_b;
     static_assert(units >= 4 && lag <= 8, "ring length");
     // tensor memory columns
-    __host__ __device__ static constexpr int s_col(int b) { return b * 128; }
+    __host__ __device__ static constexpr int s_col(int b) { return b * kt; }
     // P of key x of buffer b (two keys a column). Two row tiles leave no room of its own: P then lies over S, each
     // softmax thread's over its own keys', which it alone reads.
     __host__ __device__ static constexpr int p_col(int b, int x)
     {
-        return MT == 1 ? 256 + b * 64 + x / 2 : b * 128 + (x / kw) * kw + (x % kw) / 2;
+        return MT == 1 ? 2 * kt + b * (kt / 2) + x / 2 : b * kt + (x / kw) * kw + (x % kw) / 2;
     }
-    __host__ __device__ static constexpr int o_col(int t) { return MT == 1 ? 384 : 256 + t * 128; }
+    __host__ __device__ static constexpr int o_col(int t) { return DT == 256 ? 256 : MT == 1 ? 384 : 256 + t * 128; }
 };
 
 // whether a phase is complete, without waiting for it
@@ -120,11 +126,28 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, ui
         " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh)
         : "memory");
 }
-// N (a multiple of 32) columns of this thread's lane: all loads, one wait. The empty statements after the wait tie
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, float* v)
+{
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        " tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// N (16, or a multiple of 32) columns of this thread's lane: all loads, one wait. The empty statements after the wait tie
 // the registers to it, so no use of them is scheduled before.
 template <int N>
 __device__ __forceinline__ void tc_ld(uint32_t taddr, float* v)
 {
+    if constexpr (N == 16) {
+        tc_ld16(taddr, v);
+        return;
+    } else {
     uint32_t r[N];
 #pragma unroll
     for (int c = 0; c < N; c += 32)
@@ -145,6 +168,7 @@ __device__ __forceinline__ void tc_ld(uint32_t taddr, float* v)
                           "+r"(r[c + 6]), "+r"(r[c + 7]));
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
+    }
 }
 // pairs of fp32 in one instruction
 __device__ __forceinline__ uint64_t pair(float a, float b)
@@ -171,19 +195,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-__device__ __forceinline__ void tc_ld16(uint32_t taddr, float* v)
-{
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-        " tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ uint32_t tc_ld1(uint32_t taddr)
 {
@@ -241,7 +252,7 @@ __device__ __noinline__ bool clear_nonfinite(unsigned char* base, int row0, int 
 // The same for a tile of whole pages, by `threads` threads together, before its product: values past the last key
 // (rows from `rows` on, which may hold anything) are cleared too, without a mark. The mark is set before a value is
 // cleared: who finds it cleared (another group of threads looks at the same tile) finds the mark.
-template <typename T, int N>
+template <typename T, int KT, int N>
 __device__ __noinline__ void clear_tile(unsigned char* unit, int thread, int threads, int rows, volatile int* mark, int value)
 {
     constexpr uint32_t kExp = exp_bits<T>() * 0x10001u;
@@ -257,7 +268,7 @@ __device__ __noinline__ void clear_tile(unsigned char* unit, int thread, int thr
         for (int i = 0; i < N; ++i) {
             uint4 v = at[i * threads];
             if (!any_nonfinite<T>(v)) continue;
-            if (((thread + i * threads) >> 3) % 128 < rows) *mark = value;   // 128-byte rows, 128 of them a block
+            if (((thread + i * threads) >> 3) % KT < rows) *mark = value;   // 128-byte rows, KT of them a block
             __threadfence_block();
             v.x = finite2<T>(v.x), v.y = finite2<T>(v.y), v.z = finite2<T>(v.z), v.w = finite2<T>(v.w);
             at[i * threads] = v;
@@ -505,7 +516,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
 
     if (TMA && warp >= Cfg::w_prod && warp < Cfg::w_q) {
         // ---------------------------------- producer, whole pages ----------------------------------
-        // A tile is boxes of `box` tokens (a page, or 128 tokens of a larger one) and 64 columns; lane: one of them.
+        // A tile is boxes of `box` tokens (a page, or a tile's tokens of a larger one) and 64 columns; lane: one of them.
         // Boxes past the last key are left out: their keys are masked, their values are cleared by the softmax warps.
         const int per = KT / p.box, mine = lane * Cfg::prod_warps + warp - Cfg::w_prod, in_tile = mine % per, block = mine / per;
         const uint32_t dst0 = smem_addr(su) + block * Cfg::block_b + in_tile * p.box * 128;
@@ -515,7 +526,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         auto look_up = [&](const Cursor& c) {
             Box b;
             const int pos = c.kt * KT + in_tile * p.box, pg = p.page_div.div(pos);
-            b.live = block < Cfg::blocks && pos < c.r.seq;
+            b.live = block * 64 < p.head_dim && pos < c.r.seq;
             b.page = b.live ? __ldg(p.block_table + (int64_t)c.b * p.table_stride + pg) : 0;
             b.slot = pos - pg * p.page_size;
             b.head = c.h;
@@ -629,7 +640,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         // element offset of key `pt` of the cursor's tile (-1: past the end, or not a page of this cache)
         auto offset_of = [&](const Cursor& c) -> int64_t {
             const int pos = c.kt * KT + pt;
-            if (pos >= c.r.seq) return -1;
+            if (pt >= KT || pos >= c.r.seq) return -1;
             const int pg = p.page_div.div(pos);
             const int id = __ldg(p.block_table + (int64_t)c.b * p.table_stride + pg);
             if ((unsigned)id >= (unsigned)p.num_pages) return -1;
@@ -649,7 +660,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         int n = 0;
         for (int step = 0; step <= count; ++step) {
             if (step < count) {
-                key_off[(step & 3) * KT + pt] = off[0];
+                if (pt < KT) key_off[(step & 3) * KT + pt] = off[0];
                 named_bar_sync(3, 128);
                 issue(n++, p.k_cache, key_off + (step & 3) * KT, false);
             }
@@ -664,7 +675,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         // ---------------------------------- Q loaders ----------------------------------
         const int ql = tid - Cfg::w_q * 32, chunk = ql % CPR;
         constexpr int kRowStep = 32 * Cfg::q_warps / CPR;
-        const uint32_t dst = smem_addr(sq) + (chunk >> 3) * Cfg::block_b;
+        const uint32_t dst = smem_addr(sq) + (chunk >> 3) * Cfg::q_block_b;
         int seg = 0;
         for (int it = 0; it < count; ++it) {
             if (it == 0 || cur.kt == 0) {
@@ -680,7 +691,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                         const T* src = base + i * p.q_stride_token + g * p.q_stride_head;
 #pragma unroll
                         for (int r = row; r < MT * 128; r += RT)
-                            cp_async16(dst + (r >> 7) * Cfg::unit_b + (r & 127) * 128 + (((chunk & 7) ^ (r & 7)) << 4), src, true);
+                            cp_async16(dst + (r >> 7) * Cfg::q_tile_b + (r & 127) * 128 + (((chunk & 7) ^ (r & 7)) << 4), src, true);
                     }
                 }
                 cp_async_commit();
@@ -718,13 +729,13 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                     if (t == 0) ok = ok && wait(&full[n % NU], (n / NU) & 1);
                     if (!ok) break;
                     tcf_after();
-                    const uint32_t kd = tc_desc_low(ring + (n % NU) * Cfg::unit_b, 16), qd = tc_desc_low(q_at + t * Cfg::unit_b, 16);
+                    const uint32_t kd = tc_desc_low(ring + (n % NU) * Cfg::unit_b, 16), qd = tc_desc_low(q_at + t * Cfg::q_tile_b, 16);
                     const uint32_t dst = tmem + Cfg::s_col(buf);
 #pragma unroll
                     for (int kk = 0; kk < DT / 16; ++kk) {
-                        constexpr int kStep = 32 >> 4, kBlock = Cfg::block_b >> 4;
-                        const int at = (kk >> 2) * kBlock + (kk & 3) * kStep;
-                        if (kk < ksteps) tc_mma_ss(dst, qd + at, kd + at, idesc, kk > 0);
+                        const int block = kk >> 2, step = (kk & 3) * (32 >> 4);
+                        if (kk < ksteps)
+                            tc_mma_ss(dst, qd + block * (Cfg::q_block_b >> 4) + step, kd + block * (Cfg::block_b >> 4) + step, idesc, kk > 0);
                     }
                     tc_commit(&s_full[buf]);
                     ++used[buf];
@@ -777,8 +788,11 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
 #pragma unroll
             for (int i = 0; i < 16; ++i) z[i] = 0;
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                if ((c & 3) / (4 / REP) != rep) tc_st16(lanes + Cfg::p_col(c >> 2, (c & 3) * 32), z);
+            for (int c = 0; c < 8; ++c) {   // a quarter of a tile's keys in a buffer
+                if ((c & 3) / (4 / REP) == rep) continue;
+                if constexpr (KT == 128) tc_st16(lanes + Cfg::p_col(c >> 2, (c & 3) * (KT / 4)), z);
+                else tc_st8(lanes + Cfg::p_col(c >> 2, (c & 3) * (KT / 4)), z);
+            }
             tc_wait_st();
         }
         float m = -INFINITY, l = 0.0f;
@@ -925,7 +939,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                 const int n = v_pos(it);
                 wait_warp(&full[n % NU], (n / NU) & 1);
                 if (TMA) {
-                    clear_tile<T, Cfg::unit_b / 16 / GT>(su + (n % NU) * Cfg::unit_b, gtid, GT, ctx + seg->c.r.n - pos0, dirty + n % NU, n + 1);
+                    clear_tile<T, KT, Cfg::unit_b / 16 / GT>(su + (n % NU) * Cfg::unit_b, gtid, GT, ctx + seg->c.r.n - pos0, dirty + n % NU, n + 1);
                     named_bar_sync(bar_group, GT);
                     __syncwarp();
                 }
@@ -1157,29 +1171,33 @@ static cudaError_t launch_tc_rows(const TreeAttnParams& p, const CUtensorMap& k,
 {
     if (rows <= 32) return launch_tc<T, DT, 1, 4, TMA>(p, k, v, st);
     if (rows <= 64) return launch_tc<T, DT, 1, 2, TMA>(p, k, v, st);
-    if (rows <= 128) return launch_tc<T, DT, 1, 1, TMA>(p, k, v, st);
-    return launch_tc<T, DT, 2, 1, TMA>(p, k, v, st);
+    if constexpr (DT <= 128) {
+        if (rows > 128) return launch_tc<T, DT, 2, 1, TMA>(p, k, v, st);
+    }
+    return launch_tc<T, DT, 1, 1, TMA>(p, k, v, st);
 }
 
-template <typename T>
-static cudaError_t launch_tc_typed(TreeAttnParams p, int max_rows, cudaStream_t st)
+template <typename T, int DT>
+static cudaError_t launch_tc_dim(TreeAttnParams p, int max_rows, cudaStream_t st)
 {
     // Whole pages go by tensor copies where a tile is whole pages (or a page whole tiles) of at least a swizzle atom's
     // 8 rows; other page sizes are gathered key by key.
-    CUtensorMap k{}, v{};
-    p.box = p.page_size < 128 ? p.page_size : 128;
-    p.slot_first = p.stride_slot < p.stride_head;
+    constexpr int kt = TcCfg<DT, 1, 1, true>::kt;
     constexpr bool bf16 = !std::is_same<T, __half>::value;
-    const bool pages = p.num_pages > 0 && p.box >= 8 && 128 % p.box == 0 && p.page_size % p.box == 0 &&
+    CUtensorMap k{}, v{};
+    p.box = p.page_size < kt ? p.page_size : kt;
+    p.slot_first = p.stride_slot < p.stride_head;
+    const bool pages = p.num_pages > 0 && p.box >= 8 && kt % p.box == 0 && p.page_size % p.box == 0 &&
                        cache_map(&k, p.k_cache, p, bf16) && cache_map(&v, p.v_cache, p, bf16);
-    if (pages)
-        return p.head_dim <= 64 ? launch_tc_rows<T, 64, true>(p, k, v, max_rows, st) : launch_tc_rows<T, 128, true>(p, k, v, max_rows, st);
-    return p.head_dim <= 64 ? launch_tc_rows<T, 64, false>(p, k, v, max_rows, st) : launch_tc_rows<T, 128, false>(p, k, v, max_rows, st);
+    return pages ? launch_tc_rows<T, DT, true>(p, k, v, max_rows, st) : launch_tc_rows<T, DT, false>(p, k, v, max_rows, st);
 }
 
-cudaError_t launch_tree_attn_tc(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st)
+template <typename T>
+static cudaError_t launch_tree_attn_typed(const TreeAttnParams& p, int max_rows, cudaStream_t st)
 {
-    return dtype == 0 ? launch_tc_typed<__half>(p, max_rows, st) : launch_tc_typed<__nv_bfloat16>(p, max_rows, st);
+    if (p.head_dim <= 64) return launch_tc_dim<T, 64>(p, max_rows, st);
+    if (p.head_dim <= 128) return launch_tc_dim<T, 128>(p, max_rows, st);
+    return launch_tc_dim<T, 256>(p, max_rows, st);
 }
 
 }  // namespace dsv41

@@ -462,6 +462,17 @@ def test_cache_layouts_and_page_sizes(page, layout):
     check(build([70, 300, 0], [5, 9, 20], 4, 1, 64, page, torch.bfloat16, seed=page, layout=layout), f"{page} {layout}")
 
 
+@pytest.mark.parametrize("dim", [136, 192, 200, 256])
+@pytest.mark.parametrize("page,layout", [(8, "slots"), (64, "heads"), (192, "slots"), (24, "slots"), (1, "heads")])
+def test_head_sizes_over_128(dim, page, layout):
+    """Up to 32, 64, 128 and more rows to a KV head, whole requests and split ones, tiles of 64 keys that pages end in."""
+    dtype = torch.float16 if page == 8 else torch.bfloat16
+    check(build([63, 300, 0, 64], [5, 1, 8, 3], 8, 2, dim, page, dtype, seed=dim + page, layout=layout), f"{dim} {page} 32 rows")
+    check(build([1000, 127], [30, 33], 2, 1, dim, page, dtype, seed=dim, layout=layout), f"{dim} {page} 66 rows")
+    check(build([128, 65], [12, 15], 4, 1, dim, page, dtype, seed=page, layout=layout), f"{dim} {page} 60 rows")
+    check(build([190, 1], [64, 40], 5, 1, dim, page, dtype, seed=page, layout=layout), f"{dim} {page} 320 rows")
+
+
 def test_keys_and_values_side_by_side():
     """Both caches as slices of one tensor: equal strides, neither contiguous."""
     s = build([70, 200], [5, 9], 8, 2, 128, 16, torch.float16, seed=21)
