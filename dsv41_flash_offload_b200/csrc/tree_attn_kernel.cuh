@@ -6,7 +6,7 @@
 //                        128-byte swizzle the tensor cores read. Whole pages go by tensor copies (one or two warps, a lane
 //                        per page and 64 columns); page sizes that do not make up a tile are gathered key by key by four
 //                        warps of cp.async, whose issue rate then bounds a call (16 tokens x 8 rows over 4 x 64-128k keys:
-//                        323 us for 288)
+//                        323 us for 288, the latter now 279)
 //   Q loaders            the rows of the segment
 //   two issuers (1 thread each)  S = Q K^T (A and B from shared memory) and O += P V (A from tensor memory, V read
 //                        as it lies, N-major), fp32 accumulators in tensor memory. One thread for both left the tensor
@@ -27,12 +27,13 @@
 // in flight, the deferral makes that rare. P is rounded to the cache's type (the second product's operand), which is
 // half a unit of each weight, as much as the output's own rounding; the sum of weights is of the unrounded ones.
 //
-// Measured, 4 requests of 32-64k keys, 8 KV heads of 128, bf16, pages of 64 (floor 120 us of HBM): 32 rows 153 us,
-// 5.1 TB/s; 128 rows 172 us, 4.6 TB/s, 585 TFLOP/s; 256 rows 267 us, 753 TFLOP/s. The first two are bound by the key
+// Measured, 4 requests of 32-64k keys, 8 KV heads of 128, bf16, pages of 64 (floor 120 us of HBM): 32 rows 150 us,
+// 5.2 TB/s; 128 rows 161 us, 4.9 TB/s, 626 TFLOP/s; 256 rows 257 us, 783 TFLOP/s. The first two are bound by the key
 // stream and, at the ends of a run, by latency; the last by the softmax warps' issue (16 warps, a third of the issue
-// slots, exponentials at 40% of their pipe). Heads of 256 (floor 240 us): 285 us, 5.5 TB/s; 368 us; 592 us (two tiles of
-// 128 rows, a second trip of the keys), 680 TFLOP/s. Warp-level matrix instructions took 780 us for the first and reached
-// 120 TFLOP/s in the last.
+// slots, exponentials at 40% of their pipe). Heads of 256 (floor 240 us): 275 us, 5.7 TB/s; 302 us; 561 us (two tiles of
+// 128 rows, a second trip of the keys), 717 TFLOP/s. Warp-level matrix instructions took 780 us for the first and reached
+// 120 TFLOP/s in the last. A call of one tile takes 15 us, most of it latencies one after the other: lengths, page
+// numbers, keys, two products, the row out.
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -314,52 +315,64 @@ __device__ __noinline__ void find_nonfinite(const TreeAttnParams& p, const AttnR
     __syncwarp();
 }
 
-// Join of a segment's parts (runs fc .. lc): a thread takes 16 columns of a row (four 16-byte pieces, neighbours
-// interleaved), the row's maxima and sums first, then the parts' values, 16 loads in flight. Rows r0 .. r0 + rows - 1 of the
-// row tile at c, by `threads` threads.
+// Join of a segment's parts (runs fc .. lc): a thread takes 16 columns of a row, a batch of parts at a time with all its
+// loads in flight (one trip to L2 a batch), and rescales what it has as the softmax does. Rows r0 .. r0 + rows - 1 of
+// the row tile at c, by `threads` threads. A part is [column / 4][row][4]: neighbours in a warp are neighbouring rows
+// here and where it is written.
 template <typename T, int DT, int RT, typename Cursor>
 __device__ __noinline__ void join_parts(const TreeAttnParams& p, const Cursor& c, int fc, int lc, int r0, int rows, int thread,
                                         int threads)
 {
-    constexpr int kCols = DT / 16;
-    for (int e = thread; e < rows * kCols; e += threads) {
-        const int r = r0 + e / kCols, d0 = (e % kCols) * 4;
-        auto at = [&](int q) { return (int64_t)(2 * q + (q == fc ? 1 : 0)) * RT + r; };
-        float top = -INFINITY, sum = 0.0f;
-#pragma unroll 8
-        for (int q = fc; q <= lc; ++q) top = fmaxf(top, __ldcg(&p.part_ml[at(q)].x));
-        const float safe = top == -INFINITY ? 0.0f : top;
-        float4 acc[4];
+    constexpr int kBatch = 4;
+    const int blocks = (p.head_dim + 15) / 16;
+    for (int e = thread; e < rows * blocks; e += threads) {
+        const int block = e / rows, r = r0 + e - block * rows;
+        float mm = -INFINITY, ll = 0.0f, acc[16];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-        for (int q = fc; q <= lc; ++q) {
-            const float2 v = __ldcg(p.part_ml + at(q));
-            const float w = exp2_fast(v.x - safe);
-            sum += v.y * w;
+        for (int j = 0; j < 16; ++j) acc[j] = 0.0f;
+#pragma unroll 1
+        for (int q0 = fc; q0 <= lc; q0 += kBatch) {
+            float2 v[kBatch];
+            float4 po[kBatch][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float4 po = __ldcg(reinterpret_cast<const float4*>(p.part_o + at(q) * DT + d0 + k * (DT / 4)));
-                acc[k].x += po.x * w;
-                acc[k].y += po.y * w;
-                acc[k].z += po.z * w;
-                acc[k].w += po.w * w;
+            for (int i = 0; i < kBatch; ++i) {
+                const int q = q0 + i;
+                const int64_t slot = 2 * q + (q == fc ? 1 : 0);
+                const float4* src = reinterpret_cast<const float4*>(p.part_o + slot * RT * DT) + block * 4 * RT + r;
+                v[i] = q <= lc ? __ldcg(p.part_ml + slot * RT + r) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) po[i][k] = q <= lc ? __ldcg(src + k * RT) : make_float4(0, 0, 0, 0);
+            }
+            float top = mm;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) top = fmaxf(top, v[i].x);
+            const float safe = top == -INFINITY ? 0.0f : top, keep = exp2_fast(mm - safe);
+            ll *= keep;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[j] *= keep;
+            mm = top;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const float w = exp2_fast(v[i].x - safe);
+                ll += v[i].y * w;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    acc[4 * k] += po[i][k].x * w, acc[4 * k + 1] += po[i][k].y * w, acc[4 * k + 2] += po[i][k].z * w,
+                        acc[4 * k + 3] += po[i][k].w * w;
             }
         }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
         const int row = c.rt * RT + r, i = p.group_div.div(row), g = row - i * p.group;
         T* out = static_cast<T*>(p.out) + (int64_t)(c.r.q0 + i) * p.out_stride_token + (int64_t)(c.h * p.group + g) * p.out_stride_head;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int d = d0 + k * (DT / 4);
-            if (d >= p.head_dim) continue;
-            uint32_t* dst = reinterpret_cast<uint32_t*>(out + d);
-            dst[0] = pack2<T>(acc[k].x * inv, acc[k].y * inv);
-            dst[1] = pack2<T>(acc[k].z * inv, acc[k].w * inv);
-        }
-        if (p.lse && d0 == 0)
+        for (int j = 0; j < 16; j += 8)
+            if (block * 16 + j < p.head_dim)
+                *reinterpret_cast<uint4*>(out + block * 16 + j) =
+                    make_uint4(pack2<T>(acc[j] * inv, acc[j + 1] * inv), pack2<T>(acc[j + 2] * inv, acc[j + 3] * inv),
+                               pack2<T>(acc[j + 4] * inv, acc[j + 5] * inv), pack2<T>(acc[j + 6] * inv, acc[j + 7] * inv));
+        if (p.lse && block == 0)
             p.lse[(int64_t)(c.r.q0 + i) * p.q_heads + c.h * p.group + g] =
-                sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+                ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
     }
 }
 
@@ -416,10 +429,16 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     // ---- this CTA's run ----
-    // A segment of nkt tiles costs what nkt + extra tiles do (its rows' loads, its end), so the runs are cut from a line
-    // on which each segment begins with `extra` empty places. Every thread sums its requests' places and tiles; the
-    // one whose request holds the run's first place, and the one that holds its end, tell the others.
-    __shared__ int64_t warp_sum[Cfg::threads / 32][2];
+    // Calls whose segments can each have CTAs of their own: segments of up to 2 * R tiles stay whole, longer ones are cut into
+    // equal parts of R at most (R 4, or 8 where there is no room for 4; a place on the line is a CTA). Joining parts
+    // costs 5 to 10 us, a tile of a CTA alone 1: 3 requests of 50 rows over 13 tiles, 2 KV heads, took 43 us in parts of one
+    // tile and take 23 us, over 2 tiles 22 and 17 us; 8 segments of 16 tiles and 4 rows 20.5 and 21.5 us.
+    // Others: a segment of nkt tiles costs what nkt + extra tiles do (its rows' loads, its end), so the runs are cut from a
+    // line on which each segment begins with `extra` empty places.
+    // Every thread sums its requests' places and tiles; the one whose request holds the run's first place, and the
+    // one that holds its end, tell the others.
+    constexpr int kSums = 4;                // places on the line, tiles, parts for R = 4 and 8
+    __shared__ int64_t warp_sum[Cfg::threads / 32][kSums];
     __shared__ int64_t s_first[3], s_end;   // first: request, segment of the request, place in the segment; tiles before
     __shared__ int64_t s_tiles0;
     struct SegState {
@@ -428,58 +447,91 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
     };
     __shared__ SegState s_seg[Cfg::soft_warps];
     int64_t run, v0;
+    int part_tiles = 0;   // R (0: runs of the line)
+    auto parts = [](int nt, int r) { return nt <= 2 * r ? 1 : (nt + r - 1) / r; };
     {
         const int per = (p.batch + Cfg::threads - 1) / Cfg::threads;
         const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
         auto segments = [&](const AttnReq& r) { return r.n > 0 ? (int64_t)((r.n * p.group + RT - 1) / RT) * p.kv_heads : 0; };
         auto tiles = [&](const AttnReq& r) { return max((r.seq + KT - 1) / KT, 1); };
-        int64_t sum[2] = {0, 0};   // segments' places, tiles
+        int64_t sum[kSums] = {};
         AttnReq mine;
         for (int b = b0; b < b1; ++b) {
             mine = attn_req(p, b);
             const int64_t n = segments(mine);
-            sum[0] += n * (tiles(mine) + Cfg::extra);
-            sum[1] += n * tiles(mine);
+            const int nt = tiles(mine);
+            sum[0] += n * (nt + Cfg::extra);
+            sum[1] += n * nt;
+            sum[2] += n * parts(nt, 4);
+            sum[3] += n * parts(nt, 8);
         }
-        int64_t inc[2] = {sum[0], sum[1]};
+        int64_t inc[kSums];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
+        for (int k = 0; k < kSums; ++k) {
+            inc[k] = sum[k];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int o = 1; o < 32; o <<= 1) {
                 const int64_t y = __shfl_up_sync(0xffffffffu, inc[k], o);
                 if (lane >= o) inc[k] += y;
             }
+            if (lane == 31) warp_sum[warp][k] = inc[k];
         }
-        if (lane == 31) warp_sum[warp][0] = inc[0], warp_sum[warp][1] = inc[1];
         __syncthreads();
-        int64_t at = inc[0] - sum[0], before = inc[1] - sum[1], total = 0, all = 0;
-        for (int w = 0; w < Cfg::threads / 32; ++w) {
-            if (w < warp) at += warp_sum[w][0], before += warp_sum[w][1];
-            total += warp_sum[w][0];
-            all += warp_sum[w][1];
-        }
-        run = (total + gridDim.x - 1) / gridDim.x;
-        v0 = run * blockIdx.x;
-        const int64_t v1 = min(v0 + run, total);
-        if (tid == 0 && v1 >= total) s_end = all;
-        for (int b = b0; b < b1; ++b) {
-            if (per > 1) mine = attn_req(p, b);
-            const int64_t nt = tiles(mine), len = nt + Cfg::extra, places = segments(mine) * len;
-            auto tiles_before = [&](int64_t v) {   // tiles before place v of this request
-                const int64_t g = v / len, in = v - g * len;
-                return before + g * nt + max(in - Cfg::extra, (int64_t)0);
-            };
-            if (v0 >= at && v0 < at + places) {
-                s_first[0] = b;
-                s_first[1] = (v0 - at) / len;
-                s_first[2] = (v0 - at) % len;
-                s_tiles0 = tiles_before(v0 - at);
+        int64_t before[kSums], all[kSums];
+#pragma unroll
+        for (int k = 0; k < kSums; ++k) {
+            before[k] = inc[k] - sum[k], all[k] = 0;
+            for (int w = 0; w < Cfg::threads / 32; ++w) {
+                if (w < warp) before[k] += warp_sum[w][k];
+                all[k] += warp_sum[w][k];
             }
-            if (v1 < total && v1 >= at && v1 < at + places) s_end = tiles_before(v1 - at);
-            at += places;
-            before += segments(mine) * nt;
         }
-        if (v0 >= total && tid == 0) s_tiles0 = all;
+        part_tiles = all[2] <= gridDim.x ? 4 : all[3] <= gridDim.x ? 8 : 0;
+        if (part_tiles) {
+            int64_t at = part_tiles == 4 ? before[2] : before[3];
+            run = 1;
+            v0 = blockIdx.x;
+            if (tid == 0 && v0 >= (part_tiles == 4 ? all[2] : all[3])) s_tiles0 = s_end = 0;
+            for (int b = b0; b < b1; ++b) {
+                if (per > 1) mine = attn_req(p, b);
+                const int nt = tiles(mine), len = parts(nt, part_tiles);
+                const int64_t places = segments(mine) * len;
+                if (v0 >= at && v0 < at + places) {
+                    const int in = (int)(v0 - at), j = in % len, tpp = (nt + len - 1) / len;
+                    s_first[0] = b;
+                    s_first[1] = in / len;
+                    s_first[2] = j;
+                    s_tiles0 = j * tpp;
+                    s_end = min((j + 1) * tpp, nt);
+                }
+                at += places;
+            }
+        } else {
+            const int64_t total = all[0];
+            run = (total + gridDim.x - 1) / gridDim.x;
+            v0 = run * blockIdx.x;
+            const int64_t v1 = min(v0 + run, total);
+            if (tid == 0 && v1 >= total) s_end = all[1];
+            int64_t at = before[0], tiles0 = before[1];
+            for (int b = b0; b < b1; ++b) {
+                if (per > 1) mine = attn_req(p, b);
+                const int64_t nt = tiles(mine), len = nt + Cfg::extra, places = segments(mine) * len;
+                auto tiles_before = [&](int64_t v) {   // tiles before place v of this request
+                    const int64_t g = v / len, in = v - g * len;
+                    return tiles0 + g * nt + max(in - Cfg::extra, (int64_t)0);
+                };
+                if (v0 >= at && v0 < at + places) {
+                    s_first[0] = b;
+                    s_first[1] = (v0 - at) / len;
+                    s_first[2] = (v0 - at) % len;
+                    s_tiles0 = tiles_before(v0 - at);
+                }
+                if (v1 < total && v1 >= at && v1 < at + places) s_end = tiles_before(v1 - at);
+                at += places;
+                tiles0 += segments(mine) * nt;
+            }
+            if (v0 >= total && tid == 0) s_tiles0 = all[1];
+        }
     }
     if (p.head_dim % 16) {   // the last 16-column step of Q K^T reads past the head size: zeros there
         uint4* z = reinterpret_cast<uint4*>(sq);
@@ -500,7 +552,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
     cur.enter(p);
     cur.h = (int)s_first[1] / cur.nrt;
     cur.rt = (int)s_first[1] - cur.h * cur.nrt;
-    cur.kt = max((int)s_first[2] - Cfg::extra, 0);
+    cur.kt = part_tiles ? (int)s_tiles0 : max((int)s_first[2] - Cfg::extra, 0);
     const int ksteps = (p.head_dim + 15) / 16;
     constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(128 >> 4) << 24);   // fp32 sums, M = 128
@@ -1014,7 +1066,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             const bool whole = kt_first == 0 && kt == nkt - 1;
             if (whole) scale_o = ll == 0.0f ? 0.0f : scale_o / ll;
             const int slot = 2 * blockIdx.x + (kt_first > 0 ? 0 : 1);   // a part: its segment began in an earlier run, or not
-            float* part = p.part_o + (int64_t)slot * RT * DT;
+            float4* part = reinterpret_cast<float4*>(p.part_o + (int64_t)slot * RT * DT);   // [column / 4][row]
             auto out_ptr = [&](int r, int d) {
                 const int at = c.rt * RT + r, i = p.group_div.div(at), g = at - i * p.group;
                 return static_cast<T*>(p.out) + (int64_t)(c.r.q0 + i) * p.out_stride_token +
@@ -1028,15 +1080,14 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             // 32 columns at a time, the row's two threads half the columns each. A thread's columns of a row are whole
             // 16-byte pieces, so they go out from its registers.
             T* out_row = row < rows ? out_ptr(row, 0) : nullptr;
-            float* part_row = part + (int64_t)row * DT;
             auto put8 = [&](int d, const float* v) {
                 if (row >= rows || d >= p.head_dim) return;
                 if (whole) {
                     *reinterpret_cast<uint4*>(out_row + d) =
                         make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
                 } else {
-                    *reinterpret_cast<float4*>(part_row + d) = make_float4(v[0], v[1], v[2], v[3]);
-                    *reinterpret_cast<float4*>(part_row + d + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                    part[d / 4 * RT + row] = make_float4(v[0], v[1], v[2], v[3]);
+                    part[(d / 4 + 1) * RT + row] = make_float4(v[4], v[5], v[6], v[7]);
                 }
             };
 #pragma unroll 1
@@ -1087,7 +1138,8 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             }
             if (owner) p.part_ml[(int64_t)slot * RT + row] = make_float2(mm, ll);
             const int64_t v_seg = seg->v_seg;
-            const int fc = (int)((v_seg + Cfg::extra) / run), lc = (int)((v_seg + nkt + Cfg::extra - 1) / run);   // runs with tiles of it
+            const int fc = part_tiles ? (int)v_seg : (int)((v_seg + Cfg::extra) / run);   // runs with tiles of it
+            const int lc = part_tiles ? fc + parts(nkt, part_tiles) - 1 : (int)((v_seg + nkt + Cfg::extra - 1) / run);
             int* counter = p.counters + 2 * fc + t;
             named_bar_sync(bar_group, GT);
             if (gtid == 0) {
