@@ -179,6 +179,8 @@ def read_status(device=None) -> int:
         if index == dev.index and s == stream:
             st = C.c_int32()
             _lib.call(dev, _lib.load().dsv41_read_status, buf.data_ptr(), stream, C.byref(st))
+            if st.value:
+                buf.zero_()   # the counters of a call that gave up are not back at zero
             worst = max(worst, st.value)
     return worst
 

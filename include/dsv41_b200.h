@@ -311,9 +311,10 @@ int dsv41_store_kv(const dsv41_store_kv_args* args, void* stream);
  * that sees nothing is 0 (lse -inf); so are the rows of a request with seq_lens[b] < its new tokens or >
  * max_keys. Query head hq reads KV head hq / (q_heads / kv_heads). head_dim a multiple of 8 up to 256. dtype of q,
  * caches and out: fp16 or bf16. max_new: upper bound on a request's new tokens (a hint that picks the row
- * tile). Addresses 16-byte aligned, strides (in elements) multiples of 8. lse [num_tokens][q_heads] (natural logarithm of the sums) or NULL. The workspace is zeroed once
- * after allocation; every call leaves its counters zero. One workspace serves one stream; its status word is
- * read with dsv41_read_status (1 = a bounded device wait ran out). */
+ * tile). Addresses 16-byte aligned, strides (in elements) multiples of 8. lse [num_tokens][q_heads] (natural
+ * logarithm of the sums) or NULL. The workspace is zeroed once after allocation; every call leaves its counters
+ * zero. One workspace serves one stream; its status word is read with dsv41_read_status (1 = a bounded device
+ * wait ran out: zero the workspace before the next call). */
 typedef struct dsv41_tree_attention_args {
     int32_t dtype, batch, num_tokens, max_new;
     int32_t q_heads, kv_heads, head_dim, page_size, num_pages, max_keys;
