@@ -31,7 +31,7 @@
 // 5.2 TB/s; 128 rows 161 us, 4.9 TB/s, 626 TFLOP/s; 256 rows 257 us, 783 TFLOP/s. The first two are bound by the key
 // stream and, at the ends of a run, by latency; the last by the softmax warps' issue (16 warps, a third of the issue
 // slots, exponentials at 40% of their pipe). Heads of 256 (floor 240 us): 275 us, 5.7 TB/s; 302 us; 561 us (two tiles of
-// 128 rows, a second trip of the keys), 717 TFLOP/s. Warp-level matrix instructions took 780 us for the first and reached
+// 128 rows, a second trip of the keys), 717 TFLOP/s; 192: 250 us, 4.7 TB/s (a quarter of the ring idle). Warp-level matrix instructions took 780 us for the first and reached
 // 120 TFLOP/s in the last. A call of one tile takes 15 us, most of it latencies one after the other: lengths, page
 // numbers, keys, two products, the row out.
 #pragma once
@@ -65,8 +65,8 @@ struct TcCfg {
     static constexpr int q_b = MT * q_tile_b;
     static constexpr int own = 32 / REP;                     // of 32 columns of O, those a repeat's warps put out
     static constexpr int stage_b = soft_warps * (32 - own) * 32 * 4;   // the others', on their way to their repeat
-    // what a segment costs beside its tiles (rows' loads, its end), in tiles. 1, 2, 3, 4, 5: 32 x 64 tokens of 4 rows over
-    // 1-8k keys 271, 246, 231, 228, 228 us; 16 x 5-13 tokens over 0.1-4k keys 54, 50, 50, 57, 56 us; long lengths within 2%
+    // what a segment costs beside its tiles (rows' loads, its end), in tiles. 2, 3, 5: 32 x 64 tokens of 4 rows over
+    // 1-8k keys 237, 228, 224 us; 16 x 5-13 tokens over 0.1-4k keys 50, 50, 54 us; long lengths within 1%
     static constexpr int extra = 3;
     static constexpr int off_b = 4 * kt * 8;                 // byte offsets of the keys of four tiles
     static constexpr int ml_b = MT * 2 * 128 * 8;

@@ -473,6 +473,16 @@ def test_head_sizes_over_128(dim, page, layout):
     check(build([190, 1], [64, 40], 5, 1, dim, page, dtype, seed=page, layout=layout), f"{dim} {page} 320 rows")
 
 
+@pytest.mark.parametrize("requests,ctx,new,heads,dim", [
+    (1, 9000, 3, 2, 64), (3, 1500, 10, 5, 128),        # few segments: parts of 4 tiles
+    (40, 2500, 1, 4, 64), (44, 1100, 2, 3, 192),       # more: parts of 8
+    (50, 3900, 1, 4, 64), (60, 1300, 1, 1, 256),       # runs of the line, several segments to a CTA
+    (200, 120, 1, 4, 128), (140, 1000, 1, 2, 64)])     # whole segments, more and fewer than the processors
+def test_cuts_of_the_work(requests, ctx, new, heads, dim):
+    lens = [max(ctx - 97 * (b % 5) + 13 * (b % 3), 0) for b in range(requests)]
+    check(build(lens, [new] * requests, heads, 1, dim, 64, torch.float16, seed=requests), f"{requests} x {ctx}")
+
+
 def test_keys_and_values_side_by_side():
     """Both caches as slices of one tensor: equal strides, neither contiguous."""
     s = build([70, 200], [5, 9], 8, 2, 128, 16, torch.float16, seed=21)
