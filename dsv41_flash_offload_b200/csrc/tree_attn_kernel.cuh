@@ -317,14 +317,23 @@ __device__ __noinline__ void find_nonfinite(const TreeAttnParams& p, const AttnR
 
 // Join of a segment's parts (runs fc .. lc): a thread takes 16 columns of a row, a batch of parts at a time with all its
 // loads in flight (one trip to L2 a batch), and rescales what it has as the softmax does. Rows r0 .. r0 + rows - 1 of
-// the row tile at c, by `threads` threads. A part is [column / 4][row][4]: neighbours in a warp are neighbouring rows
-// here and where it is written.
-template <typename T, int DT, int RT, typename Cursor>
-__device__ __noinline__ void join_parts(const TreeAttnParams& p, const Cursor& c, int fc, int lc, int r0, int rows, int thread,
-                                        int threads)
+// the row tile, by `threads` threads. A part is [column / 4][row][4]: neighbours in a warp are neighbouring rows
+// here and where it is written. All by value: what a function reads through a reference (the kernel's parameters, the
+// cursor) costs a trip to L2 a field and row (50 rows of 4 parts: 13000 cycles).
+struct JoinArgs {
+    const float2* ml;
+    const float4* o;
+    void* out;            // the request's first row, the KV head's first query head
+    float* lse;           // the same, or null
+    int64_t stride_token, stride_head;
+    FastDiv group_div;
+    int group, q_heads, head_dim, row0;   // row0: first row of the row tile
+};
+template <typename T, int DT, int RT>
+__device__ __noinline__ void join_parts(const JoinArgs a, int fc, int lc, int r0, int rows, int thread, int threads)
 {
     constexpr int kBatch = 4;
-    const int blocks = (p.head_dim + 15) / 16;
+    const int blocks = (a.head_dim + 15) / 16;
     for (int e = thread; e < rows * blocks; e += threads) {
         const int block = e / rows, r = r0 + e - block * rows;
         float mm = -INFINITY, ll = 0.0f, acc[16];
@@ -338,8 +347,8 @@ __device__ __noinline__ void join_parts(const TreeAttnParams& p, const Cursor& c
             for (int i = 0; i < kBatch; ++i) {
                 const int q = q0 + i;
                 const int64_t slot = 2 * q + (q == fc ? 1 : 0);
-                const float4* src = reinterpret_cast<const float4*>(p.part_o + slot * RT * DT) + block * 4 * RT + r;
-                v[i] = q <= lc ? __ldcg(p.part_ml + slot * RT + r) : make_float2(-INFINITY, 0.0f);
+                const float4* src = a.o + slot * (RT * DT / 4) + block * 4 * RT + r;
+                v[i] = q <= lc ? __ldcg(a.ml + slot * RT + r) : make_float2(-INFINITY, 0.0f);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) po[i][k] = q <= lc ? __ldcg(src + k * RT) : make_float4(0, 0, 0, 0);
             }
@@ -362,17 +371,16 @@ __device__ __noinline__ void join_parts(const TreeAttnParams& p, const Cursor& c
             }
         }
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-        const int row = c.rt * RT + r, i = p.group_div.div(row), g = row - i * p.group;
-        T* out = static_cast<T*>(p.out) + (int64_t)(c.r.q0 + i) * p.out_stride_token + (int64_t)(c.h * p.group + g) * p.out_stride_head;
+        const int row = a.row0 + r, i = a.group_div.div(row), g = row - i * a.group;
+        T* out = static_cast<T*>(a.out) + i * a.stride_token + g * a.stride_head + block * 16;
 #pragma unroll
         for (int j = 0; j < 16; j += 8)
-            if (block * 16 + j < p.head_dim)
-                *reinterpret_cast<uint4*>(out + block * 16 + j) =
+            if (block * 16 + j < a.head_dim)
+                *reinterpret_cast<uint4*>(out + j) =
                     make_uint4(pack2<T>(acc[j] * inv, acc[j + 1] * inv), pack2<T>(acc[j + 2] * inv, acc[j + 3] * inv),
                                pack2<T>(acc[j + 4] * inv, acc[j + 5] * inv), pack2<T>(acc[j + 6] * inv, acc[j + 7] * inv));
-        if (p.lse && block == 0)
-            p.lse[(int64_t)(c.r.q0 + i) * p.q_heads + c.h * p.group + g] =
-                ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+        if (a.lse && block == 0)
+            a.lse[(int64_t)i * a.q_heads + g] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
     }
 }
 
@@ -478,10 +486,12 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         }
         __syncthreads();
         int64_t before[kSums], all[kSums];
+        const int holders = ((p.batch + per - 1) / per + 31) / 32;   // warps that hold requests
 #pragma unroll
         for (int k = 0; k < kSums; ++k) {
             before[k] = inc[k] - sum[k], all[k] = 0;
-            for (int w = 0; w < Cfg::threads / 32; ++w) {
+#pragma unroll 1
+            for (int w = 0; w < holders; ++w) {
                 if (w < warp) before[k] += warp_sum[w][k];
                 all[k] += warp_sum[w][k];
             }
@@ -1150,7 +1160,15 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             }
             named_bar_sync(bar_group, GT);
             if (*reinterpret_cast<volatile int*>(s_last + t)) {
-                join_parts<T, DT, RT>(p, c, fc, lc, t * 128, min(rows - t * 128, 128), gtid, GT);
+                JoinArgs a;
+                a.ml = p.part_ml;
+                a.o = reinterpret_cast<const float4*>(p.part_o);
+                a.out = static_cast<T*>(p.out) + c.r.q0 * p.out_stride_token + (int64_t)c.h * p.group * p.out_stride_head;
+                a.lse = p.lse ? p.lse + (int64_t)c.r.q0 * p.q_heads + c.h * p.group : nullptr;
+                a.stride_token = p.out_stride_token, a.stride_head = p.out_stride_head;
+                a.group_div = p.group_div;
+                a.group = p.group, a.q_heads = p.q_heads, a.head_dim = p.head_dim, a.row0 = c.rt * RT;
+                join_parts<T, DT, RT>(a, fc, lc, t * 128, min(rows - t * 128, 128), gtid, GT);
                 if (gtid == 0) *counter = 0;   // ready for the next call
             }
             named_bar_sync(bar_group, GT);
