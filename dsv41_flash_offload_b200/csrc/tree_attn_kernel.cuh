@@ -6,7 +6,7 @@
 //                        128-byte swizzle the tensor cores read. Whole pages go by tensor copies (one or two warps, a lane
 //                        per page and 64 columns); page sizes that do not make up a tile are gathered key by key by four
 //                        warps of cp.async, whose issue rate then bounds a call (16 tokens x 8 rows over 4 x 64-128k keys:
-//                        323 us for 288, the latter now 279)
+//                        323 us for 288, the latter now 269)
 //   Q loaders            the rows of the segment
 //   two issuers (1 thread each)  S = Q K^T (A and B from shared memory) and O += P V (A from tensor memory, V read
 //                        as it lies, N-major), fp32 accumulators in tensor memory. One thread for both left the tensor
@@ -27,13 +27,13 @@
 // in flight, the deferral makes that rare. P is rounded to the cache's type (the second product's operand), which is
 // half a unit of each weight, as much as the output's own rounding; the sum of weights is of the unrounded ones.
 //
-// Measured, 4 requests of 32-64k keys, 8 KV heads of 128, bf16, pages of 64 (floor 120 us of HBM): 32 rows 150 us,
-// 5.2 TB/s; 128 rows 161 us, 4.9 TB/s, 626 TFLOP/s; 256 rows 257 us, 783 TFLOP/s. The first two are bound by the key
+// Measured, 4 requests of 32-64k keys, 8 KV heads of 128, bf16, pages of 64 (floor 120 us of HBM): 32 rows 146 us,
+// 5.4 TB/s; 128 rows 154 us, 5.1 TB/s, 651 TFLOP/s; 256 rows 248 us, 812 TFLOP/s. The first two are bound by the key
 // stream and, at the ends of a run, by latency; the last by the softmax warps' issue (16 warps, a third of the issue
-// slots, exponentials at 40% of their pipe). Heads of 256 (floor 240 us): 275 us, 5.7 TB/s; 302 us; 561 us (two tiles of
-// 128 rows, a second trip of the keys), 717 TFLOP/s; 192: 250 us, 4.7 TB/s (a quarter of the ring idle). Warp-level matrix instructions took 780 us for the first and reached
-// 120 TFLOP/s in the last. A call of one tile takes 15 us, most of it latencies one after the other: lengths, page
-// numbers, keys, two products, the row out.
+// slots, exponentials at 40% of their pipe). Heads of 256 (floor 240 us): 267 us, 5.9 TB/s; 285 us; 522 us (two tiles of
+// 128 rows, a second trip of the keys), 770 TFLOP/s; 192: 244 us, 4.8 TB/s (a quarter of the ring idle). Warp-level
+// matrix instructions took 780 us for the first of 256 and reached 120 TFLOP/s in the last. A call of one tile takes
+// 14 us, most of it latencies one after the other: lengths, page numbers, keys, two products, the row out.
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -66,7 +66,7 @@ struct TcCfg {
     static constexpr int own = 32 / REP;                     // of 32 columns of O, those a repeat's warps put out
     static constexpr int stage_b = soft_warps * (32 - own) * 32 * 4;   // the others', on their way to their repeat
     // what a segment costs beside its tiles (rows' loads, its end), in tiles. 2, 3, 5: 32 x 64 tokens of 4 rows over
-    // 1-8k keys 237, 228, 224 us; 16 x 5-13 tokens over 0.1-4k keys 50, 50, 54 us; long lengths within 1%
+    // 1-8k keys 237, 228, 224 us (before the join's last step); 16 x 5-13 tokens over 0.1-4k keys 50, 50, 54 us; long lengths within 1%
     static constexpr int extra = 3;
     static constexpr int off_b = 4 * kt * 8;                 // byte offsets of the keys of four tiles
     static constexpr int ml_b = MT * 2 * 128 * 8;
@@ -439,8 +439,8 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
     // ---- this CTA's run ----
     // Calls whose segments can each have CTAs of their own: segments of up to 2 * R tiles stay whole, longer ones are cut into
     // equal parts of R at most (R 4, or 8 where there is no room for 4; a place on the line is a CTA). Joining parts
-    // costs 5 to 10 us, a tile of a CTA alone 1: 3 requests of 50 rows over 13 tiles, 2 KV heads, took 43 us in parts of one
-    // tile and take 23 us, over 2 tiles 22 and 17 us; 8 segments of 16 tiles and 4 rows 20.5 and 21.5 us.
+    // costs about 5 us, a tile of a CTA alone 1: 3 requests of 50 rows over 13 tiles, 2 KV heads, took 43 us in parts of one
+    // tile and take 22 us, over 2 tiles 22 and 16 us; 8 segments of 16 tiles and 4 rows 20.5 both ways.
     // Others: a segment of nkt tiles costs what nkt + extra tiles do (its rows' loads, its end), so the runs are cut from a
     // line on which each segment begins with `extra` empty places.
     // Every thread sums its requests' places and tiles; the one whose request holds the run's first place, and the
