@@ -1206,7 +1206,7 @@ static bool cache_map(CUtensorMap* m, const void* base, const TreeAttnParams& p,
 {
     auto fn = tensor_map_fn();
     if (!fn) return false;
-    auto bytes = [](int64_t s) { return (cuuint64_t)(s > 8 ? s : 8) * 2; };   // (the stride of a dimension of one may be anything)
+    auto bytes = [](int64_t s) { return (cuuint64_t)(s > 8 ? s : 8) * 2; };   // (0 is left to dimensions of one, whose stride counts for nothing)
     const int h = p.slot_first ? 2 : 1, t = 3 - h;   // dimension of heads, of slots
     cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, 0, 0, (cuuint64_t)p.num_pages}, strides[3] = {0, 0, bytes(p.stride_page)};
     cuuint32_t box[4] = {64, 1, 1, 1};
@@ -1251,13 +1251,16 @@ template <typename T, int DT>
 static cudaError_t launch_tc_dim(TreeAttnParams p, int max_rows, cudaStream_t st)
 {
     // Whole pages go by tensor copies where a tile is whole pages (or a page whole tiles) of at least a swizzle atom's
-    // 8 rows; other page sizes are gathered key by key.
+    // 8 rows; other page sizes are gathered key by key, and so are caches that repeat in memory (a view whose heads, slots
+    // or pages are one: a map has no stride of 0).
     constexpr int kt = TcCfg<DT, 1, 1, true>::kt;
     constexpr bool bf16 = !std::is_same<T, __half>::value;
     CUtensorMap k{}, v{};
     p.box = p.page_size < kt ? p.page_size : kt;
     p.slot_first = p.stride_slot < p.stride_head;
-    const bool pages = p.num_pages > 0 && p.box >= 8 && kt % p.box == 0 && p.page_size % p.box == 0 &&
+    const bool repeats = (p.stride_head == 0 && p.kv_heads > 1) || (p.stride_slot == 0 && p.page_size > 1) ||
+                         (p.stride_page == 0 && p.num_pages > 1);
+    const bool pages = p.num_pages > 0 && !repeats && p.box >= 8 && kt % p.box == 0 && p.page_size % p.box == 0 &&
                        cache_map(&k, p.k_cache, p, bf16) && cache_map(&v, p.v_cache, p, bf16);
     return pages ? launch_tc_rows<T, DT, true>(p, k, v, max_rows, st) : launch_tc_rows<T, DT, false>(p, k, v, max_rows, st);
 }

@@ -1,0 +1,24 @@
+"""The paged operators where inputs are at their ends, against plain restatements in 64 bits, with the bounds of
+test_gpu_paged.py."""
+import pytest
+import torch
+
+from dsv41_flash_offload_b200 import paged
+from test_gpu_paged import attend, build, reference
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("page", [8, 16, 24, 64, 128])
+@pytest.mark.parametrize("dim", [64, 192])
+def test_caches_that_repeat_in_memory(page, dim):
+    """One KV head read by all, one slot for a whole page, one page for all: expanded views are what they show."""
+    s = build([70, 300], [5, 9], 8, 2, dim, page, torch.float16, seed=page)
+    pages = s["kc"].shape[0]
+    for cut, full in ((lambda c: c[:, :, :1], (pages, page, 2, dim)), (lambda c: c[:, :1], (pages, page, 2, dim)),
+                      (lambda c: c[:1], (pages, page, 2, dim))):
+        views = {n: cut(s[n]).expand(full) for n in ("kc", "vc")}
+        own = dict(s, **{n: v.contiguous() for n, v in views.items()})
+        ref, bound, _ = reference(own)
+        out = attend(dict(s, **views))
+        assert bool(((out.cpu().double() - ref).abs() <= bound).all())
