@@ -17,6 +17,9 @@ static_assert(kTabNoPages == DSV41_TABLES_NO_PAGES && kTabTooWide == DSV41_TABLE
 
 static bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
+// a dimension whose entries are all one place
+static bool repeats(int64_t stride, int extent) { return stride == 0 && extent > 1; }
+
 static int launched(cudaError_t err, const char* what)
 {
     if (err == cudaSuccess) return DSV41_OK;
@@ -160,6 +163,8 @@ int dsv41_store_kv(const dsv41_store_kv_args* a, void* stream)
                                a->stride_page, a->stride_slot, a->stride_head};
     for (int64_t s : strides)
         if (s < 0 || s % 8) return set_error(DSV41_E_INVALID, "stride %lld is not a multiple of 8 elements", (long long)s);
+    if (repeats(a->stride_page, a->num_pages) || repeats(a->stride_slot, a->page_size) || repeats(a->stride_head, a->kv_heads))
+        return set_error(DSV41_E_INVALID, "the caches repeat in memory: a stride of 0 cannot be stored through");
     StoreKvParams p{};
     p.k = a->k;
     p.v = a->v;
@@ -220,6 +225,8 @@ int dsv41_tree_attention(const dsv41_tree_attention_args* a, void* workspace, si
                                a->stride_page, a->stride_slot, a->stride_head};
     for (int64_t s : strides)
         if (s < 0 || s % 8) return set_error(DSV41_E_INVALID, "stride %lld is not a multiple of 8 elements", (long long)s);
+    if (repeats(a->out_stride_token, a->num_tokens) || repeats(a->out_stride_head, a->q_heads))
+        return set_error(DSV41_E_INVALID, "out repeats in memory: a stride of 0 cannot be written through");
     if (!std::isfinite(a->scale)) return set_error(DSV41_E_INVALID, "scale %g", a->scale);
     TreeAttnParams p{};
     p.q = a->q;

@@ -3,8 +3,8 @@ test_gpu_paged.py."""
 import pytest
 import torch
 
-from dsv41_flash_offload_b200 import paged
-from test_gpu_paged import attend, build, reference
+from dsv41_flash_offload_b200 import Dsv41Error, paged
+from test_gpu_paged import DEV, attend, build, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +22,14 @@ def test_caches_that_repeat_in_memory(page, dim):
         ref, bound, _ = reference(own)
         out = attend(dict(s, **views))
         assert bool(((out.cpu().double() - ref).abs() <= bound).all())
+
+
+def test_outputs_that_repeat_in_memory_are_refused():
+    s = build([20], [3], 4, 2, 64, 16, torch.float16)
+    k = torch.zeros(3, 2, 64, dtype=torch.float16, device=DEV)
+    slots = torch.arange(3, device=DEV)
+    heads = torch.zeros(4, 16, 1, 64, dtype=torch.float16, device=DEV).expand(4, 16, 2, 64)
+    tokens = torch.zeros(1, 4, 64, dtype=torch.float16, device=DEV).expand(3, 4, 64)
+    for bad in (lambda: paged.store_kv(k, k, slots, heads, heads), lambda: attend(s, out=tokens)):
+        with pytest.raises((ValueError, Dsv41Error)):
+            bad()
