@@ -207,8 +207,9 @@ int dsv41_tree_attention(const dsv41_tree_attention_args* a, void* workspace, si
     if (a->num_tokens < 0 || a->max_new < 0) return set_error(DSV41_E_INVALID, "num_tokens=%d max_new=%d", a->num_tokens, a->max_new);
     if (a->kv_heads < 1 || a->q_heads < a->kv_heads || a->q_heads % a->kv_heads)
         return set_error(DSV41_E_INVALID, "q_heads=%d is not a multiple of kv_heads=%d", a->q_heads, a->kv_heads);
-    if ((int64_t)a->num_tokens * a->q_heads > 0x7fffffffll)
-        return set_error(DSV41_E_INVALID, "num_tokens * q_heads over 2^31 - 1");
+    // the kernel counts a request's rows and rounds them up to whole tiles in 32 bits
+    if ((int64_t)a->num_tokens * a->q_heads > 0x7fffffffll - 255)
+        return set_error(DSV41_E_INVALID, "num_tokens * q_heads over 2^31 - 256");
     if (a->page_size < 1 || a->num_pages < 0 || a->max_keys < 0)
         return set_error(DSV41_E_INVALID, "page_size=%d num_pages=%d max_keys=%d", a->page_size, a->num_pages, a->max_keys);
     if (a->max_keys > 0x7fffff00) return set_error(DSV41_E_INVALID, "max_keys=%d", a->max_keys);

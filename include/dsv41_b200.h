@@ -290,7 +290,7 @@ typedef struct dsv41_step_tables_args {
 int dsv41_step_tables(const dsv41_step_tables_args* args, void* stream);
 
 /* cache[slots[t]] = k[t], v[t]; a slot outside the cache (-1) stores nothing. 16-bit elements; head_dim a
- * multiple of 8, addresses 16-byte aligned, strides (in elements) multiples of 8. Slots that repeat within a call
+ * multiple of 8, addresses 16-byte aligned, strides (in elements) multiples of 8, the caches' not 0. Slots that repeat within a call
  * leave one of their tokens, whichever. */
 typedef struct dsv41_store_kv_args {
     int32_t num_tokens, kv_heads, head_dim, num_pages, page_size;
@@ -311,7 +311,8 @@ int dsv41_store_kv(const dsv41_store_kv_args* args, void* stream);
  * that sees nothing is 0 (lse -inf); so are the rows of a request with seq_lens[b] < its new tokens or >
  * max_keys. Query head hq reads KV head hq / (q_heads / kv_heads). head_dim a multiple of 8 up to 256. dtype of q,
  * caches and out: fp16 or bf16. max_new: upper bound on a request's new tokens (a hint that picks the row
- * tile). Addresses 16-byte aligned, strides (in elements) multiples of 8. lse [num_tokens][q_heads] (natural
+ * tile); num_tokens * q_heads up to 2^31 - 256. Addresses 16-byte aligned, strides (in elements) multiples of 8, those of
+ * out not 0. lse [num_tokens][q_heads] (natural
  * logarithm of the sums) or NULL. The workspace is zeroed once after allocation; every call leaves its counters
  * zero. One workspace serves one stream; its status word is read with dsv41_read_status (1 = a bounded device
  * wait ran out: zero the workspace before the next call). */
