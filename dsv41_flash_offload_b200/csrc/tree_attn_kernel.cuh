@@ -251,10 +251,11 @@ __device__ __noinline__ bool clear_nonfinite(unsigned char* base, int row0, int 
 }
 
 // The same for a tile of whole pages, by `threads` threads together, before its product: values past the last key
-// (rows from `rows` on, which may hold anything) are cleared too, without a mark. The mark is set before a value is
-// cleared: who finds it cleared (another group of threads looks at the same tile) finds the mark.
+// (rows from `rows` on, which may hold anything) are cleared too; `mark` is for keys that rows can see, `touched` for all.
+// Both are set before a value is cleared: who finds it cleared (another group of threads looks at the same tile)
+// finds them set.
 template <typename T, int KT, int N>
-__device__ __noinline__ void clear_tile(unsigned char* unit, int thread, int threads, int rows, volatile int* mark, int value)
+__device__ __noinline__ void clear_tile(unsigned char* unit, int thread, int threads, int rows, volatile int* mark, volatile int* touched, int value)
 {
     constexpr uint32_t kExp = exp_bits<T>() * 0x10001u;
     uint32_t least = 0xffffffffu;
@@ -269,6 +270,7 @@ __device__ __noinline__ void clear_tile(unsigned char* unit, int thread, int thr
         for (int i = 0; i < N; ++i) {
             uint4 v = at[i * threads];
             if (!any_nonfinite<T>(v)) continue;
+            *touched = value;
             if (((thread + i * threads) >> 3) % KT < rows) *mark = value;   // 128-byte rows, KT of them a block
             __threadfence_block();
             v.x = finite2<T>(v.x), v.y = finite2<T>(v.y), v.z = finite2<T>(v.z), v.w = finite2<T>(v.w);
@@ -409,7 +411,8 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
     uint64_t* pv_done = p_full + 2;        // [2] the product of a P buffer is done
     uint64_t* all_done = pv_done + 2;      // [2] per issuer
     int* dirty = reinterpret_cast<int*>(all_done + 2);   // [NU] 1 + ring position of a unit that held infinities or NaN
-    int* s_last = dirty + NU;              // [2]
+    int* touched = dirty + NU;             // [NU] the same, of one in which any were cleared
+    int* s_last = touched + NU;            // [2]
     volatile int* abort_flag = s_last + 2;
     uint32_t* tmem_slot = const_cast<uint32_t*>(reinterpret_cast<volatile uint32_t*>(abort_flag)) + 1;
 
@@ -419,7 +422,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         for (int i = 0; i < NU; ++i) {
             mbar_init(&full[i], Cfg::prod_warps);
             mbar_init(&empty[i], 1);
-            dirty[i] = 0;
+            dirty[i] = touched[i] = 0;
         }
         mbar_init(q_full, Cfg::q_warps);
         mbar_init(q_free, 1);
@@ -844,7 +847,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         const uint32_t lanes = tmem + ((uint32_t)(wq * 32) << 16);
         const int row = t * 128 + tw * 32 + lane;                     // row within the row tile
         const int gtid = tid - t * GT;                                // thread within the row tile's group
-        const int bar_group = 1 + t, bar_pair = 4 + t * 4 + wq, bar_half = 12 + half;   // 3: the producers
+        const int bar_group = 1 + t, bar_pair = 4 + t * 4 + wq, bar_half = 12 + half;   // 3: the producers, 14: both row tiles
         if (REP > 1 && half == 0) {   // P is zero outside the repeat's keys, for good
             uint32_t z[16];
 #pragma unroll
@@ -1001,8 +1004,13 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                 const int n = v_pos(it);
                 wait_warp(&full[n % NU], (n / NU) & 1);
                 if (TMA) {
-                    clear_tile<T, KT, Cfg::unit_b / 16 / GT>(su + (n % NU) * Cfg::unit_b, gtid, GT, ctx + seg->c.r.n - pos0, dirty + n % NU, n + 1);
+                    clear_tile<T, KT, Cfg::unit_b / 16 / GT>(su + (n % NU) * Cfg::unit_b, gtid, GT, ctx + seg->c.r.n - pos0, dirty + n % NU,
+                                                             touched + n % NU, n + 1);
                     named_bar_sync(bar_group, GT);
+                    // Where two groups look at the same tile, what one cleared the other finds cleared, but only the one that did
+                    // has ordered it before the tensor cores' reads: neither goes on before both have. (In every tile
+                    // with new tokens, cleared or not, that wait cost 222 -> 231 us on 32 x 64 tokens over 1-8k keys.)
+                    if (MT == 2 && rows > 128 && *reinterpret_cast<volatile int*>(touched + n % NU) == n + 1) named_bar_sync(14, 2 * GT);
                     __syncwarp();
                 }
                 fix = live && *reinterpret_cast<volatile int*>(dirty + n % NU) == n + 1;

@@ -1,5 +1,7 @@
 """The paged operators where inputs are at their ends, against plain restatements in 64 bits, with the bounds of
 test_gpu_paged.py."""
+import math
+
 import pytest
 import torch
 
@@ -7,6 +9,26 @@ from dsv41_flash_offload_b200 import Dsv41Error, paged
 from test_gpu_paged import DEV, attend, build, reference
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_two_row_tiles_share_a_cleared_tile(page, dtype):
+    """Rows of both row tiles, many times over: what one group of threads clears is cleared for the other's product too."""
+    s = build([60, 190], [64, 61], 4, 1, 128, page, dtype, seed=page)
+    clean = attend(s)
+    hidden = []                                      # tokens that only few others see: leaves of their trees
+    for b, base in ((0, 0), (1, 64)):
+        bits = [int(w) for w in s["mask"][base:base + s["new"][b], 0]]
+        leaves = [j for j in range(s["new"][b]) if sum(w >> j & 1 for w in bits) == 1]
+        for j in leaves:
+            at = s["ctx"][b] + j
+            s["vc"][int(s["table"][b, at // page]), at % page] = math.nan
+            hidden.append(base + j)
+    rest = [i for i in range(125) if i not in hidden]
+    for _ in range(30):
+        got = attend(s)
+        assert torch.equal(got[rest], clean[rest]) and bool(torch.isnan(got[hidden]).all())
 
 
 @pytest.mark.parametrize("page", [8, 16, 24, 64, 128])
