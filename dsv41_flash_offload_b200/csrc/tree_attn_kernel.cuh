@@ -197,12 +197,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ uint32_t tc_ld1(uint32_t taddr)
-{
-    uint32_t r;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n tcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(taddr) : "memory");
-    return r;
-}
 __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r)
 {
     asm volatile(
@@ -223,8 +217,8 @@ __device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t* r)
 // instruction cache.
 
 // Infinities and NaN among new tokens' values would reach rows that do not see them (0 * NaN): zero those of this
-// thread's pieces of a tile and say whether there were any; the softmax warps add them to the rows that do see them.
-// A first look only: a half-word's exponent bits, turned, are zero in a value that is not finite, and the minimum over
+// thread's pieces of a tile and say whether there were any; the softmax warps give them to the rows that do see them at
+// the end of the segment (see_nonfinite). A first look only: a half-word's exponent bits, turned, are zero in a value that is not finite, and the minimum over
 // all words finds one.
 template <typename T, int ROWS>
 __device__ __noinline__ bool clear_nonfinite(unsigned char* base, int row0, int step, int chunk)
@@ -280,41 +274,95 @@ __device__ __noinline__ void clear_tile(unsigned char* unit, int thread, int thr
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// Infinities and NaN of new tokens entered the product as zeros. A row that sees such a value takes p * v, which is
-// +inf, -inf or NaN (also where p is 0): two bits per row and column, +inf and -inf, both for NaN.
-// flags[k]: of columns col0 + k * step .. + 15, low half +inf, high half -inf. Keys x0 .. x1 - 1 of the tile at pos0.
-template <typename T, int NF, typename PCol>
-__device__ __noinline__ void find_nonfinite(const TreeAttnParams& p, const AttnReq& r, int b, int h, int tok, int pos0, int x0,
-                                            int x1, int col0, int step, PCol p_col, uint32_t (&flags)[NF])
+// Infinities and NaN of a row's sums, from the cache itself. In the products 0 * inf is NaN where the definition has no
+// such term: a repeat's P is zero outside its share of a tile's keys, a weight or a rescale may be zero in 16 or 32 bits only.
+// And new tokens' values entered them as zeros. Here a weight counts as more than zero unless its score is -inf, and
+// then 0 * inf is NaN (products of finite numbers are taken as finite). By a whole warp, a row a lane: columns col0 ..
+// col0 + n - 1 of O, scaled on the way; keys x0 .. x1 - 1, 32 at a time, a lane each, then those with such values in
+// turn, for all rows. Only segments whose sums are not finite, or that held such values of new tokens (`cleared`), come
+// here: 4 tokens over 20000 keys that are full of them take 0.6 ms. 16 columns at a time: with 32 this function's
+// registers made the caller spill its own (32 x 64 tokens over 1-8k keys 222 -> 334 us).
+template <typename T, int RT, int KT>
+__device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const UnitCursor<RT, KT>* cursor, int row, bool live, bool cleared, int x0, int x1,
+                                              int col0, int n, float scale, uint32_t o_at)
 {
-#pragma unroll
-    for (int k = 0; k < NF; ++k) flags[k] = 0;
-    const int ctx = r.seq - r.n;
+    const UnitCursor<RT, KT> c = *cursor;
+    const int lane = threadIdx.x & 31, ctx = c.r.seq - c.r.n;
+    const int at = c.rt * RT + row, i = p.group_div.div(at), g = at - i * p.group;
+    const T* q = static_cast<const T*>(p.q) + (int64_t)(c.r.q0 + i) * p.q_stride_token + (int64_t)(c.h * p.group + g) * p.q_stride_head;
+    const T* k_head = static_cast<const T*>(p.k_cache) + c.h * p.stride_head;
+    auto nonfinite = [](const T* from, int count) {
+        bool bad = false;
+        for (int d = 0; d < count; d += 8) bad |= any_nonfinite<T>(*reinterpret_cast<const uint4*>(from + d));
+        return bad;
+    };
+    const bool q_bad = live && nonfinite(q, p.head_dim);
 #pragma unroll 1
-    for (int x = x0; x < min(r.seq - pos0, x1); ++x) {
-        const int pos = pos0 + x, pg = p.page_div.div(pos);
-        const int id = p.block_table[(int64_t)b * p.table_stride + pg];
-        if ((unsigned)id >= (unsigned)p.num_pages) continue;
-        const T* src = static_cast<const T*>(p.v_cache) + id * p.stride_page + (pos - pg * p.page_size) * p.stride_slot + h * p.stride_head;
-        __syncwarp();
-        const float2 pp = unpack2<T>(tc_ld1(p_col(x)));
-        const bool zero = (x & 1 ? pp.y : pp.x) == 0.0f;
-        if (!(seen_window(p, r, tok, pos - ctx) & 1)) continue;
+    for (int col = col0; col < min(col0 + n, p.head_dim); col += 16) {
+        const int cols = min(p.head_dim - col, 16);
+        const T* v_head = static_cast<const T*>(p.v_cache) + c.h * p.stride_head + col;
+        float o[16];
+        tc_ld16(o_at + col, o);
+        bool need = cleared;
 #pragma unroll
-        for (int k = 0; k < NF; ++k) {
-            const int col = col0 + k * step;
+        for (int j = 0; j < 16; ++j) need |= j < cols && !(fabsf(o[j]) < INFINITY);
+        need = need && live;
+        const uint32_t all = (1u << cols) - 1;
+        uint32_t plus = 0, minus = 0;   // bit j: column col + j holds +inf, -inf; both: NaN
 #pragma unroll 1
-            for (int j = 0; j < 8; ++j) {
-                if (col + 2 * j >= p.head_dim) break;
-                const uint32_t raw = reinterpret_cast<const uint32_t*>(src)[col / 2 + j];
-                if (raw == finite2<T>(raw)) continue;
-                const float2 v = unpack2<T>(raw);
-                if (!(fabsf(v.x) < INFINITY)) flags[k] |= (v.x < 0 && !zero ? 0u : 1u << (2 * j)) | (v.x > 0 && !zero ? 0u : 0x10000u << (2 * j));
-                if (!(fabsf(v.y) < INFINITY)) flags[k] |= (v.y < 0 && !zero ? 0u : 2u << (2 * j)) | (v.y > 0 && !zero ? 0u : 0x20000u << (2 * j));
+        for (int base = x0; base < x1; base += 32) {
+            if (!__any_sync(0xffffffffu, need && (plus & minus) != all)) break;
+            const int pos = base + lane;
+            int64_t off = 0;
+            bool hit = false, k_bad = false;
+            if (pos < x1) {
+                const int pg = p.page_div.div(pos), id = p.block_table[(int64_t)c.b * p.table_stride + pg];
+                if ((unsigned)id < (unsigned)p.num_pages) {
+                    off = id * p.stride_page + (pos - pg * p.page_size) * p.stride_slot;
+                    hit = nonfinite(v_head + off, cols);
+                    if (hit) k_bad = nonfinite(k_head + off, p.head_dim);
+                }
             }
+            uint32_t hits = __ballot_sync(0xffffffffu, hit);
+            const uint32_t bad_keys = __ballot_sync(0xffffffffu, k_bad);
+            while (hits) {
+                const int l = __ffs(hits) - 1;
+                hits &= hits - 1;
+                const int64_t key = __shfl_sync(0xffffffffu, off, l);
+                if (!need || !(seen_window(p, c.r, i, base + l - ctx) & 1)) continue;
+                bool zero = false;
+                if (q_bad || ((bad_keys >> l) & 1)) {
+                    float score = 0.0f;
+#pragma unroll 1
+                    for (int d = 0; d < p.head_dim; d += 2) {
+                        const float2 u = unpack2<T>(*reinterpret_cast<const uint32_t*>(q + d)),
+                                     w = unpack2<T>(*reinterpret_cast<const uint32_t*>(k_head + key + d));
+                        score = fmaf(u.x, w.x, fmaf(u.y, w.y, score));
+                    }
+                    zero = (p.flip ? -score : score) == -INFINITY;
+                }
+#pragma unroll 1
+                for (int j = 0; j < cols; j += 2) {
+                    const uint32_t raw = *reinterpret_cast<const uint32_t*>(v_head + key + j);
+                    if (raw == finite2<T>(raw)) continue;
+                    const float2 w = unpack2<T>(raw);
+                    if (!(fabsf(w.x) < INFINITY)) plus |= w.x < 0 && !zero ? 0u : 1u << j, minus |= w.x > 0 && !zero ? 0u : 1u << j;
+                    if (!(fabsf(w.y) < INFINITY)) plus |= w.y < 0 && !zero ? 0u : 2u << j, minus |= w.y > 0 && !zero ? 0u : 2u << j;
+                }
+            }
+            __syncwarp();
         }
+        __syncwarp();
+        tc_ld16(o_at + col, o);
+        uint32_t u[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const bool up = (plus >> j) & 1, down = (minus >> j) & 1;
+            u[j] = __float_as_uint(up && down ? NAN : up ? INFINITY : down ? -INFINITY : scale == 0.0f ? 0.0f : o[j] * scale);
+        }
+        tc_st16(o_at + col, u);
+        tc_wait_st();
     }
-    __syncwarp();
 }
 
 // Join of a segment's parts (runs fc .. lc): a thread takes 16 columns of a row, a batch of parts at a time with all its
@@ -370,6 +418,31 @@ __device__ __noinline__ void join_parts(const JoinArgs a, int fc, int lc, int r0
                 for (int k = 0; k < 4; ++k)
                     acc[4 * k] += po[i][k].x * w, acc[4 * k + 1] += po[i][k].y * w, acc[4 * k + 2] += po[i][k].z * w,
                         acc[4 * k + 3] += po[i][k].w * w;
+            }
+        }
+        // 0 * inf is NaN where a part's weight vanishes in 32 bits: what the parts hold of infinities and NaN itself instead
+        float test = 0.0f;   // NaN if a sum is not finite (columns past the head size hold anything)
+#pragma unroll
+        for (int j = 0; j < 16; j += 8)
+            if (block * 16 + j < a.head_dim)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) test = fmaf(acc[j + c], 0.0f, test);
+        if (__builtin_expect(test != 0.0f, 0)) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float4 bad = make_float4(0, 0, 0, 0);
+#pragma unroll 1
+                for (int q = fc; q <= lc; ++q) {
+                    const float4 v = __ldcg(a.o + (int64_t)(2 * q + (q == fc ? 1 : 0)) * (RT * DT / 4) + (block * 4 + k) * RT + r);
+                    if (!(fabsf(v.x) < INFINITY)) bad.x += v.x;
+                    if (!(fabsf(v.y) < INFINITY)) bad.y += v.y;
+                    if (!(fabsf(v.z) < INFINITY)) bad.z += v.z;
+                    if (!(fabsf(v.w) < INFINITY)) bad.w += v.w;
+                }
+                if (bad.x != 0.0f) acc[4 * k] = bad.x;
+                if (bad.y != 0.0f) acc[4 * k + 1] = bad.y;
+                if (bad.z != 0.0f) acc[4 * k + 2] = bad.z;
+                if (bad.w != 0.0f) acc[4 * k + 3] = bad.w;
             }
         }
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
@@ -455,6 +528,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
     struct SegState {
         Cursor c;
         int64_t v_seg;   // place on the line where the segment begins
+        int cleared;     // its tiles held infinities or NaN of new tokens
     };
     __shared__ SegState s_seg[Cfg::soft_warps];
     int64_t run, v0;
@@ -866,6 +940,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         SegState* const seg = s_seg + warp;
         seg->c = cur;
         seg->v_seg = v0 - s_first[2];
+        seg->cleared = 0;
         __syncwarp();
         int kt = cur.kt, nkt = cur.nkt, kt_first = kt;
         int rows = min(RT, cur.r.n * p.group - cur.rt * RT);
@@ -879,6 +954,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                 c.next(p);
                 seg->c = c;
                 seg->v_seg += nkt + Cfg::extra;
+                seg->cleared = 0;
                 __syncwarp();
                 kt = kt_first = 0;
                 nkt = c.nkt;
@@ -999,7 +1075,6 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                 l += (s0 + s1) + (s2 + s3);
                 tc_wait_st();
             }
-            bool fix = false;
             if (__builtin_expect(tail, 0)) {
                 const int n = v_pos(it);
                 wait_warp(&full[n % NU], (n / NU) & 1);
@@ -1013,49 +1088,12 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                     if (MT == 2 && rows > 128 && *reinterpret_cast<volatile int*>(touched + n % NU) == n + 1) named_bar_sync(14, 2 * GT);
                     __syncwarp();
                 }
-                fix = live && *reinterpret_cast<volatile int*>(dirty + n % NU) == n + 1;
+                if (*reinterpret_cast<volatile int*>(dirty + n % NU) == n + 1) seg->cleared = 1;
             }
-            if (__builtin_expect(fix, 0)) {
-                // found now, while P is there, and added to O after the product
-                constexpr int kFix = DT / 16 / SPLIT;
-                uint32_t flags[kFix];
-                if (SPLIT == 2) {   // this thread's columns need P of all the row's keys
-                    tcf_before();
-                    named_bar_sync(bar_pair, 64);
-                    tcf_after();
-                }
-                const Cursor c = seg->c;
-                find_nonfinite<T>(p, c.r, c.b, c.h, token(), pos0, rep * (KT / REP), (rep + 1) * (KT / REP), half * 16, SPLIT * 16,
-                                  [=](int x) { return lanes + Cfg::p_col(buf, x); }, flags);
-                tcf_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[buf]);
-                __syncwarp();
-                wait_warp(&pv_done[buf], par);
-                tcf_after();
-#pragma unroll
-                for (int k = 0; k < kFix; ++k) {
-                    if (!__any_sync(0xffffffffu, flags[k] != 0)) continue;
-                    const uint32_t at = lanes + Cfg::o_col(t) + (k * SPLIT + half) * 16;
-                    float o[16];
-                    tc_ld16(at, o);
-                    uint32_t u[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        if ((flags[k] >> j) & 1) o[j] += INFINITY;
-                        if ((flags[k] >> (16 + j)) & 1) o[j] -= INFINITY;
-                        u[j] = __float_as_uint(o[j]);
-                    }
-                    tc_st16(at, u);
-                }
-                tc_wait_st();
-                tcf_before();
-            } else {
-                tcf_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[buf]);
-                __syncwarp();
-            }
+            tcf_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[buf]);
+            __syncwarp();
             ++done;
             if (__builtin_expect(!last, 1)) continue;
 
@@ -1095,6 +1133,27 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                 p.lse[(int64_t)(c.r.q0 + i) * p.q_heads + c.h * p.group + g] =
                     sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
             };
+            constexpr int kCols = DT / SPLIT;   // of this thread
+            float scale = scale_o, test = 0.0f;
+#pragma unroll 1
+            for (int col = half * kCols; col < half * kCols + kCols; col += 32) {   // test: NaN if a column is not finite
+                float o[32];
+                __syncwarp();
+                tc_ld<32>(lanes + Cfg::o_col(t) + col, o);
+#pragma unroll
+                for (int j = 0; j < 32; j += 8)
+                    if (col + j < p.head_dim)
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) test = fmaf(o[j + x], 0.0f, test);
+            }
+            // (a sum of weights that is NaN makes the row NaN by itself)
+            const bool cleared = seg->cleared;
+            const bool odd = (cleared || test != 0.0f) && row < rows && ll == ll;
+            if (__builtin_expect(__any_sync(0xffffffffu, odd), 0)) {
+                settle_nonfinite<T, RT, KT>(p, &seg->c, min(row, rows - 1), odd, cleared, kt_first * KT, min((kt + 1) * KT, c.r.seq), half * kCols,
+                                            kCols, scale, lanes + Cfg::o_col(t));
+                scale = 1.0f;
+            }
             // 32 columns at a time, the row's two threads half the columns each. A thread's columns of a row are whole
             // 16-byte pieces, so they go out from its registers.
             T* out_row = row < rows ? out_ptr(row, 0) : nullptr;
@@ -1114,7 +1173,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                 __syncwarp();
                 tc_ld<32>(lanes + Cfg::o_col(t) + col, o);   // columns past the head size hold anything: not put out
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = scale_o == 0.0f ? 0.0f : o[j] * scale_o;
+                for (int j = 0; j < 32; ++j) o[j] = scale == 0.0f ? 0.0f : o[j] * scale;
                 if (REP == 1) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 8) put8(col + j, o + j);

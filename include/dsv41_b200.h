@@ -307,8 +307,9 @@ int dsv41_store_kv(const dsv41_store_kv_args* args, void* stream);
 /* out[t][hq] = softmax(scale * q . k) v over the keys that token t of its request sees. Request b owns rows
  * cu_lens[b] .. cu_lens[b + 1] - 1 of q, its keys are the first seq_lens[b] of its pages, the last of them its
  * new tokens. Token i sees the whole context and, with tree_mask, the new tokens of its bits; without, the
- * new tokens up to itself. Keys and values that a row does not see never reach it, whatever they hold. A row
- * that sees nothing is 0 (lse -inf); so are the rows of a request with seq_lens[b] < its new tokens or >
+ * new tokens up to itself. Keys and values that a row does not see never reach it, whatever they hold. Infinite and NaN
+ * values that it sees reach it as the definition has it: a weight is zero only where the score is -inf (0 * inf is
+ * NaN). A row that sees nothing, or only scores of -inf, is 0 (lse -inf); so are the rows of a request with seq_lens[b] < its new tokens or >
  * max_keys. Query head hq reads KV head hq / (q_heads / kv_heads). head_dim a multiple of 8 up to 256. dtype of q,
  * caches and out: fp16 or bf16. max_new: upper bound on a request's new tokens (a hint that picks the row
  * tile); num_tokens * q_heads up to 2^31 - 256. Addresses 16-byte aligned, strides (in elements) multiples of 8, those of

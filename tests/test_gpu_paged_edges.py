@@ -6,9 +6,128 @@ import pytest
 import torch
 
 from dsv41_flash_offload_b200 import Dsv41Error, paged
-from test_gpu_paged import DEV, attend, build, reference
+from test_gpu_paged import DEV, HALF_UNIT, attend, build, reference
 
 pytestmark = pytest.mark.gpu
+
+
+def nonfinite_reference(s, scale=None):
+    """The definition in 64 bits, key by key: what a row sees of infinities and NaN, and nothing else."""
+    q, kc, vc = (s[n].cpu().double() for n in ("q", "kc", "vc"))
+    page, kv, dim = kc.shape[1:]
+    rep, scale = q.shape[1] // kv, dim ** -0.5 if scale is None else scale
+    out, table, base = torch.zeros_like(q), s["table"].cpu().long(), 0
+    for b, (c, n) in enumerate(zip(s["ctx"], s["new"])):
+        pos = torch.arange(c + n)
+        k, v = kc[table[b][pos // page], pos % page], vc[table[b][pos // page], pos % page]
+        for i in range(n):
+            word = (1 << (i + 1)) - 1 if s["mask"] is None else int(s["mask"][base + i, 0])
+            seen = list(range(c)) + [c + j for j in range(n) if word >> j & 1]
+            for h in range(q.shape[1]):
+                w = torch.softmax(k[seen, h // rep] @ q[base + i, h] * scale, 0)
+                out[base + i, h] = (w[:, None] * v[seen, h // rep]).sum(0)
+        base += n
+    return out
+
+
+def check_nonfinite(s, clean, what=""):
+    got, want = attend(s).cpu(), nonfinite_reference(s)
+    assert paged.read_status() == 0, what
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf].double(), want[inf]), what
+    fin = torch.isfinite(want)
+    assert torch.equal(got[fin], clean.cpu()[fin]), what    # nothing else changes, to the bit
+
+
+ROWS = [(4, 2, 64, 16, [6, 3]), (2, 1, 128, 7, [9, 4]), (4, 1, 256, 16, [7, 1]),     # up to 32 rows
+        (16, 2, 128, 32, [8, 3]), (4, 1, 80, 24, [13, 2]), (8, 1, 192, 64, [7, 5]),  # up to 64
+        (16, 2, 128, 16, [12, 3]), (8, 1, 256, 8, [16, 2]),                          # up to 128
+        (16, 1, 128, 64, [15, 9]), (8, 1, 64, 7, [30, 1])]                           # more
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim,page,new", ROWS)
+@pytest.mark.parametrize("tree", [True, False])
+def test_infinities_of_the_context(heads, kv, dim, page, new, tree, dtype):
+    """In a whole tile of the context and in the tile that the new tokens share; alone, against one of the other sign,
+    and with NaN in another column."""
+    s = build([300, 16], new, heads, kv, dim, page, dtype, seed=dim + heads, tree=tree)
+    clean = attend(s)
+
+    def put(at, column, value):
+        s["vc"][int(s["table"][0, at // page]), at % page, :, column] = value
+
+    keep = s["vc"].clone()
+    for puts in ([(5, 3, math.inf)], [(290, 3, -math.inf)], [(5, 3, -math.inf), (200, 3, -math.inf), (290, dim - 1, math.inf)],
+                 [(17, 3, math.inf), (133, 3, -math.inf), (40, 4, math.nan), (301, 4, math.inf)],
+                 [(131, 7, math.inf), (300, 7, -math.inf)]):
+        for p in puts:
+            put(*p)
+        check_nonfinite(s, clean, str(puts))
+        s["vc"].copy_(keep)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim,page,new", ROWS[::3])
+def test_infinities_under_vanishing_weights(heads, kv, dim, page, new, dtype):
+    """Weights that are zero in 16 bits, or in 32, are not zero: an infinity under them is one in the row. Scores spread
+    over some hundreds, within what 64 bits hold."""
+    s = build([300, 16], new, heads, kv, dim, page, dtype, seed=dim, q_scale=60.0)
+    clean = attend(s)
+    for at, value in ((5, math.inf), (255, -math.inf), (299, math.inf), (301, -math.inf)):
+        keep = s["vc"].clone()
+        s["vc"][int(s["table"][0, at // page]), at % page, :, 2] = value
+        check_nonfinite(s, clean, f"{at} {value}")
+        s["vc"].copy_(keep)
+
+
+@pytest.mark.parametrize("heads,dim,new", [(1, 64, 3), (8, 128, 5), (8, 128, 13), (4, 256, 33)])
+def test_infinities_in_a_split_request(heads, dim, new):
+    """The parts of a request that several processors share: one part's infinities, and parts of which one has all the weight."""
+    for q_scale in (1.0, 60.0):
+        s = build([6000], [new], heads, 1, dim, 16, torch.bfloat16, seed=dim, q_scale=q_scale)
+        clean = attend(s)
+        for puts in ([(3, 1, math.inf)], [(2500, 1, -math.inf)], [(700, 0, math.inf), (5400, 0, -math.inf), (5999, 9, math.inf)]):
+            keep = s["vc"].clone()
+            for at, column, value in puts:
+                s["vc"][int(s["table"][0, at // 16]), at % 16, :, column] = value
+            check_nonfinite(s, clean, str(puts))
+            s["vc"].copy_(keep)
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,new", ROWS[::3])
+def test_infinite_keys(heads, kv, dim, page, new):
+    """A key with an infinity has the score +inf (the row is NaN) or -inf (weight zero; its value counts only where it is
+    itself infinite, as NaN)."""
+    s = build([300, 16], new, heads, kv, dim, page, torch.float16, seed=dim + 1)
+    for value_too in (False, True):
+        for at in (7, 293):
+            keep = s["kc"].clone(), s["vc"].clone()
+            page_id = int(s["table"][0, at // page])
+            s["kc"][page_id, at % page, :, 1] = math.inf
+            if value_too:
+                s["vc"][page_id, at % page, :, 5] = math.inf
+            got, want = attend(s).cpu(), nonfinite_reference(s)
+            assert torch.equal(torch.isnan(got), torch.isnan(want))
+            fin = torch.isfinite(want)
+            s["kc"].copy_(keep[0])
+            s["vc"].copy_(keep[1])
+            # finite rows: those without this key, with the bound of one more or less of them
+            assert float((got.double() - want)[fin].abs().max()) < 8 * HALF_UNIT[torch.float16] * float(want[fin].abs().max())
+
+
+@pytest.mark.parametrize("heads,dim,new", [(4, 64, 4), (16, 128, 4), (16, 128, 20)])
+def test_a_cache_full_of_infinities(heads, dim, new):
+    """Many infinities are no slower than a bounded wait allows."""
+    s = build([20000, 100], [new, 2], heads, 1, dim, 64, torch.float16, seed=dim)
+    s["vc"][..., 0] = math.inf
+    s["vc"][..., 1] = -math.inf
+    s["vc"][..., 2] = math.nan
+    got = attend(s)
+    assert paged.read_status() == 0
+    assert bool((got[..., 0] == math.inf).all()) and bool((got[..., 1] == -math.inf).all()) and bool(torch.isnan(got[..., 2]).all())
+    assert bool(torch.isfinite(got[..., 3:]).all())
 
 
 @pytest.mark.parametrize("page", [16, 64])
