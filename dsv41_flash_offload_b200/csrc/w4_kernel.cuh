@@ -117,6 +117,18 @@ __device__ __forceinline__ void w4_words(const uint32_t* p, uint32_t (&v)[N])
     }
 }
 
+// min(silu(g), L) * clamp(u, -L, L), L = 0: no clamps. Clamps by comparison: minimum and maximum would turn a NaN product
+// into a limit.
+__device__ __forceinline__ float w4_swiglu(float g, float u, float limit)
+{
+    float s = __fdividef(g, 1.0f + __expf(-g));
+    if (limit != 0.0f) {
+        s = s > limit ? limit : s;
+        u = u > limit ? limit : u < -limit ? -limit : u;
+    }
+    return s * u;
+}
+
 // Work: one CTA per SM takes a run of whole row tiles, its warps equal runs of that run's steps (of 128 inputs), so
 // the warps of a small matrix share one tile's inputs and those of a large one take tiles of their own, by the same
 // rule. Codes, scales and zero points of a CTA's steps are contiguous; a warp keeps D steps on their way in
@@ -227,7 +239,7 @@ __global__ void __launch_bounds__(W4Cfg<TB, GATED>::warps * 32, 1) w4_kernel(con
             for (int e = 0; e < 4; ++e) {
                 const int t = t0 + b * 8 + 2 * c + (e & 1), n = tile * 16 + r + 8 * (e >> 1);
                 if (t >= p.tokens || n >= p.n) continue;
-                const float y = GATED ? act_gu(tot[0][b][e], tot[NT - 1][b][e], p.limit) : tot[0][b][e];
+                const float y = GATED ? w4_swiglu(tot[0][b][e], tot[NT - 1][b][e], p.limit) : tot[0][b][e];
                 const int64_t at = (int64_t)t * p.out_stride + n;
                 if (p.out_dtype == DSV41_DTYPE_F32) {
                     float* o = static_cast<float*>(p.out) + at;

@@ -357,7 +357,8 @@ int dsv41_w4_pack(const void* codes, const void* scales, const void* zeros, int3
 int dsv41_w4_linear(const dsv41_w4_weight* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t tokens,
                     void* out, int32_t out_dtype, int64_t out_stride, int32_t accumulate, void* stream);
 /* out[t][n] = min(silu(g), limit) * clamp(u, -limit, limit) with g, u the products with gate and up (same n,
- * k, group, scale type, both or neither with zero points); limit 0 = no clamp (the routed experts' SwiGLU). */
+ * k, group, scale type, both or neither with zero points); limit 0 = no clamp (the routed experts' SwiGLU).
+ * NaN products give NaN, and so does a gate of -inf (its silu is -inf / inf). */
 int dsv41_w4_gated(const dsv41_w4_weight* gate, const dsv41_w4_weight* up, const void* x, int32_t x_dtype,
                    int64_t x_stride, int32_t tokens, float limit, void* out, int32_t out_dtype, int64_t out_stride,
                    void* stream);
