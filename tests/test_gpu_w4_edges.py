@@ -36,3 +36,18 @@ def test_gated_keeps_nan(tokens, dtype, limit):
             assert torch.equal(got[2][inf].double(), want[inf])
             rest = [t for t in range(tokens) if t != 2]
             assert torch.equal(got[rest], clean.cpu()[rest])
+
+
+def test_silu_of_large_gates():
+    """Gates that are one input each (code 9, zero point 8, scale 1) against an up product of 1. fp32 exp, sum and divide:
+    at most 8 units of the result; below 2^-126 a result may be 0."""
+    gate, up = torch.full((31, 32), 8, dtype=torch.uint8), torch.full((31, 32), 8, dtype=torch.uint8)
+    gate[torch.arange(31), torch.arange(31)] = 9
+    up[:, 31] = 9
+    pack = lambda c: w4.W4Weight((c[:, 0::2] | c[:, 1::2] << 4).to(DEV), torch.ones(31, 1, dtype=torch.float16, device=DEV))
+    for base in (-85.0, -60.0, -30.0, -8.0, 0.0, 25.0):
+        x = torch.cat((base + torch.arange(31) * 0.34375, torch.ones(1))).half()[None]
+        got = w4.gated(x.to(DEV), pack(gate), pack(up), None, out_dtype=torch.float32).cpu().double()[0]
+        g = x[0, :31].double()
+        want = g / (1.0 + torch.exp(-g))
+        assert bool(((got - want).abs() <= 8 * 2.0 ** -23 * want.abs() + 2.0 ** -126).all()), base
