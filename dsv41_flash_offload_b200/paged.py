@@ -173,7 +173,9 @@ def _workspace(dev: torch.device, stream: int, head_dim: int) -> tuple[int, int]
 def read_status(device=None) -> int:
     """Synchronise the current stream; return (then clear) the status of its tree_attention calls: 0 = ok, 1 = a
     bounded device-side wait ran out (results since the last read are invalid)."""
-    dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    dev = torch.device(device if device is not None else "cuda")
+    if dev.index is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
     stream, worst = _lib.current_stream(dev), 0
     for (index, s, _), (_, _, buf) in list(_ws.items()):
         if index == dev.index and s == stream:

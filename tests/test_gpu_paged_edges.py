@@ -11,6 +11,14 @@ from test_gpu_paged import DEV, HALF_UNIT, attend, build, reference
 pytestmark = pytest.mark.gpu
 
 
+def test_status_of_a_device_by_name():
+    s = build([20], [3], 4, 2, 64, 16, torch.float16)
+    attend(s)
+    words = paged._ws[(torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream, 64)][2][:4].view(torch.int32)
+    words[0] = 1
+    assert paged.read_status("cuda") == 1 and paged.read_status("cuda:0") == 0 and paged.read_status(torch.device("cuda")) == 0
+
+
 def nonfinite_reference(s, scale=None):
     """The definition in 64 bits, key by key: what a row sees of infinities and NaN, and nothing else."""
     q, kc, vc = (s[n].cpu().double() for n in ("q", "kc", "vc"))
