@@ -171,20 +171,28 @@ def _workspace(dev: torch.device, stream: int, head_dim: int) -> tuple[int, int]
 
 
 def read_status(device=None) -> int:
-    """Synchronise the current stream; return (then clear) the status of its tree_attention calls: 0 = ok, 1 = a
-    bounded device-side wait ran out (results since the last read are invalid)."""
+    """Synchronise the current stream; return (then clear) the status of the device's tree_attention calls, on whichever
+    stream they ran or were captured: 0 = ok, 1 = a bounded device-side wait ran out (results since the last read are
+    invalid). Calls that other streams have still to finish report in a later read."""
     dev = torch.device(device if device is not None else "cuda")
     if dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
     stream, worst = _lib.current_stream(dev), 0
-    for (index, s, _), (_, _, buf) in list(_ws.items()):
-        if index == dev.index and s == stream:
-            st = C.c_int32()
-            _lib.call(dev, _lib.load().dsv41_read_status, buf.data_ptr(), stream, C.byref(st))
-            if st.value:
-                buf.zero_()   # the counters of a call that gave up are not back at zero
-            worst = max(worst, st.value)
+    for (index, _, _), (_, _, buf) in list(_ws.items()):
+        if index == dev.index:
+            worst = max(worst, _read_and_clear(dev, buf, stream))
     return worst
+
+
+def _read_and_clear(dev: torch.device, buf: torch.Tensor, stream: int) -> int:
+    st = C.c_int32()
+    _lib.call(dev, _lib.load().dsv41_read_status, buf.data_ptr(), stream, C.byref(st))
+    if st.value:
+        # the counters of a call that gave up are not back at zero; its stream may be another than this one
+        torch.cuda.synchronize(dev)
+        buf.zero_()
+        torch.cuda.synchronize(dev)
+    return st.value
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,

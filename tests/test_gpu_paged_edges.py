@@ -11,6 +11,30 @@ from test_gpu_paged import DEV, HALF_UNIT, attend, build, reference
 pytestmark = pytest.mark.gpu
 
 
+def test_status_of_replays_and_recovery():
+    """A wait that ran out is reported wherever its call ran, and the next call starts from clean counters."""
+    s = build([900, 2000], [5, 9], 8, 2, 128, 16, torch.float16, seed=10)
+    want = attend(s)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attend(s)
+        graph = torch.cuda.CUDAGraph()
+    side.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        out = attend(s)
+    buf = paged._ws[(torch.cuda.current_device(), side.cuda_stream, 128)][2]
+    assert paged.read_status() == 0
+    # what a call leaves that gave up: its status, and counters that are not zero
+    words = buf[:2048].view(torch.int32)
+    words[0] = 1
+    words[64:72] = 3
+    assert paged.read_status() == 1 and paged.read_status() == 0
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and paged.read_status() == 0
+
+
 def test_status_of_a_device_by_name():
     s = build([20], [3], 4, 2, 64, 16, torch.float16)
     attend(s)
