@@ -10,7 +10,9 @@ s // page_size, and row b of a block table lists the pages of request b. One ste
 
 All lengths stay on the GPU, nothing synchronises the host, and after the first tree_attention on a stream
 (whose workspace is kept per device, stream and head size) only outputs are allocated, so a step can be
-captured in a CUDA graph.
+captured in a CUDA graph. A graph uses the workspace that its capture took: the capture stream's own (made there by an
+eager call or by reserve_workspace), or one given as `workspace=`. Replays that share a workspace, and eager calls on
+that stream, have to follow one another; graphs that run at the same time need one each (attention_workspace).
 """
 from __future__ import annotations
 
@@ -149,10 +151,32 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: tor
     _lib.call(dev, _lib.load().dsv41_store_kv, C.byref(args), _lib.current_stream(dev))
 
 
-# one zeroed workspace per (device, stream, padded head size): its counters are zero between calls, and calls
-# that overlap on several streams get one each
+# one zeroed workspace per (device, stream, padded head size): its counters are zero between calls. Eager calls that
+# overlap on several streams get one each; a replayed graph uses the one of its capture, whatever stream it runs on.
 _ws_lock = threading.Lock()
 _ws: dict = {}
+
+
+def attention_workspace(head_dim: int, device=None) -> torch.Tensor:
+    """A workspace of its own for tree_attention calls of this head size (or one padded alike: up to 64, 128, 256), zeroed
+    on the current stream. For graphs that are replayed at the same time; not for two calls at once."""
+    dev = _device(device)
+    size = C.c_size_t()
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().dsv41_tree_attention_workspace_size(int(head_dim), C.byref(size)), "workspace_size")
+        return torch.zeros(size.value, dtype=torch.uint8, device=dev)
+
+
+def reserve_workspace(head_dim: int, stream: torch.cuda.Stream | None = None, device=None) -> None:
+    """Make the workspace that tree_attention calls on `stream` (default: the current one) use, before a capture."""
+    dev = stream.device if stream is not None else _device(device)
+    with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(dev)):
+        _workspace(dev, _lib.current_stream(dev), head_dim)
+
+
+def _device(device) -> torch.device:
+    dev = torch.device(device if device is not None else "cuda")
+    return dev if dev.index is not None else torch.device("cuda", torch.cuda.current_device())
 
 
 def _workspace(dev: torch.device, stream: int, head_dim: int) -> tuple[int, int]:
@@ -162,21 +186,20 @@ def _workspace(dev: torch.device, stream: int, head_dim: int) -> tuple[int, int]
     if got is None:
         with _ws_lock, torch.cuda.device(dev):
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("dsv41: workspace must be allocated before CUDA-graph capture (run once eagerly)")
-            size = C.c_size_t()
-            _lib.check(_lib.load().dsv41_tree_attention_workspace_size(head_dim, C.byref(size)), "workspace_size")
-            buf = torch.zeros(size.value, dtype=torch.uint8, device=dev)
-            got = _ws.setdefault(key, (buf.data_ptr(), size.value, buf))
+                raise RuntimeError("dsv41: workspace must be allocated before CUDA-graph capture (run once eagerly on the capture "
+                                   "stream, call paged.reserve_workspace for it, or pass workspace=)")
+            buf = attention_workspace(head_dim, dev)
+            got = _ws.setdefault(key, (buf.data_ptr(), buf.numel(), buf))
     return got[:2]
 
 
-def read_status(device=None) -> int:
+def read_status(device=None, workspace: torch.Tensor | None = None) -> int:
     """Synchronise the current stream; return (then clear) the status of the device's tree_attention calls, on whichever
-    stream they ran or were captured: 0 = ok, 1 = a bounded device-side wait ran out (results since the last read are
-    invalid). Calls that other streams have still to finish report in a later read."""
-    dev = torch.device(device if device is not None else "cuda")
-    if dev.index is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
+    stream they ran or were captured, or of those that were given `workspace`: 0 = ok, 1 = a bounded device-side wait ran
+    out (results since the last read are invalid). Calls that other streams have still to finish report in a later read."""
+    if workspace is not None:
+        return _read_and_clear(workspace.device, workspace, _lib.current_stream(workspace.device))
+    dev = _device(device)
     stream, worst = _lib.current_stream(dev), 0
     for (index, _, _), (_, _, buf) in list(_ws.items()):
         if index == dev.index:
@@ -197,7 +220,8 @@ def _read_and_clear(dev: torch.device, buf: torch.Tensor, stream: int) -> int:
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                    seq_lens: torch.Tensor, cu_lens: torch.Tensor, max_new: int, *, tree_mask: torch.Tensor | None = None,
-                   scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
+                   scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False,
+                   workspace: torch.Tensor | None = None):
     """Attention of the step's new tokens over the paged cache that already holds their keys and values.
 
     q [N, q_heads, head_dim] (the caches' dtype, head_dim up to 256); request b owns rows cu_lens[b]:cu_lens[b + 1]
@@ -205,7 +229,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     step_tables) a token sees the context and the new tokens of its bits, without it the context and the new tokens
     up to itself. max_new is an upper bound on a request's new tokens, scale defaults to head_dim ** -0.5. Query head
     h reads KV head h // (q_heads / kv_heads). A row that sees nothing is 0 with lse -inf. Returns out [N, q_heads,
-    head_dim] in q's dtype, or (out, lse fp32 [N, q_heads]); rows past cu_lens[B] are not written."""
+    head_dim] in q's dtype, or (out, lse fp32 [N, q_heads]); rows past cu_lens[B] are not written. workspace: one of
+    attention_workspace's, which no other call may use at the same time (default: the stream's own)."""
     (pages, page_size, kv_heads, dim), cs, dev = _cache(k_cache, v_cache)
     if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % kv_heads:
         raise ValueError(f"q must be [N, q_heads, {dim}] with q_heads a multiple of {kv_heads}")
@@ -234,7 +259,12 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             raise ValueError("out must be like q, with contiguous, 16-byte aligned heads")
     lse = q.new_empty((N, q_heads), dtype=torch.float32) if return_lse else None
     stream = _lib.current_stream(dev)
-    ws, ws_bytes = _workspace(dev, stream, dim)
+    if workspace is None:
+        ws, ws_bytes = _workspace(dev, stream, dim)
+    else:
+        if workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.device != dev:
+            raise ValueError(f"workspace must be one of attention_workspace's on {dev}")
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel()
     qs = q.stride()
     args = _lib.TreeAttentionArgs(
         _DTYPES[q.dtype], B, N, int(max_new), q_heads, kv_heads, dim, page_size, pages, min(width * page_size, 0x7fffff00),

@@ -43,6 +43,63 @@ def test_status_of_a_device_by_name():
     assert paged.read_status("cuda") == 1 and paged.read_status("cuda:0") == 0 and paged.read_status(torch.device("cuda")) == 0
 
 
+@pytest.mark.parametrize("dim", [64, 256])
+def test_graphs_with_workspaces_of_their_own_replay_at_once(dim):
+    """Two graphs captured on one stream that never ran a call, replayed together on two others, each with split requests."""
+    cases = [build([3000 + 500 * i, 900], [5, 9], 8, 2, dim, 16, torch.float16, seed=20 + i) for i in range(2)]
+    want = [attend(s) for s in cases]
+    graphs, outs, spaces = [], [], [paged.attention_workspace(dim) for _ in cases]
+    torch.cuda.synchronize()
+    capture = torch.cuda.Stream()
+    for s, w in zip(cases, spaces):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=capture):
+            outs.append([attend(s, workspace=w) for _ in range(4)])
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(25):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for group, w in zip(outs, want) for o in group)
+    assert [paged.read_status(workspace=w) for w in spaces] == [0, 0]
+    spaces[1][:4].view(torch.int32)[0] = 1
+    spaces[1][256:300] = 7
+    assert paged.read_status() == 0 and paged.read_status(workspace=spaces[1]) == 1
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[1]) for o in outs[1]) and paged.read_status(workspace=spaces[1]) == 0
+
+
+def test_a_reserved_stream_can_capture_at_once():
+    s = build([900, 2000], [5, 9], 8, 2, 128, 16, torch.float16, seed=30)
+    want = attend(s)
+    stream = torch.cuda.Stream()
+    paged._ws.pop((torch.cuda.current_device(), stream.cuda_stream, 128), None)   # (streams come from a pool)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="reserve_workspace"):
+        with torch.cuda.graph(graph, stream=stream):
+            attend(s)
+    paged.reserve_workspace(128, stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = attend(s)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_workspaces_that_do_not_fit_are_refused():
+    s = build([20], [3], 4, 2, 128, 16, torch.float16)
+    full = paged.attention_workspace(128)
+    assert torch.equal(attend(s, workspace=full), attend(s))
+    for bad in (full[:-256], full[128:], full.view(torch.int32), full.cpu(), full[::2]):
+        with pytest.raises((ValueError, Dsv41Error)):
+            attend(s, workspace=bad)
+    with pytest.raises(Dsv41Error):
+        paged.attention_workspace(264)
+
+
 def nonfinite_reference(s, scale=None):
     """The definition in 64 bits, key by key: what a row sees of infinities and NaN, and nothing else."""
     q, kc, vc = (s[n].cpu().double() for n in ("q", "kc", "vc"))
