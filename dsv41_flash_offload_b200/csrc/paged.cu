@@ -7,6 +7,8 @@
 // (need_b > W: the request is refused and keeps what it holds). Returned pages are pushed on the stack of
 // free pages in request order, then pages are popped in request order:
 //     the j-th popped page is entry F + G - 1 - j of the stack, F its height before, G = sum give_b
+// (where more would be left on the stack than it holds: over the requests before the first whose pages pass its end;
+// from there on all keep theirs)
 // and request b is admitted iff the running sum of takes through b fits F + G. Every quantity is a prefix
 // sum over requests, so each CTA computes the sums itself (batch <= 2048: three values per request, one
 // block scan) and then fills its own share of the outputs. A popped page that was returned in the same call
@@ -116,8 +118,16 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
     __syncthreads();
 
     const uint32_t height = (uint32_t)min(max(*p.free_count, 0), p.free_capacity);
-    const uint32_t top = sat_add(height, gv[B]);   // stack height after the returns
+    const uint32_t room = p.free_capacity - height;
+    uint32_t given = gv[B];                        // pages that go back
+    if (given > room) {
+        const uint32_t all = sat_add(height, given), popped = tk[last_le(tk, B + 1, all)];
+        if (all - popped > (uint32_t)p.free_capacity) given = gv[last_le(gv, B + 1, room)];
+    }
+    const uint32_t top = height + given;           // stack height after the returns
+    auto keeps = [&](const TabReq& r, int b) { return r.want < r.held && gv[b + 1] > given; };
     auto admitted = [&](const TabReq& r, int b) { return r.fits && (r.want <= r.held || tk[b + 1] <= top); };
+    auto flags_of = [&](const TabReq& r, int b, bool ok) { return (ok ? 0 : r.fits ? kTabNoPages : kTabTooWide) | (keeps(r, b) ? kTabNoRoom : 0); };
     // entry i of the stack after the returns (i < top)
     auto stack_page = [&](uint32_t i) {
         if (i < height) return p.free_pages[i];
@@ -135,8 +145,8 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
             p.block_table[(int64_t)b * p.table_stride + r.held + (int)(j - tk[b])] = stack_page(top - 1 - j);
     }
     // pages returned: onto the stack
-    for (uint32_t e = first; e < gv[B]; e += stride)
-        if (height + e < (uint32_t)p.free_capacity) p.free_pages[height + e] = stack_page(height + e);
+    for (uint32_t e = first; e < given; e += stride)
+        if (height + e < (uint32_t)p.free_capacity) p.free_pages[height + e] = stack_page(height + e);   // (the others are taken)
 
     // per-request outputs
     uint32_t used = 0;   // pages popped: the largest admitted running sum of takes
@@ -146,8 +156,8 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
             const bool ok = admitted(r, b);
             p.cu_lens[b] = (int)cu[b];
             p.seq_lens[b] = ok ? (int)min((int64_t)r.ctx + r.fresh, (int64_t)0x7fffffff) : 0;
-            p.held_out[b] = ok ? r.want : r.held;
-            if (!p.parents) p.status[b] = ok ? 0 : (r.fits ? kTabNoPages : kTabTooWide);
+            p.held_out[b] = ok && !keeps(r, b) ? r.want : r.held;
+            if (!p.parents) p.status[b] = flags_of(r, b, ok);
             if (ok) used = max(used, tk[b + 1] <= top ? tk[b + 1] : 0u);
         }
         used = __reduce_max_sync(0xffffffffu, used);
@@ -157,7 +167,7 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
         if (tid == 0) {
             for (int w = 1; w < kTabThreads / 32; ++w) used = max(used, warp_tot[0][w]);
             p.cu_lens[B] = (int)cu[B];
-            *p.free_count_out = (int)min(top - used, (uint32_t)p.free_capacity);
+            *p.free_count_out = (int)(top - used);
         }
     }
 
@@ -218,7 +228,7 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
     for (int b = blockIdx.x * (kTabThreads / 32) + warp; b < B; b += warps) {
         const TabReq r = tab_req(p, b);
         const bool ok = admitted(r, b);
-        int flags = ok ? 0 : (r.fits ? kTabNoPages : kTabTooWide);
+        int flags = flags_of(r, b, ok);
         for (int at = lane; at < r.fresh; at += 32) {
             const int64_t t = (int64_t)cu[b] + at;
             if (t >= p.num_tokens) break;

@@ -27,7 +27,7 @@ from . import _lib
 _DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 MAX_REQUESTS = 2048
 MAX_MASK_WORDS = 4
-NO_PAGES, TOO_WIDE, BAD_PARENT, BIG_TREE = 1, 2, 4, 8   # status bits of a request
+NO_PAGES, TOO_WIDE, BAD_PARENT, BIG_TREE, NO_ROOM = 1, 2, 4, 8, 16   # status bits of a request
 
 
 class StepTables(NamedTuple):
@@ -74,7 +74,8 @@ def step_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, held_pages: 
     batch, >= sum(new_lens). parents (int32 [num_tokens]): index within its request of each drafted token's
     parent, which must lie before it, -1 for the context; then positions are context + depth and tree_mask is
     built, for trees of up to 64 * mask_words tokens. A request that finds no pages is refused: status bit,
-    seq_lens 0, slots -1."""
+    seq_lens 0, slots -1. free_pages should have room for every page of the pool: a request whose surplus does not fit, and
+    those behind it, keep theirs (status NO_ROOM) and are served all the same."""
     dev = context_lens.device
     if not context_lens.is_cuda or context_lens.dim() != 1 or not 1 <= context_lens.shape[0] <= MAX_REQUESTS:
         raise ValueError(f"context_lens must be a CUDA int32 [B] with B in 1..{MAX_REQUESTS}")

@@ -2,13 +2,29 @@
 test_gpu_paged.py."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
 from dsv41_flash_offload_b200 import Dsv41Error, paged
-from test_gpu_paged import DEV, HALF_UNIT, attend, build, reference
+from test_gpu_paged import DEV, HALF_UNIT, attend, build, reference, run_tables
 
 pytestmark = pytest.mark.gpu
+
+
+def test_a_stack_without_room_loses_no_page():
+    ctx, new, held = [0, 0, 0, 16], [0, 0, 0, 16], [2, 3, 1, 1]
+    table = np.arange(16, dtype=np.int32).reshape(4, 4)
+    for parents in (None, [-1] * 16):
+        t, tb, fr = run_tables(ctx, new, held, table, np.array([50, 51, -1, -1, -1], np.int32), 2, 16, 16, parents)
+        # request 0's two pages fit beside the two there, request 1's three do not, request 2 waits behind it
+        assert t.held_pages.cpu().tolist() == [0, 3, 1, 2] and t.status.cpu().tolist() == [0, paged.NO_ROOM, paged.NO_ROOM, 0]
+        assert tb[3, :2].cpu().tolist() == [12, 1] and int(t.free_count) == 3 and fr[:4].cpu().tolist() == [50, 51, 0, 1]
+        assert t.seq_lens.cpu().tolist() == [0, 0, 0, 32] and t.slots.cpu().tolist() == [16 + i for i in range(16)]
+    # more comes back than the stack holds, but the same call takes it again: nothing is kept back
+    t, tb, _ = run_tables([0, 16], [0, 48], [4, 1], np.array([[4, 5, 6, 7], [1, 0, 0, 0]], np.int32), np.array([9, -1], np.int32), 1, 16, 48)
+    assert t.status.cpu().tolist() == [0, 0] and t.held_pages.cpu().tolist() == [0, 4] and int(t.free_count) == 2
+    assert tb[1].cpu().tolist() == [1, 7, 6, 5]
 
 
 def test_status_of_replays_and_recovery():
