@@ -14,7 +14,7 @@ namespace dsv41 {
 static_assert(kMaxRequests == DSV41_MAX_REQUESTS && kMaxMaskWords == DSV41_MAX_MASK_WORDS, "header limits");
 static_assert(kTabNoPages == DSV41_TABLES_NO_PAGES && kTabTooWide == DSV41_TABLES_TOO_WIDE &&
                   kTabBadParent == DSV41_TABLES_BAD_PARENT && kTabBigTree == DSV41_TABLES_BIG_TREE &&
-                  kTabNoRoom == DSV41_TABLES_NO_ROOM, "header status bits");
+                  kTabNoRoom == DSV41_TABLES_NO_ROOM && kTabPastTokens == DSV41_TABLES_PAST_TOKENS, "header status bits");
 
 static bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 

@@ -118,16 +118,22 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
     __syncthreads();
 
     const uint32_t height = (uint32_t)min(max(*p.free_count, 0), p.free_capacity);
-    const uint32_t room = p.free_capacity - height;
-    uint32_t given = gv[B];                        // pages that go back
-    if (given > room) {
+    const uint32_t room = p.free_capacity - height, tokens = p.num_tokens;
+    uint32_t given = gv[B], served = cu[B];        // pages that go back; tokens of the requests that end within the token arrays
+    const bool odd = given > room || served > tokens;
+    if (__builtin_expect(odd, 0)) {
         const uint32_t all = sat_add(height, given), popped = tk[last_le(tk, B + 1, all)];
         if (all - popped > (uint32_t)p.free_capacity) given = gv[last_le(gv, B + 1, room)];
+        if (served > tokens) served = cu[last_le(cu, B, tokens)];
     }
     const uint32_t top = height + given;           // stack height after the returns
-    auto keeps = [&](const TabReq& r, int b) { return r.want < r.held && gv[b + 1] > given; };
     auto admitted = [&](const TabReq& r, int b) { return r.fits && (r.want <= r.held || tk[b + 1] <= top); };
-    auto flags_of = [&](const TabReq& r, int b, bool ok) { return (ok ? 0 : r.fits ? kTabNoPages : kTabTooWide) | (keeps(r, b) ? kTabNoRoom : 0); };
+    auto keeps = [&](const TabReq& r, int b) { return odd && r.want < r.held && gv[b + 1] > given; };
+    // new tokens that the token arrays have no entry for: not served, for attention would take them for context
+    auto past = [&](const TabReq& r, int b) { return odd && r.fresh > 0 && cu[b + 1] > tokens; };
+    auto flags_of = [&](const TabReq& r, int b, bool ok) {
+        return (ok ? 0 : r.fits ? kTabNoPages : kTabTooWide) | (keeps(r, b) ? kTabNoRoom : 0) | (past(r, b) ? kTabPastTokens : 0);
+    };
     // entry i of the stack after the returns (i < top)
     auto stack_page = [&](uint32_t i) {
         if (i < height) return p.free_pages[i];
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
             const TabReq r = tab_req(p, b);
             const bool ok = admitted(r, b);
             p.cu_lens[b] = (int)cu[b];
-            p.seq_lens[b] = ok ? (int)min((int64_t)r.ctx + r.fresh, (int64_t)0x7fffffff) : 0;
+            p.seq_lens[b] = ok && !past(r, b) ? (int)min((int64_t)r.ctx + r.fresh, (int64_t)0x7fffffff) : 0;
             p.held_out[b] = ok && !keeps(r, b) ? r.want : r.held;
             if (!p.parents) p.status[b] = flags_of(r, b, ok);
             if (ok) used = max(used, tk[b + 1] <= top ? tk[b + 1] : 0u);
@@ -203,7 +209,7 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
                     ok = admitted(r, b);
                 }
                 const int64_t at = (int64_t)r.ctx + (t - cu[b]);
-                slot[i] = slot_of(r, b, ok, at);
+                slot[i] = slot_of(r, b, ok && t < served, at);
                 pos[i] = (int)at;
                 req[i] = b;
             }
@@ -251,7 +257,7 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
 #pragma unroll
             for (int w = 0; w < kMaxMaskWords; ++w)
                 if (w < p.mask_words) p.tree_mask[t * p.mask_words + w] = (int64_t)bits[w];
-            p.slots[t] = slot_of(r, b, ok, (int64_t)r.ctx + at);
+            p.slots[t] = slot_of(r, b, ok && t < served, (int64_t)r.ctx + at);
             p.positions[t] = (int)min((int64_t)r.ctx + depth - 1, (int64_t)0x7fffffff);
             p.requests[t] = b;
         }

@@ -7,7 +7,8 @@ namespace dsv41 {
 
 constexpr int kMaxRequests = 2048;   // requests per step
 constexpr int kMaxMaskWords = 4;     // 64-bit words of a drafted token's ancestor mask
-constexpr int kTabNoPages = 1, kTabTooWide = 2, kTabBadParent = 4, kTabBigTree = 8, kTabNoRoom = 16;   // status bits of a request
+// status bits of a request
+constexpr int kTabNoPages = 1, kTabTooWide = 2, kTabBadParent = 4, kTabBigTree = 8, kTabNoRoom = 16, kTabPastTokens = 32;
 
 struct StepTablesParams {
     const int *context_lens, *new_lens, *held_pages;   // [batch]

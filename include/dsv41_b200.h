@@ -252,7 +252,8 @@ enum {
     DSV41_TABLES_TOO_WIDE = 2,   /* its pages exceed the table's width */
     DSV41_TABLES_BAD_PARENT = 4, /* a parent is not an earlier token of the request (taken as -1) */
     DSV41_TABLES_BIG_TREE = 8,   /* tokens past 64 * mask_words: they are in no mask */
-    DSV41_TABLES_NO_ROOM = 16    /* the stack has no room for the pages it would return: it keeps them, and is served */
+    DSV41_TABLES_NO_ROOM = 16,   /* the stack has no room for the pages it would return: it keeps them, and is served */
+    DSV41_TABLES_PAST_TOKENS = 32 /* its new tokens pass num_tokens: seq_lens 0, slots -1; its pages are exchanged */
 };
 
 /* Bring the pages of every request in line with its length. Request b has context_lens[b] tokens in the
@@ -261,7 +262,8 @@ enum {
  * order; where the call would leave more on it than free_capacity, which a stack for every page of the pool never
  * meets, the first request whose pages do not fit and those behind it keep theirs), missing ones then come off its top (in request order) into the row. Entries of a row past its
  * pages are stale. All pointers are device memory; num_tokens >= sum of new_lens (the caller knows it as
- * the length of the step's token batch; later entries get slot -1, position 0, request -1).
+ * the length of the step's token batch; later entries get slot -1, position 0, request -1; a request whose tokens
+ * pass it gets a status bit).
  * Outputs: cu_lens [batch + 1] running sums of new_lens; seq_lens [batch] = context + new; held_out [batch];
  * free_count_out [1]; status [batch]; per token: slots (int64), positions, requests (its b). Without
  * parents a token's position is context + its index; with parents ([num_tokens], index of the parent

@@ -27,6 +27,16 @@ def test_a_stack_without_room_loses_no_page():
     assert tb[1].cpu().tolist() == [1, 7, 6, 5]
 
 
+def test_tokens_past_the_batch_are_refused():
+    ctx, new, held = [5, 3, 0, 9], [3, 4, 2, 0], [1, 1, 0, 1]
+    table = np.arange(16, dtype=np.int32).reshape(4, 4)
+    for parents in (None, [-1] * 5):
+        t, _, _ = run_tables(ctx, new, held, table, np.arange(90, 99, dtype=np.int32), 9, 16, 5, parents)
+        assert t.status.cpu().tolist() == [0, paged.PAST_TOKENS, paged.PAST_TOKENS, 0]
+        assert t.seq_lens.cpu().tolist() == [8, 0, 0, 9] and t.slots.cpu().tolist() == [5, 6, 7, -1, -1]
+        assert t.held_pages.cpu().tolist() == [1, 1, 1, 1] and int(t.free_count) == 8
+
+
 def test_status_of_replays_and_recovery():
     """A wait that ran out is reported wherever its call ran, and the next call starts from clean counters."""
     s = build([900, 2000], [5, 9], 8, 2, 128, 16, torch.float16, seed=10)
