@@ -12,120 +12,6 @@ from test_gpu_paged import DEV, HALF_UNIT, attend, build, reference, run_tables
 pytestmark = pytest.mark.gpu
 
 
-def test_a_stack_without_room_loses_no_page():
-    ctx, new, held = [0, 0, 0, 16], [0, 0, 0, 16], [2, 3, 1, 1]
-    table = np.arange(16, dtype=np.int32).reshape(4, 4)
-    for parents in (None, [-1] * 16):
-        t, tb, fr = run_tables(ctx, new, held, table, np.array([50, 51, -1, -1, -1], np.int32), 2, 16, 16, parents)
-        # request 0's two pages fit beside the two there, request 1's three do not, request 2 waits behind it
-        assert t.held_pages.cpu().tolist() == [0, 3, 1, 2] and t.status.cpu().tolist() == [0, paged.NO_ROOM, paged.NO_ROOM, 0]
-        assert tb[3, :2].cpu().tolist() == [12, 1] and int(t.free_count) == 3 and fr[:4].cpu().tolist() == [50, 51, 0, 1]
-        assert t.seq_lens.cpu().tolist() == [0, 0, 0, 32] and t.slots.cpu().tolist() == [16 + i for i in range(16)]
-    # more comes back than the stack holds, but the same call takes it again: nothing is kept back
-    t, tb, _ = run_tables([0, 16], [0, 48], [4, 1], np.array([[4, 5, 6, 7], [1, 0, 0, 0]], np.int32), np.array([9, -1], np.int32), 1, 16, 48)
-    assert t.status.cpu().tolist() == [0, 0] and t.held_pages.cpu().tolist() == [0, 4] and int(t.free_count) == 2
-    assert tb[1].cpu().tolist() == [1, 7, 6, 5]
-
-
-def test_tokens_past_the_batch_are_refused():
-    ctx, new, held = [5, 3, 0, 9], [3, 4, 2, 0], [1, 1, 0, 1]
-    table = np.arange(16, dtype=np.int32).reshape(4, 4)
-    for parents in (None, [-1] * 5):
-        t, _, _ = run_tables(ctx, new, held, table, np.arange(90, 99, dtype=np.int32), 9, 16, 5, parents)
-        assert t.status.cpu().tolist() == [0, paged.PAST_TOKENS, paged.PAST_TOKENS, 0]
-        assert t.seq_lens.cpu().tolist() == [8, 0, 0, 9] and t.slots.cpu().tolist() == [5, 6, 7, -1, -1]
-        assert t.held_pages.cpu().tolist() == [1, 1, 1, 1] and int(t.free_count) == 8
-
-
-def test_status_of_replays_and_recovery():
-    """A wait that ran out is reported wherever its call ran, and the next call starts from clean counters."""
-    s = build([900, 2000], [5, 9], 8, 2, 128, 16, torch.float16, seed=10)
-    want = attend(s)
-    side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(side):
-        attend(s)
-        graph = torch.cuda.CUDAGraph()
-    side.synchronize()
-    with torch.cuda.graph(graph, stream=side):
-        out = attend(s)
-    buf = paged._ws[(torch.cuda.current_device(), side.cuda_stream, 128)][2]
-    assert paged.read_status() == 0
-    # what a call leaves that gave up: its status, and counters that are not zero
-    words = buf[:2048].view(torch.int32)
-    words[0] = 1
-    words[64:72] = 3
-    assert paged.read_status() == 1 and paged.read_status() == 0
-    graph.replay()
-    torch.cuda.synchronize()
-    assert torch.equal(out, want) and paged.read_status() == 0
-
-
-def test_status_of_a_device_by_name():
-    s = build([20], [3], 4, 2, 64, 16, torch.float16)
-    attend(s)
-    words = paged._ws[(torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream, 64)][2][:4].view(torch.int32)
-    words[0] = 1
-    assert paged.read_status("cuda") == 1 and paged.read_status("cuda:0") == 0 and paged.read_status(torch.device("cuda")) == 0
-
-
-@pytest.mark.parametrize("dim", [64, 256])
-def test_graphs_with_workspaces_of_their_own_replay_at_once(dim):
-    """Two graphs captured on one stream that never ran a call, replayed together on two others, each with split requests."""
-    cases = [build([3000 + 500 * i, 900], [5, 9], 8, 2, dim, 16, torch.float16, seed=20 + i) for i in range(2)]
-    want = [attend(s) for s in cases]
-    graphs, outs, spaces = [], [], [paged.attention_workspace(dim) for _ in cases]
-    torch.cuda.synchronize()
-    capture = torch.cuda.Stream()
-    for s, w in zip(cases, spaces):
-        graphs.append(torch.cuda.CUDAGraph())
-        with torch.cuda.graph(graphs[-1], stream=capture):
-            outs.append([attend(s, workspace=w) for _ in range(4)])
-    streams = [torch.cuda.Stream() for _ in cases]
-    for _ in range(25):
-        for g, st in zip(graphs, streams):
-            with torch.cuda.stream(st):
-                g.replay()
-    torch.cuda.synchronize()
-    assert all(torch.equal(o, w) for group, w in zip(outs, want) for o in group)
-    assert [paged.read_status(workspace=w) for w in spaces] == [0, 0]
-    spaces[1][:4].view(torch.int32)[0] = 1
-    spaces[1][256:300] = 7
-    assert paged.read_status() == 0 and paged.read_status(workspace=spaces[1]) == 1
-    graphs[1].replay()
-    torch.cuda.synchronize()
-    assert all(torch.equal(o, want[1]) for o in outs[1]) and paged.read_status(workspace=spaces[1]) == 0
-
-
-def test_a_reserved_stream_can_capture_at_once():
-    s = build([900, 2000], [5, 9], 8, 2, 128, 16, torch.float16, seed=30)
-    want = attend(s)
-    stream = torch.cuda.Stream()
-    paged._ws.pop((torch.cuda.current_device(), stream.cuda_stream, 128), None)   # (streams come from a pool)
-    graph = torch.cuda.CUDAGraph()
-    with pytest.raises(RuntimeError, match="reserve_workspace"):
-        with torch.cuda.graph(graph, stream=stream):
-            attend(s)
-    paged.reserve_workspace(128, stream)
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph, stream=stream):
-        out = attend(s)
-    graph.replay()
-    torch.cuda.synchronize()
-    assert torch.equal(out, want)
-
-
-def test_workspaces_that_do_not_fit_are_refused():
-    s = build([20], [3], 4, 2, 128, 16, torch.float16)
-    full = paged.attention_workspace(128)
-    assert torch.equal(attend(s, workspace=full), attend(s))
-    for bad in (full[:-256], full[128:], full.view(torch.int32), full.cpu(), full[::2]):
-        with pytest.raises((ValueError, Dsv41Error)):
-            attend(s, workspace=bad)
-    with pytest.raises(Dsv41Error):
-        paged.attention_workspace(264)
-
-
 def nonfinite_reference(s, scale=None):
     """The definition in 64 bits, key by key: what a row sees of infinities and NaN, and nothing else."""
     q, kc, vc = (s[n].cpu().double() for n in ("q", "kc", "vc"))
@@ -289,3 +175,154 @@ def test_outputs_that_repeat_in_memory_are_refused():
     for bad in (lambda: paged.store_kv(k, k, slots, heads, heads), lambda: attend(s, out=tokens)):
         with pytest.raises((ValueError, Dsv41Error)):
             bad()
+
+
+def test_status_of_replays_and_recovery():
+    """A wait that ran out is reported wherever its call ran, and the next call starts from clean counters."""
+    s = build([900, 2000], [5, 9], 8, 2, 128, 16, torch.float16, seed=10)
+    want = attend(s)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attend(s)
+        graph = torch.cuda.CUDAGraph()
+    side.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        out = attend(s)
+    buf = paged._ws[(torch.cuda.current_device(), side.cuda_stream, 128)][2]
+    assert paged.read_status() == 0
+    # what a call leaves that gave up: its status, and counters that are not zero
+    words = buf[:2048].view(torch.int32)
+    words[0] = 1
+    words[64:72] = 3
+    assert paged.read_status() == 1 and paged.read_status() == 0
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and paged.read_status() == 0
+
+
+def test_status_of_a_device_by_name():
+    s = build([20], [3], 4, 2, 64, 16, torch.float16)
+    attend(s)
+    words = paged._ws[(torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream, 64)][2][:4].view(torch.int32)
+    words[0] = 1
+    assert paged.read_status("cuda") == 1 and paged.read_status("cuda:0") == 0 and paged.read_status(torch.device("cuda")) == 0
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_graphs_with_workspaces_of_their_own_replay_at_once(dim):
+    """Two graphs captured on one stream that never ran a call, replayed together on two others, each with split requests."""
+    cases = [build([3000 + 500 * i, 900], [5, 9], 8, 2, dim, 16, torch.float16, seed=20 + i) for i in range(2)]
+    want = [attend(s) for s in cases]
+    graphs, outs, spaces = [], [], [paged.attention_workspace(dim) for _ in cases]
+    torch.cuda.synchronize()
+    capture = torch.cuda.Stream()
+    for s, w in zip(cases, spaces):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=capture):
+            outs.append([attend(s, workspace=w) for _ in range(4)])
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(25):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for group, w in zip(outs, want) for o in group)
+    assert [paged.read_status(workspace=w) for w in spaces] == [0, 0]
+    spaces[1][:4].view(torch.int32)[0] = 1
+    spaces[1][256:300] = 7
+    assert paged.read_status() == 0 and paged.read_status(workspace=spaces[1]) == 1
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[1]) for o in outs[1]) and paged.read_status(workspace=spaces[1]) == 0
+
+
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")   # the refused capture
+def test_a_reserved_stream_can_capture_at_once():
+    s = build([900, 2000], [5, 9], 8, 2, 128, 16, torch.float16, seed=30)
+    want = attend(s)
+    stream = torch.cuda.Stream()
+    paged._ws.pop((torch.cuda.current_device(), stream.cuda_stream, 128), None)   # (streams come from a pool)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="reserve_workspace"):
+        with torch.cuda.graph(graph, stream=stream):
+            attend(s)
+    paged.reserve_workspace(128, stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = attend(s)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_workspaces_that_do_not_fit_are_refused():
+    s = build([20], [3], 4, 2, 128, 16, torch.float16)
+    full = paged.attention_workspace(128)
+    assert torch.equal(attend(s, workspace=full), attend(s))
+    for bad in (full[:-256], full[128:], full.view(torch.int32), full.cpu(), full[::2]):
+        with pytest.raises((ValueError, Dsv41Error)):
+            attend(s, workspace=bad)
+    with pytest.raises(Dsv41Error):
+        paged.attention_workspace(264)
+
+
+def test_a_stack_without_room_loses_no_page():
+    ctx, new, held = [0, 0, 0, 16], [0, 0, 0, 16], [2, 3, 1, 1]
+    table = np.arange(16, dtype=np.int32).reshape(4, 4)
+    for parents in (None, [-1] * 16):
+        t, tb, fr = run_tables(ctx, new, held, table, np.array([50, 51, -1, -1, -1], np.int32), 2, 16, 16, parents)
+        # request 0's two pages fit beside the two there, request 1's three do not, request 2 waits behind it
+        assert t.held_pages.cpu().tolist() == [0, 3, 1, 2] and t.status.cpu().tolist() == [0, paged.NO_ROOM, paged.NO_ROOM, 0]
+        assert tb[3, :2].cpu().tolist() == [12, 1] and int(t.free_count) == 3 and fr[:4].cpu().tolist() == [50, 51, 0, 1]
+        assert t.seq_lens.cpu().tolist() == [0, 0, 0, 32] and t.slots.cpu().tolist() == [16 + i for i in range(16)]
+    # more comes back than the stack holds, but the same call takes it again: nothing is kept back
+    t, tb, _ = run_tables([0, 16], [0, 48], [4, 1], np.array([[4, 5, 6, 7], [1, 0, 0, 0]], np.int32), np.array([9, -1], np.int32), 1, 16, 48)
+    assert t.status.cpu().tolist() == [0, 0] and t.held_pages.cpu().tolist() == [0, 4] and int(t.free_count) == 2
+    assert tb[1].cpu().tolist() == [1, 7, 6, 5]
+
+
+def test_tokens_past_the_batch_are_refused():
+    ctx, new, held = [5, 3, 0, 9], [3, 4, 2, 0], [1, 1, 0, 1]
+    table = np.arange(16, dtype=np.int32).reshape(4, 4)
+    for parents in (None, [-1] * 5):
+        t, _, _ = run_tables(ctx, new, held, table, np.arange(90, 99, dtype=np.int32), 9, 16, 5, parents)
+        assert t.status.cpu().tolist() == [0, paged.PAST_TOKENS, paged.PAST_TOKENS, 0]
+        assert t.seq_lens.cpu().tolist() == [8, 0, 0, 9] and t.slots.cpu().tolist() == [5, 6, 7, -1, -1]
+        assert t.held_pages.cpu().tolist() == [1, 1, 1, 1] and int(t.free_count) == 8
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim,ctx,new", [(4, 2, 64, [70, 3, 0, 129], [5, 1, 4, 9]), (16, 1, 128, [3000], [9]),
+                                                  (8, 1, 256, [500, 20], [20, 3]), (4, 1, 128, [1500, 64], [64, 40])])
+def test_sums_are_of_unrounded_weights(heads, kv, dim, ctx, new, dtype):
+    """lse = m + log l: the scores' error e (as in test_gpu_paged.py), the fp32 sum's (keys / 16 + 64) * 2^-22, 2^-21 of the
+    exponentials, and the result's own rounding with log2 and the change of base: 4 units of fp32."""
+    s = build(ctx, new, heads, kv, dim, 16, dtype, seed=dim)
+    _, lse = attend(s, return_lse=True)
+    ref = reference(s)[2]
+    q, k = s["q"].cpu().double().abs(), s["kc"].cpu().double().abs().amax((0, 1))
+    e = (dim / 16 + 8) * 2.0 ** -22 * dim ** -0.5 * torch.einsum("nhd,hd->nh", q, k.repeat_interleave(heads // kv, 0))
+    keys = max(c + n for c, n in zip(ctx, new))
+    bound = e + (keys / 16 + 64) * 2.0 ** -22 + 2.0 ** -21 + 2.0 ** -21 * ref.abs()
+    assert bool(((lse.cpu().double() - ref).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (16, 1, 128), (8, 1, 256)])
+def test_a_scale_of_zero_counts_every_key_alike(heads, kv, dim):
+    s = build([300, 0], [6, 4], heads, kv, dim, 16, torch.bfloat16, seed=3)
+    ref, bound, ref_lse = reference(s, 0.0)
+    out, lse = attend(s, scale=0.0, return_lse=True)
+    assert bool(((out.cpu().double() - ref).abs() <= bound).all())
+    assert float((lse.cpu().double() - ref_lse).abs().max()) <= 2.0 ** -18
+
+
+@pytest.mark.parametrize("page", [24, 64])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_long_prompt_chunks(page, dtype):
+    """No mask, 700 new tokens over an empty and a short context: many row tiles, those past the diagonal left out."""
+    s = build([0, 150], [700, 333], 4, 2, 64, page, dtype, seed=page, tree=False)
+    out = attend(s)
+    ref, bound, _ = reference(s)
+    assert paged.read_status() == 0
+    assert bool(((out.cpu().double() - ref).abs() <= bound).all())

@@ -51,3 +51,17 @@ def test_silu_of_large_gates():
         g = x[0, :31].double()
         want = g / (1.0 + torch.exp(-g))
         assert bool(((got - want).abs() <= 8 * 2.0 ** -23 * want.abs() + 2.0 ** -126).all()), base
+
+
+@pytest.mark.parametrize("n,k,group,zeros", [(40000, 256, 64, True), (60001, 128, 128, False), (38000, 1024, 32, False), (700, 8192, 128, True)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_tiles_of_one_warp_and_of_many(n, k, group, zeros, dtype):
+    """Warps that hold whole row tiles, and tiles that 16 warps share. fp32 sums: group / 16 matrix instructions a group,
+    one addition a group, one a warp, each off by at most 2^-22 of S = sum |w x| (tensor cores may truncate)."""
+    w, dense = make(n, k, group, zeros, dtype, n)
+    dense = dense.to(DEV)
+    for tokens in (1, 11, 25):
+        x = torch.randn(tokens, k, generator=torch.Generator().manual_seed(tokens)).to(dtype).to(DEV)
+        got = w4.linear(x, w, out_dtype=torch.float32).double()
+        bound = (group / 16 + k / group + 16) * 2.0 ** -22 * (x.double().abs() @ dense.abs().t())
+        assert bool(((got - x.double() @ dense.t()).abs() <= bound).all()), tokens
