@@ -277,14 +277,14 @@ __device__ __noinline__ void clear_tile(unsigned char* unit, int thread, int thr
 // Infinities and NaN of a row's sums, from the cache itself. In the products 0 * inf is NaN where the definition has no
 // such term: a repeat's P is zero outside its share of a tile's keys, a weight or a rescale may be zero in 16 or 32 bits only.
 // And new tokens' values entered them as zeros. Here a weight counts as more than zero unless its score is -inf, and
-// then 0 * inf is NaN (products of finite numbers are taken as finite). By a whole warp, a row a lane: columns col0 ..
-// col0 + n - 1 of O, scaled on the way; keys x0 .. x1 - 1, 32 at a time, a lane each, then those with such values in
-// turn, for all rows. Only segments whose sums are not finite, or that held such values of new tokens (`cleared`), come
-// here: 4 tokens over 20000 keys that are full of them take 0.6 ms. 16 columns at a time: with 32 this function's
-// registers made the caller spill its own (32 x 64 tokens over 1-8k keys 222 -> 334 us).
+// then 0 * inf is NaN (products of finite numbers are taken as finite). By a whole warp, a row a lane (where `live`): columns
+// col0 .. col0 + n - 1 that hold an infinity or NaN of keys x0 .. x1 - 1 are put out anew, to the output or (not null) to the part
+// at `part`. 32 keys at a time, a lane each, then those with such values in turn, for all rows. Only segments whose sums are
+// not finite, or that held such values of new tokens, come here: 4 tokens over 20000 keys that are full of them take
+// 0.6 ms. 16 columns at a time and nothing read back: what registers this function takes, the caller spills.
 template <typename T, int RT, int KT>
-__device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const UnitCursor<RT, KT>* cursor, int row, bool live, bool cleared, int x0, int x1,
-                                              int col0, int n, float scale, uint32_t o_at)
+__device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const UnitCursor<RT, KT>* cursor, int row, bool live, int x0, int x1, int col0,
+                                              int n, float4* part)
 {
     const UnitCursor<RT, KT> c = *cursor;
     const int lane = threadIdx.x & 31, ctx = c.r.seq - c.r.n;
@@ -301,17 +301,11 @@ __device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const Uni
     for (int col = col0; col < min(col0 + n, p.head_dim); col += 16) {
         const int cols = min(p.head_dim - col, 16);
         const T* v_head = static_cast<const T*>(p.v_cache) + c.h * p.stride_head + col;
-        float o[16];
-        tc_ld16(o_at + col, o);
-        bool need = cleared;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) need |= j < cols && !(fabsf(o[j]) < INFINITY);
-        need = need && live;
         const uint32_t all = (1u << cols) - 1;
         uint32_t plus = 0, minus = 0;   // bit j: column col + j holds +inf, -inf; both: NaN
 #pragma unroll 1
         for (int base = x0; base < x1; base += 32) {
-            if (!__any_sync(0xffffffffu, need && (plus & minus) != all)) break;
+            if (!__any_sync(0xffffffffu, live && (plus & minus) != all)) break;
             const int pos = base + lane;
             int64_t off = 0;
             bool hit = false, k_bad = false;
@@ -329,7 +323,7 @@ __device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const Uni
                 const int l = __ffs(hits) - 1;
                 hits &= hits - 1;
                 const int64_t key = __shfl_sync(0xffffffffu, off, l);
-                if (!need || !(seen_window(p, c.r, i, base + l - ctx) & 1)) continue;
+                if (!live || !(seen_window(p, c.r, i, base + l - ctx) & 1)) continue;
                 bool zero = false;
                 if (q_bad || ((bad_keys >> l) & 1)) {
                     float score = 0.0f;
@@ -353,16 +347,15 @@ __device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const Uni
             __syncwarp();
         }
         __syncwarp();
-        tc_ld16(o_at + col, o);
-        uint32_t u[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const bool up = (plus >> j) & 1, down = (minus >> j) & 1;
-            u[j] = __float_as_uint(up && down ? NAN : up ? INFINITY : down ? -INFINITY : scale == 0.0f ? 0.0f : o[j] * scale);
+        T* out = static_cast<T*>(p.out) + (int64_t)(c.r.q0 + i) * p.out_stride_token + (int64_t)(c.h * p.group + g) * p.out_stride_head + col;
+        for (uint32_t odd = plus | minus; odd; odd &= odd - 1) {
+            const int j = __ffs(odd) - 1;
+            const float v = (plus & minus) >> j & 1 ? NAN : plus >> j & 1 ? INFINITY : -INFINITY;
+            if (part) reinterpret_cast<float*>(part + (col + j) / 4 * RT + row)[(col + j) & 3] = v;
+            else reinterpret_cast<uint16_t*>(out)[j] = (uint16_t)pack2<T>(v, v);
         }
-        tc_st16(o_at + col, u);
-        tc_wait_st();
     }
+    __syncwarp();
 }
 
 // Join of a segment's parts (runs fc .. lc): a thread takes 16 columns of a row, a batch of parts at a time with all its
@@ -1134,31 +1127,14 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                     sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
             };
             constexpr int kCols = DT / SPLIT;   // of this thread
-            float scale = scale_o, test = 0.0f;
-#pragma unroll 1
-            for (int col = half * kCols; col < half * kCols + kCols; col += 32) {   // test: NaN if a column is not finite
-                float o[32];
-                __syncwarp();
-                tc_ld<32>(lanes + Cfg::o_col(t) + col, o);
-#pragma unroll
-                for (int j = 0; j < 32; j += 8)
-                    if (col + j < p.head_dim)
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) test = fmaf(o[j + x], 0.0f, test);
-            }
-            // (a sum of weights that is NaN makes the row NaN by itself)
-            const bool cleared = seg->cleared;
-            const bool odd = (cleared || test != 0.0f) && row < rows && ll == ll;
-            if (__builtin_expect(__any_sync(0xffffffffu, odd), 0)) {
-                settle_nonfinite<T, RT, KT>(p, &seg->c, min(row, rows - 1), odd, cleared, kt_first * KT, min((kt + 1) * KT, c.r.seq), half * kCols,
-                                            kCols, scale, lanes + Cfg::o_col(t));
-                scale = 1.0f;
-            }
             // 32 columns at a time, the row's two threads half the columns each. A thread's columns of a row are whole
             // 16-byte pieces, so they go out from its registers.
             T* out_row = row < rows ? out_ptr(row, 0) : nullptr;
+            float test = 0.0f;   // NaN if a column is not finite
             auto put8 = [&](int d, const float* v) {
                 if (row >= rows || d >= p.head_dim) return;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) test = fmaf(v[j], 0.0f, test);
                 if (whole) {
                     *reinterpret_cast<uint4*>(out_row + d) =
                         make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
@@ -1168,12 +1144,12 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                 }
             };
 #pragma unroll 1
-            for (int col = half * (DT / SPLIT); col < (half + 1) * (DT / SPLIT); col += 32) {
+            for (int col = half * kCols; col < half * kCols + kCols; col += 32) {
                 float o[32];
                 __syncwarp();
                 tc_ld<32>(lanes + Cfg::o_col(t) + col, o);   // columns past the head size hold anything: not put out
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = scale == 0.0f ? 0.0f : o[j] * scale;
+                for (int j = 0; j < 32; ++j) o[j] *= scale_o;
                 if (REP == 1) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 8) put8(col + j, o + j);
@@ -1206,6 +1182,11 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                     named_bar_sync(bar_half, 128);
                 }
             }
+            // (every repeat finds the same; a sum of weights that is NaN makes the row NaN by itself)
+            const bool odd = (test != 0.0f || (seg->cleared && row < rows)) && ll == ll;
+            if (__builtin_expect(__any_sync(0xffffffffu, odd), 0))
+                settle_nonfinite<T, RT, KT>(p, &seg->c, min(row, rows - 1), odd, kt_first * KT, min((kt + 1) * KT, c.r.seq), half * kCols, kCols,
+                                            whole ? nullptr : part);
             const bool owner = half == 0 && rep == 0 && row < rows;   // one thread per row
             if (whole) {
                 if (owner && p.lse) put_lse(row, mm, ll);
