@@ -6,7 +6,7 @@
 //                        128-byte swizzle the tensor cores read. Whole pages go by tensor copies (one or two warps, a lane
 //                        per page and 64 columns); page sizes that do not make up a tile are gathered key by key by four
 //                        warps of cp.async, whose issue rate then bounds a call (16 tokens x 8 rows over 4 x 64-128k keys:
-//                        323 us for 288, the latter now 269)
+//                        332 us for 270)
 //   Q loaders            the rows of the segment
 //   two issuers (1 thread each)  S = Q K^T (A and B from shared memory) and O += P V (A from tensor memory, V read
 //                        as it lies, N-major), fp32 accumulators in tensor memory. One thread for both left the tensor
@@ -25,13 +25,15 @@
 // The accumulator is rescaled only when a row's maximum grows by more than 2^8: P stays below 2^8, its rounding
 // is relative, and the sums are fp32, so the deferral costs no accuracy; a rescale has to wait for the product
 // in flight, the deferral makes that rare. P is rounded to the cache's type (the second product's operand), which is
-// half a unit of each weight, as much as the output's own rounding; the sum of weights is of the unrounded ones.
+// half a unit of each weight, as much as the output's own rounding; the sum of weights is of the unrounded ones. Exponentials
+// are the hardware's ex2 (2^-22 relative, results under 2^-126 are 0): far below P's rounding.
 //
-// Measured, 4 requests of 32-64k keys, 8 KV heads of 128, bf16, pages of 64 (floor 120 us of HBM): 32 rows 146 us,
-// 5.4 TB/s; 128 rows 154 us, 5.1 TB/s, 651 TFLOP/s; 256 rows 248 us, 812 TFLOP/s. The first two are bound by the key
-// stream and, at the ends of a run, by latency; the last by the softmax warps' issue (16 warps, a third of the issue
-// slots, exponentials at 40% of their pipe). Heads of 256 (floor 240 us): 267 us, 5.9 TB/s; 285 us; 522 us (two tiles of
-// 128 rows, a second trip of the keys), 770 TFLOP/s; 192: 244 us, 4.8 TB/s (a quarter of the ring idle). Warp-level
+// Measured, 4 requests of 32-64k keys, 8 KV heads of 128, bf16, pages of 64 (floor 120 us of HBM): 32 rows 145 us,
+// 5.4 TB/s; 128 rows 156 us, 5.0 TB/s, 643 TFLOP/s; 256 rows 251 us, 802 TFLOP/s. The first two are bound by the key
+// stream and, at the ends of a run, by latency; the last waits: no pipe is full (a third of the issue slots, exponentials
+// at 36% of theirs, tensor pipe 35%), its softmax warps stand at loads from tensor memory, where S is read twice, and at one
+// another. Heads of 256 (floor 240 us): 266 us, 5.9 TB/s; 288 us; 523 us (two tiles of
+// 128 rows, a second trip of the keys), 769 TFLOP/s; 192: 245 us, 4.8 TB/s (a quarter of the ring idle). Warp-level
 // matrix instructions took 780 us for the first of 256 and reached 120 TFLOP/s in the last. A call of one tile takes
 // 14 us, most of it latencies one after the other: lengths, page numbers, keys, two products, the row out.
 #pragma once

@@ -138,11 +138,13 @@ __device__ __forceinline__ float w4_swiglu(float g, float u, float limit)
 // registers, across the ends of tiles. A tile that one warp holds whole goes out from its registers; the parts of a
 // shared one lie in shared memory and its first warp adds them in order once all have ended.
 // TB: token blocks of 8 per CTA (blockIdx.y: further ones). GATED: a step is one of gate and one of up.
-// Measured: 100001 x 4096, groups of 128, 4 tokens: 50 us, 4.3 TB/s of codes and scales (floor 32 us); the instructions
-// that turn codes into fragments bound it, not the loads: 8, 16, 20 and 24 warps and 2 to 6 steps in flight are within 5%. CTAs
-// of 8 warps x 4 row tiles without a stream took 86 us. Small ones (4096 x 2048, 1 token, 10 us) are a launch and
-// one trip of the codes. At 17 tokens and more the products of 16 features x 8 tokens and, with groups of 32, their scales
-// do: 32 tokens of 2 x 2048 x 4096 12 us, 22 tokens of 2 x 5970 x 8864 51 us, 91 TFLOP/s.
+// Measured: 100001 x 4096, groups of 128, 4 tokens: 49 us, 4.3 TB/s of codes and scales (floor 32 us). No pipe is full (ALU 62%,
+// issue slots 61%, tensor pipe 26%), and 8, 16, 20 and 24 warps and 2 to 6 steps in flight are within 5%: a warp's loads and its
+// decoding wait on one another. CTAs of 8 warps x 4 row tiles without a stream took 86 us. Small ones (4096 x 2048,
+// 1 token, 10 us) are a launch and one trip of the codes. From 17 tokens on a fragment of weights feeds four products of 8 tokens
+// and a group's scales as many additions: 32 tokens of 2 x 2048 x 4096 12 us, 22 tokens of 2 x 5970 x 8864 in groups of 32 51 us,
+// 91 TFLOP/s. Every further 32 tokens read and unpack the weights again: 144 tokens of 2 x 2048 x 4096 53 us, 512 139 us.
+// Whole row tiles to a CTA leave SMs idle where the tiles are not a multiple of their number (2560 outputs: 160 tiles, 12 CTAs with two).
 template <int TB, bool GATED>
 struct W4Cfg {
     static constexpr int nt = GATED ? 2 : 1;
