@@ -279,14 +279,16 @@ __device__ __noinline__ void clear_tile(unsigned char* unit, int thread, int thr
 // Infinities and NaN of a row's sums, from the cache itself. In the products 0 * inf is NaN where the definition has no
 // such term: a repeat's P is zero outside its share of a tile's keys, a weight or a rescale may be zero in 16 or 32 bits only.
 // And new tokens' values entered them as zeros. Here a weight counts as more than zero unless its score is -inf, and
-// then 0 * inf is NaN (products of finite numbers are taken as finite). By a whole warp, a row a lane (where `live`): columns
-// col0 .. col0 + n - 1 that hold an infinity or NaN of keys x0 .. x1 - 1 are put out anew, to the output or (not null) to the part
-// at `part`. 32 keys at a time, a lane each, then those with such values in turn, for all rows. Only segments whose sums are
-// not finite, or that held such values of new tokens, come here: 4 tokens over 20000 keys that are full of them take
-// 0.6 ms. 16 columns at a time and nothing read back: what registers this function takes, the caller spills.
-template <typename T, int RT, int KT>
-__device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const UnitCursor<RT, KT>* cursor, int row, bool live, int x0, int x1, int col0,
-                                              int n, float4* part)
+// then 0 * inf is NaN (products of finite numbers are taken as finite). By a whole warp, a row a lane (where `live`): columns that hold
+// an infinity or NaN are put out anew, to the output or (not null) to the part at `part`. Keys x0 .. x1 - 1, 32 at a
+// time, a lane each, then those with such values in turn, for all rows. The warp's own columns are OWN of each 32 from col0 to
+// end; `bad` has a bit for each 32 in which they are not finite. The others can hold only what new tokens' tiles were cleared
+// of. Only segments that have either come here: 160 requests of 60000 keys, one infinity in one of them, take 2.1 ms for 0.8 (64
+// rows: 3.4); 4 tokens over 20000 keys that are full of them 0.6 ms. 16 columns at a time and nothing read back: what
+// registers this function takes, the caller spills (32 columns at a time: 32 x 64 tokens over 1-8k keys 1% slower).
+template <typename T, int RT, int KT, int OWN>
+__device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const UnitCursor<RT, KT>* cursor, int row, bool live, uint32_t bad, bool cleared,
+                                              int x0, int x1, int col0, int end, float4* part)
 {
     const UnitCursor<RT, KT> c = *cursor;
     const int lane = threadIdx.x & 31, ctx = c.r.seq - c.r.n;
@@ -300,13 +302,15 @@ __device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const Uni
     };
     const bool q_bad = live && nonfinite(q, p.head_dim);
 #pragma unroll 1
-    for (int col = col0; col < min(col0 + n, p.head_dim); col += 16) {
-        const int cols = min(p.head_dim - col, 16);
+    for (int col = col0; col < min(end, p.head_dim); col += OWN < 32 ? 32 : 16) {
+        const bool sums = __any_sync(0xffffffffu, live && (bad >> (col >> 5)) & 1);
+        if (!sums && !cleared) continue;
+        const int cols = min(p.head_dim - col, OWN < 16 ? OWN : 16), from = sums ? x0 : max(x0, ctx / KT * KT);
         const T* v_head = static_cast<const T*>(p.v_cache) + c.h * p.stride_head + col;
         const uint32_t all = (1u << cols) - 1;
         uint32_t plus = 0, minus = 0;   // bit j: column col + j holds +inf, -inf; both: NaN
 #pragma unroll 1
-        for (int base = x0; base < x1; base += 32) {
+        for (int base = from; base < x1; base += 32) {
             if (!__any_sync(0xffffffffu, live && (plus & minus) != all)) break;
             const int pos = base + lane;
             int64_t off = 0;
@@ -1132,7 +1136,8 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             // 32 columns at a time, the row's two threads half the columns each. A thread's columns of a row are whole
             // 16-byte pieces, so they go out from its registers.
             T* out_row = row < rows ? out_ptr(row, 0) : nullptr;
-            float test = 0.0f;   // NaN if a column is not finite
+            float test;          // NaN if one of 32 columns is not finite
+            uint32_t bad = 0;    // a bit for each 32 columns of which one is not
             auto put8 = [&](int d, const float* v) {
                 if (row >= rows || d >= p.head_dim) return;
 #pragma unroll
@@ -1148,6 +1153,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
 #pragma unroll 1
             for (int col = half * kCols; col < half * kCols + kCols; col += 32) {
                 float o[32];
+                test = 0.0f;
                 __syncwarp();
                 tc_ld<32>(lanes + Cfg::o_col(t) + col, o);   // columns past the head size hold anything: not put out
 #pragma unroll
@@ -1183,12 +1189,13 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                     for (int j = 0; j < OWN; j += 8) put8(col + rep * OWN + j, sum + j);
                     named_bar_sync(bar_half, 128);
                 }
+                if (test != 0.0f) bad |= 1u << (col >> 5);
             }
-            // (every repeat finds the same; a sum of weights that is NaN makes the row NaN by itself)
-            const bool odd = (test != 0.0f || (seg->cleared && row < rows)) && ll == ll;
+            // (a sum of weights that is NaN makes the row NaN by itself)
+            const bool cleared = seg->cleared, odd = (bad != 0 || (cleared && row < rows)) && ll == ll;
             if (__builtin_expect(__any_sync(0xffffffffu, odd), 0))
-                settle_nonfinite<T, RT, KT>(p, &seg->c, min(row, rows - 1), odd, kt_first * KT, min((kt + 1) * KT, c.r.seq), half * kCols, kCols,
-                                            whole ? nullptr : part);
+                settle_nonfinite<T, RT, KT, Cfg::own>(p, &seg->c, min(row, rows - 1), odd, bad, cleared, kt_first * KT, min((kt + 1) * KT, c.r.seq),
+                                                      half * kCols + rep * Cfg::own, half * kCols + kCols, whole ? nullptr : part);
             const bool owner = half == 0 && rep == 0 && row < rows;   // one thread per row
             if (whole) {
                 if (owner && p.lse) put_lse(row, mm, ll);

@@ -44,7 +44,8 @@ def check_nonfinite(s, clean, what=""):
 ROWS = [(4, 2, 64, 16, [6, 3]), (2, 1, 128, 7, [9, 4]), (4, 1, 256, 16, [7, 1]),     # up to 32 rows
         (16, 2, 128, 32, [8, 3]), (4, 1, 80, 24, [13, 2]), (8, 1, 192, 64, [7, 5]),  # up to 64
         (16, 2, 128, 16, [12, 3]), (8, 1, 256, 8, [16, 2]),                          # up to 128
-        (16, 1, 128, 64, [15, 9]), (8, 1, 64, 7, [30, 1])]                           # more
+        (16, 1, 128, 64, [15, 9]), (8, 1, 64, 7, [30, 1]),                           # more
+        (4, 2, 72, 16, [5, 3]), (8, 1, 200, 16, [9, 2]), (2, 2, 8, 32, [6, 1])]      # columns that end inside a block
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -62,7 +63,7 @@ def test_infinities_of_the_context(heads, kv, dim, page, new, tree, dtype):
     keep = s["vc"].clone()
     for puts in ([(5, 3, math.inf)], [(290, 3, -math.inf)], [(5, 3, -math.inf), (200, 3, -math.inf), (290, dim - 1, math.inf)],
                  [(17, 3, math.inf), (133, 3, -math.inf), (40, 4, math.nan), (301, 4, math.inf)],
-                 [(131, 7, math.inf), (300, 7, -math.inf)]):
+                 [(131, 7, math.inf), (300, 7, -math.inf)], [(131, slice(None, None, 2), math.inf), (300, slice(None), -math.inf)]):
         for p in puts:
             put(*p)
         check_nonfinite(s, clean, str(puts))
