@@ -283,6 +283,28 @@ def test_a_stack_without_room_loses_no_page():
     assert tb[1].cpu().tolist() == [1, 7, 6, 5]
 
 
+def test_no_page_is_lost_whatever_the_stack_holds():
+    rng = np.random.default_rng(7)
+    for case in range(60):
+        B, page, W = int(rng.integers(1, 40)), int(rng.choice([1, 3, 16])), int(rng.integers(1, 12))
+        ctx = rng.integers(0, page * W + 1, B)
+        held = np.minimum(W, -(-ctx // page) + rng.integers(0, 4, B) * rng.integers(0, 2, B))
+        ctx, new = ctx * (rng.random(B) > 0.3), rng.integers(0, 6, B)
+        spare = int(rng.integers(0, 30))
+        ids = rng.permutation(int(held.sum()) + spare).astype(np.int32)
+        table, at = np.full((B, W), -7, np.int32), 0
+        for b in range(B):
+            table[b, :held[b]] = ids[at:at + held[b]]
+            at += held[b]
+        free = np.full(spare + int(rng.choice([0, 1, 5, 20])), -9, np.int32)
+        free[:spare] = ids[at:]
+        t, tb, fr = run_tables(ctx, new, held, table, free, spare, page, int(new.sum()))
+        own = [int(p) for b in range(B) for p in tb[b, :int(t.held_pages[b])].cpu()] + fr[:int(t.free_count)].cpu().tolist()
+        assert sorted(own) == list(range(len(ids))), case
+        live = [s for s in t.slots.cpu().tolist() if s >= 0]
+        assert len(set(live)) == len(live), case
+
+
 def test_tokens_past_the_batch_are_refused():
     ctx, new, held = [5, 3, 0, 9], [3, 4, 2, 0], [1, 1, 0, 1]
     table = np.arange(16, dtype=np.int32).reshape(4, 4)
