@@ -71,9 +71,9 @@ def step_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, held_pages: 
     request order. block_table [B, W] and free_pages are updated in place; held_pages and free_count come back
     as new tensors for the next step. A finished request has lengths 0: its pages go back. Rejected drafts:
     pass the accepted context length and the surplus goes back. num_tokens is the length of the step's token
-    batch, >= sum(new_lens); requests whose tokens pass it get seq_lens 0 and slots -1 (status PAST_TOKENS). parents (int32 [num_tokens]): index within its request of each drafted token's
-    parent, which must lie before it, -1 for the context; then positions are context + depth and tree_mask is
-    built, for trees of up to 64 * mask_words tokens. A request that finds no pages is refused: status bit,
+    batch, >= sum(new_lens); requests whose tokens pass it get seq_lens 0 and slots -1 (status PAST_TOKENS). parents
+    (int32 [num_tokens]): index within its request of each drafted token's parent, which must lie before it, -1 for
+    the context; then positions are context + depth and tree_mask is built, for trees of up to 64 * mask_words tokens. A request that finds no pages is refused: status bit,
     seq_lens 0, slots -1. free_pages should have room for every page of the pool: a request whose surplus does not fit, and
     those behind it, keep theirs (status NO_ROOM) and are served all the same."""
     dev = context_lens.device

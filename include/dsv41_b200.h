@@ -260,7 +260,8 @@ enum {
  * cache, new_lens[b] new ones in this step and holds held_pages[b] pages, listed in its row of block_table.
  * It needs ceil((context + new) / page_size): surplus pages go back on the stack of free pages (in request
  * order; where the call would leave more on it than free_capacity, which a stack for every page of the pool never
- * meets, the first request whose pages do not fit and those behind it keep theirs), missing ones then come off its top (in request order) into the row. Entries of a row past its
+ * meets, the first request whose pages do not fit and those behind it keep theirs), missing ones then come off its
+ * top (in request order) into the row. Entries of a row past its
  * pages are stale. All pointers are device memory; num_tokens >= sum of new_lens (the caller knows it as
  * the length of the step's token batch; later entries get slot -1, position 0, request -1; a request whose tokens
  * pass it gets a status bit).
@@ -294,7 +295,8 @@ typedef struct dsv41_step_tables_args {
 int dsv41_step_tables(const dsv41_step_tables_args* args, void* stream);
 
 /* cache[slots[t]] = k[t], v[t]; a slot outside the cache (-1) stores nothing. 16-bit elements; head_dim a
- * multiple of 8, addresses 16-byte aligned, strides (in elements) multiples of 8, the caches' not 0. Slots that repeat within a call
+ * multiple of 8, addresses 16-byte aligned, strides (in elements) multiples of 8, the caches' not 0 (but for
+ * dimensions of one). Slots that repeat within a call
  * leave one of their tokens, whichever. */
 typedef struct dsv41_store_kv_args {
     int32_t num_tokens, kv_heads, head_dim, num_pages, page_size;
@@ -313,7 +315,8 @@ int dsv41_store_kv(const dsv41_store_kv_args* args, void* stream);
  * new tokens. Token i sees the whole context and, with tree_mask, the new tokens of its bits; without, the
  * new tokens up to itself. Keys and values that a row does not see never reach it, whatever they hold. Infinite and NaN
  * values that it sees reach it as the definition has it: a weight is zero only where the score is -inf (0 * inf is
- * NaN). A row that sees nothing, or only scores of -inf, is 0 (lse -inf); so are the rows of a request with seq_lens[b] < its new tokens or >
+ * NaN). A row that sees nothing, or only scores of -inf, is 0 (lse -inf); so are the rows of a request with
+ * seq_lens[b] < its new tokens or >
  * max_keys. Query head hq reads KV head hq / (q_heads / kv_heads). head_dim a multiple of 8 up to 256. dtype of q,
  * caches and out: fp16 or bf16. max_new: upper bound on a request's new tokens (a hint that picks the row
  * tile); num_tokens * q_heads up to 2^31 - 256. Addresses 16-byte aligned, strides (in elements) multiples of 8, those of
