@@ -322,8 +322,8 @@ int dsv41_store_kv(const dsv41_store_kv_args* args, void* stream);
  * tile); num_tokens * q_heads up to 2^31 - 256. Addresses 16-byte aligned, strides (in elements) multiples of 8, those of
  * out not 0. lse [num_tokens][q_heads] (natural
  * logarithm of the sums) or NULL. The workspace is zeroed once after allocation; every call leaves its counters
- * zero. One workspace serves one stream; its status word is read with dsv41_read_status (1 = a bounded device
- * wait ran out: zero the workspace before the next call). */
+ * zero. One workspace serves one call at a time (replays of a graph use the one it was captured with); its status
+ * word is read with dsv41_read_status (1 = a bounded device wait ran out: zero the workspace before the next call). */
 typedef struct dsv41_tree_attention_args {
     int32_t dtype, batch, num_tokens, max_new;
     int32_t q_heads, kv_heads, head_dim, page_size, num_pages, max_keys;
