@@ -28,6 +28,7 @@ SYMBOLS = (
     "dsv41_ep_peer_buffer_size", "dsv41_ep_peer_alloc", "dsv41_ep_peer_open", "dsv41_ep_peer_close", "dsv41_ep_peer_free",
     "dsv41_ep_peer_forward", "dsv41_ep_peer_read_status",
     "dsv41_step_tables", "dsv41_store_kv", "dsv41_tree_attention_workspace_size", "dsv41_tree_attention",
+    "dsv41_tree_attention_window",
     "dsv41_w4_layout_size", "dsv41_w4_pack", "dsv41_w4_linear", "dsv41_w4_gated",
     "dsv41_set_stage_timing", "dsv41_read_stage_times",
 )
@@ -178,6 +179,8 @@ def load(path: str | None = None):
         L.dsv41_tree_attention_workspace_size.argtypes = [i32, C.POINTER(C.c_size_t)]
         L.dsv41_tree_attention.restype = C.c_int
         L.dsv41_tree_attention.argtypes = [C.POINTER(TreeAttentionArgs), vp, C.c_size_t, vp]
+        L.dsv41_tree_attention_window.restype = C.c_int
+        L.dsv41_tree_attention_window.argtypes = [C.POINTER(TreeAttentionArgs), i32, i32, vp, C.c_size_t, vp]
         wp = C.POINTER(W4WeightC)
         L.dsv41_w4_layout_size.restype = C.c_int
         L.dsv41_w4_layout_size.argtypes = [i32, i32, i32, i32, C.POINTER(C.c_size_t)]

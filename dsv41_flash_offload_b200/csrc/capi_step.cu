@@ -95,6 +95,18 @@ static int w4_run(const dsv41_w4_weight* a, const dsv41_w4_weight* b, const void
     return launched(launch_w4(p, x_dtype, a->group, b != nullptr, static_cast<cudaStream_t>(stream)), "4-bit product");
 }
 
+static int check_window(int window, int sinks)
+{
+    if (window < 0 || sinks < 0) return set_error(DSV41_E_INVALID, "window=%d (0: none) sinks=%d", window, sinks);
+    if (sinks && !window) return set_error(DSV41_E_INVALID, "sinks=%d without a window", sinks);
+    return DSV41_OK;
+}
+static void set_window(TreeAttnParams& p, int window, int sinks)
+{
+    p.window = window > 0 && window < kNoWindow ? window : kNoWindow;
+    p.sinks = p.window < kNoWindow ? sinks : 0;
+}
+
 }  // namespace dsv41
 
 using namespace dsv41;
@@ -198,6 +210,12 @@ int dsv41_tree_attention_workspace_size(int32_t head_dim, size_t* bytes)
 
 int dsv41_tree_attention(const dsv41_tree_attention_args* a, void* workspace, size_t workspace_bytes, void* stream)
 {
+    return dsv41_tree_attention_window(a, 0, 0, workspace, workspace_bytes, stream);
+}
+
+int dsv41_tree_attention_window(const dsv41_tree_attention_args* a, int32_t window, int32_t sinks, void* workspace, size_t workspace_bytes,
+                                void* stream)
+{
     if (!a) return set_error(DSV41_E_INVALID, "args is NULL");
     size_t need = 0;
     int rc = dsv41_tree_attention_workspace_size(a->head_dim, &need);
@@ -213,6 +231,7 @@ int dsv41_tree_attention(const dsv41_tree_attention_args* a, void* workspace, si
         return set_error(DSV41_E_INVALID, "num_tokens * q_heads over 2^31 - 256");
     if (a->page_size < 1 || a->num_pages < 0 || a->max_keys < 0)
         return set_error(DSV41_E_INVALID, "page_size=%d num_pages=%d max_keys=%d", a->page_size, a->num_pages, a->max_keys);
+    if ((rc = check_window(window, sinks))) return rc;
     if (a->max_keys > 0x7fffff00) return set_error(DSV41_E_INVALID, "max_keys=%d", a->max_keys);
     if (a->num_tokens == 0) return DSV41_OK;
     if (!a->q || !a->k_cache || !a->v_cache || !a->block_table || !a->seq_lens || !a->cu_lens || !a->out || !workspace)
@@ -269,6 +288,7 @@ int dsv41_tree_attention(const dsv41_tree_attention_args* a, void* workspace, si
     // a scale of 0 (every key counts alike) becomes one that no score survives
     p.scale_log2 = std::fmax(std::fabs(a->scale) * 1.4426950408889634f, 1e-37f);
     p.flip = a->scale < 0.0f;
+    set_window(p, window, sinks);
     const int64_t rows = (int64_t)(a->max_new ? a->max_new : 1) * p.group;
     return launched(launch_tree_attn(p, a->dtype, (int)(rows > 1024 ? 1024 : rows), static_cast<cudaStream_t>(stream)),
                     "tree attention");

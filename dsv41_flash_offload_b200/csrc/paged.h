@@ -74,7 +74,11 @@ struct TreeAttnParams {
     int box, slot_first;                               // tensor copies: tokens, and whether slots lie within heads (set by the launch)
     float scale_log2;                                  // |scale| * log2(e), not 0 (inf * 0 is NaN)
     int flip;                                          // the scale is negative
+    int window, sinks;                                 // a token sees the last `window` keys and the first `sinks` (kNoWindow, 0: all)
+    const unsigned char* packed;                       // a cache in 4 bits instead of k_cache and v_cache
 };
+
+constexpr int kNoWindow = 1 << 30;   // longer than any cache
 
 struct AttnWorkspace {   // the status word lies at 0
     size_t counters, part_ml, part_o, total;
@@ -85,6 +89,8 @@ AttnWorkspace tree_attn_workspace(int head_dim);
 cudaError_t launch_tree_attn(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st);
 cudaError_t launch_tree_attn_f16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
 cudaError_t launch_tree_attn_bf16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
+cudaError_t launch_tree_attn_window_f16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
+cudaError_t launch_tree_attn_window_bf16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
 cudaError_t launch_step_tables(const StepTablesParams& p, cudaStream_t st);
 cudaError_t launch_store_kv(const StoreKvParams& p, cudaStream_t st);
 

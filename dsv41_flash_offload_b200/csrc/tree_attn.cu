@@ -5,7 +5,8 @@
 // hq = h * G + g:
 //     out[i, hq] = sum_j p_ij v[j, h] / sum_j p_ij,   p_ij = exp(scale * q[i, hq] . k[j, h] - m_i)
 // over the keys j that i sees: all of the context, and among the new tokens its ancestors and itself (a bit
-// mask per token), or the tokens before it and itself (no mask). A row that sees nothing is zero.
+// mask per token), or the tokens before it and itself (no mask). A row that sees nothing is zero. With a window it sees the last
+// `window` of these and those at the first `sinks` positions; tiles of keys that no row of a row tile sees are not read.
 //
 // All G query heads of a KV head and all new tokens of a request share its keys, so they are the rows
 // (r = i * G + g) of one product: each key and value is read once per tile of rows, and the softmax runs over
@@ -22,6 +23,7 @@ namespace dsv41 {
 
 cudaError_t launch_tree_attn(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st)
 {
+    if (p.window < kNoWindow) return dtype == 0 ? launch_tree_attn_window_f16(p, max_rows, st) : launch_tree_attn_window_bf16(p, max_rows, st);
     return dtype == 0 ? launch_tree_attn_f16(p, max_rows, st) : launch_tree_attn_bf16(p, max_rows, st);
 }
 

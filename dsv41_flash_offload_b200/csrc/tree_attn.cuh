@@ -81,28 +81,62 @@ __device__ __forceinline__ AttnReq attn_req(const TreeAttnParams& p, int b)
     return r;
 }
 
-// Position in the list of units: request, KV head, row tile, key tile.
+// The key tiles of a row tile, in order. Without a window: all of the request's. With one (WIN): those of the first
+// `sinks` positions, then those from the first key that the window of one of its rows reaches. Without a mask that place
+// moves with the row tile, and so does the last key; the number of tiles is the same for all row tiles of a request (so that the work can be cut
+// from sums): a span of `window` keys and the row tile's tokens wherever it begins. Tiles that are in the list
+// without need (the first row tiles of a prompt) are masked.
+template <int RT, int KT, bool WIN>
+struct KeyTiles {
+    __device__ __forceinline__ int tile(int x) const { return x; }
+    __device__ __forceinline__ int enter(const TreeAttnParams&, const AttnReq& r) { return max((r.seq + KT - 1) / KT, 1); }
+    __device__ __forceinline__ void place(const TreeAttnParams&, const AttnReq&, int, int) {}
+};
 template <int RT, int KT>
+struct KeyTiles<RT, KT, true> {
+    int sinks, skip;   // tile x of the list is tile x (x < sinks) or x + skip of the request
+    __device__ __forceinline__ int tile(int x) const { return x < sinks ? x : x + skip; }
+    // tiles of each row tile
+    __device__ __forceinline__ int enter(const TreeAttnParams& p, const AttnReq& r)
+    {
+        const int total = max((r.seq + KT - 1) / KT, 1);
+        sinks = min((min(p.sinks, r.seq) + KT - 1) / KT, total);
+        skip = 0;
+        if (p.tree_mask) return sinks + total - max(max(r.seq - r.n - p.window, 0) / KT, sinks);
+        const int span = min(p.window - 1 + min((RT - 2) / p.group + 2, r.n), r.seq);
+        return min(sinks + max(span + KT - 2, 0) / KT + 1, total);
+    }
+    __device__ __forceinline__ void place(const TreeAttnParams& p, const AttnReq& r, int rt, int count)
+    {
+        const int total = max((r.seq + KT - 1) / KT, 1), before = p.tree_mask ? 0 : p.group_div.div(rt * RT) + 1;
+        skip = min(max(max(r.seq - r.n + before - p.window, 0) / KT - sinks, 0), total - count);
+    }
+};
+
+// Position in the list of units: request, KV head, row tile, key tile.
+template <int RT, int KT, bool WIN>
 struct UnitCursor {
     int b, h, rt, kt, nrt, nkt;
     AttnReq r;
+    KeyTiles<RT, KT, WIN> keys;
     __device__ __forceinline__ void enter(const TreeAttnParams& p)
     {
         r = attn_req(p, b);
         nrt = (r.n * p.group + RT - 1) / RT;
-        nkt = max((r.seq + KT - 1) / KT, 1);
+        nkt = keys.enter(p, r);
     }
+    __device__ __forceinline__ int tile() const { return keys.tile(kt); }
     __device__ __forceinline__ void next(const TreeAttnParams& p)
     {
         if (++kt < nkt) return;
         kt = 0;
-        if (++rt < nrt) return;
+        if (++rt < nrt) return keys.place(p, r, rt, nkt);
         rt = 0;
-        if (++h < p.kv_heads) return;
+        if (++h < p.kv_heads) return keys.place(p, r, rt, nkt);
         h = 0;
         while (++b < p.batch) {
             enter(p);
-            if (r.n > 0) return;
+            if (r.n > 0) return keys.place(p, r, rt, nkt);
         }
     }
 };
@@ -120,6 +154,155 @@ __device__ __forceinline__ uint64_t seen_window(const TreeAttnParams& p, const A
     if (sh) v |= word(w + 1) << (64 - sh);
     const int left = r.n - j0;   // new tokens from j0 on
     return left >= 64 ? v : left <= 0 ? 0ull : v & (~0ull >> (64 - left));
+}
+
+// position of the first key in the window of new token i: the last `window` keys of those that it sees (negative: all of them are)
+__device__ __forceinline__ int window_start(const TreeAttnParams& p, const AttnReq& r, int i)
+{
+    const int ctx = r.seq - r.n;
+    if (!p.tree_mask) return ctx + i + 1 - p.window;
+    int seen = 0;
+    for (int j = 0; j < r.n && j < 64 * p.mask_words; j += 64) seen += __popcll(seen_window(p, r, i, j));
+    if (seen <= p.window) return ctx + seen - p.window;
+    int over = seen - p.window;   // ancestors in front of it
+    for (int j = 0;; j += 64) {
+        uint64_t v = seen_window(p, r, i, j);
+        const int here = __popcll(v);
+        if (over >= here) {
+            over -= here;
+            continue;
+        }
+        for (; over > 0; --over) v &= v - 1;
+        return ctx + j + __ffsll((long long)v) - 1;
+    }
+}
+// bits of positions pos0 .. pos0 + 63 that are among the first `sinks`, or from `start` on
+__device__ __forceinline__ uint64_t window_bits(const TreeAttnParams& p, int start, int pos0)
+{
+    const int cut = start - pos0, first = p.sinks - pos0;
+    const uint64_t in = cut <= 0 ? ~0ull : cut >= 64 ? 0ull : ~0ull << cut;
+    return in | (first <= 0 ? 0ull : first >= 64 ? ~0ull : (1ull << first) - 1);
+}
+// what new token i sees of positions pos0 .. pos0 + 63
+template <bool WIN>
+__device__ __forceinline__ uint64_t seen_keys(const TreeAttnParams& p, const AttnReq& r, int i, int pos0)
+{
+    const uint64_t seen = seen_window(p, r, i, pos0 - (r.seq - r.n));
+    return WIN ? seen & window_bits(p, window_start(p, r, i), pos0) : seen;
+}
+// whether some row of a row tile may not see all KT keys from pos0 on: last_token is its last
+template <int KT, bool WIN>
+__device__ __forceinline__ bool masked_tile(const TreeAttnParams& p, const AttnReq& r, int last_token, int pos0)
+{
+    const int ctx = r.seq - r.n;
+    if (pos0 + KT > ctx) return true;
+    return WIN && pos0 < ctx + (p.tree_mask ? r.n : last_token + 1) - p.window && pos0 + KT > p.sinks;
+}
+
+// ---- the cut of a call's units into runs, one per CTA ----
+// Calls whose segments can each have CTAs of their own: segments of up to 2 * R tiles stay whole, longer ones are cut into
+// equal parts of R at most (R = SMALL, or 2 * SMALL where there is no room for that; a place on the line is a CTA).
+// Others: a segment of nkt tiles costs what nkt + extra tiles do (its rows' loads, its end), so the runs are cut from a
+// line on which each segment begins with `extra` empty places.
+// Every thread sums its requests' places and tiles; the one whose request holds the run's first place, and the
+// one that holds its end, tell the others.
+__device__ __forceinline__ int cut_parts(int tiles, int r) { return tiles <= 2 * r ? 1 : (tiles + r - 1) / r; }
+template <int WARPS>
+struct CutShared {
+    int64_t warp_sum[WARPS][4];
+    int64_t first[3], end, tiles0;
+};
+template <int RT, int KT, bool WIN, int EXTRA, int SMALL, int WARPS>
+__device__ __forceinline__ void cut_runs(const TreeAttnParams& p, CutShared<WARPS>& sm, int64_t& run, int64_t& v0, int& part_tiles)
+{
+    constexpr int kThreads = WARPS * 32, kSums = 4;   // places on the line, tiles, parts for R = SMALL and 2 * SMALL
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (p.batch + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+    auto segments = [&](const AttnReq& r) { return r.n > 0 ? (int64_t)((r.n * p.group + RT - 1) / RT) * p.kv_heads : 0; };
+    auto tiles = [&](const AttnReq& r) {
+        return KeyTiles<RT, KT, WIN>().enter(p, r);
+    };
+    int64_t sum[kSums] = {};
+    AttnReq mine;
+    for (int b = b0; b < b1; ++b) {
+        mine = attn_req(p, b);
+        const int64_t n = segments(mine);
+        const int nt = tiles(mine);
+        sum[0] += n * (nt + EXTRA);
+        sum[1] += n * nt;
+        sum[2] += n * cut_parts(nt, SMALL);
+        sum[3] += n * cut_parts(nt, 2 * SMALL);
+    }
+    int64_t inc[kSums];
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) {
+        inc[k] = sum[k];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, inc[k], o);
+            if (lane >= o) inc[k] += y;
+        }
+        if (lane == 31) sm.warp_sum[warp][k] = inc[k];
+    }
+    __syncthreads();
+    int64_t before[kSums], all[kSums];
+    const int holders = ((p.batch + per - 1) / per + 31) / 32;   // warps that hold requests
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) {
+        before[k] = inc[k] - sum[k], all[k] = 0;
+#pragma unroll 1
+        for (int w = 0; w < holders; ++w) {
+            if (w < warp) before[k] += sm.warp_sum[w][k];
+            all[k] += sm.warp_sum[w][k];
+        }
+    }
+    part_tiles = all[2] <= gridDim.x ? SMALL : all[3] <= gridDim.x ? 2 * SMALL : 0;
+    if (part_tiles) {
+        int64_t at = part_tiles == SMALL ? before[2] : before[3];
+        run = 1;
+        v0 = blockIdx.x;
+        if (tid == 0 && v0 >= (part_tiles == SMALL ? all[2] : all[3])) sm.tiles0 = sm.end = 0;
+        for (int b = b0; b < b1; ++b) {
+            if (per > 1) mine = attn_req(p, b);
+            const int nt = tiles(mine), len = cut_parts(nt, part_tiles);
+            const int64_t places = segments(mine) * len;
+            if (v0 >= at && v0 < at + places) {
+                const int in = (int)(v0 - at), j = in % len, tpp = (nt + len - 1) / len;
+                sm.first[0] = b;
+                sm.first[1] = in / len;
+                sm.first[2] = j;
+                sm.tiles0 = j * tpp;
+                sm.end = min((j + 1) * tpp, nt);
+            }
+            at += places;
+        }
+    } else {
+        const int64_t total = all[0];
+        run = (total + gridDim.x - 1) / gridDim.x;
+        v0 = run * blockIdx.x;
+        const int64_t v1 = min(v0 + run, total);
+        if (tid == 0 && v1 >= total) sm.end = all[1];
+        int64_t at = before[0], tiles0 = before[1];
+        for (int b = b0; b < b1; ++b) {
+            if (per > 1) mine = attn_req(p, b);
+            const int64_t nt = tiles(mine), len = nt + EXTRA, places = segments(mine) * len;
+            auto tiles_before = [&](int64_t v) {   // tiles before place v of this request
+                const int64_t g = v / len, in = v - g * len;
+                return tiles0 + g * nt + max(in - EXTRA, (int64_t)0);
+            };
+            if (v0 >= at && v0 < at + places) {
+                sm.first[0] = b;
+                sm.first[1] = (v0 - at) / len;
+                sm.first[2] = (v0 - at) % len;
+                sm.tiles0 = tiles_before(v0 - at);
+            }
+            if (v1 < total && v1 >= at && v1 < at + places) sm.end = tiles_before(v1 - at);
+            at += places;
+            tiles0 += segments(mine) * nt;
+        }
+        if (v0 >= total && tid == 0) sm.tiles0 = all[1];
+    }
 }
 
 }  // namespace dsv41

@@ -5,7 +5,7 @@ namespace dsv41 {
 
 cudaError_t launch_tree_attn_bf16(const TreeAttnParams& p, int max_rows, cudaStream_t st)
 {
-    return launch_tree_attn_typed<__nv_bfloat16>(p, max_rows, st);
+    return launch_tree_attn_typed<__nv_bfloat16, false>(p, max_rows, st);
 }
 
 }  // namespace dsv41

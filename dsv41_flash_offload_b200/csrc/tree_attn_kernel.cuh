@@ -278,19 +278,19 @@ __device__ __noinline__ void clear_tile(unsigned char* unit, int thread, int thr
 
 // Infinities and NaN of a row's sums, from the cache itself. In the products 0 * inf is NaN where the definition has no
 // such term: a repeat's P is zero outside its share of a tile's keys, a weight or a rescale may be zero in 16 or 32 bits only.
-// And new tokens' values entered them as zeros. Here a weight counts as more than zero unless its score is -inf, and
+// And values that not all rows see entered them as zeros. Here a weight counts as more than zero unless its score is -inf, and
 // then 0 * inf is NaN (products of finite numbers are taken as finite). By a whole warp, a row a lane (where `live`): columns that hold
-// an infinity or NaN are put out anew, to the output or (not null) to the part at `part`. Keys x0 .. x1 - 1, 32 at a
+// an infinity or NaN are put out anew, to the output or (not null) to the part at `part`. Keys x0 .. x1 - 1 of the list of tiles, 32 at a
 // time, a lane each, then those with such values in turn, for all rows. The warp's own columns are OWN of each 32 from col0 to
 // end; `bad` has a bit for each 32 in which they are not finite. The others can hold only what new tokens' tiles were cleared
 // of. Only segments that have either come here: 160 requests of 60000 keys, one infinity in one of them, take 2.1 ms for 0.8 (64
 // rows: 3.4); 4 tokens over 20000 keys that are full of them 0.6 ms. 16 columns at a time and nothing read back: what
 // registers this function takes, the caller spills (32 columns at a time: 32 x 64 tokens over 1-8k keys 1% slower).
-template <typename T, int RT, int KT, int OWN>
-__device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const UnitCursor<RT, KT>* cursor, int row, bool live, uint32_t bad, bool cleared,
+template <typename T, int RT, int KT, int OWN, bool WIN>
+__device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const UnitCursor<RT, KT, WIN>* cursor, int row, bool live, uint32_t bad, bool cleared,
                                               int x0, int x1, int col0, int end, float4* part)
 {
-    const UnitCursor<RT, KT> c = *cursor;
+    const UnitCursor<RT, KT, WIN> c = *cursor;
     const int lane = threadIdx.x & 31, ctx = c.r.seq - c.r.n;
     const int at = c.rt * RT + row, i = p.group_div.div(at), g = at - i * p.group;
     const T* q = static_cast<const T*>(p.q) + (int64_t)(c.r.q0 + i) * p.q_stride_token + (int64_t)(c.h * p.group + g) * p.q_stride_head;
@@ -305,17 +305,17 @@ __device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const Uni
     for (int col = col0; col < min(end, p.head_dim); col += OWN < 32 ? 32 : 16) {
         const bool sums = __any_sync(0xffffffffu, live && (bad >> (col >> 5)) & 1);
         if (!sums && !cleared) continue;
-        const int cols = min(p.head_dim - col, OWN < 16 ? OWN : 16), from = sums ? x0 : max(x0, ctx / KT * KT);
+        const int cols = min(p.head_dim - col, OWN < 16 ? OWN : 16), from = sums || WIN ? x0 : max(x0, ctx / KT * KT);
         const T* v_head = static_cast<const T*>(p.v_cache) + c.h * p.stride_head + col;
         const uint32_t all = (1u << cols) - 1;
         uint32_t plus = 0, minus = 0;   // bit j: column col + j holds +inf, -inf; both: NaN
 #pragma unroll 1
-        for (int base = from; base < x1; base += 32) {
+        for (int x = from; x < x1; x += 32) {
             if (!__any_sync(0xffffffffu, live && (plus & minus) != all)) break;
-            const int pos = base + lane;
+            const int base = c.keys.tile(x / KT) * KT + x % KT, pos = base + lane;
             int64_t off = 0;
             bool hit = false, k_bad = false;
-            if (pos < x1) {
+            if (pos < c.r.seq) {
                 const int pg = p.page_div.div(pos), id = p.block_table[(int64_t)c.b * p.table_stride + pg];
                 if ((unsigned)id < (unsigned)p.num_pages) {
                     off = id * p.stride_page + (pos - pg * p.page_size) * p.stride_slot;
@@ -329,7 +329,7 @@ __device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const Uni
                 const int l = __ffs(hits) - 1;
                 hits &= hits - 1;
                 const int64_t key = __shfl_sync(0xffffffffu, off, l);
-                if (!live || !(seen_window(p, c.r, i, base + l - ctx) & 1)) continue;
+                if (!live || !(seen_keys<WIN>(p, c.r, i, base + l) & 1)) continue;
                 bool zero = false;
                 if (q_bad || ((bad_keys >> l) & 1)) {
                     float score = 0.0f;
@@ -458,13 +458,13 @@ __device__ __noinline__ void join_parts(const JoinArgs a, int fc, int lc, int r0
     }
 }
 
-template <typename T, int DT, int MT, int REP, bool TMA>
+template <typename T, int DT, int MT, int REP, bool TMA, bool WIN>
 __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn_tc_kernel(const __grid_constant__ TreeAttnParams p, const __grid_constant__ CUtensorMap tm_k,
                                                                                       const __grid_constant__ CUtensorMap tm_v)
 {
     using Cfg = TcCfg<DT, MT, REP, TMA>;
     constexpr int KT = Cfg::kt, RT = Cfg::rt, KW = Cfg::kw, NU = Cfg::units, LAG = Cfg::lag, CPR = DT / 8;
-    using Cursor = UnitCursor<RT, KT>;
+    using Cursor = UnitCursor<RT, KT, WIN>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* sq = smem;
@@ -512,113 +512,20 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     // ---- this CTA's run ----
-    // Calls whose segments can each have CTAs of their own: segments of up to 2 * R tiles stay whole, longer ones are cut into
-    // equal parts of R at most (R 4, or 8 where there is no room for 4; a place on the line is a CTA). Joining parts
-    // costs about 5 us, a tile of a CTA alone 1: 3 requests of 50 rows over 13 tiles, 2 KV heads, took 43 us in parts of one
-    // tile and take 22 us, over 2 tiles 22 and 16 us; 8 segments of 16 tiles and 4 rows 20.5 both ways.
-    // Others: a segment of nkt tiles costs what nkt + extra tiles do (its rows' loads, its end), so the runs are cut from a
-    // line on which each segment begins with `extra` empty places.
-    // Every thread sums its requests' places and tiles; the one whose request holds the run's first place, and the
-    // one that holds its end, tell the others.
-    constexpr int kSums = 4;                // places on the line, tiles, parts for R = 4 and 8
-    __shared__ int64_t warp_sum[Cfg::threads / 32][kSums];
-    __shared__ int64_t s_first[3], s_end;   // first: request, segment of the request, place in the segment; tiles before
-    __shared__ int64_t s_tiles0;
+    // Parts of 4 (8) tiles: joining parts costs about 5 us, a tile of a CTA alone 1: 3 requests of 50 rows over 13 tiles, 2 KV
+    // heads, took 43 us in parts of one tile and take 22 us, over 2 tiles 22 and 16 us; 8 segments of 16 tiles and 4 rows
+    // 20.5 both ways.
+    constexpr int kSmall = 4;
+    __shared__ CutShared<Cfg::threads / 32> cut;
     struct SegState {
         Cursor c;
         int64_t v_seg;   // place on the line where the segment begins
-        int cleared;     // its tiles held infinities or NaN of new tokens
+        int cleared;     // its tiles held infinities or NaN that not all rows see
     };
     __shared__ SegState s_seg[Cfg::soft_warps];
     int64_t run, v0;
-    int part_tiles = 0;   // R (0: runs of the line)
-    auto parts = [](int nt, int r) { return nt <= 2 * r ? 1 : (nt + r - 1) / r; };
-    {
-        const int per = (p.batch + Cfg::threads - 1) / Cfg::threads;
-        const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
-        auto segments = [&](const AttnReq& r) { return r.n > 0 ? (int64_t)((r.n * p.group + RT - 1) / RT) * p.kv_heads : 0; };
-        auto tiles = [&](const AttnReq& r) { return max((r.seq + KT - 1) / KT, 1); };
-        int64_t sum[kSums] = {};
-        AttnReq mine;
-        for (int b = b0; b < b1; ++b) {
-            mine = attn_req(p, b);
-            const int64_t n = segments(mine);
-            const int nt = tiles(mine);
-            sum[0] += n * (nt + Cfg::extra);
-            sum[1] += n * nt;
-            sum[2] += n * parts(nt, 4);
-            sum[3] += n * parts(nt, 8);
-        }
-        int64_t inc[kSums];
-#pragma unroll
-        for (int k = 0; k < kSums; ++k) {
-            inc[k] = sum[k];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t y = __shfl_up_sync(0xffffffffu, inc[k], o);
-                if (lane >= o) inc[k] += y;
-            }
-            if (lane == 31) warp_sum[warp][k] = inc[k];
-        }
-        __syncthreads();
-        int64_t before[kSums], all[kSums];
-        const int holders = ((p.batch + per - 1) / per + 31) / 32;   // warps that hold requests
-#pragma unroll
-        for (int k = 0; k < kSums; ++k) {
-            before[k] = inc[k] - sum[k], all[k] = 0;
-#pragma unroll 1
-            for (int w = 0; w < holders; ++w) {
-                if (w < warp) before[k] += warp_sum[w][k];
-                all[k] += warp_sum[w][k];
-            }
-        }
-        part_tiles = all[2] <= gridDim.x ? 4 : all[3] <= gridDim.x ? 8 : 0;
-        if (part_tiles) {
-            int64_t at = part_tiles == 4 ? before[2] : before[3];
-            run = 1;
-            v0 = blockIdx.x;
-            if (tid == 0 && v0 >= (part_tiles == 4 ? all[2] : all[3])) s_tiles0 = s_end = 0;
-            for (int b = b0; b < b1; ++b) {
-                if (per > 1) mine = attn_req(p, b);
-                const int nt = tiles(mine), len = parts(nt, part_tiles);
-                const int64_t places = segments(mine) * len;
-                if (v0 >= at && v0 < at + places) {
-                    const int in = (int)(v0 - at), j = in % len, tpp = (nt + len - 1) / len;
-                    s_first[0] = b;
-                    s_first[1] = in / len;
-                    s_first[2] = j;
-                    s_tiles0 = j * tpp;
-                    s_end = min((j + 1) * tpp, nt);
-                }
-                at += places;
-            }
-        } else {
-            const int64_t total = all[0];
-            run = (total + gridDim.x - 1) / gridDim.x;
-            v0 = run * blockIdx.x;
-            const int64_t v1 = min(v0 + run, total);
-            if (tid == 0 && v1 >= total) s_end = all[1];
-            int64_t at = before[0], tiles0 = before[1];
-            for (int b = b0; b < b1; ++b) {
-                if (per > 1) mine = attn_req(p, b);
-                const int64_t nt = tiles(mine), len = nt + Cfg::extra, places = segments(mine) * len;
-                auto tiles_before = [&](int64_t v) {   // tiles before place v of this request
-                    const int64_t g = v / len, in = v - g * len;
-                    return tiles0 + g * nt + max(in - Cfg::extra, (int64_t)0);
-                };
-                if (v0 >= at && v0 < at + places) {
-                    s_first[0] = b;
-                    s_first[1] = (v0 - at) / len;
-                    s_first[2] = (v0 - at) % len;
-                    s_tiles0 = tiles_before(v0 - at);
-                }
-                if (v1 < total && v1 >= at && v1 < at + places) s_end = tiles_before(v1 - at);
-                at += places;
-                tiles0 += segments(mine) * nt;
-            }
-            if (v0 >= total && tid == 0) s_tiles0 = all[1];
-        }
-    }
+    int part_tiles;   // R (0: runs of the line)
+    cut_runs<RT, KT, WIN, Cfg::extra, kSmall>(p, cut, run, v0, part_tiles);
     if (p.head_dim % 16) {   // the last 16-column step of Q K^T reads past the head size: zeros there
         uint4* z = reinterpret_cast<uint4*>(sq);
         for (int i = tid; i < (Cfg::q_b + NU * Cfg::unit_b) / 16; i += Cfg::threads) z[i] = make_uint4(0, 0, 0, 0);
@@ -628,21 +535,23 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
     __syncthreads();
     tcf_after();
     const uint32_t tmem = *tmem_slot;
-    const int count = (int)(s_end - s_tiles0);   // tiles of the run
+    const int count = (int)(cut.end - cut.tiles0);   // tiles of the run
     if (count <= 0) {
         if (warp == Cfg::w_s) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
         return;
     }
     Cursor cur;
-    cur.b = (int)s_first[0];
+    cur.b = (int)cut.first[0];
     cur.enter(p);
-    cur.h = (int)s_first[1] / cur.nrt;
-    cur.rt = (int)s_first[1] - cur.h * cur.nrt;
-    cur.kt = part_tiles ? (int)s_tiles0 : max((int)s_first[2] - Cfg::extra, 0);
+    cur.h = (int)cut.first[1] / cur.nrt;
+    cur.rt = (int)cut.first[1] - cur.h * cur.nrt;
+    cur.kt = part_tiles ? (int)cut.tiles0 : max((int)cut.first[2] - Cfg::extra, 0);
+    cur.keys.place(p, cur.r, cur.rt, cur.nkt);
     const int ksteps = (p.head_dim + 15) / 16;
     constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(128 >> 4) << 24);   // fp32 sums, M = 128
     auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, abort_flag, p.status); };
+    auto last_token = [&](const Cursor& c) { return p.group_div.div(min(c.rt * RT + RT, c.r.n * p.group) - 1); };   // of the row tile
     // by a whole warp, which goes on converged (the tensor memory instructions need that)
     auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
         wait(bar, parity);
@@ -663,7 +572,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         };
         auto look_up = [&](const Cursor& c) {
             Box b;
-            const int pos = c.kt * KT + in_tile * p.box, pg = p.page_div.div(pos);
+            const int pos = c.tile() * KT + in_tile * p.box, pg = p.page_div.div(pos);
             b.live = block * 64 < p.head_dim && pos < c.r.seq;
             b.page = b.live ? __ldg(p.block_table + (int64_t)c.b * p.table_stride + pg) : 0;
             b.slot = pos - pg * p.page_size;
@@ -716,7 +625,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         const uint32_t col_at = (chunk >> 3) * Cfg::block_b;
         const uint32_t ring = smem_addr(su);
         int arrived = 0;     // units handed over
-        uint32_t hist = 0;   // bit k: the unit issued k units ago holds new tokens' values
+        uint32_t hist = 0;   // bit k: the unit issued k units ago holds values that not all rows see
         auto arrive = [&](int n, bool check) {   // this thread's copies of unit n have landed
             const int slot = n % NU;
             if (__builtin_expect(check && col_live, 0)) {
@@ -777,7 +686,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         };
         // element offset of key `pt` of the cursor's tile (-1: past the end, or not a page of this cache)
         auto offset_of = [&](const Cursor& c) -> int64_t {
-            const int pos = c.kt * KT + pt;
+            const int pos = c.tile() * KT + pt;
             if (pt >= KT || pos >= c.r.seq) return -1;
             const int pg = p.page_div.div(pos);
             const int id = __ldg(p.block_table + (int64_t)c.b * p.table_stride + pg);
@@ -785,14 +694,14 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             return id * p.stride_page + (pos - pg * p.page_size) * p.stride_slot + c.h * p.stride_head;
         };
         // offsets are looked up two tiles ahead (a length, then a table entry: two trips to L2 where a request begins)
-        auto reaches_new = [](const Cursor& c) { return c.kt * KT + KT > c.r.seq - c.r.n; };
+        auto masked = [&](const Cursor& c) { return masked_tile<KT, WIN>(p, c.r, last_token(c), c.tile() * KT); };
         int64_t off[2] = {offset_of(cur), -1};
-        bool tail[2] = {reaches_new(cur), false}, tail_before = false;
+        bool tail[2] = {masked(cur), false}, tail_before = false;
         auto look_ahead = [&](int tile) {
             if (tile >= count) return;
             cur.next(p);
             off[1] = offset_of(cur);
-            tail[1] = reaches_new(cur);
+            tail[1] = masked(cur);
         };
         look_ahead(1);
         int n = 0;
@@ -938,7 +847,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         // spilled ones cost a trip to L2 each (the ring leaves no L1).
         SegState* const seg = s_seg + warp;
         seg->c = cur;
-        seg->v_seg = v0 - s_first[2];
+        seg->v_seg = v0 - cut.first[2];
         seg->cleared = 0;
         __syncwarp();
         int kt = cur.kt, nkt = cur.nkt, kt_first = kt;
@@ -967,13 +876,14 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             const bool live = t * 128 + tw * 32 < rows;
             const bool first = kt == kt_first;
             if (first) m = -INFINITY, l = 0.0f;
-            const int pos0 = kt * KT;
-            const bool tail = pos0 + KT > ctx;
+            const int pos0 = WIN ? seg->c.keys.tile(kt) * KT : kt * KT;
+            // rows differ in what they see of the tile (new tokens, a window's edge)
+            const bool tail = WIN ? masked_tile<KT, WIN>(p, seg->c.r, last_token(seg->c), pos0) : pos0 + KT > ctx;
             static_assert(KW <= 64, "one mask window per thread");
             uint64_t win = 0;
             // this row's new token
             auto token = [&]() { return p.group_div.div(min(seg->c.rt * RT + row, seg->c.r.n * p.group - 1)); };
-            if (tail && seg->c.r.seq > 0) win = seen_window(p, seg->c.r, token(), pos0 + kq - ctx);
+            if (tail && seg->c.r.seq > 0) win = seen_keys<WIN>(p, seg->c.r, token(), pos0 + kq);
             wait_warp(&s_full[buf], par);
             tcf_after();
             if (wq == 0 && half == 0 && lane == 0 && (MT == 1 || t == 1 || rows <= 128)) {   // the tile's S products have all ended
@@ -983,7 +893,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             __syncwarp();
             if (live) {
                 const uint32_t s_at = lanes + Cfg::s_col(buf) + kq, p_at = lanes + Cfg::p_col(buf, kq);
-                // Tiles that reach the new tokens: keys that the row does not see become -inf in place, before the common
+                // Tiles that reach the new tokens or a window's edge: keys that the row does not see become -inf in place, before the common
                 // path below (a negative scale is turned around there too, so that a maximum stays a maximum).
                 if (__builtin_expect(tail || p.flip, 0)) {
 #pragma unroll 1
@@ -1194,7 +1104,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             // (a sum of weights that is NaN makes the row NaN by itself)
             const bool cleared = seg->cleared, odd = (bad != 0 || (cleared && row < rows)) && ll == ll;
             if (__builtin_expect(__any_sync(0xffffffffu, odd), 0))
-                settle_nonfinite<T, RT, KT, Cfg::own>(p, &seg->c, min(row, rows - 1), odd, bad, cleared, kt_first * KT, min((kt + 1) * KT, c.r.seq),
+                settle_nonfinite<T, RT, KT, Cfg::own, WIN>(p, &seg->c, min(row, rows - 1), odd, bad, cleared, kt_first * KT, (kt + 1) * KT,
                                                       half * kCols + rep * Cfg::own, half * kCols + kCols, whole ? nullptr : part);
             const bool owner = half == 0 && rep == 0 && row < rows;   // one thread per row
             if (whole) {
@@ -1206,7 +1116,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             if (owner) p.part_ml[(int64_t)slot * RT + row] = make_float2(mm, ll);
             const int64_t v_seg = seg->v_seg;
             const int fc = part_tiles ? (int)v_seg : (int)((v_seg + Cfg::extra) / run);   // runs with tiles of it
-            const int lc = part_tiles ? fc + parts(nkt, part_tiles) - 1 : (int)((v_seg + nkt + Cfg::extra - 1) / run);
+            const int lc = part_tiles ? fc + cut_parts(nkt, part_tiles) - 1 : (int)((v_seg + nkt + Cfg::extra - 1) / run);
             int* counter = p.counters + 2 * fc + t;
             named_bar_sync(bar_group, GT);
             if (gtid == 0) {
@@ -1276,11 +1186,11 @@ static bool cache_map(CUtensorMap* m, const void* base, const TreeAttnParams& p,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DT, int MT, int REP, bool TMA>
+template <typename T, int DT, int MT, int REP, bool TMA, bool WIN>
 static cudaError_t launch_tc(const TreeAttnParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st)
 {
     using Cfg = TcCfg<DT, MT, REP, TMA>;
-    auto kernel = tree_attn_tc_kernel<T, DT, MT, REP, TMA>;
+    auto kernel = tree_attn_tc_kernel<T, DT, MT, REP, TMA, WIN>;
     static bool ready[64] = {};   // the attribute is per device and kernel, and stays
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
@@ -1293,18 +1203,18 @@ static cudaError_t launch_tc(const TreeAttnParams& p, const CUtensorMap& tm_k, c
     return cudaGetLastError();
 }
 
-template <typename T, int DT, bool TMA>
+template <typename T, int DT, bool TMA, bool WIN>
 static cudaError_t launch_tc_rows(const TreeAttnParams& p, const CUtensorMap& k, const CUtensorMap& v, int rows, cudaStream_t st)
 {
-    if (rows <= 32) return launch_tc<T, DT, 1, 4, TMA>(p, k, v, st);
-    if (rows <= 64) return launch_tc<T, DT, 1, 2, TMA>(p, k, v, st);
+    if (rows <= 32) return launch_tc<T, DT, 1, 4, TMA, WIN>(p, k, v, st);
+    if (rows <= 64) return launch_tc<T, DT, 1, 2, TMA, WIN>(p, k, v, st);
     if constexpr (DT <= 128) {
-        if (rows > 128) return launch_tc<T, DT, 2, 1, TMA>(p, k, v, st);
+        if (rows > 128) return launch_tc<T, DT, 2, 1, TMA, WIN>(p, k, v, st);
     }
-    return launch_tc<T, DT, 1, 1, TMA>(p, k, v, st);
+    return launch_tc<T, DT, 1, 1, TMA, WIN>(p, k, v, st);
 }
 
-template <typename T, int DT>
+template <typename T, int DT, bool WIN>
 static cudaError_t launch_tc_dim(TreeAttnParams p, int max_rows, cudaStream_t st)
 {
     // Whole pages go by tensor copies where a tile is whole pages (or a page whole tiles) of at least a swizzle atom's
@@ -1319,15 +1229,15 @@ static cudaError_t launch_tc_dim(TreeAttnParams p, int max_rows, cudaStream_t st
                          (p.stride_page == 0 && p.num_pages > 1);
     const bool pages = p.num_pages > 0 && !repeats && p.box >= 8 && kt % p.box == 0 && p.page_size % p.box == 0 &&
                        cache_map(&k, p.k_cache, p, bf16) && cache_map(&v, p.v_cache, p, bf16);
-    return pages ? launch_tc_rows<T, DT, true>(p, k, v, max_rows, st) : launch_tc_rows<T, DT, false>(p, k, v, max_rows, st);
+    return pages ? launch_tc_rows<T, DT, true, WIN>(p, k, v, max_rows, st) : launch_tc_rows<T, DT, false, WIN>(p, k, v, max_rows, st);
 }
 
-template <typename T>
+template <typename T, bool WIN>
 static cudaError_t launch_tree_attn_typed(const TreeAttnParams& p, int max_rows, cudaStream_t st)
 {
-    if (p.head_dim <= 64) return launch_tc_dim<T, 64>(p, max_rows, st);
-    if (p.head_dim <= 128) return launch_tc_dim<T, 128>(p, max_rows, st);
-    return launch_tc_dim<T, 256>(p, max_rows, st);
+    if (p.head_dim <= 64) return launch_tc_dim<T, 64, WIN>(p, max_rows, st);
+    if (p.head_dim <= 128) return launch_tc_dim<T, 128, WIN>(p, max_rows, st);
+    return launch_tc_dim<T, 256, WIN>(p, max_rows, st);
 }
 
 }  // namespace dsv41

@@ -219,16 +219,28 @@ def _read_and_clear(dev: torch.device, buf: torch.Tensor, stream: int) -> int:
     return st.value
 
 
+def _window(window: int | None, sinks: int) -> tuple[int, int]:
+    """Window and sinks as the library takes them (window 0: none)."""
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a window")
+        return 0, 0
+    if not 1 <= window <= 0x7fffffff or not 0 <= sinks <= 0x7fffffff:
+        raise ValueError("window must be at least 1 (None: no window), sinks at least 0")
+    return int(window), int(sinks)
+
+
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                    seq_lens: torch.Tensor, cu_lens: torch.Tensor, max_new: int, *, tree_mask: torch.Tensor | None = None,
                    scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False,
-                   workspace: torch.Tensor | None = None):
+                   workspace: torch.Tensor | None = None, window: int | None = None, sinks: int = 0):
     """Attention of the step's new tokens over the paged cache that already holds their keys and values.
 
     q [N, q_heads, head_dim] (the caches' dtype, head_dim up to 256); request b owns rows cu_lens[b]:cu_lens[b + 1]
     and the first seq_lens[b] slots of its pages, the last of them its new tokens. With tree_mask (int64 [N, words],
     step_tables) a token sees the context and the new tokens of its bits, without it the context and the new tokens
-    up to itself. max_new is an upper bound on a request's new tokens, scale defaults to head_dim ** -0.5. Query head
+    up to itself. With `window` a token sees, of these, the last `window` (itself counted) and those at the first `sinks`
+    positions of its request; tiles of keys that no token of a request sees are not read. max_new is an upper bound on a request's new tokens, scale defaults to head_dim ** -0.5. Query head
     h reads KV head h // (q_heads / kv_heads). A row that sees nothing is 0 with lse -inf. Returns out [N, q_heads,
     head_dim] in q's dtype, or (out, lse fp32 [N, q_heads]); rows past cu_lens[B] are not written. workspace: one of
     attention_workspace's, which no other call may use at the same time (default: the stream's own)."""
@@ -272,5 +284,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], table, table_stride,
         seq_lens.data_ptr(), cu_lens.data_ptr(), mask, words, dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
         os[0], os[1], lse.data_ptr() if lse is not None else None)
-    _lib.call(dev, _lib.load().dsv41_tree_attention, C.byref(args), ws, ws_bytes, stream)
+    if window is None and not sinks:
+        _lib.call(dev, _lib.load().dsv41_tree_attention, C.byref(args), ws, ws_bytes, stream)
+    else:
+        _lib.call(dev, _lib.load().dsv41_tree_attention_window, C.byref(args), *_window(window, sinks), ws, ws_bytes, stream)
     return (out, lse) if return_lse else out

@@ -345,6 +345,10 @@ typedef struct dsv41_tree_attention_args {
 } dsv41_tree_attention_args;
 int dsv41_tree_attention_workspace_size(int32_t head_dim, size_t* bytes);
 int dsv41_tree_attention(const dsv41_tree_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+/* The same through a window: of what a token sees without it, it sees the last `window` keys (itself counted, in the order
+ * of the cache) and those at the first `sinks` positions of its request. window 0: all of them (sinks 0 then). */
+int dsv41_tree_attention_window(const dsv41_tree_attention_args* args, int32_t window, int32_t sinks, void* workspace,
+                                size_t workspace_bytes, void* stream);
 
 /* 4-bit weights: w[n][k] = scale[n][k / group] * (code - zero[n][k / group]), codes 0..15, zero points
  * 0..15 (8 where there are none), groups of 32, 64 or 128 inputs, k a multiple of the group, any n.
