@@ -7,12 +7,13 @@ A drop-in for the reference (0xSero/dsv41-flash-offload) hot path behind its own
 and what a decode step with drafted tokens needs around it:
   paged                       page tables, cache store and attention of drafted trees over a paged cache
   w4                          products with 4-bit weights (projections, shared expert, head)
+  logprobs                    log probabilities of given tokens, entropy and top alternatives of rows of logits
 backed by hand-written sm_100a kernels in libdsv41_b200.so (C ABI: include/dsv41_b200.h).
 """
 from .exl3 import (Exl3MoELayer, apply_exl3_experts, apply_exl3_fused_moe, combine, decode_dense,  # noqa: F401
                    permute, read_status, workspace_bytes, FAT_EXPERT_THRESHOLD, SWIGLU_LIMIT_DEFAULT)
 from ._lib import Dsv41Error, load as load_library  # noqa: F401
-from . import paged, w4  # noqa: F401
+from . import logprobs, paged, w4  # noqa: F401
 
 __all__ = ["Exl3MoELayer", "apply_exl3_fused_moe", "apply_exl3_experts", "permute", "combine", "decode_dense",
-           "read_status", "workspace_bytes", "load_library", "Dsv41Error", "paged", "w4"]
+           "read_status", "workspace_bytes", "load_library", "Dsv41Error", "logprobs", "paged", "w4"]

@@ -30,6 +30,7 @@ SYMBOLS = (
     "dsv41_step_tables", "dsv41_store_kv", "dsv41_tree_attention_workspace_size", "dsv41_tree_attention",
     "dsv41_tree_attention_window",
     "dsv41_w4_layout_size", "dsv41_w4_pack", "dsv41_w4_linear", "dsv41_w4_gated",
+    "dsv41_token_logprobs",
     "dsv41_set_stage_timing", "dsv41_read_stage_times",
 )
 ABI_VERSION = 2
@@ -95,6 +96,12 @@ class TreeAttentionArgs(C.Structure):
 class W4WeightC(C.Structure):
     _fields_ = [("n", C.c_int32), ("k", C.c_int32), ("group", C.c_int32), ("has_zeros", C.c_int32),
                 ("scale_dtype", C.c_int32), ("data", C.c_void_p)]
+
+
+class TokenLogprobsArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("rows", C.c_int32), ("vocab", C.c_int32), ("given", C.c_int32), ("top", C.c_int32),
+                ("logits", C.c_void_p), ("row_stride", C.c_int64), ("tokens", C.c_void_p), ("logprobs", C.c_void_p),
+                ("entropy", C.c_void_p), ("lse", C.c_void_p), ("top_ids", C.c_void_p), ("top_logprobs", C.c_void_p)]
 
 
 class Dsv41Error(RuntimeError):
@@ -190,6 +197,8 @@ def load(path: str | None = None):
         L.dsv41_w4_linear.argtypes = [wp, vp, i32, C.c_int64, i32, vp, i32, C.c_int64, i32, vp]
         L.dsv41_w4_gated.restype = C.c_int
         L.dsv41_w4_gated.argtypes = [wp, wp, vp, i32, C.c_int64, i32, C.c_float, vp, i32, C.c_int64, vp]
+        L.dsv41_token_logprobs.restype = C.c_int
+        L.dsv41_token_logprobs.argtypes = [C.POINTER(TokenLogprobsArgs), vp]
         L.dsv41_set_stage_timing.restype = C.c_int
         L.dsv41_set_stage_timing.argtypes = [i32]
         L.dsv41_read_stage_times.restype = C.c_int

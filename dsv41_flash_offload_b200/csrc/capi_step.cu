@@ -6,6 +6,7 @@
 
 #include "../../include/dsv41_b200.h"
 #include "internal.h"
+#include "logprobs.h"
 #include "paged.h"
 #include "w4.h"
 
@@ -15,6 +16,7 @@ static_assert(kMaxRequests == DSV41_MAX_REQUESTS && kMaxMaskWords == DSV41_MAX_M
 static_assert(kTabNoPages == DSV41_TABLES_NO_PAGES && kTabTooWide == DSV41_TABLES_TOO_WIDE &&
                   kTabBadParent == DSV41_TABLES_BAD_PARENT && kTabBigTree == DSV41_TABLES_BIG_TREE &&
                   kTabNoRoom == DSV41_TABLES_NO_ROOM && kTabPastTokens == DSV41_TABLES_PAST_TOKENS, "header status bits");
+static_assert(kMaxTop == DSV41_MAX_TOP && kMaxGiven == DSV41_MAX_GIVEN, "header limits");
 
 static bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
@@ -329,6 +331,36 @@ int dsv41_w4_gated(const dsv41_w4_weight* gate, const dsv41_w4_weight* up, const
 {
     if (!up) return set_error(DSV41_E_INVALID, "up weight is NULL");
     return w4_run(gate, up, x, x_dtype, x_stride, tokens, limit, out, out_dtype, out_stride, 0, stream);
+}
+
+int dsv41_token_logprobs(const dsv41_token_logprobs_args* a, void* stream)
+{
+    if (!a) return set_error(DSV41_E_INVALID, "args is NULL");
+    if (a->dtype < DSV41_DTYPE_F16 || a->dtype > DSV41_DTYPE_F32) return set_error(DSV41_E_INVALID, "dtype %d (fp16, bf16 or fp32)", a->dtype);
+    if (a->rows < 0 || a->rows > (1 << 27)) return set_error(DSV41_E_INVALID, "rows=%d (0..2^27)", a->rows);
+    if (a->vocab < 1 || a->vocab > 0x7fffff00) return set_error(DSV41_E_INVALID, "vocab=%d", a->vocab);
+    if (a->given < 0 || a->given > kMaxGiven) return set_error(DSV41_E_INVALID, "given=%d (0..%d tokens a row)", a->given, kMaxGiven);
+    if (a->top < 0 || a->top > kMaxTop) return set_error(DSV41_E_INVALID, "top=%d (0..%d)", a->top, kMaxTop);
+    if (a->row_stride < 0) return set_error(DSV41_E_INVALID, "row_stride %lld", (long long)a->row_stride);
+    if (a->rows == 0) return DSV41_OK;
+    if (!a->logits || !a->entropy || !a->lse || (a->given && (!a->tokens || !a->logprobs)) || (a->top && (!a->top_ids || !a->top_logprobs)))
+        return set_error(DSV41_E_INVALID, "NULL pointer");
+    if (!aligned(a->logits, a->dtype == DSV41_DTYPE_F32 ? 4 : 2) || !aligned(a->tokens, 8) || !aligned(a->top_ids, 8))
+        return set_error(DSV41_E_INVALID, "logits, tokens or top_ids is misaligned");
+    LogprobParams p{};
+    p.logits = a->logits;
+    p.row_stride = a->row_stride;
+    p.tokens = a->tokens;
+    p.rows = a->rows;
+    p.vocab = a->vocab;
+    p.given = a->given;
+    p.top = a->top;
+    p.logprobs = a->logprobs;
+    p.entropy = a->entropy;
+    p.lse = a->lse;
+    p.top_ids = a->top_ids;
+    p.top_logprobs = a->top_logprobs;
+    return launched(launch_logprobs(p, a->dtype, static_cast<cudaStream_t>(stream)), "log probabilities");
 }
 
 }  // extern "C"

@@ -15,7 +15,7 @@ import ctypes as C
 
 import torch
 
-from . import _lib
+from . import _lib, logprobs
 
 _X_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 _OUT_DTYPES = {**_X_DTYPES, torch.float32: _lib.DTYPE_F32}
@@ -140,3 +140,19 @@ def shared_expert(x: torch.Tensor, gate: W4Weight, up: W4Weight, down: W4Weight,
     """out [T, H] fp32 (the routed experts' sum, exl3.apply_exl3_fused_moe) += down(gated(x)); the activations
     between the two products have x's type."""
     return linear(gated(x, gate, up, limit), down, out=out, accumulate=True)
+
+
+_HEAD_ROWS = 256   # rows of logits at a time: 100 MB at a vocabulary of 100000, where they stay in L2
+
+
+def head_logprobs(x: torch.Tensor, head: W4Weight, tokens: torch.Tensor, top: int = 0) -> logprobs.TokenLogprobs:
+    """What the head answers for hidden states x [N, k]: log probabilities of the given tokens [N] or [N, m] (drafted
+    children, a prompt's next tokens), entropy and the `top` likeliest tokens of each row (logprobs.token_logprobs), from fp32 logits, which
+    are formed and scored a few hundred rows at a time."""
+    if x.dim() != 2:
+        raise ValueError(f"x must be [N, {head.k}]")
+    if tokens.dim() not in (1, 2) or tokens.shape[0] != x.shape[0]:
+        raise ValueError(f"tokens must be [{x.shape[0]}] or [{x.shape[0]}, m]")
+    parts = [logprobs.token_logprobs(linear(x[r:r + _HEAD_ROWS], head, out_dtype=torch.float32), tokens[r:r + _HEAD_ROWS], top)
+             for r in range(0, max(x.shape[0], 1), _HEAD_ROWS)]
+    return parts[0] if len(parts) == 1 else logprobs.TokenLogprobs(*(torch.cat(t) for t in zip(*parts)))

@@ -374,6 +374,26 @@ int dsv41_w4_gated(const dsv41_w4_weight* gate, const dsv41_w4_weight* up, const
                    int64_t x_stride, int32_t tokens, float limit, void* out, int32_t out_dtype, int64_t out_stride,
                    void* stream);
 
+/* Scores of rows of logits [rows][row_stride] (fp16, bf16 or fp32; any stride in elements, rows need no alignment beyond
+ * their type's). Per row, with p the softmax of its vocab logits: logprobs[given] = log p of the given tokens (-inf for
+ * one outside 0..vocab - 1), entropy = -sum p log p, lse = log of the sum of exponentials, and the `top` tokens
+ * with the largest logits in descending order, equal ones by the lowest index, with their log p. Tokens with a logit
+ * of -inf are no alternatives: places that find none hold id -1 and -inf. A row of -inf alone: -inf, entropy 0, lse
+ * -inf. A row that holds NaN or +inf has no distribution: NaN throughout, ids -1. */
+enum { DSV41_MAX_TOP = 32, DSV41_MAX_GIVEN = 1024 };
+typedef struct dsv41_token_logprobs_args {
+    int32_t dtype, rows, vocab, given, top;
+    const void* logits;
+    int64_t row_stride;
+    const int64_t* tokens;        /* [rows][given] */
+    float* logprobs;              /* [rows][given] */
+    float* entropy;               /* [rows] */
+    float* lse;                   /* [rows] */
+    int64_t* top_ids;             /* [rows][top] */
+    float* top_logprobs;          /* [rows][top] */
+} dsv41_token_logprobs_args;
+int dsv41_token_logprobs(const dsv41_token_logprobs_args* args, void* stream);
+
 /* Profiling (no counterpart in the reference; used by bench.py to time each kernel on the stream
  * it runs on). While enabled, dsv41_moe_forward records CUDA events at its stage boundaries for up
  * to DSV41_TIMING_MAX_CALLS calls (not under stream capture). dsv41_read_stage_times synchronises
