@@ -29,6 +29,7 @@ SYMBOLS = (
     "dsv41_ep_peer_forward", "dsv41_ep_peer_read_status",
     "dsv41_step_tables", "dsv41_store_kv", "dsv41_tree_attention_workspace_size", "dsv41_tree_attention",
     "dsv41_tree_attention_window",
+    "dsv41_kv4_cache_size", "dsv41_kv4_store", "dsv41_kv4_load", "dsv41_kv4_move", "dsv41_tree_attention4",
     "dsv41_w4_layout_size", "dsv41_w4_pack", "dsv41_w4_linear", "dsv41_w4_gated",
     "dsv41_token_logprobs",
     "dsv41_set_stage_timing", "dsv41_read_stage_times",
@@ -91,6 +92,17 @@ class TreeAttentionArgs(C.Structure):
                 ("cu_lens", C.c_void_p), ("tree_mask", C.c_void_p), ("mask_words", C.c_int32), ("scale", C.c_float),
                 ("out", C.c_void_p), ("out_stride_token", C.c_int64), ("out_stride_head", C.c_int64),
                 ("lse", C.c_void_p)]
+
+
+class Kv4Cache(C.Structure):
+    _fields_ = [("num_pages", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("data", C.c_void_p)]
+
+
+class Kv4Tokens(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("num_tokens", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_stride_token", C.c_int64), ("k_stride_head", C.c_int64), ("v_stride_token", C.c_int64),
+                ("v_stride_head", C.c_int64), ("slots", C.c_void_p)]
 
 
 class W4WeightC(C.Structure):
@@ -188,6 +200,17 @@ def load(path: str | None = None):
         L.dsv41_tree_attention.argtypes = [C.POINTER(TreeAttentionArgs), vp, C.c_size_t, vp]
         L.dsv41_tree_attention_window.restype = C.c_int
         L.dsv41_tree_attention_window.argtypes = [C.POINTER(TreeAttentionArgs), i32, i32, vp, C.c_size_t, vp]
+        kp, tp = C.POINTER(Kv4Cache), C.POINTER(Kv4Tokens)
+        L.dsv41_kv4_cache_size.restype = C.c_int
+        L.dsv41_kv4_cache_size.argtypes = [i32, i32, i32, i32, C.POINTER(C.c_size_t)]
+        L.dsv41_kv4_store.restype = C.c_int
+        L.dsv41_kv4_store.argtypes = [kp, tp, vp]
+        L.dsv41_kv4_load.restype = C.c_int
+        L.dsv41_kv4_load.argtypes = [kp, tp, vp]
+        L.dsv41_kv4_move.restype = C.c_int
+        L.dsv41_kv4_move.argtypes = [kp, vp, vp, i32, vp, C.c_size_t, vp]
+        L.dsv41_tree_attention4.restype = C.c_int
+        L.dsv41_tree_attention4.argtypes = [C.POINTER(TreeAttentionArgs), kp, i32, i32, vp, C.c_size_t, vp]
         wp = C.POINTER(W4WeightC)
         L.dsv41_w4_layout_size.restype = C.c_int
         L.dsv41_w4_layout_size.argtypes = [i32, i32, i32, i32, C.POINTER(C.c_size_t)]

@@ -6,6 +6,7 @@
 
 #include "../../include/dsv41_b200.h"
 #include "internal.h"
+#include "kv4.cuh"
 #include "logprobs.h"
 #include "paged.h"
 #include "w4.h"
@@ -107,6 +108,138 @@ static void set_window(TreeAttnParams& p, int window, int sinks)
 {
     p.window = window > 0 && window < kNoWindow ? window : kNoWindow;
     p.sinks = p.window < kNoWindow ? sinks : 0;
+}
+
+// checks of an attention call and the kernel's parameters; cache: in 4 bits, instead of k_cache and v_cache
+static int attn_params(TreeAttnParams& p, const dsv41_tree_attention_args* a, const dsv41_kv4_cache* cache, int window, int sinks, void* workspace,
+                       size_t workspace_bytes, bool* run)
+{
+    if (!a) return set_error(DSV41_E_INVALID, "args is NULL");
+    size_t need = 0;
+    int rc = dsv41_tree_attention_workspace_size(a->head_dim, &need);
+    if (rc) return rc;
+    if (a->dtype != DSV41_DTYPE_F16 && a->dtype != DSV41_DTYPE_BF16)
+        return set_error(DSV41_E_INVALID, "dtype %d (fp16 or bf16)", a->dtype);
+    if (a->batch < 1 || a->batch > kMaxRequests) return set_error(DSV41_E_INVALID, "batch=%d (1..%d)", a->batch, kMaxRequests);
+    if (a->num_tokens < 0 || a->max_new < 0) return set_error(DSV41_E_INVALID, "num_tokens=%d max_new=%d", a->num_tokens, a->max_new);
+    if (a->kv_heads < 1 || a->q_heads < a->kv_heads || a->q_heads % a->kv_heads)
+        return set_error(DSV41_E_INVALID, "q_heads=%d is not a multiple of kv_heads=%d", a->q_heads, a->kv_heads);
+    // the kernel counts a request's rows and rounds them up to whole tiles in 32 bits
+    if ((int64_t)a->num_tokens * a->q_heads > 0x7fffffffll - 255)
+        return set_error(DSV41_E_INVALID, "num_tokens * q_heads over 2^31 - 256");
+    if (a->page_size < 1 || a->num_pages < 0 || a->max_keys < 0)
+        return set_error(DSV41_E_INVALID, "page_size=%d num_pages=%d max_keys=%d", a->page_size, a->num_pages, a->max_keys);
+    if ((rc = check_window(window, sinks))) return rc;
+    if (a->max_keys > 0x7fffff00) return set_error(DSV41_E_INVALID, "max_keys=%d", a->max_keys);
+    *run = a->num_tokens > 0;
+    if (!*run) return DSV41_OK;
+    if (!a->q || (!cache && (!a->k_cache || !a->v_cache)) || !a->block_table || !a->seq_lens || !a->cu_lens || !a->out || !workspace)
+        return set_error(DSV41_E_INVALID, "NULL pointer");
+    if (a->tree_mask && (a->mask_words < 1 || a->mask_words > kMaxMaskWords))
+        return set_error(DSV41_E_INVALID, "mask_words=%d (1..%d)", a->mask_words, kMaxMaskWords);
+    if (!aligned(a->q, 16) || !aligned(a->out, 16) || (!cache && (!aligned(a->k_cache, 16) || !aligned(a->v_cache, 16))))
+        return set_error(DSV41_E_INVALID, "q, out and the caches must be 16-byte aligned");
+    if (!aligned(workspace, 256)) return set_error(DSV41_E_INVALID, "the workspace must be 256-byte aligned");
+    if (workspace_bytes < need) return set_error(DSV41_E_WORKSPACE, "workspace %zu bytes < required %zu", workspace_bytes, need);
+    const int64_t strides[] = {a->q_stride_token, a->q_stride_head, a->out_stride_token, a->out_stride_head,
+                               cache ? 0 : a->stride_page, cache ? 0 : a->stride_slot, cache ? 0 : a->stride_head};
+    for (int64_t s : strides)
+        if (s < 0 || s % 8) return set_error(DSV41_E_INVALID, "stride %lld is not a multiple of 8 elements", (long long)s);
+    if (repeats(a->out_stride_token, a->num_tokens) || repeats(a->out_stride_head, a->q_heads))
+        return set_error(DSV41_E_INVALID, "out repeats in memory: a stride of 0 cannot be written through");
+    if (!std::isfinite(a->scale)) return set_error(DSV41_E_INVALID, "scale %g", a->scale);
+    p.q = a->q;
+    p.q_stride_token = a->q_stride_token;
+    p.q_stride_head = a->q_stride_head;
+    p.k_cache = a->k_cache;
+    p.v_cache = a->v_cache;
+    p.stride_page = a->stride_page;
+    p.stride_slot = a->stride_slot;
+    p.stride_head = a->stride_head;
+    p.packed = cache ? static_cast<const unsigned char*>(cache->data) : nullptr;
+    p.block_table = a->block_table;
+    p.table_stride = a->table_stride;
+    p.seq_lens = a->seq_lens;
+    p.cu_lens = a->cu_lens;
+    p.tree_mask = a->tree_mask;
+    p.out = a->out;
+    p.out_stride_token = a->out_stride_token;
+    p.out_stride_head = a->out_stride_head;
+    p.lse = a->lse;
+    const AttnWorkspace w = tree_attn_workspace(a->head_dim);
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    p.status = reinterpret_cast<int*>(ws);
+    p.counters = reinterpret_cast<int*>(ws + w.counters);
+    p.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
+    p.part_o = reinterpret_cast<float*>(ws + w.part_o);
+    p.batch = a->batch;
+    p.num_tokens = a->num_tokens;
+    p.q_heads = a->q_heads;
+    p.kv_heads = a->kv_heads;
+    p.group = a->q_heads / a->kv_heads;
+    p.head_dim = a->head_dim;
+    p.page_size = a->page_size;
+    p.num_pages = a->num_pages;
+    p.max_keys = a->max_keys;
+    p.mask_words = a->mask_words;
+    p.page_div = FastDiv::make(a->page_size);
+    p.group_div = FastDiv::make(p.group);
+    // a scale of 0 (every key counts alike) becomes one that no score survives
+    p.scale_log2 = std::fmax(std::fabs(a->scale) * 1.4426950408889634f, 1e-37f);
+    p.flip = a->scale < 0.0f;
+    set_window(p, window, sinks);
+    return DSV41_OK;
+}
+// upper bound on a request's rows (picks the row tile)
+static int attn_rows(const dsv41_tree_attention_args* a)
+{
+    const int64_t rows = (int64_t)(a->max_new ? a->max_new : 1) * (a->q_heads / a->kv_heads);
+    return (int)(rows > 1024 ? 1024 : rows);
+}
+
+static int check_kv4(const dsv41_kv4_cache* c, bool data)
+{
+    if (!c) return set_error(DSV41_E_INVALID, "cache is NULL");
+    if (c->num_pages < 0 || c->kv_heads < 1) return set_error(DSV41_E_INVALID, "num_pages=%d kv_heads=%d", c->num_pages, c->kv_heads);
+    if (c->page_size < kKv4Tokens || c->page_size % kKv4Tokens)
+        return set_error(DSV41_E_INVALID, "page_size=%d (a multiple of %d for a cache in 4 bits)", c->page_size, kKv4Tokens);
+    if (c->head_dim < kKv4Chunk || c->head_dim > 256 || c->head_dim % kKv4Chunk)
+        return set_error(DSV41_E_INVALID, "head_dim=%d (a multiple of %d up to 256 for a cache in 4 bits)", c->head_dim, kKv4Chunk);
+    if ((int64_t)c->page_size * c->kv_heads > (1 << 24)) return set_error(DSV41_E_INVALID, "pages of %d tokens and %d heads", c->page_size, c->kv_heads);
+    if (data && c->num_pages && (!c->data || !aligned(c->data, 16))) return set_error(DSV41_E_INVALID, "the cache's data must be 16-byte aligned");
+    return DSV41_OK;
+}
+static void kv4_cache(Kv4Params& p, const dsv41_kv4_cache* c)
+{
+    p.data = static_cast<unsigned char*>(c->data);
+    p.num_pages = c->num_pages;
+    p.page_size = c->page_size;
+    p.kv_heads = c->kv_heads;
+    p.chunks = c->head_dim / kKv4Chunk;
+}
+static int kv4_params(Kv4Params& p, const dsv41_kv4_cache* c, const dsv41_kv4_tokens* a)
+{
+    const int rc = check_kv4(c, true);
+    if (rc) return rc;
+    if (!a) return set_error(DSV41_E_INVALID, "tokens is NULL");
+    if (a->dtype != DSV41_DTYPE_F16 && a->dtype != DSV41_DTYPE_BF16) return set_error(DSV41_E_INVALID, "dtype %d (fp16 or bf16)", a->dtype);
+    if (a->num_tokens < 0) return set_error(DSV41_E_INVALID, "num_tokens=%d", a->num_tokens);
+    if (a->num_tokens == 0) return DSV41_OK;
+    if (!a->k || !a->v || !a->slots) return set_error(DSV41_E_INVALID, "NULL pointer");
+    if (!aligned(a->k, 16) || !aligned(a->v, 16)) return set_error(DSV41_E_INVALID, "k and v must be 16-byte aligned");
+    const int64_t strides[] = {a->k_stride_token, a->k_stride_head, a->v_stride_token, a->v_stride_head};
+    for (int64_t s : strides)
+        if (s < 0 || s % 8) return set_error(DSV41_E_INVALID, "stride %lld is not a multiple of 8 elements", (long long)s);
+    kv4_cache(p, c);
+    p.k = a->k;
+    p.v = a->v;
+    p.k_stride_token = a->k_stride_token;
+    p.k_stride_head = a->k_stride_head;
+    p.v_stride_token = a->v_stride_token;
+    p.v_stride_head = a->v_stride_head;
+    p.slots = a->slots;
+    p.num_tokens = a->num_tokens;
+    return DSV41_OK;
 }
 
 }  // namespace dsv41
@@ -218,82 +351,74 @@ int dsv41_tree_attention(const dsv41_tree_attention_args* a, void* workspace, si
 int dsv41_tree_attention_window(const dsv41_tree_attention_args* a, int32_t window, int32_t sinks, void* workspace, size_t workspace_bytes,
                                 void* stream)
 {
-    if (!a) return set_error(DSV41_E_INVALID, "args is NULL");
-    size_t need = 0;
-    int rc = dsv41_tree_attention_workspace_size(a->head_dim, &need);
-    if (rc) return rc;
-    if (a->dtype != DSV41_DTYPE_F16 && a->dtype != DSV41_DTYPE_BF16)
-        return set_error(DSV41_E_INVALID, "dtype %d (fp16 or bf16)", a->dtype);
-    if (a->batch < 1 || a->batch > kMaxRequests) return set_error(DSV41_E_INVALID, "batch=%d (1..%d)", a->batch, kMaxRequests);
-    if (a->num_tokens < 0 || a->max_new < 0) return set_error(DSV41_E_INVALID, "num_tokens=%d max_new=%d", a->num_tokens, a->max_new);
-    if (a->kv_heads < 1 || a->q_heads < a->kv_heads || a->q_heads % a->kv_heads)
-        return set_error(DSV41_E_INVALID, "q_heads=%d is not a multiple of kv_heads=%d", a->q_heads, a->kv_heads);
-    // the kernel counts a request's rows and rounds them up to whole tiles in 32 bits
-    if ((int64_t)a->num_tokens * a->q_heads > 0x7fffffffll - 255)
-        return set_error(DSV41_E_INVALID, "num_tokens * q_heads over 2^31 - 256");
-    if (a->page_size < 1 || a->num_pages < 0 || a->max_keys < 0)
-        return set_error(DSV41_E_INVALID, "page_size=%d num_pages=%d max_keys=%d", a->page_size, a->num_pages, a->max_keys);
-    if ((rc = check_window(window, sinks))) return rc;
-    if (a->max_keys > 0x7fffff00) return set_error(DSV41_E_INVALID, "max_keys=%d", a->max_keys);
-    if (a->num_tokens == 0) return DSV41_OK;
-    if (!a->q || !a->k_cache || !a->v_cache || !a->block_table || !a->seq_lens || !a->cu_lens || !a->out || !workspace)
-        return set_error(DSV41_E_INVALID, "NULL pointer");
-    if (a->tree_mask && (a->mask_words < 1 || a->mask_words > kMaxMaskWords))
-        return set_error(DSV41_E_INVALID, "mask_words=%d (1..%d)", a->mask_words, kMaxMaskWords);
-    if (!aligned(a->q, 16) || !aligned(a->out, 16) || !aligned(a->k_cache, 16) || !aligned(a->v_cache, 16))
-        return set_error(DSV41_E_INVALID, "q, out and the caches must be 16-byte aligned");
-    if (!aligned(workspace, 256)) return set_error(DSV41_E_INVALID, "the workspace must be 256-byte aligned");
-    if (workspace_bytes < need) return set_error(DSV41_E_WORKSPACE, "workspace %zu bytes < required %zu", workspace_bytes, need);
-    const int64_t strides[] = {a->q_stride_token, a->q_stride_head, a->out_stride_token, a->out_stride_head,
-                               a->stride_page, a->stride_slot, a->stride_head};
-    for (int64_t s : strides)
-        if (s < 0 || s % 8) return set_error(DSV41_E_INVALID, "stride %lld is not a multiple of 8 elements", (long long)s);
-    if (repeats(a->out_stride_token, a->num_tokens) || repeats(a->out_stride_head, a->q_heads))
-        return set_error(DSV41_E_INVALID, "out repeats in memory: a stride of 0 cannot be written through");
-    if (!std::isfinite(a->scale)) return set_error(DSV41_E_INVALID, "scale %g", a->scale);
     TreeAttnParams p{};
-    p.q = a->q;
-    p.q_stride_token = a->q_stride_token;
-    p.q_stride_head = a->q_stride_head;
-    p.k_cache = a->k_cache;
-    p.v_cache = a->v_cache;
-    p.stride_page = a->stride_page;
-    p.stride_slot = a->stride_slot;
-    p.stride_head = a->stride_head;
-    p.block_table = a->block_table;
-    p.table_stride = a->table_stride;
-    p.seq_lens = a->seq_lens;
-    p.cu_lens = a->cu_lens;
-    p.tree_mask = a->tree_mask;
-    p.out = a->out;
-    p.out_stride_token = a->out_stride_token;
-    p.out_stride_head = a->out_stride_head;
-    p.lse = a->lse;
-    const AttnWorkspace w = tree_attn_workspace(a->head_dim);
-    unsigned char* ws = static_cast<unsigned char*>(workspace);
-    p.status = reinterpret_cast<int*>(ws);
-    p.counters = reinterpret_cast<int*>(ws + w.counters);
-    p.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
-    p.part_o = reinterpret_cast<float*>(ws + w.part_o);
-    p.batch = a->batch;
-    p.num_tokens = a->num_tokens;
-    p.q_heads = a->q_heads;
-    p.kv_heads = a->kv_heads;
-    p.group = a->q_heads / a->kv_heads;
-    p.head_dim = a->head_dim;
-    p.page_size = a->page_size;
-    p.num_pages = a->num_pages;
-    p.max_keys = a->max_keys;
-    p.mask_words = a->mask_words;
-    p.page_div = FastDiv::make(a->page_size);
-    p.group_div = FastDiv::make(p.group);
-    // a scale of 0 (every key counts alike) becomes one that no score survives
-    p.scale_log2 = std::fmax(std::fabs(a->scale) * 1.4426950408889634f, 1e-37f);
-    p.flip = a->scale < 0.0f;
-    set_window(p, window, sinks);
-    const int64_t rows = (int64_t)(a->max_new ? a->max_new : 1) * p.group;
-    return launched(launch_tree_attn(p, a->dtype, (int)(rows > 1024 ? 1024 : rows), static_cast<cudaStream_t>(stream)),
-                    "tree attention");
+    bool run = false;
+    const int rc = attn_params(p, a, nullptr, window, sinks, workspace, workspace_bytes, &run);
+    if (rc || !run) return rc;
+    return launched(launch_tree_attn(p, a->dtype, attn_rows(a), static_cast<cudaStream_t>(stream)), "tree attention");
+}
+
+int dsv41_kv4_cache_size(int32_t num_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim, size_t* bytes)
+{
+    if (!bytes) return set_error(DSV41_E_INVALID, "bytes is NULL");
+    const dsv41_kv4_cache c{num_pages, page_size, kv_heads, head_dim, nullptr};
+    const int rc = check_kv4(&c, false);
+    if (rc) return rc;
+    *bytes = (size_t)num_pages * kv_heads * 2 * kv4_block(page_size, head_dim / kKv4Chunk);
+    return DSV41_OK;
+}
+
+int dsv41_kv4_store(const dsv41_kv4_cache* cache, const dsv41_kv4_tokens* a, void* stream)
+{
+    Kv4Params p{};
+    const int rc = kv4_params(p, cache, a);
+    if (rc || p.num_tokens == 0) return rc;
+    return launched(launch_kv4_store(p, a->dtype, static_cast<cudaStream_t>(stream)), "store in 4 bits");
+}
+
+int dsv41_kv4_load(const dsv41_kv4_cache* cache, const dsv41_kv4_tokens* a, void* stream)
+{
+    Kv4Params p{};
+    const int rc = kv4_params(p, cache, a);
+    if (rc || p.num_tokens == 0) return rc;
+    if (repeats(a->k_stride_token, a->num_tokens) || repeats(a->v_stride_token, a->num_tokens) || repeats(a->k_stride_head, cache->kv_heads) ||
+        repeats(a->v_stride_head, cache->kv_heads))
+        return set_error(DSV41_E_INVALID, "k or v repeats in memory: a stride of 0 cannot be written through");
+    return launched(launch_kv4_load(p, a->dtype, static_cast<cudaStream_t>(stream)), "load from 4 bits");
+}
+
+int dsv41_kv4_move(const dsv41_kv4_cache* cache, const int64_t* from, const int64_t* to, int32_t num_tokens, void* room, size_t room_bytes,
+                   void* stream)
+{
+    const int rc = check_kv4(cache, true);
+    if (rc) return rc;
+    if (num_tokens < 0) return set_error(DSV41_E_INVALID, "num_tokens=%d", num_tokens);
+    if (num_tokens == 0) return DSV41_OK;
+    if (!from || !to || !room) return set_error(DSV41_E_INVALID, "NULL pointer");
+    if (!aligned(room, 16)) return set_error(DSV41_E_INVALID, "room must be 16-byte aligned");
+    Kv4Params p{};
+    kv4_cache(p, cache);
+    const size_t need = (size_t)num_tokens * p.kv_heads * 2 * p.chunks * 20;
+    if (room_bytes < need) return set_error(DSV41_E_WORKSPACE, "room %zu bytes < required %zu", room_bytes, need);
+    p.slots = from;
+    p.moved = static_cast<unsigned char*>(room);
+    p.num_tokens = num_tokens;
+    return launched(launch_kv4_move(p, to, static_cast<cudaStream_t>(stream)), "move within a cache in 4 bits");
+}
+
+int dsv41_tree_attention4(const dsv41_tree_attention_args* a, const dsv41_kv4_cache* cache, int32_t window, int32_t sinks, void* workspace,
+                          size_t workspace_bytes, void* stream)
+{
+    if (!a) return set_error(DSV41_E_INVALID, "args is NULL");
+    int rc = check_kv4(cache, true);
+    if (rc) return rc;
+    if (a->kv_heads != cache->kv_heads || a->head_dim != cache->head_dim || a->page_size != cache->page_size || a->num_pages != cache->num_pages)
+        return set_error(DSV41_E_INVALID, "the arguments' heads, head_dim, page_size or num_pages are not the cache's");
+    TreeAttnParams p{};
+    bool run = false;
+    rc = attn_params(p, a, cache, window, sinks, workspace, workspace_bytes, &run);
+    if (rc || !run) return rc;
+    return launched(launch_tree_attn4(p, a->dtype, attn_rows(a), static_cast<cudaStream_t>(stream)), "tree attention over 4 bits");
 }
 
 int dsv41_w4_layout_size(int32_t n, int32_t k, int32_t group, int32_t has_zeros, size_t* bytes)

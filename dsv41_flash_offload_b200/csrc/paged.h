@@ -79,6 +79,17 @@ struct TreeAttnParams {
 };
 
 constexpr int kNoWindow = 1 << 30;   // longer than any cache
+constexpr int kAttnCtas = 4;         // most CTAs of an attention kernel on an SM
+
+// a cache in 4 bits (kv4.cuh has its layout), and the tokens of a call
+struct Kv4Params {
+    unsigned char* data;
+    const void *k, *v;                                 // [num_tokens][kv_heads][32 * chunks], 16-bit elements (load: written)
+    int64_t k_stride_token, k_stride_head, v_stride_token, v_stride_head;
+    const int64_t* slots;
+    unsigned char* moved;                              // move: room for the tokens' codes and scales
+    int num_tokens, kv_heads, chunks, num_pages, page_size;
+};
 
 struct AttnWorkspace {   // the status word lies at 0
     size_t counters, part_ml, part_o, total;
@@ -91,6 +102,13 @@ cudaError_t launch_tree_attn_f16(const TreeAttnParams& p, int max_rows, cudaStre
 cudaError_t launch_tree_attn_bf16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
 cudaError_t launch_tree_attn_window_f16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
 cudaError_t launch_tree_attn_window_bf16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
+cudaError_t launch_kv4_store(const Kv4Params& p, int dtype, cudaStream_t st);
+cudaError_t launch_kv4_load(const Kv4Params& p, int dtype, cudaStream_t st);
+cudaError_t launch_kv4_move(const Kv4Params& p, const int64_t* to, cudaStream_t st);
+// attention over a cache in 4 bits (p.packed)
+cudaError_t launch_tree_attn4(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st);
+cudaError_t launch_tree_attn4_f16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
+cudaError_t launch_tree_attn4_bf16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
 cudaError_t launch_step_tables(const StepTablesParams& p, cudaStream_t st);
 cudaError_t launch_store_kv(const StoreKvParams& p, cudaStream_t st);
 

@@ -27,7 +27,13 @@ cudaError_t launch_tree_attn(const TreeAttnParams& p, int dtype, int max_rows, c
     return dtype == 0 ? launch_tree_attn_f16(p, max_rows, st) : launch_tree_attn_bf16(p, max_rows, st);
 }
 
-// Most parts a call can leave: two per CTA (one CTA per SM), of a row tile of the padded head size.
+cudaError_t launch_tree_attn4(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st)
+{
+    return dtype == 0 ? launch_tree_attn4_f16(p, max_rows, st) : launch_tree_attn4_bf16(p, max_rows, st);
+}
+
+// Most parts a call can leave: two per CTA, of a row tile of the padded head size; CTAs that share an SM (up to kAttnCtas) have
+// smaller row tiles.
 AttnWorkspace tree_attn_workspace(int head_dim)
 {
     const int64_t dt = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
@@ -35,7 +41,7 @@ AttnWorkspace tree_attn_workspace(int head_dim)
     AttnWorkspace w;
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     w.counters = 256;
-    w.part_ml = w.counters + up(2 * ctas * sizeof(int));
+    w.part_ml = w.counters + up(kAttnCtas * ctas * sizeof(int));
     w.part_o = w.part_ml + up(rows * sizeof(float2));
     w.total = w.part_o + up(rows * dt * sizeof(float));
     return w;

@@ -1,5 +1,5 @@
-// Device helpers of the attention kernel: 16-bit pairs, asynchronous
-// copies, the kernel's view of a request, positions in the list of units, and the mask windows.
+// Device helpers of the attention kernels: 16-bit pairs, asynchronous copies, a kernel's view of a request, key tiles and
+// positions in the list of units, mask windows, the cut of the work, and the join of what was cut.
 #pragma once
 #include <cuda_bf16.h>
 
@@ -190,13 +190,16 @@ __device__ __forceinline__ uint64_t seen_keys(const TreeAttnParams& p, const Att
     const uint64_t seen = seen_window(p, r, i, pos0 - (r.seq - r.n));
     return WIN ? seen & window_bits(p, window_start(p, r, i), pos0) : seen;
 }
-// whether some row of a row tile may not see all KT keys from pos0 on: last_token is its last
+// from where on the windows of all rows of a row tile have begun (context); last_token is its last
+__device__ __forceinline__ int window_edge(const TreeAttnParams& p, const AttnReq& r, int last_token)
+{
+    return r.seq - r.n + (p.tree_mask ? r.n : last_token + 1) - p.window;
+}
+// whether some row of a row tile may not see all KT keys from pos0 on
 template <int KT, bool WIN>
 __device__ __forceinline__ bool masked_tile(const TreeAttnParams& p, const AttnReq& r, int last_token, int pos0)
 {
-    const int ctx = r.seq - r.n;
-    if (pos0 + KT > ctx) return true;
-    return WIN && pos0 < ctx + (p.tree_mask ? r.n : last_token + 1) - p.window && pos0 + KT > p.sinks;
+    return pos0 + KT > r.seq - r.n || (WIN && pos0 < window_edge(p, r, last_token) && pos0 + KT > p.sinks);
 }
 
 // ---- the cut of a call's units into runs, one per CTA ----
@@ -302,6 +305,100 @@ __device__ __forceinline__ void cut_runs(const TreeAttnParams& p, CutShared<WARP
             tiles0 += segments(mine) * nt;
         }
         if (v0 >= total && tid == 0) sm.tiles0 = all[1];
+    }
+}
+
+// Join of a segment's parts (runs fc .. lc): a thread takes 16 columns of a row, a batch of parts at a time with all its
+// loads in flight (one trip to L2 a batch), and rescales what it has as the softmax does. Rows r0 .. r0 + rows - 1 of
+// the row tile, by `threads` threads. A part is [column / 4][row][4]: neighbours in a warp are neighbouring rows
+// here and where it is written. All by value: what a function reads through a reference (the kernel's parameters, the
+// cursor) costs a trip to L2 a field and row (50 rows of 4 parts: 13000 cycles).
+struct JoinArgs {
+    const float2* ml;
+    const float4* o;
+    void* out;            // the request's first row, the KV head's first query head
+    float* lse;           // the same, or null
+    int64_t stride_token, stride_head;
+    FastDiv group_div;
+    int group, q_heads, head_dim, row0;   // row0: first row of the row tile
+};
+template <typename T, int DT, int RT>
+__device__ __noinline__ void join_parts(const JoinArgs a, int fc, int lc, int r0, int rows, int thread, int threads)
+{
+    constexpr int kBatch = 4;
+    const int blocks = (a.head_dim + 15) / 16;
+    for (int e = thread; e < rows * blocks; e += threads) {
+        const int block = e / rows, r = r0 + e - block * rows;
+        float mm = -INFINITY, ll = 0.0f, acc[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[j] = 0.0f;
+#pragma unroll 1
+        for (int q0 = fc; q0 <= lc; q0 += kBatch) {
+            float2 v[kBatch];
+            float4 po[kBatch][4];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int q = q0 + i;
+                const int64_t slot = 2 * q + (q == fc ? 1 : 0);
+                const float4* src = a.o + slot * (RT * DT / 4) + block * 4 * RT + r;
+                v[i] = q <= lc ? __ldcg(a.ml + slot * RT + r) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) po[i][k] = q <= lc ? __ldcg(src + k * RT) : make_float4(0, 0, 0, 0);
+            }
+            float top = mm;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) top = fmaxf(top, v[i].x);
+            const float safe = top == -INFINITY ? 0.0f : top, keep = exp2_fast(mm - safe);
+            ll *= keep;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[j] *= keep;
+            mm = top;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const float w = exp2_fast(v[i].x - safe);
+                ll += v[i].y * w;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    acc[4 * k] += po[i][k].x * w, acc[4 * k + 1] += po[i][k].y * w, acc[4 * k + 2] += po[i][k].z * w,
+                        acc[4 * k + 3] += po[i][k].w * w;
+            }
+        }
+        // 0 * inf is NaN where a part's weight vanishes in 32 bits: what the parts hold of infinities and NaN itself instead
+        float test = 0.0f;   // NaN if a sum is not finite (columns past the head size hold anything)
+#pragma unroll
+        for (int j = 0; j < 16; j += 8)
+            if (block * 16 + j < a.head_dim)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) test = fmaf(acc[j + c], 0.0f, test);
+        if (__builtin_expect(test != 0.0f, 0)) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float4 bad = make_float4(0, 0, 0, 0);
+#pragma unroll 1
+                for (int q = fc; q <= lc; ++q) {
+                    const float4 v = __ldcg(a.o + (int64_t)(2 * q + (q == fc ? 1 : 0)) * (RT * DT / 4) + (block * 4 + k) * RT + r);
+                    if (!(fabsf(v.x) < INFINITY)) bad.x += v.x;
+                    if (!(fabsf(v.y) < INFINITY)) bad.y += v.y;
+                    if (!(fabsf(v.z) < INFINITY)) bad.z += v.z;
+                    if (!(fabsf(v.w) < INFINITY)) bad.w += v.w;
+                }
+                if (bad.x != 0.0f) acc[4 * k] = bad.x;
+                if (bad.y != 0.0f) acc[4 * k + 1] = bad.y;
+                if (bad.z != 0.0f) acc[4 * k + 2] = bad.z;
+                if (bad.w != 0.0f) acc[4 * k + 3] = bad.w;
+            }
+        }
+        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+        const int row = a.row0 + r, i = a.group_div.div(row), g = row - i * a.group;
+        T* out = static_cast<T*>(a.out) + i * a.stride_token + g * a.stride_head + block * 16;
+#pragma unroll
+        for (int j = 0; j < 16; j += 8)
+            if (block * 16 + j < a.head_dim)
+                *reinterpret_cast<uint4*>(out + j) =
+                    make_uint4(pack2<T>(acc[j] * inv, acc[j + 1] * inv), pack2<T>(acc[j + 2] * inv, acc[j + 3] * inv),
+                               pack2<T>(acc[j + 4] * inv, acc[j + 5] * inv), pack2<T>(acc[j + 6] * inv, acc[j + 7] * inv));
+        if (a.lse && block == 0)
+            a.lse[(int64_t)i * a.q_heads + g] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
     }
 }
 

@@ -126,12 +126,12 @@ def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[torch.Size, tu
     return shape, strides, dev
 
 
-def _heads(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor) -> torch.Tensor:
+def _heads(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
     """t of this shape with contiguous, 16-byte aligned heads (copied if they are not)."""
-    if t.shape != shape or t.device != like.device:
-        raise ValueError(f"{name} must be {list(shape)} on {like.device}")
-    if t.dtype is not like.dtype:
-        raise TypeError(f"{name} is {t.dtype}, the cache {like.dtype}")
+    if t.shape != shape or t.device != dev:
+        raise ValueError(f"{name} must be {list(shape)} on {dev}")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} is {t.dtype}, the cache {dtype}")
     s = t.stride()
     if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
@@ -144,8 +144,8 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: tor
     (pages, page_size, heads, dim), cs, dev = _cache(k_cache, v_cache)
     N = slots.shape[0] if slots.dim() else 0
     slots = _vector(slots, "slots", N, torch.int64, dev)
-    k = _heads(k, "k", (N, heads, dim), k_cache)
-    v = _heads(v, "v", (N, heads, dim), k_cache)
+    k = _heads(k, "k", (N, heads, dim), k_cache.dtype, dev)
+    v = _heads(v, "v", (N, heads, dim), k_cache.dtype, dev)
     ks, vs = k.stride(), v.stride()
     args = _lib.StoreKvArgs(N, heads, dim, pages, page_size, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
                             slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2])
@@ -245,10 +245,18 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     head_dim] in q's dtype, or (out, lse fp32 [N, q_heads]); rows past cu_lens[B] are not written. workspace: one of
     attention_workspace's, which no other call may use at the same time (default: the stream's own)."""
     (pages, page_size, kv_heads, dim), cs, dev = _cache(k_cache, v_cache)
+    return _attend(q, k_cache.dtype, dev, (kv_heads, dim, page_size, pages), (k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2]),
+                   None, block_table, seq_lens, cu_lens, max_new, tree_mask, scale, out, return_lse, workspace, window, sinks)
+
+
+def _attend(q, dtype, dev, sizes, cache, packed, block_table, seq_lens, cu_lens, max_new, tree_mask, scale, out, return_lse, workspace,
+            window, sinks):
+    """Attention over a cache: `cache` its addresses and strides, or `packed` the library's view of one in 4 bits."""
+    kv_heads, dim, page_size, pages = sizes
     if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % kv_heads:
         raise ValueError(f"q must be [N, q_heads, {dim}] with q_heads a multiple of {kv_heads}")
     N, q_heads, _ = q.shape
-    q = _heads(q, "q", (N, q_heads, dim), k_cache)
+    q = _heads(q, "q", (N, q_heads, dim), dtype, dev)
     if seq_lens.dim() != 1:
         raise ValueError("seq_lens must be int32 [B]")
     B = seq_lens.shape[0]
@@ -280,12 +288,88 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         ws, ws_bytes = workspace.data_ptr(), workspace.numel()
     qs = q.stride()
     args = _lib.TreeAttentionArgs(
-        _DTYPES[q.dtype], B, N, int(max_new), q_heads, kv_heads, dim, page_size, pages, min(width * page_size, 0x7fffff00),
-        q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], table, table_stride,
+        _DTYPES[dtype], B, N, int(max_new), q_heads, kv_heads, dim, page_size, pages, min(width * page_size, 0x7fffff00),
+        q.data_ptr(), qs[0], qs[1], *cache, table, table_stride,
         seq_lens.data_ptr(), cu_lens.data_ptr(), mask, words, dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
         os[0], os[1], lse.data_ptr() if lse is not None else None)
-    if window is None and not sinks:
+    if packed is not None:
+        _lib.call(dev, _lib.load().dsv41_tree_attention4, C.byref(args), packed, *_window(window, sinks), ws, ws_bytes, stream)
+    elif window is None and not sinks:
         _lib.call(dev, _lib.load().dsv41_tree_attention, C.byref(args), ws, ws_bytes, stream)
     else:
         _lib.call(dev, _lib.load().dsv41_tree_attention_window, C.byref(args), *_window(window, sinks), ws, ws_bytes, stream)
     return (out, lse) if return_lse else out
+
+
+# ------------------------------------------------------------------------------------------------
+# a cache in 4 bits
+# ------------------------------------------------------------------------------------------------
+class Cache4:
+    """Keys and values of a layer in 4 bits: [num_pages, page_size, kv_heads, head_dim] of `dtype` in 5 bits a value, on the GPU.
+
+    Columns come in groups of 32. With lo and hi the smallest and largest value of a token's group, s = (hi - lo) / 15 in `dtype`
+    and code = round((x - lo) / s), a code stands for lo + s * code, rounded once to `dtype`. A group with NaN or an infinity
+    stands for NaN. page_size is a multiple of 8, head_dim one of 32 up to 256. The layout of `data` (uint8, [num_pages, kv_heads, 2, ...]:
+    pages can be copied whole) is the library's own; one of your own must have that size, be contiguous and 16-byte aligned."""
+
+    def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16, device=None,
+                 data: torch.Tensor | None = None):
+        if dtype not in _DTYPES:
+            raise TypeError(f"unsupported cache dtype {dtype} (fp16 or bf16)")
+        size = C.c_size_t()
+        _lib.check(_lib.load().dsv41_kv4_cache_size(num_pages, page_size, kv_heads, head_dim, C.byref(size)), "dsv41_kv4_cache_size")
+        if data is None:
+            data = torch.zeros(size.value, dtype=torch.uint8, device=_device(device))
+        if not data.is_cuda or data.dtype is not torch.uint8 or data.numel() != size.value or not data.is_contiguous() or data.data_ptr() % 16:
+            raise ValueError(f"data must be {size.value} contiguous, 16-byte aligned uint8 on a CUDA device")
+        self.data = data.view(num_pages, kv_heads, 2, -1) if num_pages else data.view(0, kv_heads, 2, page_size * head_dim // 32 * 20)
+        self.num_pages, self.page_size, self.kv_heads, self.head_dim = num_pages, page_size, kv_heads, head_dim
+        self.dtype, self.device = dtype, data.device
+        self._c = _lib.Kv4Cache(num_pages, page_size, kv_heads, head_dim, self.data.data_ptr())
+        self._ref = C.byref(self._c)
+
+
+def _tokens4(cache: Cache4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor):
+    ks, vs = k.stride(), v.stride()
+    return C.byref(_lib.Kv4Tokens(_DTYPES[cache.dtype], slots.shape[0], k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr()))
+
+
+def store_kv4(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Cache4) -> None:
+    """Round new keys and values [N, kv_heads, head_dim] (any strides with contiguous heads) into the cache's slots int64 [N]; -1
+    stores nothing. A slot may not come twice in a call."""
+    N, dev = slots.shape[0] if slots.dim() else 0, cache.device
+    slots = _vector(slots, "slots", N, torch.int64, dev)
+    shape = (N, cache.kv_heads, cache.head_dim)
+    k = _heads(k, "k", shape, cache.dtype, dev)
+    v = _heads(v, "v", shape, cache.dtype, dev)
+    _lib.call(dev, _lib.load().dsv41_kv4_store, cache._ref, _tokens4(cache, k, v, slots), _lib.current_stream(dev))
+
+
+def load_kv4(slots: torch.Tensor, cache: Cache4) -> tuple[torch.Tensor, torch.Tensor]:
+    """What the cache's slots (int64 [N]) stand for: (k, v) [N, kv_heads, head_dim] in its dtype, zeros for a slot of -1. For handing tokens
+    on: to a 16-bit cache (store_kv), to another engine."""
+    N, dev = slots.shape[0] if slots.dim() else 0, cache.device
+    slots = _vector(slots, "slots", N, torch.int64, dev)
+    k, v = (torch.empty((N, cache.kv_heads, cache.head_dim), dtype=cache.dtype, device=dev) for _ in range(2))
+    _lib.call(dev, _lib.load().dsv41_kv4_load, cache._ref, _tokens4(cache, k, v, slots), _lib.current_stream(dev))
+    return k, v
+
+
+def move_kv4(src: torch.Tensor, dst: torch.Tensor, cache: Cache4) -> None:
+    """Copy the tokens of slots src[i] to dst[i] (int64 [N]) with the bits they have, e.g. an accepted path of drafted tokens to the end
+    of its context. All are read before any is written, so a slot may be in both; none may come twice in dst. -1 in either: nothing."""
+    N, dev = src.shape[0] if src.dim() else 0, cache.device
+    src = _vector(src, "src", N, torch.int64, dev)
+    dst = _vector(dst, "dst", N, torch.int64, dev)
+    room = torch.empty(N * cache.kv_heads * cache.head_dim // 32 * 40, dtype=torch.uint8, device=dev)
+    _lib.call(dev, _lib.load().dsv41_kv4_move, cache._ref, src.data_ptr(), dst.data_ptr(), N, room.data_ptr(), room.numel(), _lib.current_stream(dev))
+
+
+def tree_attention4(q: torch.Tensor, cache: Cache4, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_lens: torch.Tensor, max_new: int, *,
+                    tree_mask: torch.Tensor | None = None, scale: float | None = None, out: torch.Tensor | None = None,
+                    return_lse: bool = False, workspace: torch.Tensor | None = None, window: int | None = None, sinks: int = 0):
+    """tree_attention over a cache in 4 bits: as over a 16-bit cache of the values that its codes stand for. q and out have the
+    cache's dtype. Workspaces are tree_attention's (one of a head size serves both)."""
+    sizes = (cache.kv_heads, cache.head_dim, cache.page_size, cache.num_pages)
+    return _attend(q, cache.dtype, cache.device, sizes, (None, None, 0, 0, 0), cache._ref, block_table, seq_lens, cu_lens, max_new, tree_mask,
+                   scale, out, return_lse, workspace, window, sinks)
