@@ -17,7 +17,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdsv41_b200.so")
 SOURCES = ["capi.cu", "permute.cu", "transform.cu", "gemv.cu", "gemm.cu", "noalloc.cu", "ep_peer.cu", "router.cu",
            "paged.cu", "tree_attn.cu", "tree_attn_f16.cu", "tree_attn_bf16.cu",
-           "tree_attn_window_f16.cu", "tree_attn_window_bf16.cu", "kv4.cu", "tree_attn4_f16.cu", "tree_attn4_bf16.cu", "w4.cu", "w4_f16.cu",
+           "tree_attn_window_f16.cu", "tree_attn_window_bf16.cu", "kv4.cu", "tree_attn4_f16.cu",
+           "tree_attn4_bf16.cu", "tree_attn4_rows_f16.cu", "tree_attn4_rows_bf16.cu", "w4.cu", "w4_f16.cu",
            "w4_bf16.cu", "logprobs.cu", "capi_step.cu"]
 HEADERS = ["common.cuh", "internal.h", "gemm.h", "paged.h", "tree_attn.cuh", "tree_attn_kernel.cuh",
            "kv4.cuh", "tree_attn4_rows.cuh", "w4.h",

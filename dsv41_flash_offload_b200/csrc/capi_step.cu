@@ -156,7 +156,6 @@ static int attn_params(TreeAttnParams& p, const dsv41_tree_attention_args* a, co
     p.stride_page = a->stride_page;
     p.stride_slot = a->stride_slot;
     p.stride_head = a->stride_head;
-    p.packed = cache ? static_cast<const unsigned char*>(cache->data) : nullptr;
     p.block_table = a->block_table;
     p.table_stride = a->table_stride;
     p.seq_lens = a->seq_lens;
@@ -172,6 +171,8 @@ static int attn_params(TreeAttnParams& p, const dsv41_tree_attention_args* a, co
     p.counters = reinterpret_cast<int*>(ws + w.counters);
     p.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
     p.part_o = reinterpret_cast<float*>(ws + w.part_o);
+    // (a cache without pages: what its keys are read from and thrown away has to exist)
+    p.packed = !cache ? nullptr : cache->num_pages ? static_cast<const unsigned char*>(cache->data) : ws;
     p.batch = a->batch;
     p.num_tokens = a->num_tokens;
     p.q_heads = a->q_heads;
@@ -206,6 +207,8 @@ static int check_kv4(const dsv41_kv4_cache* c, bool data)
     if (c->head_dim < kKv4Chunk || c->head_dim > 256 || c->head_dim % kKv4Chunk)
         return set_error(DSV41_E_INVALID, "head_dim=%d (a multiple of %d up to 256 for a cache in 4 bits)", c->head_dim, kKv4Chunk);
     if ((int64_t)c->page_size * c->kv_heads > (1 << 24)) return set_error(DSV41_E_INVALID, "pages of %d tokens and %d heads", c->page_size, c->kv_heads);
+    if ((int64_t)c->num_pages * c->kv_heads * 2 * (c->page_size / kKv4Tokens) > 0x7fffffffll)
+        return set_error(DSV41_E_INVALID, "num_pages=%d: over 2^31 - 1 records of %d tokens", c->num_pages, kKv4Tokens);
     if (data && c->num_pages && (!c->data || !aligned(c->data, 16))) return set_error(DSV41_E_INVALID, "the cache's data must be 16-byte aligned");
     return DSV41_OK;
 }

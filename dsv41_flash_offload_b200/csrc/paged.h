@@ -109,6 +109,8 @@ cudaError_t launch_kv4_move(const Kv4Params& p, const int64_t* to, cudaStream_t 
 cudaError_t launch_tree_attn4(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st);
 cudaError_t launch_tree_attn4_f16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
 cudaError_t launch_tree_attn4_bf16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
+cudaError_t launch_tree_attn4_rows_f16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
+cudaError_t launch_tree_attn4_rows_bf16(const TreeAttnParams& p, int max_rows, cudaStream_t st);
 cudaError_t launch_step_tables(const StepTablesParams& p, cudaStream_t st);
 cudaError_t launch_store_kv(const StoreKvParams& p, cudaStream_t st);
 

@@ -27,8 +27,11 @@ cudaError_t launch_tree_attn(const TreeAttnParams& p, int dtype, int max_rows, c
     return dtype == 0 ? launch_tree_attn_f16(p, max_rows, st) : launch_tree_attn_bf16(p, max_rows, st);
 }
 
+constexpr int kFewRows = 16;   // up to which codes are decoded into fragments of warp-level instructions
+
 cudaError_t launch_tree_attn4(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st)
 {
+    if (max_rows <= kFewRows) return dtype == 0 ? launch_tree_attn4_rows_f16(p, max_rows, st) : launch_tree_attn4_rows_bf16(p, max_rows, st);
     return dtype == 0 ? launch_tree_attn4_f16(p, max_rows, st) : launch_tree_attn4_bf16(p, max_rows, st);
 }
 

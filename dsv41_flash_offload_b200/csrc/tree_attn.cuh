@@ -82,34 +82,34 @@ __device__ __forceinline__ AttnReq attn_req(const TreeAttnParams& p, int b)
 }
 
 // The key tiles of a row tile, in order. Without a window: all of the request's. With one (WIN): those of the first
-// `sinks` positions, then those from the first key that the window of one of its rows reaches. Without a mask that place
-// moves with the row tile, and so does the last key; the number of tiles is the same for all row tiles of a request (so that the work can be cut
-// from sums): a span of `window` keys and the row tile's tokens wherever it begins. Tiles that are in the list
-// without need (the first row tiles of a prompt) are masked.
+// `sinks` positions, then those from the first key that the window of one of its rows reaches; without a mask also only up to the last
+// token of the row tile, so that a prompt's row tiles have lists of their own (a list that is the same for all, long enough for the
+// longest, cost 1330 us for 900 on 2 x 6000-8192 tokens through a window of 2048: the tiles too many are masked, the
+// slowest kind).
 template <int RT, int KT, bool WIN>
 struct KeyTiles {
     __device__ __forceinline__ int tile(int x) const { return x; }
-    __device__ __forceinline__ int enter(const TreeAttnParams&, const AttnReq& r) { return max((r.seq + KT - 1) / KT, 1); }
-    __device__ __forceinline__ void place(const TreeAttnParams&, const AttnReq&, int, int) {}
+    // of row tile rt; how many there are
+    __device__ __forceinline__ int place(const TreeAttnParams&, const AttnReq& r, int) { return max((r.seq + KT - 1) / KT, 1); }
 };
 template <int RT, int KT>
 struct KeyTiles<RT, KT, true> {
     int sinks, skip;   // tile x of the list is tile x (x < sinks) or x + skip of the request
     __device__ __forceinline__ int tile(int x) const { return x < sinks ? x : x + skip; }
-    // tiles of each row tile
-    __device__ __forceinline__ int enter(const TreeAttnParams& p, const AttnReq& r)
+    __device__ __forceinline__ int place(const TreeAttnParams& p, const AttnReq& r, int rt)
     {
-        const int total = max((r.seq + KT - 1) / KT, 1);
-        sinks = min((min(p.sinks, r.seq) + KT - 1) / KT, total);
-        skip = 0;
-        if (p.tree_mask) return sinks + total - max(max(r.seq - r.n - p.window, 0) / KT, sinks);
-        const int span = min(p.window - 1 + min((RT - 2) / p.group + 2, r.n), r.seq);
-        return min(sinks + max(span + KT - 2, 0) / KT + 1, total);
-    }
-    __device__ __forceinline__ void place(const TreeAttnParams& p, const AttnReq& r, int rt, int count)
-    {
-        const int total = max((r.seq + KT - 1) / KT, 1), before = p.tree_mask ? 0 : p.group_div.div(rt * RT) + 1;
-        skip = min(max(max(r.seq - r.n + before - p.window, 0) / KT - sinks, 0), total - count);
+        sinks = skip = 0;
+        if (r.seq <= 0) return 1;
+        const int ctx = r.seq - r.n;
+        int before = 0, last = r.seq - 1;   // the row tile's first token (and itself), if it says where the window begins; its last key
+        if (!p.tree_mask) {
+            before = p.group_div.div(rt * RT) + 1;
+            last = ctx + p.group_div.div(min(rt * RT + RT, r.n * p.group) - 1);
+        }
+        const int end = last / KT + 1, first = max(ctx + before - p.window, 0) / KT;
+        sinks = min((min(p.sinks, r.seq) + KT - 1) / KT, end);
+        skip = max(first - sinks, 0);
+        return end - skip;
     }
 };
 
@@ -123,20 +123,24 @@ struct UnitCursor {
     {
         r = attn_req(p, b);
         nrt = (r.n * p.group + RT - 1) / RT;
-        nkt = keys.enter(p, r);
+        if (!WIN) nkt = keys.place(p, r, 0);
+    }
+    __device__ __forceinline__ void place(const TreeAttnParams& p)
+    {
+        if (WIN) nkt = keys.place(p, r, rt);
     }
     __device__ __forceinline__ int tile() const { return keys.tile(kt); }
     __device__ __forceinline__ void next(const TreeAttnParams& p)
     {
         if (++kt < nkt) return;
         kt = 0;
-        if (++rt < nrt) return keys.place(p, r, rt, nkt);
+        if (++rt < nrt) return place(p);
         rt = 0;
-        if (++h < p.kv_heads) return keys.place(p, r, rt, nkt);
+        if (++h < p.kv_heads) return place(p);
         h = 0;
         while (++b < p.batch) {
             enter(p);
-            if (r.n > 0) return keys.place(p, r, rt, nkt);
+            if (r.n > 0) return place(p);
         }
     }
 };
@@ -190,16 +194,28 @@ __device__ __forceinline__ uint64_t seen_keys(const TreeAttnParams& p, const Att
     const uint64_t seen = seen_window(p, r, i, pos0 - (r.seq - r.n));
     return WIN ? seen & window_bits(p, window_start(p, r, i), pos0) : seen;
 }
-// from where on the windows of all rows of a row tile have begun (context); last_token is its last
-__device__ __forceinline__ int window_edge(const TreeAttnParams& p, const AttnReq& r, int last_token)
+// Where the rows of a row tile (tokens first .. last) may differ in what they see: keys from `from` on are new tokens that not
+// all of them see, keys before `edge` lie in front of the window of one of them (the first p.sinks do not).
+template <bool WIN>
+struct MaskedKeys {
+    int from, edge;
+    __device__ __forceinline__ MaskedKeys() {}
+    __device__ __forceinline__ MaskedKeys(const TreeAttnParams& p, const AttnReq& r, int first, int last)
+    {
+        const int ctx = r.seq - r.n;
+        from = p.tree_mask ? ctx : ctx + first + 1;
+        edge = ctx + (p.tree_mask ? r.n : last + 1) - p.window;
+    }
+    template <int KT>
+    __device__ __forceinline__ bool tile(const TreeAttnParams& p, int pos0) const
+    {
+        return pos0 + KT > from || (WIN && pos0 < edge && pos0 + KT > p.sinks);
+    }
+};
+template <int RT, bool WIN, typename Cursor>
+__device__ __forceinline__ MaskedKeys<WIN> masked_keys(const TreeAttnParams& p, const Cursor& c)
 {
-    return r.seq - r.n + (p.tree_mask ? r.n : last_token + 1) - p.window;
-}
-// whether some row of a row tile may not see all KT keys from pos0 on
-template <int KT, bool WIN>
-__device__ __forceinline__ bool masked_tile(const TreeAttnParams& p, const AttnReq& r, int last_token, int pos0)
-{
-    return pos0 + KT > r.seq - r.n || (WIN && pos0 < window_edge(p, r, last_token) && pos0 + KT > p.sinks);
+    return MaskedKeys<WIN>(p, c.r, p.group_div.div(c.rt * RT), p.group_div.div(min(c.rt * RT + RT, c.r.n * p.group) - 1));
 }
 
 // ---- the cut of a call's units into runs, one per CTA ----
@@ -215,6 +231,33 @@ struct CutShared {
     int64_t warp_sum[WARPS][4];
     int64_t first[3], end, tiles0;
 };
+// Sums over the row tiles of one head of a request, each with its own number of key tiles (WIN, no mask): places, tiles, parts for
+// R = SMALL and 2 * SMALL. By a whole warp, a request a lane: those with many row tiles are summed by all lanes together.
+template <int RT, int KT, int EXTRA, int SMALL>
+__device__ __noinline__ void head_sums(const TreeAttnParams& p, int n, int seq, int64_t* s)
+{
+    const int lane = threadIdx.x & 31, nrt = n > 0 ? (n * p.group + RT - 1) / RT : 0;
+    auto add = [&](const AttnReq& r, int rt, int64_t* to) {
+        const int nt = KeyTiles<RT, KT, true>().place(p, r, rt);
+        to[0] += nt + EXTRA, to[1] += nt, to[2] += cut_parts(nt, SMALL), to[3] += cut_parts(nt, 2 * SMALL);
+    };
+    s[0] = s[1] = s[2] = s[3] = 0;
+    if (nrt <= 4)
+        for (int rt = 0; rt < nrt; ++rt) add(AttnReq{0, n, seq}, rt, s);
+    for (uint32_t many = __ballot_sync(0xffffffffu, nrt > 4); many; many &= many - 1) {
+        const int l = __ffs(many) - 1, tiles = __shfl_sync(0xffffffffu, nrt, l);
+        const AttnReq r{0, __shfl_sync(0xffffffffu, n, l), __shfl_sync(0xffffffffu, seq, l)};
+        int64_t v[4] = {0, 0, 0, 0};
+        for (int rt = lane; rt < tiles; rt += 32) add(r, rt, v);
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+            if (lane == l) s[k] = v[k];
+        }
+        __syncwarp();
+    }
+}
+
 template <int RT, int KT, bool WIN, int EXTRA, int SMALL, int WARPS>
 __device__ __forceinline__ void cut_runs(const TreeAttnParams& p, CutShared<WARPS>& sm, int64_t& run, int64_t& v0, int& part_tiles)
 {
@@ -222,20 +265,23 @@ __device__ __forceinline__ void cut_runs(const TreeAttnParams& p, CutShared<WARP
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (p.batch + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
-    auto segments = [&](const AttnReq& r) { return r.n > 0 ? (int64_t)((r.n * p.group + RT - 1) / RT) * p.kv_heads : 0; };
-    auto tiles = [&](const AttnReq& r) {
-        return KeyTiles<RT, KT, WIN>().enter(p, r);
+    const bool own_lists = WIN && !p.tree_mask;   // row tiles of a request differ in their number of key tiles
+    auto row_tiles = [&](const AttnReq& r) { return r.n > 0 ? (r.n * p.group + RT - 1) / RT : 0; };
+    auto tiles = [&](const AttnReq& r) { return KeyTiles<RT, KT, WIN>().place(p, r, 0); };
+    // sums over one head of request b (of this thread's; all threads go round together)
+    auto sums = [&](const AttnReq& r, int64_t* s) {
+        if (WIN && own_lists) return head_sums<RT, KT, EXTRA, SMALL>(p, r.n, r.seq, s);
+        const int64_t n = row_tiles(r);
+        const int nt = tiles(r);
+        s[0] = n * (nt + EXTRA), s[1] = n * nt, s[2] = n * cut_parts(nt, SMALL), s[3] = n * cut_parts(nt, 2 * SMALL);
     };
-    int64_t sum[kSums] = {};
-    AttnReq mine;
-    for (int b = b0; b < b1; ++b) {
-        mine = attn_req(p, b);
-        const int64_t n = segments(mine);
-        const int nt = tiles(mine);
-        sum[0] += n * (nt + EXTRA);
-        sum[1] += n * nt;
-        sum[2] += n * cut_parts(nt, SMALL);
-        sum[3] += n * cut_parts(nt, 2 * SMALL);
+    int64_t sum[kSums] = {}, head[kSums];
+    AttnReq mine{0, 0, 0};
+    for (int i = 0; i < per; ++i) {
+        mine = b0 + i < b1 ? attn_req(p, b0 + i) : AttnReq{0, 0, 0};
+        sums(mine, head);
+#pragma unroll
+        for (int k = 0; k < kSums; ++k) sum[k] += head[k] * p.kv_heads;
     }
     int64_t inc[kSums];
 #pragma unroll
@@ -261,50 +307,66 @@ __device__ __forceinline__ void cut_runs(const TreeAttnParams& p, CutShared<WARP
         }
     }
     part_tiles = all[2] <= gridDim.x ? SMALL : all[3] <= gridDim.x ? 2 * SMALL : 0;
-    if (part_tiles) {
-        int64_t at = part_tiles == SMALL ? before[2] : before[3];
-        run = 1;
-        v0 = blockIdx.x;
-        if (tid == 0 && v0 >= (part_tiles == SMALL ? all[2] : all[3])) sm.tiles0 = sm.end = 0;
-        for (int b = b0; b < b1; ++b) {
-            if (per > 1) mine = attn_req(p, b);
-            const int nt = tiles(mine), len = cut_parts(nt, part_tiles);
-            const int64_t places = segments(mine) * len;
-            if (v0 >= at && v0 < at + places) {
-                const int in = (int)(v0 - at), j = in % len, tpp = (nt + len - 1) / len;
-                sm.first[0] = b;
-                sm.first[1] = in / len;
-                sm.first[2] = j;
-                sm.tiles0 = j * tpp;
-                sm.end = min((j + 1) * tpp, nt);
-            }
-            at += places;
+    auto places_in = [&](const int64_t* s) { return part_tiles == SMALL ? s[2] : part_tiles ? s[3] : s[0]; };
+    const int64_t total = places_in(all);
+    run = part_tiles ? 1 : (total + gridDim.x - 1) / gridDim.x;
+    v0 = run * blockIdx.x;
+    const int64_t v1 = min(v0 + run, total);
+    if (tid == 0) {
+        if (v0 >= total) sm.tiles0 = sm.end = 0;
+        else if (!part_tiles && v1 >= total) sm.end = all[1];
+    }
+    int64_t at = places_in(before), tiles0 = before[1];
+    for (int i = 0; i < per; ++i) {
+        if (per > 1) {
+            mine = b0 + i < b1 ? attn_req(p, b0 + i) : AttnReq{0, 0, 0};
+            sums(mine, head);
         }
-    } else {
-        const int64_t total = all[0];
-        run = (total + gridDim.x - 1) / gridDim.x;
-        v0 = run * blockIdx.x;
-        const int64_t v1 = min(v0 + run, total);
-        if (tid == 0 && v1 >= total) sm.end = all[1];
-        int64_t at = before[0], tiles0 = before[1];
-        for (int b = b0; b < b1; ++b) {
-            if (per > 1) mine = attn_req(p, b);
-            const int64_t nt = tiles(mine), len = nt + EXTRA, places = segments(mine) * len;
-            auto tiles_before = [&](int64_t v) {   // tiles before place v of this request
-                const int64_t g = v / len, in = v - g * len;
-                return tiles0 + g * nt + max(in - EXTRA, (int64_t)0);
-            };
-            if (v0 >= at && v0 < at + places) {
-                sm.first[0] = b;
-                sm.first[1] = (v0 - at) / len;
-                sm.first[2] = (v0 - at) % len;
-                sm.tiles0 = tiles_before(v0 - at);
+        const int64_t per_head = places_in(head), places = per_head * p.kv_heads;
+        // place v of this request: its segment, the place within that, and the tiles before it
+        struct Found {
+            int64_t segment, in, tiles;
+            int nt;
+        };
+        auto find = [&](int64_t v) {
+            Found f;
+            const int64_t h = v / per_head;
+            f.in = v - h * per_head;
+            auto places_of = [&](int nt) { return part_tiles ? cut_parts(nt, part_tiles) : nt + EXTRA; };
+            int64_t rt = 0, passed = 0;
+            if (WIN && own_lists) {
+                for (;; ++rt) {
+                    f.nt = KeyTiles<RT, KT, WIN>().place(p, mine, (int)rt);
+                    if (f.in < places_of(f.nt)) break;
+                    f.in -= places_of(f.nt);
+                    passed += f.nt;
+                }
+            } else {
+                f.nt = tiles(mine);
+                rt = f.in / places_of(f.nt);
+                f.in -= rt * places_of(f.nt);
+                passed = rt * f.nt;
             }
-            if (v1 < total && v1 >= at && v1 < at + places) sm.end = tiles_before(v1 - at);
-            at += places;
-            tiles0 += segments(mine) * nt;
+            f.segment = h * row_tiles(mine) + rt;
+            f.tiles = tiles0 + h * head[1] + passed + max(f.in - EXTRA, (int64_t)0);
+            return f;
+        };
+        if (v0 >= at && v0 < at + places) {
+            const Found f = find(v0 - at);
+            sm.first[0] = b0 + i;
+            sm.first[1] = f.segment;
+            sm.first[2] = f.in;
+            if (part_tiles) {
+                const int len = cut_parts(f.nt, part_tiles), tpp = (f.nt + len - 1) / len;
+                sm.tiles0 = f.in * tpp;
+                sm.end = min((f.in + 1) * tpp, (int64_t)f.nt);
+            } else {
+                sm.tiles0 = f.tiles;
+            }
         }
-        if (v0 >= total && tid == 0) sm.tiles0 = all[1];
+        if (!part_tiles && v1 < total && v1 >= at && v1 < at + places) sm.end = find(v1 - at).tiles;
+        at += places;
+        tiles0 += head[1] * p.kv_heads;
     }
 }
 

@@ -67,13 +67,13 @@ template <int N>
 __device__ __forceinline__ void load_words(const unsigned char* from, uint32_t* w)
 {
     if constexpr (N == 4) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(from));
+        const uint4 v = load_early16(from);
         w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     } else if constexpr (N == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(from));
+        const uint2 v = load_early8(from);
         w[0] = v.x, w[1] = v.y;
     } else {
-        w[0] = __ldg(reinterpret_cast<const uint32_t*>(from));
+        w[0] = load_early4(from);
     }
 }
 
@@ -128,73 +128,75 @@ __global__ void __launch_bounds__(RowsCfg<NC, NT>::threads, RowsCfg<NC, NT>::cta
     ahead.h = (int)cut.first[1] / ahead.nrt;
     ahead.rt = (int)cut.first[1] - ahead.h * ahead.nrt;
     ahead.kt = part_tiles ? (int)cut.tiles0 : max((int)cut.first[2] - Cfg::extra, 0);
-    ahead.keys.place(p, ahead.r, ahead.rt, ahead.nkt);
+    ahead.place(p);
     if (tid == 0) s_seg = ahead;
     if (tid < Cfg::warps * RT) s_nan[tid / RT][tid % RT] = 0;
     __syncthreads();
     int64_t v_seg = v0 - cut.first[2];
 
     // ---- keys and values on their way ----
-    const int64_t block = kv4_block(p.page_size, NC);
     constexpr int kRecord = kv4_record(NC);
-    // this warp's record x of a tile, x = 0, 1 by lane parity: the page, or -1 (past the end, or not a page of this cache)
-    auto look_up = [&](const Cursor& c, int& in_page) {
-        const int pos = c.tile() * KT + warp * 16 + (lane & 1) * kKv4Tokens;
-        if (pos >= c.r.seq) return -1;
-        const int pg = p.page_div.div(pos), id = __ldg(p.block_table + (int64_t)c.b * p.table_stride + pg);
+    const int ps8 = p.page_size / kKv4Tokens;
+    // this warp's record x of a tile, x = 0, 1 by lane parity: a page number that is on its way, and where in the page
+    int id = -1, in_page = 0, head = 0;
+    auto look_up = [&](const Cursor& c) {
+        const int pos = c.tile() * KT + warp * 16 + (lane & 1) * kKv4Tokens, pg = p.page_div.div(pos);
+        id = pos < c.r.seq ? __ldg(p.block_table + (int64_t)c.b * p.table_stride + pg) : -1;
         in_page = pos - pg * p.page_size;
-        return (unsigned)id < (unsigned)p.num_pages ? id : -1;
-    };
-    const unsigned char* rec[2];   // keys' records of the tile under way (null: zeros); values `block` further
-    auto resolve = [&](int id, int in_page, int head) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int i = __shfl_sync(0xffffffffu, id, x), s = __shfl_sync(0xffffffffu, in_page, x);
-            rec[x] = i < 0 ? nullptr : p.packed + ((int64_t)i * p.kv_heads + head) * 2 * block + (s / kKv4Tokens) * kRecord;
-        }
+        head = c.h;
     };
     uint32_t kc[2][NC], ks[2][Cfg::wide ? NC / 4 : NC == 2 ? 1 : NC];         // keys: [record][word]
     uint32_t vc[2][2][VS][VW], vs[2][2][VS];                                  // values: [record][key t, t + 4][slice][word]
-    constexpr int KS = sizeof(ks[0]) / 4;
+    constexpr int KS = sizeof(ks[0]) / 4, W = NC / KS;
     const int kx = (g >> 1) + 4 * (g & 1);                                    // this lane's key of a record
+    // a lane's codes and scales within a record of keys, of values
+    const unsigned char* const k_codes = p.packed + Cfg::k_chunk(0, t) * kKv4Codes + kx * 16 + Cfg::k_word(0, t) * 4;
+    const unsigned char* const k_scales = p.packed + NC * kKv4Codes + Cfg::k_chunk(0, t) * kKv4Scales + kx * 4;
+    const int v_chunk = VW == 2 ? g >> 1 : g >> 2, v_word = VW == 2 ? 2 * (g & 1) : g & 3;   // of a slice
+    const unsigned char* const v_codes = p.packed + v_chunk * kKv4Codes + t * 16 + v_word * 4;
+    const unsigned char* const v_scales = p.packed + NC * kKv4Codes + v_chunk * kKv4Scales + t * 4;
+    // The records of a tile, by number; 0 where there is none (past the end, or not a page of this cache): what is read there becomes
+    // zeros before it is used.
+    int rec[2];
+    bool none[2] = {false, false}, none_next[2];
+    auto resolve = [&]() {
+        const int at = (unsigned)id < (unsigned)p.num_pages ? (id * p.kv_heads + head) * 2 * ps8 + in_page / kKv4Tokens : -1;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            rec[x] = __shfl_sync(0xffffffffu, at, x);
+            none_next[x] = rec[x] < 0;
+            rec[x] = max(rec[x], 0);
+        }
+    };
     auto load_keys = [&]() {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const unsigned char* at = rec[x];
-            if (at == nullptr) {
+            const unsigned char* codes = k_codes + (int64_t)rec[x] * kRecord;
+            const unsigned char* scales = k_scales + (int64_t)rec[x] * kRecord;
 #pragma unroll
-                for (int i = 0; i < NC; ++i) kc[x][i] = 0;
-#pragma unroll
-                for (int i = 0; i < KS; ++i) ks[x][i] = 0;
-                continue;
-            }
-            constexpr int W = Cfg::wide ? 4 : NC == 2 ? 2 : 1;
-#pragma unroll
-            for (int i = 0; i < NC; i += W) {
-                const int c = Cfg::k_chunk(i, t);
-                load_words<W>(at + c * kKv4Codes + kx * 16 + Cfg::k_word(i, t) * 4, kc[x] + i);
-                load_words<1>(at + NC * kKv4Codes + c * kKv4Scales + kx * 4, ks[x] + i / W);
+            for (int i = 0; i < NC; i += W) {   // (a lane's chunks: 4 apart, or neighbours, or one)
+                load_words<W>(codes + (W == 4 ? i : i / W) * kKv4Codes, kc[x] + i);
+                load_words<1>(scales + (W == 4 ? i : i / W) * kKv4Scales, ks[x] + i / W);
             }
         }
     };
     auto load_values = [&]() {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
+            const int at = none_next[x] ? 0 : rec[x] + ps8;
+            const unsigned char* codes = v_codes + (int64_t)at * kRecord;
+            const unsigned char* scales = v_scales + (int64_t)at * kRecord;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int s = 0; s < VS; ++s) {
-                    // word w of the slice's: chunk c, word of the chunk
-                    const int c = VW == 2 ? 4 * s + (g >> 1) : 2 * s + (g >> 2), w = VW == 2 ? 2 * (g & 1) : g & 3;
-                    if (rec[x] == nullptr || c >= NC) {
-#pragma unroll
-                        for (int i = 0; i < VW; ++i) vc[x][j][s][i] = 0;
-                        vs[x][j][s] = 0;
+                    constexpr int kChunks = 2 * VW;
+                    if ((NC % kChunks) && s == VS - 1 && v_chunk >= NC % kChunks) {   // (an odd number of chunks: half of the last slice)
+                        vc[x][j][s][0] = vs[x][j][s] = 0;
                         continue;
                     }
-                    const unsigned char* at = rec[x] + block;
-                    load_words<VW>(at + c * kKv4Codes + (t + 4 * j) * 16 + w * 4, vc[x][j][s]);
-                    load_words<1>(at + NC * kKv4Codes + c * kKv4Scales + (t + 4 * j) * 4, vs[x][j] + s);
+                    load_words<VW>(codes + s * kChunks * kKv4Codes + j * 64, vc[x][j][s]);
+                    load_words<1>(scales + s * kChunks * kKv4Scales + j * 16, vs[x][j] + s);
                 }
         }
     };
@@ -223,18 +225,15 @@ __global__ void __launch_bounds__(RowsCfg<NC, NT>::threads, RowsCfg<NC, NT>::cta
         }
     };
 
-    int id = 0, in_page = 0;
-    id = look_up(ahead, in_page);
-    resolve(id, in_page, ahead.h);
+    look_up(ahead);
+    resolve();
     load_keys();
     load_values();
-    int next_head = 0;
     auto look_ahead = [&](int tile) {   // tile: the one that `ahead` goes to
         id = -1;
         if (tile >= count) return;
         ahead.next(p);
-        id = look_up(ahead, in_page);
-        next_head = ahead.h;
+        look_up(ahead);
     };
     look_ahead(1);
     load_rows();
@@ -243,21 +242,32 @@ __global__ void __launch_bounds__(RowsCfg<NC, NT>::threads, RowsCfg<NC, NT>::cta
 
     const float f = p.flip ? -p.scale_log2 : p.scale_log2;
     int kt = s_seg.kt, nkt = s_seg.nkt, kt_first = kt;
-    int sinks, skip, ctx, edge;   // of the segment: its list of tiles, its context, where the windows of all rows have begun
+    int sinks, skip;            // of the segment: its list of tiles
+    MaskedKeys<true> mask;
     auto enter = [&]() {
         const Cursor& c = s_seg;
-        sinks = c.keys.sinks, skip = c.keys.skip, ctx = c.r.seq - c.r.n;
-        edge = window_edge(p, c.r, p.group_div.div(min(c.rt * RT + RT, c.r.n * p.group) - 1));
+        sinks = c.keys.sinks, skip = c.keys.skip;
+        mask = masked_keys<RT, true>(p, c);
     };
     enter();
     for (int it = 0; it < count; ++it) {
+        none[0] = none_next[0], none[1] = none_next[1];
+        if (__builtin_expect(none[0] || none[1], 0)) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                if (!none[x]) continue;
+#pragma unroll
+                for (int i = 0; i < KS; ++i) ks[x][i] = 0;
+#pragma unroll
+                for (int i = 0; i < 2 * VS; ++i) (&vs[x][0][0])[i] = 0;
+            }
+        }
         // ---- scores ----
         float s[NT][4];
 #pragma unroll
         for (int i = 0; i < NT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
 #pragma unroll
         for (int x = 0; x < NC; ++x) {
-            constexpr int W = Cfg::wide ? 4 : NC == 2 ? 2 : 1;
             const uint32_t sa = ks[0][x / W], sb = ks[1][x / W];
             const uint32_t sa2 = prmt(sa, sa, 0x1010), la2 = prmt(sa, sa, 0x3232), sb2 = prmt(sb, sb, 0x1010), lb2 = prmt(sb, sb, 0x3232);
             const uint32_t a0[4] = {kv4_pair<T, 0>(kc[0][x], sa2, la2), kv4_pair<T, 0>(kc[1][x], sb2, lb2),
@@ -272,7 +282,7 @@ __global__ void __launch_bounds__(RowsCfg<NC, NT>::threads, RowsCfg<NC, NT>::cta
             }
         }
         // ---- the next tile's keys ----
-        resolve(id, in_page, next_head);
+        resolve();
         load_keys();
         look_ahead(it + 2);
 
@@ -282,7 +292,7 @@ __global__ void __launch_bounds__(RowsCfg<NC, NT>::threads, RowsCfg<NC, NT>::cta
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[i][j] *= f;
-        if (__builtin_expect(pos0 + KT > ctx || (pos0 < edge && pos0 + KT > p.sinks), 0)) {   // rows differ in what they see
+        if (__builtin_expect(mask.template tile<KT>(p, pos0), 0)) {   // rows differ in what they see
             const AttnReq r = s_seg.r;
 #pragma unroll
             for (int i = 0; i < NT; ++i)

@@ -41,12 +41,17 @@
 #include <cudaTypedefs.h>
 
 #include "internal.h"
+#include "kv4.cuh"
 #include "tree_attn.cuh"
 
 namespace dsv41 {
 
-template <int DT, int MT, int REP, bool TMA>
+// where keys and values come from
+enum Source { kGather, kPages, kPacked };
+
+template <int DT, int MT, int REP, int SRC>
 struct TcCfg {
+    static constexpr bool TMA = SRC == kPages;
     static_assert(MT == 1 || REP == 1, "repeats are for a single tile of 128 rows");
     static_assert(MT == 1 || DT <= 128, "tensor memory holds one row tile of 256 columns");
     static constexpr int kt = DT == 256 ? 64 : 128;          // keys per tile (256 columns of O leave room for two S of 64)
@@ -57,7 +62,7 @@ struct TcCfg {
     static constexpr int group = 128 * split;                // softmax threads per 128 rows
     static constexpr int soft_warps = 4 * split * MT;
     // one warp's tensor copies of 16-token pages (16 a unit) take 1200 cycles to issue; two share them where there is room
-    static constexpr int prod_warps = TMA ? (MT == 2 ? 1 : 2) : 4, q_warps = TMA && MT == 2 ? 1 : 2;
+    static constexpr int prod_warps = TMA ? (MT == 2 ? 1 : 2) : SRC == kPacked && REP == 4 ? 8 : 4, q_warps = TMA && MT == 2 ? 1 : 2;
     static constexpr int w_prod = soft_warps, w_q = w_prod + prod_warps, w_s = w_q + q_warps, w_o = w_s + 1;
     static constexpr int threads = (w_o + 1) * 32;
     static constexpr int blocks = DT / 64;                   // blocks of 64 columns (128 bytes), swizzled
@@ -90,6 +95,18 @@ struct TcCfg {
     }
     __host__ __device__ static constexpr int o_col(int t) { return DT == 256 ? 256 : MT == 1 ? 384 : 256 + t * 128; }
 };
+
+// what a thread holds of a key or value in 4 bits: C chunks
+template <int C>
+struct CodePiece {
+    uint4 codes[C];
+    uint32_t scales[C];
+};
+
+__device__ __forceinline__ void st_shared16(uint32_t at, const uint4& v)
+{
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 
 // whether a phase is complete, without waiting for it
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity)
@@ -364,11 +381,64 @@ __device__ __noinline__ void settle_nonfinite(const TreeAttnParams& p, const Uni
     __syncwarp();
 }
 
-template <typename T, int DT, int MT, int REP, bool TMA, bool WIN>
-__global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn_tc_kernel(const __grid_constant__ TreeAttnParams p, const __grid_constant__ CUtensorMap tm_k,
+// The same for a cache in 4 bits, whose chunks stand for NaN in all columns or in none: in tiles that all rows see such a chunk reaches
+// them by itself, what was cleared of the others (tiles kt0 .. kt1 of the list) makes the chunk's columns NaN in the rows that see it.
+template <typename T, int RT, int KT, int OWN, bool WIN>
+__device__ __noinline__ void settle_packed(const TreeAttnParams& p, const UnitCursor<RT, KT, WIN>* cursor, int row, bool live, int kt0, int kt1, int col0,
+                                           int end, float4* part)
+{
+    const UnitCursor<RT, KT, WIN> c = *cursor;
+    const int lane = threadIdx.x & 31, nc = p.head_dim / kKv4Chunk;
+    const int at = c.rt * RT + row, i = p.group_div.div(at), g = at - i * p.group;
+    const MaskedKeys<WIN> mask = masked_keys<RT, WIN>(p, c);
+    uint32_t chunks = 0;
+#pragma unroll 1
+    for (int x = kt0; x <= kt1; ++x) {
+        const int pos0 = c.keys.tile(x) * KT;
+        if (!mask.template tile<KT>(p, pos0)) continue;
+#pragma unroll 1
+        for (int base = pos0; base < pos0 + KT; base += 32) {
+            const int pos = base + lane;
+            uint32_t nan = 0;
+            if (pos < c.r.seq) {
+                const int pg = p.page_div.div(pos), id = p.block_table[(int64_t)c.b * p.table_stride + pg], in_page = pos - pg * p.page_size;
+                if ((unsigned)id < (unsigned)p.num_pages) {
+                    const unsigned char* rec = p.packed + (((int64_t)id * p.kv_heads + c.h) * 2 + 1) * kv4_block(p.page_size, nc) +
+                                               (in_page / kKv4Tokens) * kv4_record(nc) + nc * kKv4Codes + (in_page % kKv4Tokens) * 4;
+                    for (int j = 0; j < nc; ++j) nan |= (uint32_t)kv4_nan<T>(*reinterpret_cast<const uint32_t*>(rec + j * kKv4Scales)) << j;
+                }
+            }
+            uint32_t hits = __ballot_sync(0xffffffffu, nan != 0);
+            while (hits) {
+                const int l = __ffs(hits) - 1;
+                hits &= hits - 1;
+                const uint32_t of = __shfl_sync(0xffffffffu, nan, l);
+                if (live && (seen_keys<WIN>(p, c.r, i, base + l) & 1)) chunks |= of;
+            }
+            __syncwarp();
+        }
+    }
+    T* out = static_cast<T*>(p.out) + (int64_t)(c.r.q0 + i) * p.out_stride_token + (int64_t)(c.h * p.group + g) * p.out_stride_head;
+#pragma unroll 1
+    for (int col = col0; live && col < min(end, p.head_dim); col += OWN < 32 ? 32 : 16) {
+        if (!((chunks >> (col / kKv4Chunk)) & 1)) continue;
+        for (int j = col; j < col + (OWN < 16 ? OWN : 16); ++j) {
+            if (part) reinterpret_cast<float*>(part + j / 4 * RT + row)[j & 3] = NAN;
+            else reinterpret_cast<uint16_t*>(out)[j] = (uint16_t)pack2<T>(NAN, NAN);
+        }
+    }
+    __syncwarp();
+}
+
+template <typename T, int DT, int MT, int REP, int SRC, bool WIN>
+__global__ void __launch_bounds__(TcCfg<DT, MT, REP, SRC>::threads, 1) tree_attn_tc_kernel(const __grid_constant__ TreeAttnParams p, const __grid_constant__ CUtensorMap tm_k,
                                                                                       const __grid_constant__ CUtensorMap tm_v)
 {
-    using Cfg = TcCfg<DT, MT, REP, TMA>;
+    using Cfg = TcCfg<DT, MT, REP, SRC>;
+    constexpr bool TMA = Cfg::TMA;
+    // without a tree mask, tiles of new tokens before all of the row tile's are ordinary ones (plain calls over a 16-bit cache
+    // mask every tile with new tokens)
+    constexpr bool kRowMasks = WIN || SRC == kPacked;
     constexpr int KT = Cfg::kt, RT = Cfg::rt, KW = Cfg::kw, NU = Cfg::units, LAG = Cfg::lag, CPR = DT / 8;
     using Cursor = UnitCursor<RT, KT, WIN>;
     extern __shared__ unsigned char smem_raw[];
@@ -427,6 +497,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         Cursor c;
         int64_t v_seg;   // place on the line where the segment begins
         int cleared;     // its tiles held infinities or NaN that not all rows see
+        MaskedKeys<WIN> mask;
     };
     __shared__ SegState s_seg[Cfg::soft_warps];
     int64_t run, v0;
@@ -452,12 +523,16 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
     cur.h = (int)cut.first[1] / cur.nrt;
     cur.rt = (int)cut.first[1] - cur.h * cur.nrt;
     cur.kt = part_tiles ? (int)cut.tiles0 : max((int)cut.first[2] - Cfg::extra, 0);
-    cur.keys.place(p, cur.r, cur.rt, cur.nkt);
+    cur.place(p);
     const int ksteps = (p.head_dim + 15) / 16;
     constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(128 >> 4) << 24);   // fp32 sums, M = 128
     auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, abort_flag, p.status); };
-    auto last_token = [&](const Cursor& c) { return p.group_div.div(min(c.rt * RT + RT, c.r.n * p.group) - 1); };   // of the row tile
+    // whether rows differ in what they see of the cursor's tile (new tokens, a window's edge)
+    auto masked = [&](const Cursor& c) {
+        if constexpr (kRowMasks) return masked_keys<RT, WIN>(p, c).template tile<KT>(p, c.tile() * KT);
+        else return c.kt * KT + KT > c.r.seq - c.r.n;
+    };
     // by a whole warp, which goes on converged (the tensor memory instructions need that)
     auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
         wait(bar, parity);
@@ -523,7 +598,116 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             while (!mbar_try_wait(&full[u % NU], (u / NU) & 1) && globaltimer_ns() - t0 < kWaitLimitNs) {}
         }
         __syncwarp();
-    } else if (!TMA && warp >= Cfg::w_prod && warp < Cfg::w_q) {
+    } else if (SRC == kPacked && warp >= Cfg::w_prod && warp < Cfg::w_q) {
+        if constexpr (SRC == kPacked) {
+        // ---------------------------------- producers, codes ----------------------------------
+        // A thread decodes the chunks of one key that are its group's: codes and scales of a tile's keys (values) are read into registers while
+        // the ones before are decoded. Eight neighbouring keys' 16-byte pieces fall into different banks by the swizzle.
+        constexpr int PT = Cfg::prod_warps * 32, G = PT / KT, C = DT / kKv4Chunk / G;   // groups of threads; chunks of each
+        static_assert(G >= 1 && C >= 1 && G * C * kKv4Chunk == DT, "chunks are dealt out evenly");
+        const int pt = tid - Cfg::w_prod * 32, key = pt % KT, c0 = pt / KT * C;
+        const int nc = p.head_dim / kKv4Chunk;
+        const int64_t block = kv4_block(p.page_size, nc);
+        const uint32_t scales_at = nc * kKv4Codes;
+        using Piece = CodePiece<C>;
+        // this thread's key of the cursor's tile: a page number that is on its way, and where in the page
+        struct Place {
+            int id, in_page, head;
+        };
+        auto place_of = [&](const Cursor& c) {
+            const int pos = c.tile() * KT + key, pg = p.page_div.div(pos);
+            Place a;
+            a.id = pos < c.r.seq ? __ldg(p.block_table + (int64_t)c.b * p.table_stride + pg) : -1;
+            a.in_page = pos - pg * p.page_size;
+            a.head = c.h;
+            return a;
+        };
+        // its keys' record; null: past the end, or not a page of this cache
+        auto record_of = [&](const Place& a) -> const unsigned char* {
+            return (unsigned)a.id < (unsigned)p.num_pages
+                       ? p.packed + ((int64_t)a.id * p.kv_heads + a.head) * 2 * block + (a.in_page / kKv4Tokens) * kv4_record(nc) + (key % kKv4Tokens) * 16
+                       : nullptr;
+        };
+        // (chunks past the head size repeat the last one: the products do not read their columns. No record: anything that can
+        // be read, its scales become zeros)
+        auto load = [&](Piece& u, const unsigned char* rec) {
+            const unsigned char* at = rec ? rec : p.packed;
+            const unsigned char* scales = at + (rec ? scales_at - (key % kKv4Tokens) * 12 : 0);
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const int c = min(c0 + i, nc - 1);
+                u.codes[i] = load_early16(at + c * kKv4Codes);
+                u.scales[i] = load_early4(scales + c * kKv4Scales);
+            }
+        };
+        auto put = [&](int n, Piece& u, bool live, bool check) {
+            const int slot = n % NU;
+            wait_warp(&empty[slot], ((n / NU) & 1) ^ 1);
+            unsigned char* row = su + slot * Cfg::unit_b + key * 128;
+            if (!live) {
+#pragma unroll
+                for (int i = 0; i < C; ++i) u.scales[i] = 0;
+            }
+            if (__builtin_expect(check, 0)) {
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+                    if (kv4_nan<T>(u.scales[i])) {   // not all rows see it: zeros (settle_packed)
+                        *reinterpret_cast<volatile int*>(dirty + slot) = n + 1;
+                        u.scales[i] = 0;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const int c = c0 + i;
+                const uint32_t sc = u.scales[i], s2 = prmt(sc, sc, 0x1010), lo2 = prmt(sc, sc, 0x3232);
+                const uint32_t w[4] = {u.codes[i].x, u.codes[i].y, u.codes[i].z, u.codes[i].w};
+                uint4 v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v[j] = make_uint4(kv4_pair<T, 0>(w[j], s2, lo2), kv4_pair<T, 1>(w[j], s2, lo2), kv4_pair<T, 2>(w[j], s2, lo2), kv4_pair<T, 3>(w[j], s2, lo2));
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    st_shared16(smem_addr(row) + (c >> 1) * Cfg::block_b + ((((c & 1) * 4 + j) ^ (key & 7)) << 4), v[j]);
+            }
+            fence_proxy_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[slot]);
+            __syncwarp();
+        };
+        // a tile's pages are looked up a tile ahead of its loads, those are a tile ahead of the decoding
+        Piece k, v;
+        const unsigned char* rec = record_of(place_of(cur));   // of tile `step`
+        const unsigned char* rec_v = nullptr;                  // of the tile before
+        bool mask = masked(cur), mask_v = false, mask_next = false;
+        Place next{-1, 0, 0};
+        auto look_ahead = [&](int tile) {
+            if (tile >= count) return;
+            cur.next(p);
+            next = place_of(cur);
+            mask_next = masked(cur);
+        };
+        load(k, rec);
+        look_ahead(1);
+        int n = 0;
+        for (int step = 0; step <= count; ++step) {
+            const unsigned char* rec_k = rec;
+            if (step < count) {
+                put(n++, k, rec != nullptr, false);
+                if (step + 1 < count) {
+                    rec_k = record_of(next);
+                    load(k, rec_k);
+                }
+            }
+            if (step > 0) put(n++, v, rec_v != nullptr, mask_v);
+            if (step < count) load(v, rec ? rec + block : nullptr);
+            rec_v = rec;
+            mask_v = mask;
+            rec = rec_k;
+            mask = mask_next;
+            look_ahead(step + 2);
+        }
+        }
+    } else if (SRC == kGather && warp >= Cfg::w_prod && warp < Cfg::w_q) {
         // ---------------------------------- producers ----------------------------------
         const int pt = tid - Cfg::w_prod * 32, chunk = pt % CPR, row0 = pt / CPR;
         constexpr int kRowStep = 128 / CPR;
@@ -600,7 +784,6 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             return id * p.stride_page + (pos - pg * p.page_size) * p.stride_slot + c.h * p.stride_head;
         };
         // offsets are looked up two tiles ahead (a length, then a table entry: two trips to L2 where a request begins)
-        auto masked = [&](const Cursor& c) { return masked_tile<KT, WIN>(p, c.r, last_token(c), c.tile() * KT); };
         int64_t off[2] = {offset_of(cur), -1};
         bool tail[2] = {masked(cur), false}, tail_before = false;
         auto look_ahead = [&](int tile) {
@@ -755,6 +938,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
         seg->c = cur;
         seg->v_seg = v0 - cut.first[2];
         seg->cleared = 0;
+        if (kRowMasks) seg->mask = masked_keys<RT, WIN>(p, cur);
         __syncwarp();
         int kt = cur.kt, nkt = cur.nkt, kt_first = kt;
         int rows = min(RT, cur.r.n * p.group - cur.rt * RT);
@@ -769,6 +953,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                 seg->c = c;
                 seg->v_seg += nkt + Cfg::extra;
                 seg->cleared = 0;
+                if (kRowMasks) seg->mask = masked_keys<RT, WIN>(p, c);
                 __syncwarp();
                 kt = kt_first = 0;
                 nkt = c.nkt;
@@ -784,7 +969,7 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
             if (first) m = -INFINITY, l = 0.0f;
             const int pos0 = WIN ? seg->c.keys.tile(kt) * KT : kt * KT;
             // rows differ in what they see of the tile (new tokens, a window's edge)
-            const bool tail = WIN ? masked_tile<KT, WIN>(p, seg->c.r, last_token(seg->c), pos0) : pos0 + KT > ctx;
+            const bool tail = kRowMasks ? seg->mask.template tile<KT>(p, pos0) : pos0 + KT > ctx;
             static_assert(KW <= 64, "one mask window per thread");
             uint64_t win = 0;
             // this row's new token
@@ -1008,8 +1193,11 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, TMA>::threads, 1) tree_attn
                 if (test != 0.0f) bad |= 1u << (col >> 5);
             }
             // (a sum of weights that is NaN makes the row NaN by itself)
-            const bool cleared = seg->cleared, odd = (bad != 0 || (cleared && row < rows)) && ll == ll;
-            if (__builtin_expect(__any_sync(0xffffffffu, odd), 0))
+            const bool cleared = seg->cleared, odd = ((SRC != kPacked && bad != 0) || (cleared && row < rows)) && ll == ll;
+            if (SRC == kPacked && __builtin_expect(cleared, 0))
+                settle_packed<T, RT, KT, Cfg::own, WIN>(p, &seg->c, min(row, rows - 1), odd, kt_first, kt, half * kCols + rep * Cfg::own,
+                                                        half * kCols + kCols, whole ? nullptr : part);
+            else if (SRC != kPacked && __builtin_expect(__any_sync(0xffffffffu, odd), 0))
                 settle_nonfinite<T, RT, KT, Cfg::own, WIN>(p, &seg->c, min(row, rows - 1), odd, bad, cleared, kt_first * KT, (kt + 1) * KT,
                                                       half * kCols + rep * Cfg::own, half * kCols + kCols, whole ? nullptr : part);
             const bool owner = half == 0 && rep == 0 && row < rows;   // one thread per row
@@ -1092,11 +1280,11 @@ static bool cache_map(CUtensorMap* m, const void* base, const TreeAttnParams& p,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DT, int MT, int REP, bool TMA, bool WIN>
+template <typename T, int DT, int MT, int REP, int SRC, bool WIN>
 static cudaError_t launch_tc(const TreeAttnParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st)
 {
-    using Cfg = TcCfg<DT, MT, REP, TMA>;
-    auto kernel = tree_attn_tc_kernel<T, DT, MT, REP, TMA, WIN>;
+    using Cfg = TcCfg<DT, MT, REP, SRC>;
+    auto kernel = tree_attn_tc_kernel<T, DT, MT, REP, SRC, WIN>;
     static bool ready[64] = {};   // the attribute is per device and kernel, and stays
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
@@ -1109,15 +1297,15 @@ static cudaError_t launch_tc(const TreeAttnParams& p, const CUtensorMap& tm_k, c
     return cudaGetLastError();
 }
 
-template <typename T, int DT, bool TMA, bool WIN>
+template <typename T, int DT, int SRC, bool WIN>
 static cudaError_t launch_tc_rows(const TreeAttnParams& p, const CUtensorMap& k, const CUtensorMap& v, int rows, cudaStream_t st)
 {
-    if (rows <= 32) return launch_tc<T, DT, 1, 4, TMA, WIN>(p, k, v, st);
-    if (rows <= 64) return launch_tc<T, DT, 1, 2, TMA, WIN>(p, k, v, st);
+    if (rows <= 32) return launch_tc<T, DT, 1, 4, SRC, WIN>(p, k, v, st);
+    if (rows <= 64) return launch_tc<T, DT, 1, 2, SRC, WIN>(p, k, v, st);
     if constexpr (DT <= 128) {
-        if (rows > 128) return launch_tc<T, DT, 2, 1, TMA, WIN>(p, k, v, st);
+        if (rows > 128) return launch_tc<T, DT, 2, 1, SRC, WIN>(p, k, v, st);
     }
-    return launch_tc<T, DT, 1, 1, TMA, WIN>(p, k, v, st);
+    return launch_tc<T, DT, 1, 1, SRC, WIN>(p, k, v, st);
 }
 
 template <typename T, int DT, bool WIN>
@@ -1126,7 +1314,7 @@ static cudaError_t launch_tc_dim(TreeAttnParams p, int max_rows, cudaStream_t st
     // Whole pages go by tensor copies where a tile is whole pages (or a page whole tiles) of at least a swizzle atom's
     // 8 rows; other page sizes are gathered key by key, and so are caches that repeat in memory (a view whose heads, slots
     // or pages are one: a map has no stride of 0).
-    constexpr int kt = TcCfg<DT, 1, 1, true>::kt;
+    constexpr int kt = TcCfg<DT, 1, 1, kPages>::kt;
     constexpr bool bf16 = !std::is_same<T, __half>::value;
     CUtensorMap k{}, v{};
     p.box = p.page_size < kt ? p.page_size : kt;
@@ -1135,7 +1323,7 @@ static cudaError_t launch_tc_dim(TreeAttnParams p, int max_rows, cudaStream_t st
                          (p.stride_page == 0 && p.num_pages > 1);
     const bool pages = p.num_pages > 0 && !repeats && p.box >= 8 && kt % p.box == 0 && p.page_size % p.box == 0 &&
                        cache_map(&k, p.k_cache, p, bf16) && cache_map(&v, p.v_cache, p, bf16);
-    return pages ? launch_tc_rows<T, DT, true, WIN>(p, k, v, max_rows, st) : launch_tc_rows<T, DT, false, WIN>(p, k, v, max_rows, st);
+    return pages ? launch_tc_rows<T, DT, kPages, WIN>(p, k, v, max_rows, st) : launch_tc_rows<T, DT, kGather, WIN>(p, k, v, max_rows, st);
 }
 
 template <typename T, bool WIN>
@@ -1144,6 +1332,16 @@ static cudaError_t launch_tree_attn_typed(const TreeAttnParams& p, int max_rows,
     if (p.head_dim <= 64) return launch_tc_dim<T, 64, WIN>(p, max_rows, st);
     if (p.head_dim <= 128) return launch_tc_dim<T, 128, WIN>(p, max_rows, st);
     return launch_tc_dim<T, 256, WIN>(p, max_rows, st);
+}
+
+// over a cache in 4 bits
+template <typename T, bool WIN>
+static cudaError_t launch_tree_attn4_typed(const TreeAttnParams& p, int max_rows, cudaStream_t st)
+{
+    const CUtensorMap none{};
+    if (p.head_dim <= 64) return launch_tc_rows<T, 64, kPacked, WIN>(p, none, none, max_rows, st);
+    if (p.head_dim <= 128) return launch_tc_rows<T, 128, kPacked, WIN>(p, none, none, max_rows, st);
+    return launch_tc_rows<T, 256, kPacked, WIN>(p, none, none, max_rows, st);
 }
 
 }  // namespace dsv41

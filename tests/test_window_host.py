@@ -30,19 +30,16 @@ def test_window_refusals():
 
 def key_tiles(seq, n, group, window, sinks, tree, RT, KT):
     """Tiles of each row tile, as KeyTiles lists them."""
-    ctx, total = seq - n, max(-(-seq // KT), 1)
-    ns = min(-(-min(sinks, seq) // KT), total)
-    if tree:
-        count = ns + total - max(max(ctx - window, 0) // KT, ns)
-    else:
-        span = min(window - 1 + min((RT - 2) // group + 2, n), seq)
-        count = min(ns + max(span + KT - 2, 0) // KT + 1, total)
-    lists = []
+    ctx, lists = seq - n, []
     for rt in range(-(-n * group // RT)):
-        before = 0 if tree else rt * RT // group + 1
-        skip = min(max(max(ctx + before - window, 0) // KT - ns, 0), total - count)
-        lists.append([x if x < ns else x + skip for x in range(count)])
-    return lists, total
+        before, last = 0, seq - 1
+        if not tree:
+            before, last = rt * RT // group + 1, ctx + (min(rt * RT + RT, n * group) - 1) // group
+        end, first = last // KT + 1, max(ctx + before - window, 0) // KT
+        ns = min(-(-min(sinks, seq) // KT), end)
+        skip = max(first - ns, 0)
+        lists.append([x if x < ns else x + skip for x in range(end - skip)])
+    return lists, max(-(-seq // KT), 1)
 
 
 def test_every_visible_key_is_in_the_list_once():
