@@ -30,7 +30,7 @@ __device__ __forceinline__ Kv4At kv4_at(const Kv4Params& p, int64_t slot, int he
     const int in_page = (int)(slot - page * p.page_size), t = in_page % kKv4Tokens;
     unsigned char* rec = p.data + ((page * p.kv_heads + head) * 2 + which) * kv4_block(p.page_size, p.chunks) +
                          (int64_t)(in_page / kKv4Tokens) * kv4_record(p.chunks);
-    return {rec + c * kKv4Codes + t * 16, rec + p.chunks * kKv4Codes + c * kKv4Scales + t * 4};
+    return {rec + c * kKv4Codes + kv4_place(c, t) * 16, rec + p.chunks * kKv4Codes + c * kKv4Scales + t * 4};
 }
 
 template <typename T>
@@ -120,8 +120,7 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_load_kernel(const Kv4Params p
         if (slot >= 0 && slot < slots) {
             const Kv4At at = kv4_at(p, slot, head, which, c);
             const uint32_t w = reinterpret_cast<const uint32_t*>(at.codes)[part], sc = *reinterpret_cast<const uint32_t*>(at.scales);
-            const uint32_t s2 = prmt(sc, sc, 0x1010), lo2 = prmt(sc, sc, 0x3232);
-            v = make_uint4(kv4_pair<T, 0>(w, s2, lo2), kv4_pair<T, 1>(w, s2, lo2), kv4_pair<T, 2>(w, s2, lo2), kv4_pair<T, 3>(w, s2, lo2));
+            v = kv4_word<T>(w, Scale2<T>(sc));
         }
         T* dst = static_cast<T*>(const_cast<void*>(which ? p.v : p.k)) + t * (which ? p.v_stride_token : p.k_stride_token) +
                  head * (which ? p.v_stride_head : p.k_stride_head) + c * kKv4Chunk + part * 8;

@@ -625,18 +625,18 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, SRC>::threads, 1) tree_attn
         // its keys' record; null: past the end, or not a page of this cache
         auto record_of = [&](const Place& a) -> const unsigned char* {
             return (unsigned)a.id < (unsigned)p.num_pages
-                       ? p.packed + ((int64_t)a.id * p.kv_heads + a.head) * 2 * block + (a.in_page / kKv4Tokens) * kv4_record(nc) + (key % kKv4Tokens) * 16
+                       ? p.packed + ((int64_t)a.id * p.kv_heads + a.head) * 2 * block + (a.in_page / kKv4Tokens) * kv4_record(nc)
                        : nullptr;
         };
         // (chunks past the head size repeat the last one: the products do not read their columns. No record: anything that can
         // be read, its scales become zeros)
         auto load = [&](Piece& u, const unsigned char* rec) {
             const unsigned char* at = rec ? rec : p.packed;
-            const unsigned char* scales = at + (rec ? scales_at - (key % kKv4Tokens) * 12 : 0);
+            const unsigned char* scales = at + scales_at + (key % kKv4Tokens) * 4;
 #pragma unroll
             for (int i = 0; i < C; ++i) {
                 const int c = min(c0 + i, nc - 1);
-                u.codes[i] = load_early16(at + c * kKv4Codes);
+                u.codes[i] = load_early16(at + c * kKv4Codes + kv4_place(c, key % kKv4Tokens) * 16);   // (pages are whole records)
                 u.scales[i] = load_early4(scales + c * kKv4Scales);
             }
         };
@@ -659,12 +659,11 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, SRC>::threads, 1) tree_attn
 #pragma unroll
             for (int i = 0; i < C; ++i) {
                 const int c = c0 + i;
-                const uint32_t sc = u.scales[i], s2 = prmt(sc, sc, 0x1010), lo2 = prmt(sc, sc, 0x3232);
+                const Scale2<T> sc(u.scales[i]);
                 const uint32_t w[4] = {u.codes[i].x, u.codes[i].y, u.codes[i].z, u.codes[i].w};
                 uint4 v[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    v[j] = make_uint4(kv4_pair<T, 0>(w[j], s2, lo2), kv4_pair<T, 1>(w[j], s2, lo2), kv4_pair<T, 2>(w[j], s2, lo2), kv4_pair<T, 3>(w[j], s2, lo2));
+                for (int j = 0; j < 4; ++j) v[j] = kv4_word<T>(w[j], sc);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     st_shared16(smem_addr(row) + (c >> 1) * Cfg::block_b + ((((c & 1) * 4 + j) ^ (key & 7)) << 4), v[j]);

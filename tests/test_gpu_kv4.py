@@ -29,13 +29,19 @@ def quantize(x):
     return code.to(torch.uint8), s, lo.to(x.dtype), value.flatten(-2)
 
 
+def places(chunks):
+    """Where token t of chunk c has its codes within the chunk's 8 places: [chunks, 8]."""
+    return torch.arange(8) ^ torch.tensor([0, 5, 2, 7]).repeat(2)[:chunks, None]
+
+
 def codes_of(cache, slots):
     """(codes [N, heads, 2, chunks, 32], scales [N, heads, 2, chunks, 2]) as they lie in the cache."""
     d, page = cache.data.cpu(), cache.page_size
     chunks = cache.head_dim // 32
     rec = d.view(cache.num_pages, cache.kv_heads, 2, page // 8, chunks * 160)
     words = rec[..., :chunks * 128].reshape(*rec.shape[:4], chunks, 8, 4, 4).to(torch.int64)      # [.., token, word, byte]
-    word = (words << torch.tensor([0, 8, 16, 24])).sum(-1)
+    word = (words << torch.tensor([0, 8, 16, 24])).sum(-1)                                         # [page, h, kv, group, chunk, place, word]
+    word = word.gather(5, places(chunks)[..., None].expand(*word.shape))
     column = torch.arange(8)
     shift = 4 * (column // 2) + 16 * (column % 2)
     code = ((word[..., None] >> shift) & 15).flatten(-2)                                           # [page, h, kv, group, chunk, token, 32]
@@ -293,13 +299,14 @@ def test_slots_past_the_end_may_hold_anything():
         x = torch.arange(c + n)
         used[table[b].long()[x // page] * page + x % page] = True
     chunks = 4
+    back = places(chunks).to(DEV)                           # place p holds token back[p] (the exchange is its own reverse)
     rec = s["cache"].data.view(-1, 2, 2, page // 8, chunks * 160)
     free = (~used).view(-1, page // 8, 8).to(DEV)
     for fill in (0xFF, 0x7C, 0x7F):
         codes = rec[..., :chunks * 128].unflatten(-1, (chunks, 8, 16))
         scales = rec[..., chunks * 128:].unflatten(-1, (chunks, 8, 4))
         at = free[:, None, None, :, None, :, None]
-        codes.copy_(torch.where(at, torch.full_like(codes, fill), codes))
+        codes.copy_(torch.where(free[:, :, back][:, None, None, :, :, :, None], torch.full_like(codes, fill), codes))
         scales.copy_(torch.where(at, torch.full_like(scales, fill), scales))
         assert torch.equal(attend4(s), want)
 
