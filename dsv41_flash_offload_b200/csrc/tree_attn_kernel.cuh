@@ -62,7 +62,7 @@ struct TcCfg {
     static constexpr int group = 128 * split;                // softmax threads per 128 rows
     static constexpr int soft_warps = 4 * split * MT;
     // one warp's tensor copies of 16-token pages (16 a unit) take 1200 cycles to issue; two share them where there is room
-    static constexpr int prod_warps = TMA ? (MT == 2 ? 1 : 2) : SRC == kPacked && REP == 4 ? 8 : 4, q_warps = TMA && MT == 2 ? 1 : 2;
+    static constexpr int prod_warps = TMA ? (MT == 2 ? 1 : 2) : SRC == kPacked && REP > 1 ? 8 : 4, q_warps = TMA && MT == 2 ? 1 : 2;
     static constexpr int w_prod = soft_warps, w_q = w_prod + prod_warps, w_s = w_q + q_warps, w_o = w_s + 1;
     static constexpr int threads = (w_o + 1) * 32;
     static constexpr int blocks = DT / 64;                   // blocks of 64 columns (128 bytes), swizzled
@@ -606,45 +606,59 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, SRC>::threads, 1) tree_attn
         constexpr int PT = Cfg::prod_warps * 32, G = PT / KT, C = DT / kKv4Chunk / G;   // groups of threads; chunks of each
         static_assert(G >= 1 && C >= 1 && G * C * kKv4Chunk == DT, "chunks are dealt out evenly");
         const int pt = tid - Cfg::w_prod * 32, key = pt % KT, c0 = pt / KT * C;
-        const int nc = p.head_dim / kKv4Chunk;
-        const int64_t block = kv4_block(p.page_size, nc);
-        const uint32_t scales_at = nc * kKv4Codes;
+        const int nc = p.head_dim / kKv4Chunk, ps8 = p.page_size / kKv4Tokens, record_b = kv4_record(nc);
         using Piece = CodePiece<C>;
-        // this thread's key of the cursor's tile: a page number that is on its way, and where in the page
-        struct Place {
-            int id, in_page, head;
+        // this thread's codes and scales within a record (chunks past the head size repeat the last one: the products do not
+        // read their columns), and its pieces of a row in shared memory
+        uint32_t codes_at[C], scales_at[C];
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int c = min(c0 + i, nc - 1);
+            codes_at[i] = c * kKv4Codes + kv4_place(c, key % kKv4Tokens) * 16;
+            scales_at[i] = nc * kKv4Codes + c * kKv4Scales + key % kKv4Tokens * 4;
+        }
+        const uint32_t row = smem_addr(su) + (c0 >> 1) * Cfg::block_b + key * 128 + ((((c0 & 1) * 4) ^ (key & 7)) << 4);
+        // (what every tile asks for, out of the parameters once)
+        const FastDiv page_div = p.page_div;
+        const int page_size = p.page_size, num_pages = p.num_pages, kv_heads = p.kv_heads;
+        const unsigned char* const packed = p.packed;
+        const int* pages = p.block_table + (int64_t)cur.b * p.table_stride;
+        // this thread's key of the cursor's tile: a page number that is on its way, and which record of the page
+        int id = -1, in_page = 0, head = 0;
+        MaskedKeys<WIN> masks = masked_keys<RT, WIN>(p, cur);
+        bool mask = false;
+        auto look_up = [&]() {
+            const int pos0 = cur.tile() * KT, pos = pos0 + key, pg = page_div.div(pos);
+            id = pos < cur.r.seq ? __ldg(pages + pg) : -1;
+            in_page = (pos - pg * page_size) / kKv4Tokens;
+            head = cur.h;
+            mask = masks.template tile<KT>(p, pos0);
         };
-        auto place_of = [&](const Cursor& c) {
-            const int pos = c.tile() * KT + key, pg = p.page_div.div(pos);
-            Place a;
-            a.id = pos < c.r.seq ? __ldg(p.block_table + (int64_t)c.b * p.table_stride + pg) : -1;
-            a.in_page = pos - pg * p.page_size;
-            a.head = c.h;
-            return a;
+        auto look_ahead = [&](int tile) {
+            if (tile >= count) return;
+            if (__builtin_expect(cur.kt + 1 < cur.nkt, 1)) {
+                ++cur.kt;
+            } else {
+                cur.next(p);
+                masks = masked_keys<RT, WIN>(p, cur);
+                pages = p.block_table + (int64_t)cur.b * p.table_stride;
+            }
+            look_up();
         };
-        // its keys' record; null: past the end, or not a page of this cache
-        auto record_of = [&](const Place& a) -> const unsigned char* {
-            return (unsigned)a.id < (unsigned)p.num_pages
-                       ? p.packed + ((int64_t)a.id * p.kv_heads + a.head) * 2 * block + (a.in_page / kKv4Tokens) * kv4_record(nc)
-                       : nullptr;
-        };
-        // (chunks past the head size repeat the last one: the products do not read their columns. No record: anything that can
-        // be read, its scales become zeros)
-        auto load = [&](Piece& u, const unsigned char* rec) {
-            const unsigned char* at = rec ? rec : p.packed;
-            const unsigned char* scales = at + scales_at + (key % kKv4Tokens) * 4;
+        // its keys' record by number; -1: past the end, or not a page of this cache (record 0 is read, its scales become zeros)
+        auto record = [&]() { return (unsigned)id < (unsigned)num_pages ? (id * kv_heads + head) * 2 * ps8 + in_page : -1; };
+        auto load = [&](Piece& u, int rec) {
+            const unsigned char* at = packed + (int64_t)max(rec, 0) * record_b;
 #pragma unroll
             for (int i = 0; i < C; ++i) {
-                const int c = min(c0 + i, nc - 1);
-                u.codes[i] = load_early16(at + c * kKv4Codes + kv4_place(c, key % kKv4Tokens) * 16);   // (pages are whole records)
-                u.scales[i] = load_early4(scales + c * kKv4Scales);
+                u.codes[i] = load_early16(at + codes_at[i]);
+                u.scales[i] = load_early4(at + scales_at[i]);
             }
         };
         auto put = [&](int n, Piece& u, bool live, bool check) {
             const int slot = n % NU;
             wait_warp(&empty[slot], ((n / NU) & 1) ^ 1);
-            unsigned char* row = su + slot * Cfg::unit_b + key * 128;
-            if (!live) {
+            if (__builtin_expect(!live, 0)) {
 #pragma unroll
                 for (int i = 0; i < C; ++i) u.scales[i] = 0;
             }
@@ -656,17 +670,14 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, SRC>::threads, 1) tree_attn
                         u.scales[i] = 0;
                     }
             }
+            const uint32_t to = row + slot * Cfg::unit_b;
 #pragma unroll
             for (int i = 0; i < C; ++i) {
-                const int c = c0 + i;
                 const Scale2<T> sc(u.scales[i]);
                 const uint32_t w[4] = {u.codes[i].x, u.codes[i].y, u.codes[i].z, u.codes[i].w};
-                uint4 v[4];
+                // (an even number of chunks a thread begins at an even one)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = kv4_word<T>(w[j], sc);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    st_shared16(smem_addr(row) + (c >> 1) * Cfg::block_b + ((((c & 1) * 4 + j) ^ (key & 7)) << 4), v[j]);
+                for (int j = 0; j < 4; ++j) st_shared16((to ^ (((i & 1) * 4 + j) << 4)) + (i >> 1) * Cfg::block_b, kv4_word<T>(w[j], sc));
             }
             fence_proxy_smem();
             __syncwarp();
@@ -675,34 +686,27 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, SRC>::threads, 1) tree_attn
         };
         // a tile's pages are looked up a tile ahead of its loads, those are a tile ahead of the decoding
         Piece k, v;
-        const unsigned char* rec = record_of(place_of(cur));   // of tile `step`
-        const unsigned char* rec_v = nullptr;                  // of the tile before
-        bool mask = masked(cur), mask_v = false, mask_next = false;
-        Place next{-1, 0, 0};
-        auto look_ahead = [&](int tile) {
-            if (tile >= count) return;
-            cur.next(p);
-            next = place_of(cur);
-            mask_next = masked(cur);
-        };
+        look_up();
+        int rec = record(), rec_v = -1;   // of tile `step`, and the one before
+        bool mask_k = mask, mask_v = false;
         load(k, rec);
         look_ahead(1);
         int n = 0;
         for (int step = 0; step <= count; ++step) {
-            const unsigned char* rec_k = rec;
+            int next = -1;
             if (step < count) {
-                put(n++, k, rec != nullptr, false);
+                put(n++, k, rec >= 0, false);
                 if (step + 1 < count) {
-                    rec_k = record_of(next);
-                    load(k, rec_k);
+                    next = record();
+                    load(k, next);
                 }
             }
-            if (step > 0) put(n++, v, rec_v != nullptr, mask_v);
-            if (step < count) load(v, rec ? rec + block : nullptr);
+            if (step > 0) put(n++, v, rec_v >= 0, mask_v);
+            if (step < count) load(v, rec < 0 ? -1 : rec + ps8);
             rec_v = rec;
-            mask_v = mask;
-            rec = rec_k;
-            mask = mask_next;
+            mask_v = mask_k;
+            rec = next;
+            mask_k = mask;
             look_ahead(step + 2);
         }
         }
