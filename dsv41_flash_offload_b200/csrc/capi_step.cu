@@ -219,6 +219,8 @@ static void kv4_cache(Kv4Params& p, const dsv41_kv4_cache* c)
     p.page_size = c->page_size;
     p.kv_heads = c->kv_heads;
     p.chunks = c->head_dim / kKv4Chunk;
+    p.page_div = FastDiv::make(c->page_size);
+    p.few_slots = (int64_t)c->num_pages * c->page_size <= 0x7fffffffll;
 }
 static int kv4_params(Kv4Params& p, const dsv41_kv4_cache* c, const dsv41_kv4_tokens* a)
 {

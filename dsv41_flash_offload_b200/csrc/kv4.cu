@@ -20,17 +20,34 @@ namespace dsv41 {
 
 constexpr int kKv4Threads = 256;
 
-// where chunk c of token slot lies: codes, and scales
+// where chunk c of a slot's key lies: codes, and scales (the value's: `values` bytes further)
 struct Kv4At {
     unsigned char *codes, *scales;
+    int64_t values;
 };
-__device__ __forceinline__ Kv4At kv4_at(const Kv4Params& p, int64_t slot, int head, int which, int c)
+__device__ __forceinline__ Kv4At kv4_at(const Kv4Params& p, int64_t slot, int head, int c)
 {
-    const int64_t page = slot / p.page_size;
-    const int in_page = (int)(slot - page * p.page_size), t = in_page % kKv4Tokens;
-    unsigned char* rec = p.data + ((page * p.kv_heads + head) * 2 + which) * kv4_block(p.page_size, p.chunks) +
-                         (int64_t)(in_page / kKv4Tokens) * kv4_record(p.chunks);
-    return {rec + c * kKv4Codes + kv4_place(c, t) * 16, rec + p.chunks * kKv4Codes + c * kKv4Scales + t * 4};
+    const int page = p.few_slots ? p.page_div.div((int)slot) : (int)(slot / p.page_size);
+    const int in_page = (int)(slot - (int64_t)page * p.page_size), t = in_page % kKv4Tokens, ps8 = p.page_size / kKv4Tokens;
+    const int record = (page * p.kv_heads + head) * 2 * ps8 + in_page / kKv4Tokens, bytes = kv4_record(p.chunks);   // (records are below 2^31)
+    unsigned char* at = p.data + (int64_t)record * bytes;
+    return {at + c * kKv4Codes + kv4_place(c, t) * 16, at + p.chunks * kKv4Codes + c * kKv4Scales + t * 4, (int64_t)ps8 * bytes};
+}
+
+// f(token, head, chunk, quarter of the chunk, in a token) for every quarter (8 columns) of the call's chunks. A CTA takes as many tokens
+// at a time as it has threads for; all its threads go round together, those without a token or a quarter with a token of -1.
+template <typename F>
+__device__ __forceinline__ void each_quarter(const Kv4Params& p, F f)
+{
+    const int per_token = p.kv_heads * p.chunks * 4, many = max(kKv4Threads / per_token, 1);
+    const int mine = per_token < kKv4Threads ? threadIdx.x / per_token : 0, first = threadIdx.x - mine * per_token;
+    for (int64_t t0 = (int64_t)blockIdx.x * many; t0 < p.num_tokens; t0 += (int64_t)gridDim.x * many) {
+        const int64_t t = mine < many && t0 + mine < p.num_tokens ? t0 + mine : -1;
+        for (int u0 = 0; u0 < per_token; u0 += kKv4Threads) {
+            const int u = u0 + first, hc = u >> 2, head = hc / p.chunks;
+            f(u < per_token ? t : -1, head, hc - head * p.chunks, u & 3);
+        }
+    }
 }
 
 template <typename T>
@@ -44,88 +61,110 @@ __device__ __forceinline__ float of_bits16(uint32_t v)
     return unpack2<T>(v).x;
 }
 
-// code of x in a chunk from lo with steps of s (not 0), inv about 1 / s
-__device__ __forceinline__ uint32_t kv4_code(float x, float lo, float s, float inv)
+// The word of 8 codes of x in a chunk from lo with steps of s (not 0). A quotient from the reciprocal is off by a few units of 2^-23:
+// where one comes near a half, all 8 are decided exactly.
+__device__ __noinline__ uint32_t kv4_word_exact(float4 a, float4 b, float lo, float s)
 {
-    const float d = x - lo, r = d * inv;
-    float n = rintf(r);
-    if (__builtin_expect(fabsf(r - n) > 0.4999f, 0)) {   // near a half (r is off by a few units of 2^-23): which side is the exact one on?
-        const float h = floorf(r) + 0.5f, low = d + lo, err = (x - low) + ((low - d) - lo);   // x - lo is d + err exactly
-        const float rest = fmaf(-h, s, d) + err;
-        n = rest > 0.0f ? h + 0.5f : rest < 0.0f ? h - 0.5f : rintf(h);
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    const float up = s < 1e-30f ? 0x1p64f : 1.0f;   // (1 / s would pass fp32)
+    lo *= up, s *= up;
+    const float inv = 1.0f / s;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = x[i] * up, d = v - lo, r = d * inv;
+        float n = rintf(r);
+        if (fabsf(r - n) > 0.4999f) {   // which side of the half is the exact quotient on?
+            const float h = floorf(r) + 0.5f, low = d + lo, err = (v - low) + ((low - d) - lo);   // v - lo is d + err exactly
+            const float rest = fmaf(-h, s, d) + err;
+            n = rest > 0.0f ? h + 0.5f : rest < 0.0f ? h - 0.5f : rintf(h);
+        }
+        word |= (uint32_t)fminf(fmaxf(n, 0.0f), 15.0f) << (4 * (i >> 1) + 16 * (i & 1));
     }
-    return (uint32_t)fminf(fmaxf(n, 0.0f), 15.0f);
+    return word;
+}
+__device__ __forceinline__ uint32_t kv4_word_of(const float* x, float lo, float s)
+{
+    constexpr float kRound = 12582912.0f;   // 1.5 * 2^23: a sum's low bits are the rounded number
+    const float inv = 1.0f / s;
+    float worst = s < 1e-30f ? 1.0f : 0.0f;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float r = fminf((x[i] - lo) * inv, 15.0f), t = r + kRound;
+        worst = fmaxf(worst, fabsf(r - (t - kRound)));
+        word |= (__float_as_uint(t) & 15u) << (4 * (i >> 1) + 16 * (i & 1));
+    }
+    return __builtin_expect(worst > 0.4999f, 0) ? kv4_word_exact(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), lo, s) : word;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kKv4Threads) kv4_store_kernel(const Kv4Params p)
 {
-    const int64_t per_token = (int64_t)p.kv_heads * 2 * p.chunks * 4, units = per_token * p.num_tokens, slots = (int64_t)p.num_pages * p.page_size;
-    const int64_t stride = (int64_t)gridDim.x * kKv4Threads;
-    // whole warps go round together: the four threads of a chunk exchange their extremes
-    for (int64_t u0 = (int64_t)blockIdx.x * kKv4Threads + (threadIdx.x & ~31); u0 < units; u0 += stride) {
-        const int64_t u = u0 + (threadIdx.x & 31);
-        const int part = (int)(u & 3);
-        const int64_t t = u / per_token;
-        const int rest = (int)(u - t * per_token) >> 2, c = rest % p.chunks, wh = rest / p.chunks, which = wh / p.kv_heads, head = wh - which * p.kv_heads;
-        const int64_t slot = u < units ? p.slots[t] : -1;
+    const int64_t slots = (int64_t)p.num_pages * p.page_size;
+    each_quarter(p, [&](int64_t t, int head, int c, int part) {
+        const int64_t slot = t >= 0 ? p.slots[t] : -1;
         const bool live = slot >= 0 && slot < slots;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (live)
-            raw = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(which ? p.v : p.k) + t * (which ? p.v_stride_token : p.k_stride_token) +
-                                                        head * (which ? p.v_stride_head : p.k_stride_head) + c * kKv4Chunk + part * 8));
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack2<T>(w[i]);
-            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};   // of keys, values
+        if (live) {
+            raw[0] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(p.k) + t * p.k_stride_token + head * p.k_stride_head + c * kKv4Chunk + part * 8));
+            raw[1] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(p.v) + t * p.v_stride_token + head * p.v_stride_head + c * kKv4Chunk + part * 8));
         }
-        float lo = x[0], hi = x[0], test = 0.0f;   // test: NaN if one is not finite
+        const Kv4At at = kv4_at(p, live ? slot : 0, head, c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]), test = fmaf(x[i], 0.0f, test);
+        for (int which = 0; which < 2; ++which) {
+            const uint32_t w[4] = {raw[which].x, raw[which].y, raw[which].z, raw[which].w};
+            float x[8];
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            test += __shfl_xor_sync(0xffffffffu, test, o);
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = unpack2<T>(w[i]);
+                x[2 * i] = f.x, x[2 * i + 1] = f.y;
+            }
+            float lo = x[0], hi = x[0], test = 0.0f;   // test: NaN if one is not finite
+#pragma unroll
+            for (int i = 0; i < 8; ++i) lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]), test = fmaf(x[i], 0.0f, test);
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                test += __shfl_xor_sync(0xffffffffu, test, o);
+            }
+            uint32_t sb = bits16<T>(__fdiv_rn(hi - lo, 15.0f));
+            float s = of_bits16<T>(sb);
+            const bool fine = test == 0.0f && fabsf(s) < INFINITY;
+            if (fine && (bits16<T>(fmaf(15.0f, s, lo)) & exp_bits<T>()) == exp_bits<T>()) s = of_bits16<T>(--sb);
+            uint32_t code = 0;
+            if (fine && s > 0.0f) code = kv4_word_of(x, lo, s);
+            if (!live) continue;
+            reinterpret_cast<uint32_t*>(at.codes + which * at.values)[part] = code;
+            if (part == 0) *reinterpret_cast<uint32_t*>(at.scales + which * at.values) = fine ? sb | bits16<T>(lo) << 16 : 0x7fff0000u;   // (0x7fff: NaN in both types)
         }
-        uint32_t sb = bits16<T>(__fdiv_rn(hi - lo, 15.0f));
-        float s = of_bits16<T>(sb);
-        const bool fine = test == 0.0f && fabsf(s) < INFINITY;
-        if (fine && (bits16<T>(fmaf(15.0f, s, lo)) & exp_bits<T>()) == exp_bits<T>()) s = of_bits16<T>(--sb);
-        uint32_t code = 0;
-        if (fine && s > 0.0f) {
-            const float up = s < 1e-30f ? 0x1p64f : 1.0f, inv = 1.0f / (s * up);   // (1 / s would pass fp32)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) code |= kv4_code(x[i] * up, lo * up, s * up, inv) << (4 * (i >> 1) + 16 * (i & 1));
-        }
-        if (!live) continue;
-        const Kv4At at = kv4_at(p, slot, head, which, c);
-        reinterpret_cast<uint32_t*>(at.codes)[part] = code;
-        if (part == 0) *reinterpret_cast<uint32_t*>(at.scales) = fine ? sb | bits16<T>(lo) << 16 : 0x7fff0000u;   // (0x7fff: NaN in both types)
-    }
+    });
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kKv4Threads) kv4_load_kernel(const Kv4Params p)
 {
-    const int64_t per_token = (int64_t)p.kv_heads * 2 * p.chunks * 4, units = per_token * p.num_tokens, slots = (int64_t)p.num_pages * p.page_size;
-    for (int64_t u = (int64_t)blockIdx.x * kKv4Threads + threadIdx.x; u < units; u += (int64_t)gridDim.x * kKv4Threads) {
-        const int part = (int)(u & 3);
-        const int64_t t = u / per_token;
-        const int rest = (int)(u - t * per_token) >> 2, c = rest % p.chunks, wh = rest / p.chunks, which = wh / p.kv_heads, head = wh - which * p.kv_heads;
+    const int64_t slots = (int64_t)p.num_pages * p.page_size;
+    each_quarter(p, [&](int64_t t, int head, int c, int part) {
+        if (t < 0) return;
         const int64_t slot = p.slots[t];
-        uint4 v = make_uint4(0, 0, 0, 0);
+        uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if (slot >= 0 && slot < slots) {
-            const Kv4At at = kv4_at(p, slot, head, which, c);
-            const uint32_t w = reinterpret_cast<const uint32_t*>(at.codes)[part], sc = *reinterpret_cast<const uint32_t*>(at.scales);
-            v = kv4_word<T>(w, Scale2<T>(sc));
+            const Kv4At at = kv4_at(p, slot, head, c);
+            uint32_t w[2], sc[2];
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                w[which] = reinterpret_cast<const uint32_t*>(at.codes + which * at.values)[part];
+                sc[which] = *reinterpret_cast<const uint32_t*>(at.scales + which * at.values);
+            }
+#pragma unroll
+            for (int which = 0; which < 2; ++which) v[which] = kv4_word<T>(w[which], Scale2<T>(sc[which]));
         }
-        T* dst = static_cast<T*>(const_cast<void*>(which ? p.v : p.k)) + t * (which ? p.v_stride_token : p.k_stride_token) +
-                 head * (which ? p.v_stride_head : p.k_stride_head) + c * kKv4Chunk + part * 8;
-        *reinterpret_cast<uint4*>(dst) = v;
-    }
+        T *k = static_cast<T*>(const_cast<void*>(p.k)), *val = static_cast<T*>(const_cast<void*>(p.v));
+        *reinterpret_cast<uint4*>(k + t * p.k_stride_token + head * p.k_stride_head + c * kKv4Chunk + part * 8) = v[0];
+        *reinterpret_cast<uint4*>(val + t * p.v_stride_token + head * p.v_stride_head + c * kKv4Chunk + part * 8) = v[1];
+    });
 }
 
 // out: from the cache to `moved` ([token][head, keys or values][chunk] codes, then scales), or back
@@ -140,7 +179,8 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_move_kernel(const Kv4Params p
         const int64_t t = u / per_token, slot = p.slots[t], far = other[t];
         if (slot < 0 || slot >= slots || far < 0 || far >= slots) continue;   // both or neither
         const int rest = (int)(u - t * per_token), c = rest % p.chunks, wh = rest / p.chunks, which = wh / p.kv_heads, head = wh - which * p.kv_heads;
-        const Kv4At at = kv4_at(p, slot, head, which, c);
+        Kv4At at = kv4_at(p, slot, head, c);
+        at.codes += which * at.values, at.scales += which * at.values;
         if (OUT) {
             codes[u] = *reinterpret_cast<const uint4*>(at.codes);
             scales[u] = *reinterpret_cast<const uint32_t*>(at.scales);
@@ -156,20 +196,24 @@ static int kv4_grid(int64_t units)
     const int64_t ctas = (units + kKv4Threads - 1) / kKv4Threads, cap = 16 * (int64_t)num_sms();
     return (int)(ctas > cap ? cap : ctas);
 }
+static int quarters_grid(const Kv4Params& p)
+{
+    const int per_token = p.kv_heads * p.chunks * 4, many = per_token < kKv4Threads ? kKv4Threads / per_token : 1;
+    const int64_t ctas = ((int64_t)p.num_tokens + many - 1) / many, cap = 16 * (int64_t)num_sms();
+    return (int)(ctas > cap ? cap : ctas);
+}
 
 cudaError_t launch_kv4_store(const Kv4Params& p, int dtype, cudaStream_t st)
 {
-    const int grid = kv4_grid((int64_t)p.num_tokens * p.kv_heads * 2 * p.chunks * 4);
-    if (dtype == 0) kv4_store_kernel<__half><<<grid, kKv4Threads, 0, st>>>(p);
-    else kv4_store_kernel<__nv_bfloat16><<<grid, kKv4Threads, 0, st>>>(p);
+    if (dtype == 0) kv4_store_kernel<__half><<<quarters_grid(p), kKv4Threads, 0, st>>>(p);
+    else kv4_store_kernel<__nv_bfloat16><<<quarters_grid(p), kKv4Threads, 0, st>>>(p);
     return cudaGetLastError();
 }
 
 cudaError_t launch_kv4_load(const Kv4Params& p, int dtype, cudaStream_t st)
 {
-    const int grid = kv4_grid((int64_t)p.num_tokens * p.kv_heads * 2 * p.chunks * 4);
-    if (dtype == 0) kv4_load_kernel<__half><<<grid, kKv4Threads, 0, st>>>(p);
-    else kv4_load_kernel<__nv_bfloat16><<<grid, kKv4Threads, 0, st>>>(p);
+    if (dtype == 0) kv4_load_kernel<__half><<<quarters_grid(p), kKv4Threads, 0, st>>>(p);
+    else kv4_load_kernel<__nv_bfloat16><<<quarters_grid(p), kKv4Threads, 0, st>>>(p);
     return cudaGetLastError();
 }
 

@@ -28,15 +28,43 @@ namespace dsv41 {
 
 constexpr int kLpThreads = 512;
 constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kPlainCtas = 3;    // CTAs on an SM where no alternatives are asked for
 constexpr int kLpRoom = 6144;    // keys of the list of candidates
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLpNone = -140.0f;   // e^-140 is 0 in fp32 (results under 2^-126 are)
 
-__device__ __forceinline__ float lp_exp(float x)
+__device__ __forceinline__ float lp_exp2(float x)
 {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * kLog2e));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float lp_exp(float x) { return lp_exp2(x * kLog2e); }
+// pairs of fp32 in one instruction
+__device__ __forceinline__ uint64_t pair2(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
 __device__ __forceinline__ float max_nan(float a, float b)   // NaN if one is
 {
@@ -48,7 +76,24 @@ __device__ __forceinline__ float max_nan(float a, float b)   // NaN if one is
 template <typename T>
 struct LpVec {
     static constexpr int n = 16 / sizeof(T);
+    static constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;   // -inf
     float v[n];
+    // the largest element (NaN counts for nothing)
+    __device__ __forceinline__ static float largest(const uint4& u)
+    {
+        if constexpr (sizeof(T) == 4) {
+            return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const __half2* h = reinterpret_cast<const __half2*>(&u);
+            const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+            return fmaxf(f.x, f.y);
+        } else {
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+            const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+            return fmaxf(f.x, f.y);
+        }
+    }
+    __device__ __forceinline__ static uint4 none() { return make_uint4(kNone, kNone, kNone, kNone); }
     __device__ __forceinline__ void unpack(const uint4& u)
     {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -72,19 +117,18 @@ template <typename T>
 struct LpRow {
     static constexpr int n = LpVec<T>::n;
     const T* x;        // element 0
-    int head, vocab, vectors;
+    int head, vocab, vectors, whole0, whole1;   // (vectors whole0 .. whole1 - 1 are)
     __device__ __forceinline__ LpRow(const void* logits, int64_t at, int vocab_) : x(static_cast<const T*>(logits) + at), vocab(vocab_)
     {
         head = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
         vectors = (int)(((int64_t)vocab + head + n - 1) / n);
+        whole0 = head > 0, whole1 = (int)(((int64_t)vocab + head) / n);
     }
-    __device__ __forceinline__ bool whole(int i) const { return (i > 0 || head == 0) && (int64_t)(i + 1) * n <= (int64_t)vocab + head; }
     __device__ __forceinline__ const uint4* at(int i) const { return reinterpret_cast<const uint4*>(x - head + (int64_t)i * n); }
     __device__ __forceinline__ int first(int i) const { return i * n - head; }   // element of the vector's first place (may be outside)
     __device__ __noinline__ uint4 partial(int i) const
     {
-        constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-        uint32_t w[4] = {none, none, none, none};
+        uint32_t w[4] = {LpVec<T>::kNone, LpVec<T>::kNone, LpVec<T>::kNone, LpVec<T>::kNone};
         for (int j = 0; j < n; ++j) {
             const int64_t e = (int64_t)i * n - head + j;
             if (e < 0 || e >= vocab) continue;
@@ -97,7 +141,7 @@ struct LpRow {
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
-    __device__ __forceinline__ uint4 load(int i) const { return whole(i) ? __ldg(at(i)) : partial(i); }
+    __device__ __forceinline__ uint4 load(int i) const { return __builtin_expect(i >= whole0 && i < whole1, 1) ? __ldg(at(i)) : partial(i); }
 };
 
 // orders tokens by logit, then by the lowest index; 0: none (a logit of -inf)
@@ -175,7 +219,7 @@ __device__ __forceinline__ void lp_join(float& m, float& l, float& e, float m2, 
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LogprobParams p)
+__global__ void __launch_bounds__(kLpThreads, TOP ? 2 : kPlainCtas) logprobs_kernel(const LogprobParams p)
 {
     using Row = LpRow<T>;
     constexpr int n = Row::n, kBatch = 4;
@@ -188,39 +232,46 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LogprobPa
     const int step = kLpThreads * ranks, i0 = rank * kLpThreads + tid;   // this thread's vectors: i0, i0 + step, ...
 
     // ---- sums ----
-    float m = -INFINITY, l = 0.0f, e = 0.0f;   // m: the largest logit so far
+    float m = -INFINITY;                       // the largest logit so far
+    uint64_t l2 = 0, e2 = 0;                   // sums, as pairs
     int at = -1;                               // first vector of the batch that it came with
-    for (int64_t i = i0; i < row.vectors; i += (int64_t)kBatch * step) {
+    for (int i = i0; i < row.vectors; i += kBatch * step) {   // (a row has less than 2^30 vectors, kBatch * step is 2^14 at most)
         uint4 u[kBatch];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            const int64_t v = i + (int64_t)b * step;
-            constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-            u[b] = v < row.vectors ? row.load((int)v) : make_uint4(none, none, none, none);
+            const int v = i + b * step;
+            u[b] = v < row.vectors ? row.load(v) : LpVec<T>::none();
         }
-        LpVec<T> x[kBatch];
         float top = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            x[b].unpack(u[b]);
-#pragma unroll
-            for (int j = 0; j < n; ++j) top = fmaxf(top, x[b].v[j]);
-        }
-        if (top > m) at = (int)i;
+        for (int b = 0; b < kBatch; ++b) top = fmaxf(top, LpVec<T>::largest(u[b]));
+        if (top > m) at = i;
         const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now;
         const float d = max_nan(m - base, kLpNone), keep = lp_exp(d);
-        e = fmaf(l, d, e) * keep;
-        l *= keep;
+        e2 = mul2(fma2(l2, pair2(d, d), e2), pair2(keep, keep));
+        l2 = mul2(l2, pair2(keep, keep));
         m = now;
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b)
+        for (int b = 0; b < kBatch; ++b) {
+            LpVec<T> x;
+            x.unpack(u[b]);
 #pragma unroll
-            for (int j = 0; j < n; ++j) {
-                const float z = max_nan(x[b].v[j] - base, kLpNone), w = lp_exp(z);
-                l += w;
-                e = fmaf(w, z, e);
+            for (int j = 0; j < n; j += 2) {
+                float z0, z1;
+                split2(add2(pair2(x.v[j], x.v[j + 1]), pair2(-base, -base)), z0, z1);
+                const uint64_t z = pair2(max_nan(z0, kLpNone), max_nan(z1, kLpNone));
+                split2(mul2(z, pair2(kLog2e, kLog2e)), z0, z1);
+                const uint64_t w = pair2(lp_exp2(z0), lp_exp2(z1));
+                l2 = add2(l2, w);
+                e2 = fma2(w, z, e2);
             }
+        }
     }
+    float l, e, other;
+    split2(l2, l, other);
+    l += other;
+    split2(e2, e, other);
+    e += other;
     float jm = m, jl = l, je = e;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
@@ -232,15 +283,19 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LogprobPa
     if (TOP) {
         uint64_t mine = 0;   // the largest key of this thread's elements
         if (at >= 0) {
-#pragma unroll 1
-            for (int b = 0; b < kBatch && mine == 0; ++b) {
-                const int64_t i = (int64_t)at + (int64_t)b * step;
-                if (i >= row.vectors) break;
+            uint4 u[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int i = at + b * step;
+                u[b] = i < row.vectors ? row.load(i) : LpVec<T>::none();
+            }
+#pragma unroll
+            for (int b = kBatch - 1; b >= 0; --b) {   // (the first one that has it is the last to be set)
                 LpVec<T> x;
-                x.unpack(row.load((int)i));
+                x.unpack(u[b]);
 #pragma unroll
                 for (int j = n - 1; j >= 0; --j)
-                    if (x.v[j] == m) mine = lp_key(m, row.first((int)i) + j);
+                    if (x.v[j] == m) mine = lp_key(m, row.first(at + b * step) + j);
             }
         }
         keys[tid] = mine;
@@ -250,27 +305,37 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LogprobPa
         if (mine >= least && mine > 0) s.hot[atomicAdd(&s.hots, 1)] = tid;
         __syncthreads();
         const int per = (row.vectors + step - 1) / step, work = s.hots * per;
-        for (int w0 = 0; w0 < work; w0 += kLpThreads) {
-            const int have = s.count;
-            __syncthreads();   // (all have read it before any adds to it)
-            if (have > kLpRoom - kLpThreads * n - 32) {   // no room for what this round may find
-                lp_select(s, keys, have);
-                if (warp == 0) keys[lane] = s.best[0][lane];
-                if (tid == 0) s.count = 32;
-                __syncthreads();
+        auto vector_of = [&](int w) { return w < work ? rank * kLpThreads + s.hot[w / per] + w % per * step : row.vectors; };
+        constexpr int kRounds = 4;   // whose vectors are read together
+        for (int w0 = 0; w0 < work; w0 += kRounds * kLpThreads) {
+            uint4 u[kRounds];
+            int first[kRounds];
+#pragma unroll
+            for (int q = 0; q < kRounds; ++q) {
+                const int i = vector_of(w0 + q * kLpThreads + tid);
+                u[q] = i < row.vectors ? row.load(i) : LpVec<T>::none();
+                first[q] = row.first(i);
             }
-            const int w = w0 + tid;
-            const int64_t i = w < work ? (int64_t)rank * kLpThreads + s.hot[w / per] + (int64_t)(w % per) * step : row.vectors;
-            if (i < row.vectors) {
+#pragma unroll
+            for (int q = 0; q < kRounds; ++q) {
+                if (w0 + q * kLpThreads >= work) break;
+                const int have = s.count;
+                __syncthreads();   // (all have read it before any adds to it)
+                if (have > kLpRoom - kLpThreads * n - 32) {   // no room for what this round may find
+                    lp_select(s, keys, have);
+                    if (warp == 0) keys[lane] = s.best[0][lane];
+                    if (tid == 0) s.count = 32;
+                    __syncthreads();
+                }
                 LpVec<T> x;
-                x.unpack(row.load((int)i));
+                x.unpack(u[q]);
 #pragma unroll
                 for (int j = 0; j < n; ++j) {
-                    const uint64_t k = lp_key(x.v[j], row.first((int)i) + j);
+                    const uint64_t k = lp_key(x.v[j], first[q] + j);
                     if (k >= least && k > 0) keys[atomicAdd(&s.count, 1)] = k;
                 }
+                __syncthreads();
             }
-            __syncthreads();
         }
         lp_select(s, keys, s.count);
     }
@@ -335,9 +400,10 @@ static cudaError_t launch_lp(const LogprobParams& p, cudaStream_t st)
         if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return err;
         if (dev < 64) ready[dev] = true;
     }
-    // two CTAs fit on an SM: few rows are shared by up to 8 CTAs, of at least 4096 logits each
+    // Few rows are shared by up to 8 CTAs each, of at least 4096 logits, as long as every CTA has an SM of its own. (Up to two on each: 100
+    // rows of 32768 with 20 alternatives 32 us for 21, on five 56: what a CTA does beside its sums does not shrink.)
     int ranks = 1;
-    while (ranks < 8 && (int64_t)p.rows * ranks < 2 * num_sms() && p.vocab / (2 * ranks) >= 4096) ranks *= 2;
+    while (ranks < 8 && (int64_t)p.rows * ranks * 2 <= 2 * num_sms() && p.vocab / (2 * ranks) >= 4096) ranks *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.rows * ranks));
     cfg.blockDim = dim3(kLpThreads);

@@ -89,6 +89,8 @@ struct Kv4Params {
     const int64_t* slots;
     unsigned char* moved;                              // move: room for the tokens' codes and scales
     int num_tokens, kv_heads, chunks, num_pages, page_size;
+    FastDiv page_div;
+    int few_slots;                                     // slots fit page_div
 };
 
 struct AttnWorkspace {   // the status word lies at 0
