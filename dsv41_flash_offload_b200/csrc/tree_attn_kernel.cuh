@@ -2,7 +2,8 @@
 // mathematics, the rows and the cut of the work into runs).
 //
 // One CTA per SM walks its run of (request, KV head, row tile, key tile) units:
-//   producers            key and value tiles (128 keys; 64 for head sizes over 128) into a ring of units, in the
+//   producers            (over a cache in 4 bits: four or eight warps that decode codes into the same tiles)
+//                        key and value tiles (128 keys; 64 for head sizes over 128) into a ring of units, in the
 //                        128-byte swizzle the tensor cores read. Whole pages go by tensor copies (one or two warps, a lane
 //                        per page and 64 columns); page sizes that do not make up a tile are gathered key by key by four
 //                        warps of cp.async, whose issue rate then bounds a call (16 tokens x 8 rows over 4 x 64-128k keys:
@@ -75,11 +76,13 @@ struct TcCfg {
     // what a segment costs beside its tiles (rows' loads, its end), in tiles. 2, 3, 5: 32 x 64 tokens of 4 rows over
     // 1-8k keys 237, 228, 224 us (before the join's last step); 16 x 5-13 tokens over 0.1-4k keys 50, 50, 54 us; long lengths within 1%
     static constexpr int extra = 3;
-    static constexpr int off_b = 4 * kt * 8;                 // byte offsets of the keys of four tiles
+    static constexpr int off_b = SRC == kPacked ? 0 : 4 * kt * 8;   // byte offsets of the keys of four tiles
+    static constexpr int raw_unit_b = kt * DT / kKv4Chunk * 20, raw_units = DT == 256 ? 1 : 2,
+                         raw_b = SRC == kPacked ? raw_units * raw_unit_b : 0;   // codes and scales of a tile's keys, values (of either: 256 columns)
     static constexpr int ml_b = MT * 2 * 128 * 8;
     static constexpr int mx_b = MT * 4 * 128 * 4;            // tile maxima of the threads that share a row
     static constexpr int bars_b = 1024;
-    static constexpr int fixed_b = 1024 + q_b + stage_b + off_b + ml_b + mx_b + bars_b;
+    static constexpr int fixed_b = 1024 + q_b + stage_b + off_b + raw_b + ml_b + mx_b + bars_b;
     static constexpr int units_fit = (232448 - fixed_b) / unit_b;
     static constexpr int units = units_fit < 10 ? units_fit : 10;
     static constexpr int lag = units - 2;                    // cp.async: units in flight when the next is issued
@@ -96,16 +99,27 @@ struct TcCfg {
     __host__ __device__ static constexpr int o_col(int t) { return DT == 256 ? 256 : MT == 1 ? 384 : 256 + t * 128; }
 };
 
-// what a thread holds of a key or value in 4 bits: C chunks
-template <int C>
-struct CodePiece {
-    uint4 codes[C];
-    uint32_t scales[C];
-};
-
 __device__ __forceinline__ void st_shared16(uint32_t at, const uint4& v)
 {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+__device__ __forceinline__ uint4 ld_shared16(uint32_t at)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_shared4(uint32_t at)
+{
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool live)
+{
+    const int n = live ? 4 : 0;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
 // whether a phase is complete, without waiting for it
@@ -447,7 +461,8 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, SRC>::threads, 1) tree_attn
     unsigned char* su = sq + Cfg::q_b;
     float* stage = reinterpret_cast<float*>(su + NU * Cfg::unit_b);
     int64_t* key_off = reinterpret_cast<int64_t*>(reinterpret_cast<unsigned char*>(stage) + Cfg::stage_b);
-    float2* ml = reinterpret_cast<float2*>(key_off + 4 * KT);
+    unsigned char* raw = reinterpret_cast<unsigned char*>(stage) + Cfg::stage_b + Cfg::off_b;
+    float2* ml = reinterpret_cast<float2*>(raw + Cfg::raw_b);
     float* mx = reinterpret_cast<float*>(ml + MT * 2 * 128);
     uint64_t* bars = reinterpret_cast<uint64_t*>(mx + MT * 4 * 128);
     uint64_t* full = bars;                 // [NU] a unit's copies have landed (4 producer warps)
@@ -601,36 +616,28 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, SRC>::threads, 1) tree_attn
     } else if (SRC == kPacked && warp >= Cfg::w_prod && warp < Cfg::w_q) {
         if constexpr (SRC == kPacked) {
         // ---------------------------------- producers, codes ----------------------------------
-        // A thread decodes the chunks of one key that are its group's: codes and scales of a tile's keys (values) are read into registers while
-        // the ones before are decoded. Eight neighbouring keys' 16-byte pieces fall into different banks by the swizzle.
+        // A thread decodes the chunks of one key that are its group's. Their codes and scales go to places of its own in shared memory
+        // (cp.async) a tile ahead, keys and values in turn. (In registers they were read as early, but two tiles' pieces left
+        // too few of them where 256 rows share a CTA, and decoding them had to be written out for every chunk, twice: code
+        // that the instruction cache did not hold: 32 x 64 tokens of 4 rows over 1-8k keys 328 us for 242, 16 small trees over
+        // 0.1-16k keys 137 us for 127.)
+        // Eight neighbouring keys' 16-byte pieces fall into different banks by the swizzle.
         constexpr int PT = Cfg::prod_warps * 32, G = PT / KT, C = DT / kKv4Chunk / G;   // groups of threads; chunks of each
         static_assert(G >= 1 && C >= 1 && G * C * kKv4Chunk == DT, "chunks are dealt out evenly");
         const int pt = tid - Cfg::w_prod * 32, key = pt % KT, c0 = pt / KT * C;
         const int nc = p.head_dim / kKv4Chunk, ps8 = p.page_size / kKv4Tokens, record_b = kv4_record(nc);
-        using Piece = CodePiece<C>;
-        // this thread's codes and scales within a record (chunks past the head size repeat the last one: the products do not
-        // read their columns), and its pieces of a row in shared memory
-        uint32_t codes_at[C], scales_at[C];
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = min(c0 + i, nc - 1);
-            codes_at[i] = c * kKv4Codes + kv4_place(c, key % kKv4Tokens) * 16;
-            scales_at[i] = nc * kKv4Codes + c * kKv4Scales + key % kKv4Tokens * 4;
-        }
+        const int chunks = min(C, nc - c0);   // of this thread (none: past the head size)
+        const uint32_t raw_codes = smem_addr(raw) + pt * 16, raw_scales = smem_addr(raw) + PT * C * 16 + pt * 4;   // [chunk][thread]
         const uint32_t row = smem_addr(su) + (c0 >> 1) * Cfg::block_b + key * 128 + ((((c0 & 1) * 4) ^ (key & 7)) << 4);
-        // (what every tile asks for, out of the parameters once)
-        const FastDiv page_div = p.page_div;
-        const int page_size = p.page_size, num_pages = p.num_pages, kv_heads = p.kv_heads;
-        const unsigned char* const packed = p.packed;
-        const int* pages = p.block_table + (int64_t)cur.b * p.table_stride;
         // this thread's key of the cursor's tile: a page number that is on its way, and which record of the page
+        const int* pages = p.block_table + (int64_t)cur.b * p.table_stride;
         int id = -1, in_page = 0, head = 0;
         MaskedKeys<WIN> masks = masked_keys<RT, WIN>(p, cur);
         bool mask = false;
         auto look_up = [&]() {
-            const int pos0 = cur.tile() * KT, pos = pos0 + key, pg = page_div.div(pos);
+            const int pos0 = cur.tile() * KT, pos = pos0 + key, pg = p.page_div.div(pos);
             id = pos < cur.r.seq ? __ldg(pages + pg) : -1;
-            in_page = (pos - pg * page_size) / kKv4Tokens;
+            in_page = (pos - pg * p.page_size) / kKv4Tokens;
             head = cur.h;
             mask = masks.template tile<KT>(p, pos0);
         };
@@ -645,64 +652,73 @@ __global__ void __launch_bounds__(TcCfg<DT, MT, REP, SRC>::threads, 1) tree_attn
             }
             look_up();
         };
-        // its keys' record by number; -1: past the end, or not a page of this cache (record 0 is read, its scales become zeros)
-        auto record = [&]() { return (unsigned)id < (unsigned)num_pages ? (id * kv_heads + head) * 2 * ps8 + in_page : -1; };
-        auto load = [&](Piece& u, int rec) {
-            const unsigned char* at = packed + (int64_t)max(rec, 0) * record_b;
-#pragma unroll
-            for (int i = 0; i < C; ++i) {
-                u.codes[i] = load_early16(at + codes_at[i]);
-                u.scales[i] = load_early4(at + scales_at[i]);
+        // its keys' record by number; -1: past the end, or not a page of this cache (zeros)
+        auto record = [&]() { return (unsigned)id < (unsigned)p.num_pages ? (id * p.kv_heads + head) * 2 * ps8 + in_page : -1; };
+        auto send = [&](int unit, int rec) {   // unit: 0 keys, 1 values
+            const unsigned char* at = p.packed + (int64_t)max(rec, 0) * record_b;
+            const int token = key % kKv4Tokens;
+#pragma unroll 1
+            for (int i = 0; i < chunks; ++i) {
+                const int c = c0 + i;
+                cp_async16(raw_codes + unit * Cfg::raw_unit_b + i * PT * 16, at + c * kKv4Codes + kv4_place(c, token) * 16, rec >= 0);
+                cp_async4(raw_scales + unit * Cfg::raw_unit_b + i * PT * 4, at + nc * kKv4Codes + c * kKv4Scales + token * 4, rec >= 0);
             }
+            cp_async_commit();
         };
-        auto put = [&](int n, Piece& u, bool live, bool check) {
+        auto put = [&](int n, int unit, bool check) {
             const int slot = n % NU;
+            cp_async_wait<Cfg::raw_units - 1>();   // (the last sent for may still be on their way)
             wait_warp(&empty[slot], ((n / NU) & 1) ^ 1);
-            if (__builtin_expect(!live, 0)) {
-#pragma unroll
-                for (int i = 0; i < C; ++i) u.scales[i] = 0;
-            }
-            if (__builtin_expect(check, 0)) {
-#pragma unroll
-                for (int i = 0; i < C; ++i)
-                    if (kv4_nan<T>(u.scales[i])) {   // not all rows see it: zeros (settle_packed)
-                        *reinterpret_cast<volatile int*>(dirty + slot) = n + 1;
-                        u.scales[i] = 0;
-                    }
-            }
-            const uint32_t to = row + slot * Cfg::unit_b;
-#pragma unroll
-            for (int i = 0; i < C; ++i) {
-                const Scale2<T> sc(u.scales[i]);
-                const uint32_t w[4] = {u.codes[i].x, u.codes[i].y, u.codes[i].z, u.codes[i].w};
+            const uint32_t to = row + slot * Cfg::unit_b, codes = raw_codes + unit * Cfg::raw_unit_b, scales = raw_scales + unit * Cfg::raw_unit_b;
+#pragma unroll 1
+            for (int i = 0; i < chunks; ++i) {
+                uint32_t sv = ld_shared4(scales + i * PT * 4);
+                const uint4 u = ld_shared16(codes + i * PT * 16);
+                if (__builtin_expect(check && kv4_nan<T>(sv), 0)) {   // not all rows see it: zeros (settle_packed)
+                    *reinterpret_cast<volatile int*>(dirty + slot) = n + 1;
+                    sv = 0;
+                }
+                const Scale2<T> sc(sv);
                 // (an even number of chunks a thread begins at an even one)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) st_shared16((to ^ (((i & 1) * 4 + j) << 4)) + (i >> 1) * Cfg::block_b, kv4_word<T>(w[j], sc));
+                const uint32_t at = (to ^ ((i & 1) << 6)) + (i >> 1) * Cfg::block_b;
+                st_shared16(at, kv4_word<T>(u.x, sc));
+                st_shared16(at ^ 16, kv4_word<T>(u.y, sc));
+                st_shared16(at ^ 32, kv4_word<T>(u.z, sc));
+                st_shared16(at ^ 48, kv4_word<T>(u.w, sc));
             }
             fence_proxy_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[slot]);
             __syncwarp();
         };
-        // a tile's pages are looked up a tile ahead of its loads, those are a tile ahead of the decoding
-        Piece k, v;
+        // a tile's pages are looked up a tile ahead of sending for it, which is a tile (one place for both: half a tile) ahead of
+        // its decoding
+        constexpr bool kBoth = Cfg::raw_units == 2;
+        constexpr int kValues = kBoth ? 1 : 0;
+        auto values = [&](int rec) { send(kValues, rec < 0 ? -1 : rec + ps8); };
         look_up();
         int rec = record(), rec_v = -1;   // of tile `step`, and the one before
         bool mask_k = mask, mask_v = false;
-        load(k, rec);
+        send(0, rec);
+        if (kBoth) cp_async_commit();     // (no values yet)
         look_ahead(1);
         int n = 0;
         for (int step = 0; step <= count; ++step) {
-            int next = -1;
+            const bool more = step + 1 < count;
+            const int next = more ? record() : -1;
             if (step < count) {
-                put(n++, k, rec >= 0, false);
-                if (step + 1 < count) {
-                    next = record();
-                    load(k, next);
-                }
+                put(n++, 0, false);
+                if (kBoth || (step == 0 && more)) send(0, next);
+                else values(step > 0 ? rec_v : rec);
+            } else if (kBoth) {
+                cp_async_commit();        // (no keys after the last values)
             }
-            if (step > 0) put(n++, v, rec_v >= 0, mask_v);
-            if (step < count) load(v, rec < 0 ? -1 : rec + ps8);
+            if (step > 0) {
+                put(n++, kValues, mask_v);
+                if (!kBoth && more) send(0, next);
+                else if (!kBoth && step < count) values(rec);
+            }
+            if (kBoth && step < count) values(rec);
             rec_v = rec;
             mask_v = mask_k;
             rec = next;
