@@ -108,6 +108,8 @@ static void set_window(TreeAttnParams& p, int window, int sinks)
 {
     p.window = window > 0 && window < kNoWindow ? window : kNoWindow;
     p.sinks = p.window < kNoWindow ? sinks : 0;
+    // (positions are taken against the window: no request is longer than "none" reaches)
+    if ((window || p.packed) && p.max_keys > kNoWindow) p.max_keys = kNoWindow;
 }
 
 // checks of an attention call and the kernel's parameters; cache: in 4 bits, instead of k_cache and v_cache

@@ -78,7 +78,7 @@ struct TreeAttnParams {
     const unsigned char* packed;                       // a cache in 4 bits instead of k_cache and v_cache
 };
 
-constexpr int kNoWindow = 1 << 30;   // longer than any cache
+constexpr int kNoWindow = 1 << 30;   // as long as the longest request of a windowed call, or over 4 bits
 constexpr int kAttnCtas = 4;         // most CTAs of an attention kernel on an SM
 
 // a cache in 4 bits (kv4.cuh has its layout), and the tokens of a call

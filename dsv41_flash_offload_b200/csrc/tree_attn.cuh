@@ -270,7 +270,7 @@ __device__ __forceinline__ void cut_runs(const TreeAttnParams& p, CutShared<WARP
     auto tiles = [&](const AttnReq& r) { return KeyTiles<RT, KT, WIN>().place(p, r, 0); };
     // sums over one head of request b (of this thread's; all threads go round together)
     auto sums = [&](const AttnReq& r, int64_t* s) {
-        if (WIN && own_lists) return head_sums<RT, KT, EXTRA, SMALL>(p, r.n, r.seq, s);
+        if (WIN && own_lists && __any_sync(0xffffffffu, row_tiles(r) > 1)) return head_sums<RT, KT, EXTRA, SMALL>(p, r.n, r.seq, s);
         const int64_t n = row_tiles(r);
         const int nt = tiles(r);
         s[0] = n * (nt + EXTRA), s[1] = n * nt, s[2] = n * cut_parts(nt, SMALL), s[3] = n * cut_parts(nt, 2 * SMALL);

@@ -346,7 +346,8 @@ typedef struct dsv41_tree_attention_args {
 int dsv41_tree_attention_workspace_size(int32_t head_dim, size_t* bytes);
 int dsv41_tree_attention(const dsv41_tree_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 /* The same through a window: of what a token sees without it, it sees the last `window` keys (itself counted, in the order
- * of the cache) and those at the first `sinks` positions of its request. window 0: all of them (sinks 0 then). */
+ * of the cache) and those at the first `sinks` positions of its request. window 0: all of them (sinks 0 then). With a window
+ * seq_lens go up to 2^30. */
 int dsv41_tree_attention_window(const dsv41_tree_attention_args* args, int32_t window, int32_t sinks, void* workspace,
                                 size_t workspace_bytes, void* stream);
 
@@ -354,7 +355,7 @@ int dsv41_tree_attention_window(const dsv41_tree_attention_args* args, int32_t w
  * to 256). Columns come in groups of 32: with lo and hi the smallest and largest value of a token's group, T the type (fp16 or
  * bf16), s = T((hi - lo) / 15) (the next smaller number where T(lo + 15 s) would not be finite), code = round((x - lo) / s) in
  * 0..15, halves to even, 0 where s is 0, a code stands for T(lo + s code), rounded once. A group with a value or an s that is
- * not finite stands for NaN. 20 bytes a group. data: dsv41_kv4_cache_size bytes, 16-byte aligned, its layout the library's own
+ * not finite stands for NaN. 20 bytes a group. Up to 2^31 - 1 records of 8 tokens of a head, page_size * kv_heads up to 2^24. data: dsv41_kv4_cache_size bytes, 16-byte aligned, its layout the library's own
  * ([page][head][keys, values], pages contiguous). One cache holds one type: that of the calls that store into it. */
 typedef struct dsv41_kv4_cache {
     int32_t num_pages, page_size, kv_heads, head_dim;
@@ -378,7 +379,7 @@ int dsv41_kv4_load(const dsv41_kv4_cache* cache, const dsv41_kv4_tokens* tokens,
 int dsv41_kv4_move(const dsv41_kv4_cache* cache, const int64_t* from, const int64_t* to, int32_t num_tokens, void* room, size_t room_bytes,
                    void* stream);
 /* dsv41_tree_attention_window over a cache in 4 bits: k_cache, v_cache and their strides are not read, kv_heads, head_dim, page_size and num_pages
- * are the cache's, dtype is that of q, out and the cache. The same workspaces. */
+ * are the cache's, dtype is that of q, out and the cache. The same workspaces. seq_lens go up to 2^30. */
 int dsv41_tree_attention4(const dsv41_tree_attention_args* args, const dsv41_kv4_cache* cache, int32_t window, int32_t sinks, void* workspace,
                           size_t workspace_bytes, void* stream);
 

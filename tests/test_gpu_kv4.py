@@ -276,6 +276,39 @@ def test_nan_reaches_those_who_see_it(heads, kv, dim, new, window, dtype):
     assert torch.equal(torch.isnan(attend4(d, window=window, sinks=sinks).cpu()), torch.isnan(win.reference(d, w, sinks)[0]))
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 64), (16, 2, 128), (2, 1, 256)])
+@pytest.mark.parametrize("window", [None, 70])
+def test_nan_within_a_prompt_chunk(heads, kv, dim, window):
+    """Without a mask a tile of new tokens is an ordinary one for the row tiles behind it: what is NaN there reaches them, and no
+    token before."""
+    s = build([90, 0], [310, 130], heads, kv, dim, 16, BF16, seed=dim, tree=False)
+    sinks = 2 if window else 0
+    clean = attend4(in4(s), window=window, sinks=sinks).cpu()
+    vc, table = s["vc"].clone(), s["table"].cpu()
+    for b, x, col in ((0, 90, 0), (0, 140, dim - 1), (0, 399, 0), (1, 1, 3), (1, 64, dim - 1)):
+        vc[int(table[b, x // 16]), x % 16, :, col] = math.nan
+    d = in4(dict(s, vc=vc))
+    got = attend4(d, window=window, sinks=sinks).cpu()
+    nan = torch.isnan(win.reference(d, window or 10 ** 6, sinks)[0])
+    assert bool(nan.any()) and torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], clean[~nan])
+
+
+def test_a_cache_without_pages():
+    """Every table entry lies outside it: keys and values of zeros."""
+    for heads, new in ((4, 1), (4, 30)):
+        c = paged.Cache4(0, 16, 2, 64, dtype=F16, device=DEV)
+        q = torch.randn(new, heads, 64, device=DEV).half()
+        out, lse = paged.tree_attention4(q, c, torch.zeros(1, 4, dtype=torch.int32, device=DEV), torch.tensor([40], dtype=torch.int32, device=DEV),
+                                         torch.tensor([0, new], dtype=torch.int32, device=DEV), new, return_lse=True)
+        assert not bool(out.any())
+        keys = 40 - new + 1 + torch.arange(new)
+        assert torch.allclose(lse.cpu(), keys.float().log()[:, None].expand(new, heads), atol=1e-5)
+        slots = torch.zeros(new, dtype=torch.int64, device=DEV)
+        paged.store_kv4(q[:, :2], q[:, :2], slots, c)
+        assert not bool(paged.load_kv4(slots, c)[0].any())
+        paged.move_kv4(slots, slots, c)
+
+
 def test_nan_in_a_split_request():
     s = build([9000, 40], [3, 2], 4, 2, 128, 16, BF16)
     clean = attend4(in4(s)).cpu()

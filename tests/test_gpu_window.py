@@ -155,6 +155,24 @@ def test_infinities_and_nan_outside_a_window(heads, kv, dim, page, new, tree):
     assert paged.read_status() == 0
 
 
+@pytest.mark.parametrize("heads,kv,dim,page", [(4, 1, 64, 16), (16, 2, 128, 64), (8, 1, 128, 7), (2, 1, 256, 24)])
+def test_infinities_within_a_prompt_chunk(heads, kv, dim, page):
+    """Without a mask a tile of new tokens is an ordinary one for the row tiles behind it: what it holds of infinities reaches
+    those whose window does, and no token before."""
+    s = build([90, 0], [310, 130], heads, kv, dim, page, F16, seed=dim, tree=False)
+    clean = attend(s, window=70, sinks=2).cpu()
+    vc, table = s["vc"].clone(), s["table"].cpu()
+    for b, x, col, value in ((0, 90, 0, math.inf), (0, 140, dim - 1, math.nan), (0, 399, 0, -math.inf), (1, 1, 3, math.inf), (1, 64, dim - 1, -math.inf)):
+        vc[int(table[b, x // page]), x % page, :, col] = value
+    d = dict(s, vc=vc)
+    got, want = attend(d, window=70, sinks=2).cpu(), reference(d, 70, 2)[0]
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    inf = torch.isinf(want)
+    assert bool(inf.any()) and torch.equal(torch.isinf(got), inf) and torch.equal(got[inf].double(), want[inf])
+    fin = torch.isfinite(want)
+    assert torch.equal(got[fin], clean[fin]) and paged.read_status() == 0
+
+
 def test_windowed_calls_in_a_graph_and_on_another_stream():
     s = build([3000, 77, 900], [9, 4, 1], 8, 2, 128, 16, BF16)
     want = attend(s, window=500, sinks=4)
