@@ -7,8 +7,9 @@
 // x - lo is formed in fp32 with its rounding error, the quotient from a reciprocal; where that comes near a half, the remainder of the
 // half decides, so every code is the exact quotient's.
 //
-// Four threads share a chunk, 8 columns (16 bytes) each: loads are whole, and a chunk's codes leave as 16 contiguous bytes. Bound by
-// HBM: 64 bytes in and 20 out a chunk.
+// Four threads share a chunk, 8 columns (16 bytes) of keys and of values each: loads are whole, and a chunk's codes leave as 16 contiguous
+// bytes. 64 bytes in and 20 out a chunk: 16384 tokens of 8 heads of 128 in 43 us (floor 13 us), bound by instructions (73% of the issue
+// slots, 16 a value); reading back 27 us, moving 33 us; 100 tokens 8, 6 and 10 us.
 //
 // Load is the reverse, and move copies codes and scales as they are (a drafted path that is accepted keeps its bits): all
 // are read before any is written, so slots may be both source and destination of one call.
