@@ -94,26 +94,6 @@ __device__ __forceinline__ uint4 kv4_word(uint32_t w, const Scale2<T>& sc)   // 
     return make_uint4(kv4_pair<T, 0>(w, sc), kv4_pair<T, 1>(w, sc), kv4_pair<T, 2>(w, sc), kv4_pair<T, 3>(w, sc));
 }
 
-// Loads that stay where they are written, ahead of the work that hides their latency (a plain one may be moved to its first use).
-__device__ __forceinline__ uint4 load_early16(const void* from)
-{
-    uint4 v;
-    asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(from));
-    return v;
-}
-__device__ __forceinline__ uint2 load_early8(const void* from)
-{
-    uint2 v;
-    asm volatile("ld.global.nc.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(from));
-    return v;
-}
-__device__ __forceinline__ uint32_t load_early4(const void* from)
-{
-    uint32_t v;
-    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(from));
-    return v;
-}
-
 // whether a chunk stands for NaN (lo is)
 template <typename T>
 __device__ __forceinline__ bool kv4_nan(uint32_t scales)

@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kLpThreads, TOP ? 2 : kPlainCtas) logprobs_ker
                 if (w0 + q * kLpThreads >= work) break;
                 const int have = s.count;
                 __syncthreads();   // (all have read it before any adds to it)
-                if (have > kLpRoom - kLpThreads * n - 32) {   // no room for what this round may find
+                if (have > kLpRoom - kLpThreads * n - 32) {   // no room for what these vectors may hold
                     lp_select(s, keys, have);
                     if (warp == 0) keys[lane] = s.best[0][lane];
                     if (tid == 0) s.count = 32;

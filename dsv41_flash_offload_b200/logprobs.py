@@ -49,13 +49,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     top = int(top)
     if logits.stride(1) != 1 and vocab > 1:
         logits = logits.contiguous()
-    tokens = tokens.to(torch.int64).contiguous()
-    logprobs = logits.new_empty(tokens.shape, dtype=torch.float32)
-    stats = logits.new_empty((2, n), dtype=torch.float32)
+    if tokens.dtype is not torch.int64 or not tokens.is_contiguous():
+        tokens = tokens.to(torch.int64).contiguous()
+    # one allocation for all that is fp32
+    floats = logits.new_empty(n * (given + 2 + top), dtype=torch.float32)
+    logprobs, entropy, lse, top_logprobs = floats.split_with_sizes((n * given, n, n, n * top))
     ids = tokens.new_empty((n, top))
-    top_logprobs = logits.new_empty((n, top), dtype=torch.float32)
-    base = stats.data_ptr()
+    base = floats.data_ptr()
+    at = base + 4 * n * given
     args = _lib.TokenLogprobsArgs(_DTYPES[logits.dtype], n, vocab, given, top, logits.data_ptr(), logits.stride(0), tokens.data_ptr(),
-                                  logprobs.data_ptr(), base, base + 4 * n, ids.data_ptr(), top_logprobs.data_ptr())
+                                  base, at, at + 4 * n, ids.data_ptr(), at + 8 * n)
     _lib.call(dev, _lib.load().dsv41_token_logprobs, C.byref(args), _lib.current_stream(dev))
-    return TokenLogprobs(logprobs, stats[0], stats[1], ids, top_logprobs)
+    return TokenLogprobs(logprobs if tokens.dim() == 1 else logprobs.view(n, given), entropy, lse, ids, top_logprobs.view(n, top))
