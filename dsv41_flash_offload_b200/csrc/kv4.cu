@@ -3,7 +3,8 @@
 // Store. For 32 columns x of a token's head, lo and hi their smallest and largest:
 //     s = T((hi - lo) / 15),   code = round((x - lo) / s) in 0..15 (halves to even; s = 0: 0),   x stands for T(lo + s code)
 // lo is one of the values and exact. Where the 15th code would round past T's largest number s is the next smaller one. A
-// chunk whose values or whose s are not finite stands for NaN throughout: it has no codes that say which of its columns are not.
+// chunk with a value that is not finite stands for NaN throughout: it has no codes that say which of its columns are not. So does
+// one whose hi - lo passes fp32, where s is formed: bf16 chunks of 3.4e38 and more from end to end.
 // x - lo is formed in fp32 with its rounding error, the quotient from a reciprocal; where that comes near a half, the remainder of the
 // half decides, so every code is the exact quotient's.
 //

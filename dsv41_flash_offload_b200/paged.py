@@ -312,8 +312,9 @@ class Cache4:
 
     Columns come in groups of 32. With lo and hi the smallest and largest value of a token's group, s = (hi - lo) / 15 in `dtype`
     and code = round((x - lo) / s), a code stands for lo + s * code, rounded once to `dtype`. A group with NaN or an infinity
-    stands for NaN. page_size is a multiple of 8, head_dim one of 32 up to 256. The layout of `data` (uint8, [num_pages, kv_heads, 2, ...]:
-    pages can be copied whole) is the library's own; one of your own must have that size, be contiguous and 16-byte aligned."""
+    stands for NaN, and so does a bfloat16 group whose range hi - lo passes fp32 (3.4e38: a value below -1.7e38 beside one above 1.7e38).
+    page_size is a multiple of 8, head_dim one of 32 up to 256. The layout of `data` (uint8, [num_pages, kv_heads, 2, ...]: pages can
+    be copied whole) is the library's own; one of your own must have that size, be contiguous and 16-byte aligned."""
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16, device=None,
                  data: torch.Tensor | None = None):

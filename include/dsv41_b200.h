@@ -354,9 +354,11 @@ int dsv41_tree_attention_window(const dsv41_tree_attention_args* args, int32_t w
 /* A cache in 4 bits: keys and values of num_pages pages of page_size tokens (a multiple of 8), kv_heads heads of head_dim (a multiple of 32 up
  * to 256). Columns come in groups of 32: with lo and hi the smallest and largest value of a token's group, T the type (fp16 or
  * bf16), s = T((hi - lo) / 15) (the next smaller number where T(lo + 15 s) would not be finite), code = round((x - lo) / s) in
- * 0..15, halves to even, 0 where s is 0, a code stands for T(lo + s code), rounded once. A group with a value or an s that is
- * not finite stands for NaN. 20 bytes a group. Up to 2^31 - 1 records of 8 tokens of a head, page_size * kv_heads up to 2^24. data: dsv41_kv4_cache_size bytes, 16-byte aligned, its layout the library's own
- * ([page][head][keys, values], pages contiguous). One cache holds one type: that of the calls that store into it. */
+ * 0..15, halves to even, 0 where s is 0, a code stands for T(lo + s code), rounded once. A group stands for NaN if one of its
+ * values is not finite, or if hi - lo is not in fp32 (bf16 only: 3.4e38 or more from end to end, whatever lies between).
+ * 20 bytes a group. Up to 2^31 - 1 records of 8 tokens of a head, page_size * kv_heads up to 2^24. data:
+ * dsv41_kv4_cache_size bytes, 16-byte aligned, its layout the library's own ([page][head][keys, values], pages contiguous).
+ * One cache holds one type: that of the calls that store into it. */
 typedef struct dsv41_kv4_cache {
     int32_t num_pages, page_size, kv_heads, head_dim;
     void* data;
