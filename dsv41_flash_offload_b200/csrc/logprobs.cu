@@ -403,10 +403,14 @@ static cudaError_t launch_lp(const LogprobParams& p, cudaStream_t st)
         if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return err;
         if (dev < 64) ready[dev] = true;
     }
-    // Few rows are shared by up to 8 CTAs each, of at least 4096 logits, as long as every CTA has an SM of its own. (Up to two on each: 100
-    // rows of 32768 with 20 alternatives 32 us for 21, on five 56: what a CTA does beside its sums does not shrink.)
+    // Few rows are shared by up to 8 CTAs each, of at least 4096 logits. With alternatives as long as every CTA has an SM of its own, for
+    // what a CTA does beside its sums does not shrink with its share: with 5 alternatives, 37 rows of 128000 bf16 logits take 23 us in
+    // four CTAs each and 31 in eight, 74 rows 23 in two and 33 in four, 100 rows of 32768 17 in one and 21 in two (75 rows of
+    // 128000 fp32 logits lose: 30 for 28). Without alternatives up to two CTAs on an SM: 100 rows of 128000 fp32 logits take 21 us in
+    // two each, 27 in one.
+    const int64_t places = (TOP ? 1 : 2) * (int64_t)num_sms();
     int ranks = 1;
-    while (ranks < 8 && (int64_t)p.rows * ranks * 2 <= 2 * num_sms() && p.vocab / (2 * ranks) >= 4096) ranks *= 2;
+    while (ranks < 8 && (int64_t)p.rows * ranks * 2 <= places && p.vocab / (2 * ranks) >= 4096) ranks *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.rows * ranks));
     cfg.blockDim = dim3(kLpThreads);
