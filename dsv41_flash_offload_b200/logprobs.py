@@ -1,9 +1,11 @@
 """Scores of a step's logits: log probabilities of given tokens, entropy, and the likeliest alternatives of every row, in one
 pass over the logits.
 
-`token_logprobs` takes logits as they are (a head's output, a slice of a padded one, any type); `w4.head_logprobs` goes from hidden states
-through a 4-bit head. All work runs on the current CUDA stream, nothing synchronises the host and nothing but the
-outputs is allocated, so the calls can be captured in a CUDA graph.
+`token_logprobs` takes logits as they are (a head's output, a slice of a padded one, any type); `w4.head_logprobs` goes from
+hidden states through a 4-bit head. All work runs on the current CUDA stream and nothing synchronises the host, so the calls can
+be captured in a CUDA graph. Beside the outputs, token_logprobs allocates a copy of tokens that are not contiguous int64 and of
+logits whose columns do not lie together; head_logprobs allocates its logits, fp32, of up to 256 rows at a time, and what it joins
+the results of more rows from. A captured graph keeps these in its pool.
 """
 from __future__ import annotations
 

@@ -8,12 +8,12 @@ s // page_size, and row b of a block table lists the pages of request b. One ste
     per layer:  store_kv(k, v, t.slots, k_cache, v_cache)
                 out = tree_attention(q, k_cache, v_cache, block_table, t.seq_lens, t.cu_lens, max_new, tree_mask=t.tree_mask)
 
-The same over a cache in 4 bits: Cache4 with store_kv4, tree_attention4, load_kv4 and move_kv4. `window=` and `sinks=` of both attentions leave
-the middle of long contexts out.
+The same over a cache in 4 bits: Cache4 with store_kv4, tree_attention4, load_kv4 and move_kv4. `window=` and `sinks=` of both
+attentions leave the middle of long contexts out.
 
 All lengths stay on the GPU, nothing synchronises the host, and after the first tree_attention on a stream
-(whose workspace is kept per device, stream and head size) only outputs are allocated, so a step can be
-captured in a CUDA graph. A graph uses the workspace that its capture took: the capture stream's own (made there by an
+(whose workspace is kept per device, stream and head size) only outputs are allocated, and what move_kv4 moves, so a
+step can be captured in a CUDA graph. A graph uses the workspace that its capture took: the capture stream's own (made there by an
 eager call or by reserve_workspace), or one given as `workspace=`. Replays that share a workspace, and eager calls on
 that stream, have to follow one another; graphs that run at the same time need one each (attention_workspace).
 """
