@@ -76,8 +76,8 @@ def step_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, held_pages: 
     pass the accepted context length and the surplus goes back. num_tokens is the length of the step's token
     batch, >= sum(new_lens); requests whose tokens pass it get seq_lens 0 and slots -1 (status PAST_TOKENS). parents
     (int32 [num_tokens]): index within its request of each drafted token's parent, which must lie before it, -1 for
-    the context; then positions are context + depth and tree_mask is built, for trees of up to 64 * mask_words tokens. A request that finds no pages is refused: status bit,
-    seq_lens 0, slots -1. free_pages should have room for every page of the pool: a request whose surplus does not fit, and
+    the context; then positions are context + depth and tree_mask is built, for trees of up to 64 * mask_words tokens. A request
+    that finds no pages is refused: status bit, seq_lens 0, slots -1. free_pages should have room for every page of the pool: a request whose surplus does not fit, and
     those behind it, keep theirs (status NO_ROOM) and are served all the same."""
     dev = context_lens.device
     if not context_lens.is_cuda or context_lens.dim() != 1 or not 1 <= context_lens.shape[0] <= MAX_REQUESTS:
@@ -243,8 +243,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     and the first seq_lens[b] slots of its pages, the last of them its new tokens. With tree_mask (int64 [N, words],
     step_tables) a token sees the context and the new tokens of its bits, without it the context and the new tokens
     up to itself. With `window` a token sees, of these, the last `window` (itself counted) and those at the first `sinks`
-    positions of its request; tiles of keys that no token of a request sees are not read. max_new is an upper bound on a request's new tokens, scale defaults to head_dim ** -0.5. Query head
-    h reads KV head h // (q_heads / kv_heads). A row that sees nothing is 0 with lse -inf. Returns out [N, q_heads,
+    positions of its request; tiles of keys that no token of a request sees are not read. max_new is an upper bound on a request's
+    new tokens, scale defaults to head_dim ** -0.5. Query head h reads KV head h // (q_heads / kv_heads). A row that sees nothing is 0 with lse -inf. Returns out [N, q_heads,
     head_dim] in q's dtype, or (out, lse fp32 [N, q_heads]); rows past cu_lens[B] are not written. workspace: one of
     attention_workspace's, which no other call may use at the same time (default: the stream's own)."""
     (pages, page_size, kv_heads, dim), cs, dev = _cache(k_cache, v_cache)
@@ -312,9 +312,9 @@ class Cache4:
 
     Columns come in groups of 32. With lo and hi the smallest and largest value of a token's group, s = (hi - lo) / 15 in `dtype`
     and code = round((x - lo) / s), a code stands for lo + s * code, rounded once to `dtype`. A group with NaN or an infinity
-    stands for NaN, and so does a bfloat16 group whose range hi - lo passes fp32 (3.4e38: a value below -1.7e38 beside one above 1.7e38).
-    page_size is a multiple of 8, head_dim one of 32 up to 256. The layout of `data` (uint8, [num_pages, kv_heads, 2, ...]: pages can
-    be copied whole) is the library's own; one of your own must have that size, be contiguous and 16-byte aligned."""
+    stands for NaN, and so does a bfloat16 group whose range hi - lo passes fp32 (3.4e38: a value below -1.7e38 beside one above
+    1.7e38). page_size is a multiple of 8, head_dim one of 32 up to 256. The layout of `data` (uint8, [num_pages, kv_heads, 2, ...]:
+    pages can be copied whole) is the library's own; one of your own must have that size, be contiguous and 16-byte aligned."""
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16, device=None,
                  data: torch.Tensor | None = None):
@@ -350,8 +350,8 @@ def store_kv4(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Cach
 
 
 def load_kv4(slots: torch.Tensor, cache: Cache4) -> tuple[torch.Tensor, torch.Tensor]:
-    """What the cache's slots (int64 [N]) stand for: (k, v) [N, kv_heads, head_dim] in its dtype, zeros for a slot of -1. For handing tokens
-    on: to a 16-bit cache (store_kv), to another engine."""
+    """What the cache's slots (int64 [N]) stand for: (k, v) [N, kv_heads, head_dim] in its dtype, zeros for a slot of -1. For
+    handing tokens on: to a 16-bit cache (store_kv), to another engine."""
     N, dev = slots.shape[0] if slots.dim() else 0, cache.device
     slots = _vector(slots, "slots", N, torch.int64, dev)
     k, v = (torch.empty((N, cache.kv_heads, cache.head_dim), dtype=cache.dtype, device=dev) for _ in range(2))
@@ -360,8 +360,9 @@ def load_kv4(slots: torch.Tensor, cache: Cache4) -> tuple[torch.Tensor, torch.Te
 
 
 def move_kv4(src: torch.Tensor, dst: torch.Tensor, cache: Cache4) -> None:
-    """Copy the tokens of slots src[i] to dst[i] (int64 [N]) with the bits they have, e.g. an accepted path of drafted tokens to the end
-    of its context. All are read before any is written, so a slot may be in both; none may come twice in dst. -1 in either: nothing."""
+    """Copy the tokens of slots src[i] to dst[i] (int64 [N]) with the bits they have, e.g. an accepted path of drafted tokens to
+    the end of its context. All are read before any is written, so a slot may be in both; none may come twice in dst. -1 in either:
+    nothing."""
     N, dev = src.shape[0] if src.dim() else 0, cache.device
     src = _vector(src, "src", N, torch.int64, dev)
     dst = _vector(dst, "dst", N, torch.int64, dev)

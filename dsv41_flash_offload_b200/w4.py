@@ -142,8 +142,9 @@ def shared_expert(x: torch.Tensor, gate: W4Weight, up: W4Weight, down: W4Weight,
     return linear(gated(x, gate, up, limit), down, out=out, accumulate=True)
 
 
-# Rows of logits at a time, which bounds what they take: 100 MB at a vocabulary of 100000. The number hardly matters for time, which is
-# the product's: 512 rows of 4096 through a head of 100001, with 20 alternatives, 2080 us in pieces of 64, 1990 of 128, 1950 of 256, 1935 of 512.
+# Rows of logits at a time, which bounds what they take: 100 MB at a vocabulary of 100000. The number hardly matters for time, which
+# is the product's: 512 rows of 4096 through a head of 100001, with 20 alternatives, 2080 us in pieces of 64, 1990 of 128, 1950 of
+# 256, 1935 of 512.
 _HEAD_ROWS = 256
 
 

@@ -351,8 +351,8 @@ int dsv41_tree_attention(const dsv41_tree_attention_args* args, void* workspace,
 int dsv41_tree_attention_window(const dsv41_tree_attention_args* args, int32_t window, int32_t sinks, void* workspace,
                                 size_t workspace_bytes, void* stream);
 
-/* A cache in 4 bits: keys and values of num_pages pages of page_size tokens (a multiple of 8), kv_heads heads of head_dim (a multiple of 32 up
- * to 256). Columns come in groups of 32: with lo and hi the smallest and largest value of a token's group, T the type (fp16 or
+/* A cache in 4 bits: keys and values of num_pages pages of page_size tokens (a multiple of 8), kv_heads heads of head_dim
+ * (a multiple of 32 up to 256). Columns come in groups of 32: with lo and hi the smallest and largest value of a token's group, T the type (fp16 or
  * bf16), s = T((hi - lo) / 15) (the next smaller number where T(lo + 15 s) would not be finite), code = round((x - lo) / s) in
  * 0..15, halves to even, 0 where s is 0, a code stands for T(lo + s code), rounded once. A group stands for NaN if one of its
  * values is not finite, or if hi - lo is not in fp32 (bf16 only: 3.4e38 or more from end to end, whatever lies between).
@@ -372,16 +372,16 @@ typedef struct dsv41_kv4_tokens {
     const int64_t* slots;
 } dsv41_kv4_tokens;
 int dsv41_kv4_cache_size(int32_t num_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim, size_t* bytes);
-/* store: k and v into the tokens' slots; a slot outside the cache stores nothing. A slot may not come twice in a call (its codes and
- * scales could be of different tokens). load: what the slots stand for into k and v (strides not 0), zeros for a slot outside. move: the
- * codes of from[t] to to[t] as they are, all read before any is written (a slot may be in both; none twice in `to`); nothing
- * where either lies outside. room: num_tokens * kv_heads * head_dim / 32 * 40 bytes, 16-byte aligned. */
+/* store: k and v into the tokens' slots; a slot outside the cache stores nothing. A slot may not come twice in a call (its
+ * codes and scales could be of different tokens). load: what the slots stand for into k and v (strides not 0), zeros for a slot
+ * outside. move: the codes of from[t] to to[t] as they are, all read before any is written (a slot may be in both; none twice
+ * in `to`); nothing where either lies outside. room: num_tokens * kv_heads * head_dim / 32 * 40 bytes, 16-byte aligned. */
 int dsv41_kv4_store(const dsv41_kv4_cache* cache, const dsv41_kv4_tokens* tokens, void* stream);
 int dsv41_kv4_load(const dsv41_kv4_cache* cache, const dsv41_kv4_tokens* tokens, void* stream);
 int dsv41_kv4_move(const dsv41_kv4_cache* cache, const int64_t* from, const int64_t* to, int32_t num_tokens, void* room, size_t room_bytes,
                    void* stream);
-/* dsv41_tree_attention_window over a cache in 4 bits: k_cache, v_cache and their strides are not read, kv_heads, head_dim, page_size and num_pages
- * are the cache's, dtype is that of q, out and the cache. The same workspaces. seq_lens go up to 2^30. */
+/* dsv41_tree_attention_window over a cache in 4 bits: k_cache, v_cache and their strides are not read, kv_heads, head_dim,
+ * page_size and num_pages are the cache's, dtype is that of q, out and the cache. The same workspaces. seq_lens go up to 2^30. */
 int dsv41_tree_attention4(const dsv41_tree_attention_args* args, const dsv41_kv4_cache* cache, int32_t window, int32_t sinks, void* workspace,
                           size_t workspace_bytes, void* stream);
 
