@@ -27,9 +27,10 @@ cudaError_t launch_tree_attn(const TreeAttnParams& p, int dtype, int max_rows, c
     return dtype == 0 ? launch_tree_attn_f16(p, max_rows, st) : launch_tree_attn_bf16(p, max_rows, st);
 }
 
-// Over a cache in 4 bits, up to 16 rows codes are decoded straight into the fragments of warp-level matrix instructions (tree_attn4_rows.cuh), more
-// go through shared memory to the fifth-generation tensor cores: 4 requests of 32-64k keys, 8 KV heads of 128, 8 rows 90 us (148 the other way), 16 rows
-// 111 (148); with 24 rows the first would read the keys twice, 200 us for 152. Heads of 64: 64, 78 (113) and 115; of 256: 158, 203 (387) and 390.
+// Over a cache in 4 bits, up to 16 rows codes are decoded straight into the fragments of warp-level matrix instructions
+// (tree_attn4_rows.cuh), more go through shared memory to the fifth-generation tensor cores. 4 requests of 32-64k keys, 8 KV heads of
+// 128: 8 rows 80 us (141 the other way), 16 rows 100 (140), 24 rows, for which the first reads the keys twice, 169 and 142. Heads of 64:
+// 60 (109), 72 (107), 118 and 107; of 256: 141 (377), 180 (380), 311 and 385 (there the first would still be the faster one).
 constexpr int kFewRows = 16;
 
 cudaError_t launch_tree_attn4(const TreeAttnParams& p, int dtype, int max_rows, cudaStream_t st)

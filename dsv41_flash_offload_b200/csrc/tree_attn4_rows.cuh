@@ -20,7 +20,7 @@
 // other kernel (tree_attn_kernel.cuh).
 //
 // Measured: one token of 8 rows a KV head (8 heads of 128, bf16) over 4 requests of 65-131k keys 141 us, 3.5 TB/s of codes (floor 75 us);
-// one request of 131k keys 70 us (26); 4 of 32-64k keys 90 us, with 16 rows 111 us. Bound by instructions: 420 a step of 16 keys, 256 of
+// one request of 131k keys 68 us (26); 4 of 32-64k keys 80 us, with 16 rows 100 us. Bound by instructions: 420 a step of 16 keys, 256 of
 // them the decoding (a shift or mask, two 16-bit operations for two values), at 0.6 a cycle and scheduler: ALU 41%, fp16 and
 // integer products 43% of their pipes, matrix instructions 16%, loads hardly waited for. A fifth or more of a call this size is start (lengths,
 // pages, first records: 8 us) and join. More CTAs an SM, loads to registers, bulk copies measured the same or slower.

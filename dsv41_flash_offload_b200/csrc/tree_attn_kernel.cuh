@@ -33,9 +33,10 @@
 // 5.4 TB/s; 128 rows 156 us, 5.0 TB/s, 643 TFLOP/s; 256 rows 251 us, 802 TFLOP/s. The first two are bound by the key
 // stream and, at the ends of a run, by latency; the last waits: no pipe is full (a third of the issue slots, exponentials
 // at 36% of theirs, tensor pipe 35%), its softmax warps stand at loads from tensor memory, where S is read twice, and at one
-// another. Over a cache in 4 bits, same lengths: 24 or 32 rows 152 us, 64 rows 166 us, 128 rows 193 us; 32 x 64 tokens of 4 rows over 1-8k
-// keys 240 us (16 bits: 223), the decoding warps' instructions and fences. Through a window of 2048: prompt chunks of 6000 and 8192
-// tokens, 32/8 heads of 128, 856 us, 520 TFLOP/s of the pairs that are seen (3 of the 19 tiles that a row tile walks are masked).
+// another. Over a cache in 4 bits, same lengths: 24 or 32 rows 145 us, 64 rows 160 us, 128 rows 182 us, 256 rows 264 us; heads of 256 384,
+// 401, 473 and 897 us (codes of one unit at a time); 32 x 64 tokens of 4 rows over 1-8k keys 240 us (16 bits: 223). Through a window of
+// 2048: prompt chunks of 6000 and 8192 tokens, 32/8 heads of 128, 856 us, 520 TFLOP/s of the pairs that are seen (3 of the 19 tiles
+// that a row tile walks are masked).
 // Heads of 256 (floor 240 us): 266 us, 5.9 TB/s; 288 us; 523 us (two tiles of
 // 128 rows, a second trip of the keys), 769 TFLOP/s; 192: 245 us, 4.8 TB/s (a quarter of the ring idle). Warp-level
 // matrix instructions took 780 us for the first of 256 and reached 120 TFLOP/s in the last. A call of one tile takes
